@@ -25,7 +25,7 @@
 #include <stdint.h>
 
 /* The version of these entry points' signatures (kvq_abi_version): changes with any of them. */
-#define KVQ_ABI_VERSION 12
+#define KVQ_ABI_VERSION 13
 
 #ifdef __cplusplus
 extern "C" {
@@ -269,6 +269,66 @@ int kvq_stream_scatter(const void* key, int64_t key_st, int64_t key_sh, const vo
                        int64_t val_sh, int8_t* k_cache, int8_t* v_cache, int64_t c_sb, int64_t c_sn, int64_t c_sh,
                        const int64_t* slot_mapping, int64_t n_tokens, int64_t num_heads, int64_t head_dim,
                        int64_t num_blocks, int64_t block_size, void* stream);
+
+/* ---- Block-scaled INT8 cache: no calibrated scales, no counterpart in the reference ----
+ * A block is `group` consecutive positions of a page (group = 16, 32, 64 or 128, at most block_size; block b of a page
+ * is its slots b group .. + group - 1). Each (page, kv head, block) has one fp32 scale for K and one for V: at
+ * page * s_sb + head * s_sh + b * s_sg floats of k_scale / v_scale (the same strides for both). A cached value is
+ * code * scale. Caches, tables and lengths as above (16-byte aligned rows; head_dim 64 or 128). */
+
+/* Quantize a step's new tokens into their blocks: request r's tokens cu_seqlens_q[r] .. cu_seqlens_q[r + 1] - 1 of key /
+ * value are its last positions (up to seq_lens[r] - 1), in pages of its row of block_table. For each block touched and
+ * head, over the block's new values x, with s_old the block's scale if it holds earlier positions of the request, else 0:
+ *   s = max(s_old, fl(max |x| / 127), 1e-8)   (finite x; an infinite one saturates, a NaN's code is any)
+ *   new slots sat127(rint(fl(x / s))), the request's earlier slots of the block rint(fl(code * fl(s_old / s))) if s > s_old
+ * Other slots and scales stay as they are. A page id outside [0, num_blocks) and a token at a negative position
+ * (seq_lens[r] < its tokens) are skipped, as are tokens from num_tokens on (the rows key / value hold). The pages that
+ * a call writes must belong to one request each. Stream-ordered, allocates nothing, bit-reproducible. */
+int kvq_quant_block_cache(const void* key, int64_t key_st, int64_t key_sh, const void* value, int64_t val_st,
+                          int64_t val_sh, int64_t num_tokens, int8_t* k_cache, int64_t kc_sb, int64_t kc_sn,
+                          int64_t kc_sh, int8_t* v_cache, int64_t vc_sb, int64_t vc_sn, int64_t vc_sh,
+                          int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, float* k_scale,
+                          float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group,
+                          const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+                          int64_t bt_stride, int64_t num_seqs, void* stream);
+
+/* Read ranges of keys back: positions starts[r] .. of request r become rows cu_seqlens_k[r] .. cu_seqlens_k[r + 1] - 1
+ * of k_out / v_out (bf16 [num_rows, H, D], strides (st, sh, 1)): bf16_rne(code * scale). Rows past cu_seqlens_k's last
+ * entry are left as they were, rows from num_rows on are not written, a negative start reads nothing. */
+int kvq_read_block_cache(const int8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, const int8_t* v_cache,
+                         int64_t vc_sb, int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size,
+                         int64_t num_heads, int64_t head_dim, const float* k_scale, const float* v_scale, int64_t s_sb,
+                         int64_t s_sh, int64_t s_sg, int64_t group, const int32_t* starts, const int32_t* cu_seqlens_k,
+                         const int32_t* block_table, int64_t bt_stride, int64_t num_seqs, void* k_out, int64_t ko_st,
+                         int64_t ko_sh, void* v_out, int64_t vo_st, int64_t vo_sh, int64_t num_rows, void* stream);
+
+/* Attention over a block-scaled cache for requests with 1 <= q_len <= qmax:
+ *   o = softmax(q . (k_code * k_scale) * softmax_scale) (v_code * v_scale),  bottom-right causal, bf16 q and out;
+ * a row that sees no key is zero. Neither q nor the softmax's weights are rounded to 8 bits. Rows, skipped requests, split
+ * buffers and the other arguments as kvq_int8_decode_attention_ex. */
+int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
+                               int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
+                               int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+                               int64_t head_dim, const float* k_scale, const float* v_scale, int64_t s_sb, int64_t s_sh,
+                               int64_t s_sg, int64_t group, void* out, int64_t o_st, int64_t o_sh,
+                               const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+                               int64_t bt_stride, int64_t num_seqs, int64_t num_q_heads, double softmax_scale,
+                               float* segm_out, float* segm_max, float* segm_sum, int64_t seg_st, int64_t seg_sh,
+                               int64_t num_splits, int64_t segm_rows, int64_t target_waves, int64_t max_query_len,
+                               int64_t qmax, void* stream);
+
+/* The same attention for the rows of a work list, as kvq_int8_prefill_attention_ex takes it (tile_piece NULL: every
+ * entry reads all of its rows' keys). */
+int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
+                                int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
+                                int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+                                int64_t head_dim, const float* k_scale, const float* v_scale, int64_t s_sb, int64_t s_sh,
+                                int64_t s_sg, int64_t group, void* out, int64_t o_st, int64_t o_sh,
+                                const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+                                int64_t bt_stride, int64_t num_q_heads, const int32_t* tile_req, const int32_t* tile_row,
+                                int64_t num_tiles, int64_t rows_per_tile, double softmax_scale, const int32_t* tile_piece,
+                                const int32_t* tile_slot, const int32_t* merge, int64_t num_merge, float* part_out,
+                                float* part_ml, void* stream);
 
 /* Text of the last error on this thread ("" if none). */
 const char* kvq_last_error(void);

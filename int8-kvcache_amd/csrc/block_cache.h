@@ -1,0 +1,528 @@
+// The block-scaled INT8 cache: no calibrated scales, one fp32 scale for each block of 16 .. 128 consecutive positions
+// of a page and kv head, K and V apart, made as the cache is written. Part of kvq_int8.hip (included at its end: it
+// shares the helpers above it).
+//
+//   quant_block_kernel   quantize a step's new K/V into their blocks, raising scales (and requantizing) where needed
+//   read_block_kernel    ranges of the requests' keys back to bf16 rows
+//   block_rows_kernel    attention, one wavefront per (query token, q head)
+//
+// A cached value is code * scale; attention is that of those values and the bf16 q, without further rounding of either.
+
+namespace {
+
+constexpr int BLK_MIN = 16, BLK_MAX = 128;   // positions per scale
+
+// Where the scales lie: that of (page p, head h, block b) at p * sb + h * sh + b * sg floats of ks / vs.
+struct BlockScales {
+  const float* ks;
+  const float* vs;
+  int64_t sb, sh, sg;
+  int lg;   // log2 of the positions per scale
+};
+
+// The request that holds slot u of a line on which request r starts at (cu[r] >> lg) + 2 r: as long as cu[r] counts
+// rows of consecutive positions, r's rows touch at most (rows >> lg) + 2 aligned blocks of 2^lg positions, so its
+// blocks fit before the next request's start wherever its first position lies in a block. A launch sizes its grid
+// from the row count alone. 64-way search, the lanes a probe each; every lane returns the same r.
+__device__ __forceinline__ int request_of_slot(const int* __restrict__ cu, int num_seqs, int lg, int u, int lane) {
+  int lo = 0, n = num_seqs;
+  while (n > 1) {
+    const int step = (n + WAVE - 1) / WAVE, r = lo + lane * step;
+    const bool in = lane * step < n && (cu[r] >> lg) + 2 * r <= u;
+    // (the first probe always holds: request lo starts at or before u)
+    const int k = __builtin_popcountll(__ballot(in)) - 1;
+    lo += max(k, 0) * step;
+    n = min(step, num_seqs - lo);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+inline int64_t block_slots(int64_t rows, int64_t num_seqs, int lg) { return (rows >> lg) + 2 * num_seqs; }
+
+__device__ __forceinline__ int page_at(const int* __restrict__ bt, int64_t bt_stride, int r, int page) {
+  return __builtin_amdgcn_readfirstlane(bt[(int64_t)r * bt_stride + page]);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Quantize a step's new K / V rows into their blocks. Request r's new tokens are its last q_r positions; one item is
+// one (request, block, head), whose W = block / 16 wavefronts take 16 positions each, K and V. With x the block's new
+// values and s_old its scale if it holds earlier positions of the request (else 0):
+//   s = max(s_old, fl(max |x| / 127), 1e-8);  new slots: sat127(rint(fl(x / s)));  old: rint(fl(code * fl(s_old / s)))
+// The items of a call touch disjoint blocks, so nothing is shared between wavefronts of different items.
+// ------------------------------------------------------------------------------------------------
+struct QuantBlockArgs {
+  const uint16_t* key;
+  const uint16_t* value;
+  int8_t* kc;
+  int8_t* vc;
+  float* ks;
+  float* vs;
+  const int* cu_q;
+  const int* seq_lens;
+  const int* block_table;
+  int64_t key_st, key_sh, val_st, val_sh, kc_sb, kc_sn, kc_sh, vc_sb, vc_sn, vc_sh, s_sb, s_sh, s_sg, bt_stride;
+  int num_seqs, num_tokens, heads, num_blocks, lbs, lg, items;
+};
+
+// largest finite |x| of 8 bf16
+__device__ __forceinline__ float absmax8(u32x4 w) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = __builtin_fabsf(bf16_lo(w[j])), b = __builtin_fabsf(bf16_hi(w[j]));
+    m = __builtin_fmaxf(m, a < INFINITY ? a : 0.f);
+    m = __builtin_fmaxf(m, b < INFINITY ? b : 0.f);
+  }
+  return m;
+}
+__device__ __forceinline__ u32x2 codes8(u32x4 w, float s, float y) {
+  float t[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    t[2 * j] = code_magic(bf16_lo(w[j]), s, y);
+    t[2 * j + 1] = code_magic(bf16_hi(w[j]), s, y);
+  }
+  return u32x2{pack_magic4(t[0], t[1], t[2], t[3]), pack_magic4(t[4], t[5], t[6], t[7])};
+}
+// 8 codes at another scale: rint(fl(code * ratio)), ratio <= 1
+__device__ __forceinline__ u32x2 rescaled8(u32x2 c, float ratio) {
+  float t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = (float)(int8_t)(c[e / 4] >> (8 * (e % 4))) * ratio + QC_MAGIC;
+  return u32x2{pack_magic4(t[0], t[1], t[2], t[3]), pack_magic4(t[4], t[5], t[6], t[7])};
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(WAVE * (W < 4 ? 4 : W)) void quant_block_kernel(QuantBlockArgs a) {
+  constexpr int LPR = D / 8;              // lanes per row
+  constexpr int RPL = WAVE / LPR;         // rows per load
+  constexpr int N = 16 / RPL;             // loads per matrix and wavefront
+  constexpr int WPB = W < 4 ? 4 : W;      // wavefronts per workgroup
+  __shared__ float top[WPB][2];
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int item = blockIdx.x * (WPB / W) + wave / W, part = wave % W;
+  bool live = item < a.items;
+  int h = 0, p0 = 0, first = 0, last = 0, tok0 = 0, page = 0, off = 0;
+  if (live) {
+    const int u = item / a.heads;
+    h = item - u * a.heads;
+    const int r = request_of_slot(a.cu_q, a.num_seqs, a.lg, u, lane);
+    const int tok = a.cu_q[r], q = min(a.cu_q[r + 1], a.num_tokens) - tok, len = a.seq_lens[r];
+    p0 = len - (a.cu_q[r + 1] - tok);                                     // first new position (negative ones: no slot)
+    const int blk = (max(p0, 0) >> a.lg) + u - ((tok >> a.lg) + 2 * r);   // the item's block of the request's positions
+    const int b0 = blk << a.lg;
+    first = max(max(p0, 0), b0);                                          // new positions [first, last) of the block
+    last = min(p0 + q, b0 + (1 << a.lg));
+    live = first < last;
+    if (live) {
+      page = page_at(a.block_table, a.bt_stride, r, b0 >> a.lbs);
+      live = page >= 0 && page < a.num_blocks;                            // a bad id: nothing is written
+    }
+    off = b0 & ((1 << a.lbs) - 1);                                        // the block's first slot of the page
+    tok0 = tok - p0;                                                      // token of position p: tok0 + p
+    p0 = b0;
+  }
+  const int row = lane / LPR, d0 = 8 * (lane % LPR);
+  u32x4 kin[N], vin[N];
+  u32x2 kold[N], vold[N];
+  int8_t* kc = a.kc + (int64_t)page * a.kc_sb + (int64_t)(off + 16 * part) * a.kc_sn + (int64_t)h * a.kc_sh + d0;
+  int8_t* vc = a.vc + (int64_t)page * a.vc_sb + (int64_t)(off + 16 * part) * a.vc_sn + (int64_t)h * a.vc_sh + d0;
+  const bool begun = live && first > p0;                                  // earlier positions of the request share the block
+  float km = 0.f, vm = 0.f, ks_old = 0.f, vs_old = 0.f;
+  float* ksp = a.ks + (int64_t)page * a.s_sb + (int64_t)h * a.s_sh + (int64_t)(off >> a.lg) * a.s_sg;
+  float* vsp = a.vs + (int64_t)page * a.s_sb + (int64_t)h * a.s_sh + (int64_t)(off >> a.lg) * a.s_sg;
+  if (begun) {
+    ks_old = *ksp;
+    vs_old = *vsp;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = row + RPL * j, p = p0 + 16 * part + i;
+    kin[j] = vin[j] = u32x4{0u, 0u, 0u, 0u};
+    kold[j] = vold[j] = u32x2{0u, 0u};
+    if (live && p >= first && p < last) {
+      const int64_t t = tok0 + p;
+      kin[j] = *reinterpret_cast<const u32x4*>(a.key + t * a.key_st + (int64_t)h * a.key_sh + d0);
+      vin[j] = *reinterpret_cast<const u32x4*>(a.value + t * a.val_st + (int64_t)h * a.val_sh + d0);
+    } else if (begun && p < first) {
+      kold[j] = *reinterpret_cast<const u32x2*>(kc + (int64_t)i * a.kc_sn);
+      vold[j] = *reinterpret_cast<const u32x2*>(vc + (int64_t)i * a.vc_sn);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    km = __builtin_fmaxf(km, absmax8(kin[j]));
+    vm = __builtin_fmaxf(vm, absmax8(vin[j]));
+  }
+  km = wave_max(km);
+  vm = wave_max(vm);
+  if constexpr (W > 1) {   // the block's wavefronts agree on the maxima
+    if (lane == 0) {
+      top[wave][0] = km;
+      top[wave][1] = vm;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      km = __builtin_fmaxf(km, top[wave - part + k][0]);
+      vm = __builtin_fmaxf(vm, top[wave - part + k][1]);
+    }
+  }
+  if (!live) return;
+  const float ks = __builtin_fmaxf(__builtin_fmaxf(km / 127.f, 1e-8f), ks_old);
+  const float vs = __builtin_fmaxf(__builtin_fmaxf(vm / 127.f, 1e-8f), vs_old);
+  if (lane == 0 && part == 0) {
+    *ksp = ks;
+    *vsp = vs;
+  }
+  const float ky = 1.f / ks, vy = 1.f / vs, kr = ks_old / ks, vr = vs_old / vs;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = row + RPL * j, p = p0 + 16 * part + i;
+    u32x2* kp = reinterpret_cast<u32x2*>(kc + (int64_t)i * a.kc_sn);
+    u32x2* vp = reinterpret_cast<u32x2*>(vc + (int64_t)i * a.vc_sn);
+    if (p >= first && p < last) {
+      *kp = codes8(kin[j], ks, ky);
+      *vp = codes8(vin[j], vs, vy);
+    } else if (begun && p < first) {
+      if (ks > ks_old) *kp = rescaled8(kold[j], kr);
+      if (vs > vs_old) *vp = rescaled8(vold[j], vr);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Read ranges of keys back: request r's positions start[r] .. are rows cu_k[r] .. cu_k[r + 1] - 1 of k_out / v_out,
+// bf16_rne(code * scale). One wavefront takes one aligned run of 16 positions (one page, one scale) of one head.
+// ------------------------------------------------------------------------------------------------
+struct ReadBlockArgs {
+  const int8_t* kc;
+  const int8_t* vc;
+  uint16_t* ko;
+  uint16_t* vo;
+  const int* start;
+  const int* cu_k;
+  const int* block_table;
+  BlockScales s;
+  int64_t kc_sb, kc_sn, kc_sh, vc_sb, vc_sn, vc_sh, ko_st, ko_sh, vo_st, vo_sh, bt_stride;
+  int num_seqs, num_rows, heads, num_blocks, lbs, items;
+};
+
+template <int D>
+__global__ __launch_bounds__(256) void read_block_kernel(ReadBlockArgs a) {
+  constexpr int LPR = D / 8, RPL = WAVE / LPR, N = 16 / RPL;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int item = blockIdx.x * 4 + wave;
+  if (item >= a.items) return;
+  const int u = item / a.heads, h = item - u * a.heads;
+  const int r = request_of_slot(a.cu_k, a.num_seqs, 4, u, lane);
+  const int row0 = a.cu_k[r], n = min(a.cu_k[r + 1], a.num_rows) - row0, start = a.start[r];
+  if (start < 0) return;
+  const int b0 = ((start >> 4) + u - ((row0 >> 4) + 2 * r)) << 4;
+  const int first = max(start, b0), last = min(start + n, b0 + 16);
+  if (first >= last) return;
+  int page = page_at(a.block_table, a.bt_stride, r, b0 >> a.lbs);
+  page = page >= 0 && page < a.num_blocks ? page : 0;
+  const int off = b0 & ((1 << a.lbs) - 1);
+  const int64_t si = (int64_t)page * a.s.sb + (int64_t)h * a.s.sh + (int64_t)(off >> a.s.lg) * a.s.sg;
+  const float ks = a.s.ks[si], vs = a.s.vs[si];
+  const int row = lane / LPR, d0 = 8 * (lane % LPR);
+  const int8_t* kc = a.kc + (int64_t)page * a.kc_sb + (int64_t)off * a.kc_sn + (int64_t)h * a.kc_sh + d0;
+  const int8_t* vc = a.vc + (int64_t)page * a.vc_sb + (int64_t)off * a.vc_sn + (int64_t)h * a.vc_sh + d0;
+  float ksc[8], vsc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    ksc[e] = ks;
+    vsc[e] = vs;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = row + RPL * j, p = b0 + i;
+    if (p < first || p >= last) continue;
+    const int64_t t = row0 + p - start;
+    const u32x2 k = *reinterpret_cast<const u32x2*>(kc + (int64_t)i * a.kc_sn);
+    const u32x2 v = *reinterpret_cast<const u32x2*>(vc + (int64_t)i * a.vc_sn);
+    *reinterpret_cast<u32x4*>(a.ko + t * a.ko_st + (int64_t)h * a.ko_sh + d0) = dq8x(k.x, k.y, ksc);
+    *reinterpret_cast<u32x4*>(a.vo + t * a.vo_st + (int64_t)h * a.vo_sh + d0) = dq8x(v.x, v.y, vsc);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Attention of one (query token, q head) by one wavefront: a lane scores one of 64 keys, then the lanes own D / 64
+// channels each and add the 64 keys' values. fp32 throughout.
+// ------------------------------------------------------------------------------------------------
+struct BlockRowsArgs {
+  const uint16_t* q;
+  const int8_t* kc;
+  const int8_t* vc;
+  uint16_t* out;
+  const int* cu_q;
+  const int* seq_lens;
+  const int* block_table;
+  const int* tile_req;    // long-query calls: the rows of entry blockIdx.x (NULL: every token of the batch)
+  const int* tile_row;
+  BlockScales s;
+  int64_t q_st, q_sh, o_st, o_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, bt_stride;
+  float sm_log2;
+  int num_seqs, hkv, G, qmax, num_blocks, lbs;
+};
+
+template <int D>
+__device__ __forceinline__ void attend_row(const BlockRowsArgs& a, int r, int tok, int qlen, int t, int kvh, int head, int lane,
+                                           float* lq) {
+  const int len = a.seq_lens[r], lim = min(len, len - qlen + 1 + t);
+  const uint16_t* qp = a.q + (int64_t)(tok + t) * a.q_st + (int64_t)head * a.q_sh;
+  for (int d = lane; d < D; d += WAVE) lq[d] = __uint_as_float((uint32_t)qp[d] << 16) * a.sm_log2;
+  __builtin_amdgcn_wave_barrier();
+  const int bsm = (1 << a.lbs) - 1;
+  constexpr int CPL = D / WAVE;
+  float m = -1e30f, l = 0.f, acc[CPL];
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
+  for (int k0 = 0; k0 < lim; k0 += WAVE) {
+    const int key = min(k0 + lane, lim - 1);
+    int page = a.block_table[(int64_t)r * a.bt_stride + (key >> a.lbs)];
+    page = page >= 0 && page < a.num_blocks ? page : 0;
+    const int slot = key & bsm;
+    const int64_t si = (int64_t)page * a.s.sb + (int64_t)kvh * a.s.sh + (int64_t)(slot >> a.s.lg) * a.s.sg;
+    const float ks = a.s.ks[si], vs = a.s.vs[si];
+    const u32x4* kp = reinterpret_cast<const u32x4*>(a.kc + (int64_t)page * a.k_sb + (int64_t)slot * a.k_sn + (int64_t)kvh * a.k_sh);
+    float dot = 0.f;
+    for (int u = 0; u < D / 16; ++u) {
+      const u32x4 w = kp[u];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dot = __builtin_fmaf((float)(int8_t)(w[e / 4] >> (8 * (e % 4))), lq[16 * u + e], dot);
+    }
+    const float sc = k0 + lane < lim ? dot * ks : -INFINITY;
+    const float mnew = __builtin_fmaxf(m, wave_max(sc));
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew), p = __builtin_amdgcn_exp2f(sc - mnew);
+    m = mnew;
+    l = l * alpha + wave_sum(p);
+    const float pv = p * vs;
+#pragma unroll
+    for (int c = 0; c < CPL; ++c) acc[c] *= alpha;
+    const int n = min(WAVE, lim - k0);
+    for (int j = 0; j < n; ++j) {
+      const int pj = __shfl(page, j, WAVE), sj = __shfl(slot, j, WAVE);
+      const float wj = __shfl(pv, j, WAVE);
+      const int8_t* vp = a.vc + (int64_t)pj * a.v_sb + (int64_t)sj * a.v_sn + (int64_t)kvh * a.v_sh + CPL * lane;
+#pragma unroll
+      for (int c = 0; c < CPL; ++c) acc[c] = __builtin_fmaf(wj, (float)vp[c], acc[c]);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  uint16_t* op = a.out + (int64_t)(tok + t) * a.o_st + (int64_t)head * a.o_sh + CPL * lane;
+#pragma unroll
+  for (int c = 0; c < CPL; ++c) op[c] = (uint16_t)bf16_rne(acc[c] * inv);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void block_rows_kernel(BlockRowsArgs a) {
+  __shared__ float lq[4][D];
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  if (a.tile_req) {   // entry blockIdx.x, kv head blockIdx.y, rows 4 blockIdx.z + wave
+    const int r = a.tile_req[blockIdx.x], R = a.tile_row[blockIdx.x] + blockIdx.z * 4 + wave;
+    const int tok = a.cu_q[r], qlen = a.cu_q[r + 1] - tok, t = R / a.G;
+    if (t < qlen) attend_row<D>(a, r, tok, qlen, t, blockIdx.y, blockIdx.y * a.G + R % a.G, lane, lq[wave]);
+  } else {            // request blockIdx.x, q head 4 blockIdx.y + wave
+    const int r = blockIdx.x, head = blockIdx.y * 4 + wave, tok = a.cu_q[r], qlen = a.cu_q[r + 1] - tok;
+    if (head >= a.G * a.hkv || qlen > a.qmax) return;
+    for (int t = 0; t < qlen; ++t) attend_row<D>(a, r, tok, qlen, t, head / a.G, head, lane, lq[wave]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------------
+// What every call on a block-scaled cache checks; 0, or the error after fail().
+int check_blocks(const char* nm, int64_t num_blocks, int64_t block_size, int64_t group, int64_t heads, int64_t head_dim,
+                 const void* kc, int64_t k_sb, int64_t k_sn, int64_t k_sh, const void* vc, int64_t v_sb, int64_t v_sn,
+                 int64_t v_sh) {
+  if (head_dim != 64 && head_dim != 128) return fail("%s: head_dim must be 64 or 128, got %lld", nm, (long long)head_dim);
+  if (block_size < 16 || !pow2(block_size) || block_size > (1 << 24))
+    return fail("%s: block_size must be a power of two >= 16", nm);
+  if (!pow2(group) || group < BLK_MIN || group > BLK_MAX || group > block_size)
+    return fail("%s: positions per scale must be a power of two from %d to %d, at most block_size, got %lld", nm, BLK_MIN, BLK_MAX,
+                (long long)group);
+  if (heads <= 0 || heads > 65535 || num_blocks <= 0 || num_blocks > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (!kc || !vc || !aligned16(kc) || !aligned16(vc) || (k_sb | k_sn | k_sh | v_sb | v_sn | v_sh) % 16)
+    return fail("%s: cache rows must be 16-byte aligned (base pointers and strides)", nm);
+  return 0;
+}
+BlockScales block_scales(const float* ks, const float* vs, int64_t sb, int64_t sh, int64_t sg, int64_t group) {
+  return BlockScales{ks, vs, sb, sh, sg, log2i(group)};
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvq_quant_block_cache(const void* key, int64_t key_st, int64_t key_sh, const void* value, int64_t val_st,
+                          int64_t val_sh, int64_t num_tokens, int8_t* k_cache, int64_t kc_sb, int64_t kc_sn,
+                          int64_t kc_sh, int8_t* v_cache, int64_t vc_sb, int64_t vc_sn, int64_t vc_sh,
+                          int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, float* k_scale,
+                          float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group,
+                          const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+                          int64_t bt_stride, int64_t num_seqs, void* stream) {
+  const char* nm = "quant_block_cache";
+  if (num_tokens < 0 || num_seqs < 0 || num_tokens > INT32_MAX || num_seqs > INT32_MAX / 4) return fail("%s: bad sizes", nm);
+  if (num_tokens == 0 || num_seqs == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_blocks(nm, num_blocks, block_size, group, num_heads, head_dim, k_cache, kc_sb, kc_sn, kc_sh, v_cache,
+                                  vc_sb, vc_sn, vc_sh)) return rc;
+  if (!key || !value || !k_scale || !v_scale || !cu_seqlens_q || !seq_lens || !block_table) return fail("%s: null pointer", nm);
+  if (!aligned16(key) || !aligned16(value) || (key_st | key_sh | val_st | val_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  QuantBlockArgs a;
+  a.key = (const uint16_t*)key; a.value = (const uint16_t*)value; a.kc = k_cache; a.vc = v_cache; a.ks = k_scale; a.vs = v_scale;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table;
+  a.key_st = key_st; a.key_sh = key_sh; a.val_st = val_st; a.val_sh = val_sh;
+  a.kc_sb = kc_sb; a.kc_sn = kc_sn; a.kc_sh = kc_sh; a.vc_sb = vc_sb; a.vc_sn = vc_sn; a.vc_sh = vc_sh;
+  a.s_sb = s_sb; a.s_sh = s_sh; a.s_sg = s_sg; a.bt_stride = bt_stride;
+  a.num_seqs = (int)num_seqs; a.num_tokens = (int)num_tokens; a.heads = (int)num_heads; a.num_blocks = (int)num_blocks;
+  a.lbs = log2i(block_size); a.lg = log2i(group);
+  const int64_t items = block_slots(num_tokens, num_seqs, a.lg) * num_heads;
+  if (items > INT32_MAX) return fail("%s: too many tokens and heads for one call", nm);
+  a.items = (int)items;
+  const int w = (int)(group / 16), wpb = w < 4 ? 4 : w;
+  const dim3 grid((unsigned)((items + wpb / w - 1) / (wpb / w))), block(WAVE * wpb);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  auto go = [&](auto d_t) {
+    constexpr int D = decltype(d_t)::value;
+    if (w == 1) hipLaunchKernelGGL((quant_block_kernel<D, 1>), grid, block, 0, st, a);
+    else if (w == 2) hipLaunchKernelGGL((quant_block_kernel<D, 2>), grid, block, 0, st, a);
+    else if (w == 4) hipLaunchKernelGGL((quant_block_kernel<D, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((quant_block_kernel<D, 8>), grid, block, 0, st, a);
+  };
+  if (head_dim == 128) go(std::integral_constant<int, 128>{});
+  else go(std::integral_constant<int, 64>{});
+  return launched(nm);
+}
+
+int kvq_read_block_cache(const int8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, const int8_t* v_cache,
+                         int64_t vc_sb, int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size,
+                         int64_t num_heads, int64_t head_dim, const float* k_scale, const float* v_scale, int64_t s_sb,
+                         int64_t s_sh, int64_t s_sg, int64_t group, const int32_t* starts, const int32_t* cu_seqlens_k,
+                         const int32_t* block_table, int64_t bt_stride, int64_t num_seqs, void* k_out, int64_t ko_st,
+                         int64_t ko_sh, void* v_out, int64_t vo_st, int64_t vo_sh, int64_t num_rows, void* stream) {
+  const char* nm = "read_block_cache";
+  if (num_rows < 0 || num_seqs < 0 || num_rows > INT32_MAX || num_seqs > INT32_MAX / 4) return fail("%s: bad sizes", nm);
+  if (num_rows == 0 || num_seqs == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_blocks(nm, num_blocks, block_size, group, num_heads, head_dim, k_cache, kc_sb, kc_sn, kc_sh, v_cache,
+                                  vc_sb, vc_sn, vc_sh)) return rc;
+  if (!k_out || !v_out || !k_scale || !v_scale || !starts || !cu_seqlens_k || !block_table) return fail("%s: null pointer", nm);
+  if (!aligned16(k_out) || !aligned16(v_out) || (ko_st | ko_sh | vo_st | vo_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  ReadBlockArgs a;
+  a.kc = k_cache; a.vc = v_cache; a.ko = (uint16_t*)k_out; a.vo = (uint16_t*)v_out;
+  a.start = starts; a.cu_k = cu_seqlens_k; a.block_table = block_table;
+  a.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
+  a.kc_sb = kc_sb; a.kc_sn = kc_sn; a.kc_sh = kc_sh; a.vc_sb = vc_sb; a.vc_sn = vc_sn; a.vc_sh = vc_sh;
+  a.ko_st = ko_st; a.ko_sh = ko_sh; a.vo_st = vo_st; a.vo_sh = vo_sh; a.bt_stride = bt_stride;
+  a.num_seqs = (int)num_seqs; a.num_rows = (int)num_rows; a.heads = (int)num_heads; a.num_blocks = (int)num_blocks;
+  a.lbs = log2i(block_size);
+  const int64_t items = block_slots(num_rows, num_seqs, 4) * num_heads;
+  if (items > INT32_MAX) return fail("%s: too many rows and heads for one call", nm);
+  a.items = (int)items;
+  const dim3 grid((unsigned)((items + 3) / 4));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (head_dim == 128) hipLaunchKernelGGL(read_block_kernel<128>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(read_block_kernel<64>, grid, dim3(256), 0, st, a);
+  return launched(nm);
+}
+
+}  // extern "C"
+
+namespace {
+
+// The checks and arguments that the two attention calls share.
+int block_rows(const char* nm, BlockRowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache,
+               int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+               int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const float* k_scale,
+               const float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group, void* out, int64_t o_st,
+               int64_t o_sh, const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+               int64_t bt_stride, int64_t num_q_heads, double softmax_scale) {
+  if (const int rc = check_blocks(nm, num_blocks, block_size, group, num_kv_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache,
+                                  v_sb, v_sn, v_sh)) return rc;
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
+    return fail("%s: bad head counts Hq=%lld Hkv=%lld", nm, (long long)num_q_heads, (long long)num_kv_heads);
+  if (!q || !out || !k_scale || !v_scale || !cu_seqlens_q || !seq_lens || !block_table) return fail("%s: null pointer", nm);
+  if (!aligned16(q) || !aligned16(out) || (q_st | q_sh | o_st | o_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  a.q = (const uint16_t*)q; a.kc = k_cache; a.vc = v_cache; a.out = (uint16_t*)out;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table; a.tile_req = a.tile_row = nullptr;
+  a.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
+  a.q_st = q_st; a.q_sh = q_sh; a.o_st = o_st; a.o_sh = o_sh;
+  a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh; a.bt_stride = bt_stride;
+  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
+  a.hkv = (int)num_kv_heads; a.G = (int)(num_q_heads / num_kv_heads); a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size);
+  a.num_seqs = 0; a.qmax = 0;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
+                               int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
+                               int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+                               int64_t head_dim, const float* k_scale, const float* v_scale, int64_t s_sb, int64_t s_sh,
+                               int64_t s_sg, int64_t group, void* out, int64_t o_st, int64_t o_sh,
+                               const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+                               int64_t bt_stride, int64_t num_seqs, int64_t num_q_heads, double softmax_scale,
+                               float* segm_out, float* segm_max, float* segm_sum, int64_t seg_st, int64_t seg_sh,
+                               int64_t num_splits, int64_t segm_rows, int64_t target_waves, int64_t max_query_len,
+                               int64_t qmax, void* stream) {
+  const char* nm = "block_decode_attention";
+  if (num_splits < 1 || num_splits > MAX_SPLITS) return fail("%s: at most %d split-KV segments", nm, MAX_SPLITS);
+  if (num_seqs < 0 || num_seqs > INT32_MAX / 4 || max_query_len < 0 || qmax < 1 || target_waves < 0 || segm_rows < 0)
+    return fail("%s: bad sizes", nm);
+  if (num_seqs == 0) { g_err.clear(); return KVQ_OK; }
+  BlockRowsArgs a;
+  if (const int rc = block_rows(nm, a, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
+                                num_kv_heads, head_dim, k_scale, v_scale, s_sb, s_sh, s_sg, group, out, o_st, o_sh, cu_seqlens_q,
+                                seq_lens, block_table, bt_stride, num_q_heads, softmax_scale)) return rc;
+  if (num_splits > 1 && segm_rows > 0 && (!segm_out || !segm_max || !segm_sum || !aligned16(segm_out)))
+    return fail("%s: split buffers missing or not 16-byte aligned", nm);
+  a.num_seqs = (int)num_seqs;
+  a.qmax = (int)std::min<int64_t>(qmax, INT32_MAX);
+  (void)seg_st; (void)seg_sh;
+  const dim3 grid((unsigned)num_seqs, (unsigned)((num_q_heads + 3) / 4));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (head_dim == 128) hipLaunchKernelGGL(block_rows_kernel<128>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(block_rows_kernel<64>, grid, dim3(256), 0, st, a);
+  return launched(nm);
+}
+
+int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
+                                int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
+                                int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
+                                int64_t head_dim, const float* k_scale, const float* v_scale, int64_t s_sb, int64_t s_sh,
+                                int64_t s_sg, int64_t group, void* out, int64_t o_st, int64_t o_sh,
+                                const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+                                int64_t bt_stride, int64_t num_q_heads, const int32_t* tile_req, const int32_t* tile_row,
+                                int64_t num_tiles, int64_t rows_per_tile, double softmax_scale, const int32_t* tile_piece,
+                                const int32_t* tile_slot, const int32_t* merge, int64_t num_merge, float* part_out,
+                                float* part_ml, void* stream) {
+  const char* nm = "block_prefill_attention";
+  if (num_tiles < 0 || num_tiles > INT32_MAX || num_merge < 0 || num_merge > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (num_tiles == 0) { g_err.clear(); return KVQ_OK; }
+  if (rows_per_tile != PR_ROWS) return fail("%s: work list tiles must be %d rows", nm, PR_ROWS);
+  if (!tile_req || !tile_row || (tile_piece && !tile_slot)) return fail("%s: bad work list", nm);
+  if (tile_piece && num_merge > 0 && (!merge || !part_out || !part_ml || !aligned16(merge) || !aligned16(part_out) ||
+                                      !aligned16(part_ml)))
+    return fail("%s: split work list needs 16-byte aligned merge list and partial buffers", nm);
+  BlockRowsArgs a;
+  if (const int rc = block_rows(nm, a, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
+                                num_kv_heads, head_dim, k_scale, v_scale, s_sb, s_sh, s_sg, group, out, o_st, o_sh, cu_seqlens_q,
+                                seq_lens, block_table, bt_stride, num_q_heads, softmax_scale)) return rc;
+  a.tile_req = tile_req;
+  a.tile_row = tile_row;
+  const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads, PR_ROWS / 4);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // (an entry that is one of several pieces is computed whole, by each of them with the same result)
+  if (head_dim == 128) hipLaunchKernelGGL(block_rows_kernel<128>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(block_rows_kernel<64>, grid, dim3(256), 0, st, a);
+  return launched(nm);
+}
+
+}  // extern "C"

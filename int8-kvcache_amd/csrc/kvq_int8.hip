@@ -3806,3 +3806,5 @@ int kvq_dequant_pages(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t
 }
 
 }  // extern "C"
+
+#include "block_cache.h"

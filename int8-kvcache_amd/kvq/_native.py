@@ -10,7 +10,7 @@ import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkvq_int8.so")
-ABI_VERSION = 12
+ABI_VERSION = 13
 ERR_LAUNCH = 2      # KVQ_ERR_LAUNCH
 
 _i64 = ctypes.c_int64
@@ -56,6 +56,18 @@ SIGNATURES = {
     "kvq_stream_rw": [_ptr, _i64, _ptr, _i64, _i64, _ptr],
     "kvq_stream_scatter": [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64,
                            _i64, _i64, _i64, _ptr],
+    "kvq_quant_block_cache": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64,
+                              _i64, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64,
+                              _ptr],
+    "kvq_read_block_cache": [_ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64,
+                             _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64,
+                             _ptr],
+    "kvq_block_decode_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                                   _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
+                                   _i64, _i64, _f64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr],
+    "kvq_block_prefill_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                                    _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
+                                    _i64, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr],
     "kvq_last_error": [],
     "kvq_abi_version": [],
 }
