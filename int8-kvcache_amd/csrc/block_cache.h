@@ -331,6 +331,412 @@ __global__ __launch_bounds__(256) void block_rows_kernel(BlockRowsArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// Attention of short queries: attn_kernel's plan, pieces and tiles (int8 MFMA on the codes as they lie in the cache),
+// with operands that keep what an int8 code would lose. Per (request, kv head) and 32-key tile, log2 domain:
+//   S    = q16 . k_code            q16 = rint(q / sq), |q16| <= 16256 = 127 * 128: two int8 planes q16 = 128 hi + lo
+//   e    = S sq scale k_scale + log2(v_scale)      the V scale rides in the exponent, so that one maximum serves both
+//   P    = 2^(e - m)               m: the row's reference maximum of e;  l += P / v_scale
+//   O   += (P14 . v_code) ps       P14 = rint(P / ps), ps = the tile's largest P / 16320: two planes again
+// so the scales cost one multiplication (K) and one addition (V) per 16-key half tile, not one per element, and the
+// products are exact integers. A half tile lies in one block (blocks are 16 positions or more).
+// PACK: at most 8 (token, q head) rows per kv head: the hi planes are the MFMA's columns 0 .. 7, the lo planes columns
+// 8 .. 15, so both planes cost one MFMA each, as a single int8 plane of 16 rows does; lanes n and n + 8 hold the same
+// row and exchange their half of S by a 16-lane rotation. Otherwise 16 rows and two MFMAs per product.
+// ------------------------------------------------------------------------------------------------
+struct BlockAttnArgs {
+  AttnArgs a;   // (first: fresh_args)
+  BlockScales s;
+};
+static_assert(offsetof(BlockAttnArgs, a) == 0 && sizeof(AttnArgs) % 8 == 0, "AttnArgs lead the kernel arguments");
+__device__ __forceinline__ const BlockScales& fresh_scales() {
+  auto* p = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const BlockScales*)(const void*)(p + offsetof(BlockAttnArgs, s));
+}
+
+constexpr float Q16_MAX = 16256.f;   // 127 * 128: the hi plane of rint(q / sq) stays an int8
+constexpr float P14_MAX = 16320.f;   // below 16383 by more than the reciprocal's error: the hi plane stays below 128
+constexpr float MIN_VSCALE = 1e-30f; // a block's V scale counts as at least this (its logarithm and reciprocal are taken)
+
+__device__ __forceinline__ int ror8(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true); }
+__device__ __forceinline__ float ror8(float x) { return __int_as_float(ror8(__float_as_int(x))); }
+
+// Four 14-bit integers (in the low mantissa bits of t) as the bytes of one plane, keys in the order 0, 2, 1, 3 (the V
+// operand's too): bits [SH, SH + 7) of each. sh: 7 (hi plane) or 0 (lo).
+__device__ __forceinline__ uint32_t plane4(uint32_t w01, uint32_t w23, int sh) {
+  const uint32_t a = w01 >> sh, b = w23 << (8 - sh);
+  return ((a & 0x00ff00ffu) | (b & ~0x00ff00ffu)) & 0x7f7f7f7fu;
+}
+
+template <int D, int PF, bool PACK>
+__device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int seqlen, int kvh, int row0, int c_begin,
+                                              int c_end, int ks, int KS, int rtile, int part, int nparts, float* lds,
+                                              int lane) {
+  const AttnArgs& a = fresh_args();
+  const BlockScales& bs_ = fresh_scales();
+  constexpr int RT = PACK ? 8 : 16;        // rows of this wavefront's tile
+  constexpr int NP = PACK ? 1 : 2;         // planes in separate MFMAs
+  constexpr int KPL = D / 4, KSTEPS = D / 64, VT = D / 16, VW = D / 64, OPL = D / 4;
+  const int G = PACK ? a.G >> 1 : a.G;     // (PACK: the plan counts plane rows, two a row)
+  const bool active = row0 < qlen * G;
+  const int num_blocks = a.num_blocks, lbs = a.lbs, lg = bs_.lg;
+  const int64_t k_sb = a.k_sb, k_sn = a.k_sn, v_sb = a.v_sb, v_sn = a.v_sn, s_sb = bs_.sb, s_sg = bs_.sg;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tok = __builtin_amdgcn_readfirstlane(tok);
+  qlen = __builtin_amdgcn_readfirstlane(qlen);
+  kvh = __builtin_amdgcn_readfirstlane(kvh);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
+  c_begin = __builtin_amdgcn_readfirstlane(c_begin);
+  c_end = __builtin_amdgcn_readfirstlane(c_end);
+  part = __builtin_amdgcn_readfirstlane(part);
+  nparts = __builtin_amdgcn_readfirstlane(nparts);
+  ks = __builtin_amdgcn_readfirstlane(ks);
+  KS = __builtin_amdgcn_readfirstlane(KS);
+  const int n = lane & 15, g = lane >> 4;
+  const int L = __builtin_amdgcn_readfirstlane(seqlen);
+  if (L <= 0 || !active) c_end = c_begin;
+  const int nt = c_begin + ks < c_end ? (c_end - c_begin - ks + KS - 1) / KS : 0;
+  auto tile = [&](int j) { return c_begin + ks + j * KS; };
+  const int* bt = a.block_table + (int64_t)seq * a.bt_stride;
+  const int bs = 1 << lbs;
+  auto div_g = [&](int x) { return G == 1 ? x : a.g_inv ? (int)__umulhi((unsigned)x, a.g_inv) : x / G; };
+
+  const int R = row0 + (n & (RT - 1)), rtok = div_g(R), rh = R - rtok * G;
+  const int lim_lo = L - qlen + 1 + __builtin_amdgcn_readfirstlane(div_g(row0));
+  const int8_t* kbase = a.kc + (int64_t)kvh * a.k_sh;
+  const int8_t* vbase = a.vc + (int64_t)kvh * a.v_sh;
+  const int koff = n * (int)k_sn + g * KPL;
+  const int voff = 4 * g * (int)v_sn + n * VT;
+  const int vsn = (int)v_sn;
+  // a tile's four scales, one load: lane l takes that of half l / 2 % 2, K (l even) or V
+  const float* sbase = ((lane & 1) ? bs_.vs : bs_.ks) + (int64_t)kvh * bs_.sh;
+
+  auto page_of = [&](int key) -> int {
+    const int idx = __builtin_amdgcn_readfirstlane(key >> lbs);
+    const int p = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[idx]);
+    return (p >= 0 && p < num_blocks) ? p : 0;
+  };
+  struct Tile {
+    KVTile<D> kv;
+    float sc;
+  };
+  auto load = [&](Tile& r, int c) {
+    const int n0 = c * TILE, n1 = n0 + 16;
+    const int p0 = page_of(n0);
+    const int p1 = n1 < L ? page_of(n1) : p0;
+    const int o0 = n0 & (bs - 1), o1 = n1 < L ? (n1 & (bs - 1)) : o0;
+    const int8_t* kb0 = kbase + (int64_t)p0 * k_sb + (int64_t)o0 * k_sn;
+    const int8_t* kb1 = kbase + (int64_t)p1 * k_sb + (int64_t)o1 * k_sn;
+    const int8_t* vb0 = vbase + (int64_t)p0 * v_sb + (int64_t)o0 * v_sn;
+    const int8_t* vb1 = vbase + (int64_t)p1 * v_sb + (int64_t)o1 * v_sn;
+    const int64_t s0 = (int64_t)p0 * s_sb + (int64_t)(o0 >> lg) * s_sg, s1 = (int64_t)p1 * s_sb + (int64_t)(o1 >> lg) * s_sg;
+    r.sc = sbase[(lane & 2) ? s1 : s0];
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      r.kv.k[0][s] = ldk(reinterpret_cast<const i32x4*>(kb0 + koff + 16 * s));
+      r.kv.k[1][s] = ldk(reinterpret_cast<const i32x4*>(kb1 + koff + 16 * s));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VW == 2) {
+        const u32x2 w0 = ldv(reinterpret_cast<const u32x2*>(vb0 + voff + i * vsn));
+        const u32x2 w1 = ldv(reinterpret_cast<const u32x2*>(vb1 + voff + i * vsn));
+        r.kv.v[i][0] = w0.x; r.kv.v[i][1] = w0.y;
+        r.kv.v[4 + i][0] = w1.x; r.kv.v[4 + i][1] = w1.y;
+      } else {
+        r.kv.v[i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb0 + voff + i * vsn));
+        r.kv.v[4 + i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb1 + voff + i * vsn));
+      }
+    }
+  };
+
+  Tile ring[PF];
+  // the q row is requested before the first tiles, and made two planes while they are in flight
+  const bool qrow = rtok < qlen;
+  u32x4 qraw[KPL / 8];
+#pragma unroll
+  for (int u = 0; u < KPL / 8; ++u) qraw[u] = u32x4{0u, 0u, 0u, 0u};
+  if (qrow) {
+    const u32x4* qp = reinterpret_cast<const u32x4*>(a.q + (int64_t)(tok + rtok) * a.q_st +
+                                                     (int64_t)(kvh * G + rh) * a.q_sh + g * KPL);
+#pragma unroll
+    for (int u = 0; u < KPL / 8; ++u) qraw[u] = qp[u];
+  }
+  if (nt > 0) {
+#pragma unroll
+    for (int j = 0; j < PF - 1; ++j) load(ring[j], tile(min(j, nt - 1)));
+  }
+  i32x4 qop[NP][KSTEPS];
+  float rs;
+  {
+    float x[KPL], amax = 0.f;
+#pragma unroll
+    for (int u = 0; u < KPL / 8; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[8 * u + 2 * j] = bf16_lo(qraw[u][j]);
+        x[8 * u + 2 * j + 1] = bf16_hi(qraw[u][j]);
+      }
+#pragma unroll
+    for (int e = 0; e < KPL; ++e) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[e]));
+    amax = __builtin_fmaxf(group4_fmax(amax), 1e-30f);
+    const float inv = Q16_MAX / amax;
+    rs = amax / Q16_MAX * a.sm_log2;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t hi = 0u, lo = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = (int)__builtin_rintf(x[16 * s + 4 * w + e] * inv), h = (v + 64) >> 7;
+          hi |= (uint32_t)(h & 0xff) << (8 * e);
+          lo |= (uint32_t)((v - 128 * h) & 0xff) << (8 * e);
+        }
+        if constexpr (PACK) {
+          qop[0][s][w] = n < 8 ? (int)hi : (int)lo;
+        } else {
+          qop[0][s][w] = (int)hi;
+          qop[NP - 1][s][w] = (int)lo;
+        }
+      }
+  }
+  const int lim = rtok < qlen ? L - qlen + 1 + rtok : L;
+  const int sh = n < 8 ? 7 : 0;            // PACK: this lane's plane
+
+  float m = -1e30f, l = 0.f, acc[VT][4];
+#pragma unroll
+  for (int t = 0; t < VT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+
+  auto compute = [&](auto masked_t, const Tile& tl, int c) {
+    constexpr bool MASKED = decltype(masked_t)::value;
+    const KVTile<D>& r = tl.kv;
+    const int n0 = c * TILE;
+    // ---- QK: S^T[key][row] of the tile's two 16-key halves ----
+    int sc[2][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      i32x4 z[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        z[p] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) z[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.k[b][s], qop[p][s], z[p], 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (PACK) {
+          const int own = z[0][i] << sh;
+          sc[b][i] = own + ror8(own);
+        } else {
+          sc[b][i] = (z[0][i] << 7) + z[NP - 1][i];
+        }
+      }
+    }
+    // ---- V^T operands, the keys of a lane's 4-key runs in the order 0, 2, 1, 3 ----
+    long vop[VT];
+    {
+      uint32_t lo[VT], hi[VT];
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        transpose4x4(r.v[0][w], r.v[2][w], r.v[1][w], r.v[3][w], lo[4 * w], lo[4 * w + 1], lo[4 * w + 2], lo[4 * w + 3]);
+        transpose4x4(r.v[4][w], r.v[6][w], r.v[5][w], r.v[7][w], hi[4 * w], hi[4 * w + 1], hi[4 * w + 2], hi[4 * w + 3]);
+      }
+#pragma unroll
+      for (int t = 0; t < VT; ++t) vop[t] = (long)(((uint64_t)hi[t] << 32) | lo[t]);
+    }
+    // ---- the halves' scales ----
+    const float vfl = __builtin_fmaxf(tl.sc, MIN_VSCALE);
+    const float lg2 = __builtin_amdgcn_logf(vfl), rcp = __builtin_amdgcn_rcpf(vfl);
+    auto of_lane = [](float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
+    const float f[2] = {rs * of_lane(tl.sc, 0), rs * of_lane(tl.sc, 2)};
+    const float lv[2] = {of_lane(lg2, 1), of_lane(lg2, 3)}, iv[2] = {of_lane(rcp, 1), of_lane(rcp, 3)};
+    // ---- online softmax; key of accumulator (b, i) = n0 + 16 b + 4 g + i ----
+    bool ok[2][4];
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      int mx = INT32_MIN;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ok[b][i] = MASKED ? n0 + 16 * b + 4 * g + i < lim : true;
+        mx = ok[b][i] ? max(mx, sc[b][i]) : mx;
+      }
+      // (a dot product never reaches INT32_MIN: it marks a half without a visible key)
+      const float tb = __builtin_fmaf((float)mx, f[b], lv[b]);
+      tmax = (MASKED && mx == INT32_MIN) ? tmax : __builtin_fmaxf(tmax, tb);
+    }
+    tmax = group4_fmax(tmax);
+    const bool raise = tmax > m + ATTN_SLACK;
+    const float mnew = raise ? tmax : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+    m = mnew;
+    const float ps = __builtin_fmaxf(__builtin_amdgcn_exp2f(tmax - mnew) * (1.f / P14_MAX), 1e-30f);
+    const float ri = __builtin_amdgcn_rcpf(ps);
+    uint32_t w[2][2];
+    float sum[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const float e0 = lv[b] - mnew;
+      uint32_t t[4];
+      sum[b] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf((float)sc[b][i], f[b], e0));
+        if (MASKED) p = ok[b][i] ? p : 0.f;
+        sum[b] += p;
+        t[i] = __float_as_uint(__builtin_fmaf(p, ri, QC_MAGIC));
+      }
+      w[b][0] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100u);   // keys 1 : 0
+      w[b][1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100u);   // keys 3 : 2
+    }
+    l = __builtin_fmaf(sum[0], iv[0], __builtin_fmaf(sum[1], iv[1], l * alpha));
+    if (__any(raise)) {
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] *= alpha;
+    }
+    // ---- PV: O^T[channel][row] += (V^T . P^T) ps ----
+    long pop[NP];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int s = PACK ? sh : p == 0 ? 7 : 0;
+      pop[p] = (long)(((uint64_t)plane4(w[1][0], w[1][1], s) << 32) | plane4(w[0][0], w[0][1], s));
+    }
+    const float psl = PACK && sh ? ps * 128.f : ps;
+#pragma unroll
+    for (int t = 0; t < VT; ++t) {
+      i32x4 z[NP];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) z[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(vop[t], pop[p], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int zi = PACK ? z[0][i] : (z[0][i] << 7) + z[NP - 1][i];
+        acc[t][i] = __builtin_fmaf((float)zi, psl, acc[t][i]);
+      }
+    }
+  };
+
+  // the ring of attn_kernel: PF - 1 tiles in flight, loads past the end re-read the last tile
+  if (nt > 0) {
+    const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
+    const int j_full = min(nt, full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0);
+    int j0 = 0;
+    for (; j0 + PF <= j_full; j0 += PF) {
+#pragma unroll
+      for (int jj = 0; jj < PF; ++jj) {
+        load(ring[(jj + PF - 1) % PF], tile(min(j0 + jj + PF - 1, nt - 1)));
+        compute(std::false_type{}, ring[jj], tile(j0 + jj));
+      }
+    }
+    for (; j0 < nt; j0 += PF) {
+#pragma unroll
+      for (int jj = 0; jj < PF; ++jj) {
+        const int j = j0 + jj;
+        if (j >= nt) break;
+        load(ring[(jj + PF - 1) % PF], tile(min(j + PF - 1, nt - 1)));
+        compute(std::true_type{}, ring[jj], tile(j));
+      }
+    }
+  }
+
+  // ---- epilogue: lane (n, g) holds channels (D/4) g + (D/16) i + t of its row in acc[t][i] ----
+  l = group4_sum(l);
+  if constexpr (PACK) {   // both planes of a row: lanes n and n + 8 end with the same sums
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] += ror8(acc[t][i]);
+  }
+  if (KS > 1) {   // attn_kernel's merge of the key splits
+    static_assert(VT * 4 + 2 <= MERGE_FIELDS, "merge slot too small");
+    auto slot = [&](int k) { return lds + (size_t)((k - 1) * a.rt + rtile) * MERGE_FIELDS * WAVE + lane; };
+    if (ks > 0 && active) {
+      float* sl = slot(ks);
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sl[(4 * t + i) * WAVE] = acc[t][i];
+      sl[(4 * VT) * WAVE] = m;
+      sl[(4 * VT + 1) * WAVE] = l;
+    }
+    __syncthreads();
+    if (ks == 0 && active) {
+      float M = m;
+      for (int k = 1; k < KS; ++k) M = __builtin_fmaxf(M, slot(k)[(4 * VT) * WAVE]);
+      const float w0 = __builtin_amdgcn_exp2f(m - M);
+      l *= w0;
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] *= w0;
+      for (int k = 1; k < KS; ++k) {
+        const float* src = slot(k);
+        const float wk = __builtin_amdgcn_exp2f(src[(4 * VT) * WAVE] - M);
+        l = __builtin_fmaf(wk, src[(4 * VT + 1) * WAVE], l);
+#pragma unroll
+        for (int t = 0; t < VT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(wk, src[(4 * t + i) * WAVE], acc[t][i]);
+      }
+      m = M;
+    }
+    __syncthreads();
+  }
+  if (ks > 0 || !active || rtok >= qlen || (PACK && n >= 8)) return;
+  // ---- the end of a piece: bf16 out of a whole segment, or the fp32 partial of a cut one (as finish_segment) ----
+  const AttnArgs& o = fresh_args();
+  const int qt = tok + rtok, head = kvh * G + rh;
+  if (nparts == 1) {
+    if (o.max_splits > 1 && qt < o.cut_rows && g == 0)
+      o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh] = -1.f;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint32_t w[OPL / 2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < VT; t += 2) w[(VT * i + t) / 2] = pack_bf16x2(acc[t][i] * inv, acc[t + 1][i] * inv);
+    u32x4* op = reinterpret_cast<u32x4*>(o.out + (int64_t)qt * o.o_st + (int64_t)head * o.o_sh + OPL * g);
+#pragma unroll
+    for (int u = 0; u < OPL / 8; ++u) op[u] = u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+  } else {
+    const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh + part;
+    if (g == 0) {
+      o.segm_max[sidx] = m;
+      o.segm_sum[sidx] = part == nparts - 1 ? -2.f - l : l;
+    }
+    float* sp = o.segm_out + sidx * D + OPL * g;
+#pragma unroll
+    for (int u = 0; u < OPL / 4; ++u) {
+      const int c0 = 4 * u;
+      reinterpret_cast<float4*>(sp)[u] = float4{acc[(c0 + 0) % VT][(c0 + 0) / VT], acc[(c0 + 1) % VT][(c0 + 1) / VT],
+                                                acc[(c0 + 2) % VT][(c0 + 2) / VT], acc[(c0 + 3) % VT][(c0 + 3) / VT]};
+    }
+  }
+}
+
+template <int D, int PF, bool PACK>
+__global__ __launch_bounds__(256) void block_attn_kernel(BlockAttnArgs args) {
+  touch_args();
+  const AttnArgs& a = args.a;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int rt = a.rt, ksplit = a.ksplit, kspl = div_row_tiles(wave, rt), rtile = wave - kspl * rt;
+  extern __shared__ float merge_lds[];
+  int solo = 0;
+  walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
+    const int row0 = (rg * rt + rtile) * (PACK ? 8 : 16);
+    if (ksplit > 1 && c1 - c0 >= a.coop) {
+      attend_blocks<D, PF, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, kspl, ksplit, rtile, part, nparts, merge_lds, lane);
+    } else {
+      if (solo % ksplit == kspl)
+        attend_blocks<D, PF, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, 0, 1, rtile, part, nparts, merge_lds, lane);
+      ++solo;
+    }
+  });
+}
+
+// ------------------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------------------
 // What every call on a block-scaled cache checks; 0, or the error after fail().
@@ -433,13 +839,12 @@ int kvq_read_block_cache(const int8_t* k_cache, int64_t kc_sb, int64_t kc_sn, in
 
 namespace {
 
-// The checks and arguments that the two attention calls share.
-int block_rows(const char* nm, BlockRowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache,
-               int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
-               int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const float* k_scale,
-               const float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group, void* out, int64_t o_st,
-               int64_t o_sh, const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
-               int64_t bt_stride, int64_t num_q_heads, double softmax_scale) {
+// What the two attention calls check.
+int check_attention(const char* nm, const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
+                    int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                    int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const float* k_scale,
+                    const float* v_scale, int64_t group, void* out, int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q,
+                    const int32_t* seq_lens, const int32_t* block_table, int64_t num_q_heads) {
   if (const int rc = check_blocks(nm, num_blocks, block_size, group, num_kv_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache,
                                   v_sb, v_sn, v_sh)) return rc;
   if (num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
@@ -447,6 +852,17 @@ int block_rows(const char* nm, BlockRowsArgs& a, const void* q, int64_t q_st, in
   if (!q || !out || !k_scale || !v_scale || !cu_seqlens_q || !seq_lens || !block_table) return fail("%s: null pointer", nm);
   if (!aligned16(q) || !aligned16(out) || (q_st | q_sh | o_st | o_sh) % 8)
     return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  return 0;
+}
+int block_rows(const char* nm, BlockRowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache,
+               int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+               int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const float* k_scale,
+               const float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group, void* out, int64_t o_st,
+               int64_t o_sh, const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
+               int64_t bt_stride, int64_t num_q_heads, double softmax_scale) {
+  if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
+                                     num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q, seq_lens,
+                                     block_table, num_q_heads)) return rc;
   a.q = (const uint16_t*)q; a.kc = k_cache; a.vc = v_cache; a.out = (uint16_t*)out;
   a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table; a.tile_req = a.tile_row = nullptr;
   a.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
@@ -477,20 +893,66 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   if (num_seqs < 0 || num_seqs > INT32_MAX / 4 || max_query_len < 0 || qmax < 1 || target_waves < 0 || segm_rows < 0)
     return fail("%s: bad sizes", nm);
   if (num_seqs == 0) { g_err.clear(); return KVQ_OK; }
-  BlockRowsArgs a;
-  if (const int rc = block_rows(nm, a, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
-                                num_kv_heads, head_dim, k_scale, v_scale, s_sb, s_sh, s_sg, group, out, o_st, o_sh, cu_seqlens_q,
-                                seq_lens, block_table, bt_stride, num_q_heads, softmax_scale)) return rc;
+  if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks,
+                                     block_size, num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q,
+                                     seq_lens, block_table, num_q_heads)) return rc;
   if (num_splits > 1 && segm_rows > 0 && (!segm_out || !segm_max || !segm_sum || !aligned16(segm_out)))
     return fail("%s: split buffers missing or not 16-byte aligned", nm);
-  a.num_seqs = (int)num_seqs;
+  if ((int64_t)block_size * k_sn > INT32_MAX || 16 * v_sn > INT32_MAX || k_sn < 0 || v_sn < 0)
+    return fail("%s: page too large for 32-bit lane offsets", nm);
+  const int G = (int)(num_q_heads / num_kv_heads);
+  const int64_t maxq = std::min<int64_t>(std::max<int64_t>(max_query_len, 1), qmax), rows = (int64_t)G * maxq;
+  if (rows > INT32_MAX / 4) return fail("%s: grid too large", nm);
+  // the row tile: 8 rows, both planes in one MFMA, where that holds all of a request's rows; else 16
+  const bool pack = rows <= 8;
+  const int rt = (int)std::min<int64_t>(MAX_ROW_TILES, (rows + 15) / 16);
+  const Tuning tune = read_tuning();
+  const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
+                     : num_splits == 1 || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? MAX_ROW_TILES : DEFAULT_KSPLIT;
+  const int ks = std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = rt * ks;
+  BlockAttnArgs b;
+  b.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
+  AttnArgs& a = b.a;
+  a.q = (const uint16_t*)q; a.kc = k_cache; a.vc = v_cache; a.out = (uint16_t*)out;
+  a.segm_out = segm_out; a.segm_max = segm_max; a.segm_sum = segm_sum;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table;
+  a.ks = a.vs = nullptr; a.ks_pc = a.vs_pc = 0;
+  a.q_st = q_st; a.q_sh = q_sh; a.o_st = o_st; a.o_sh = o_sh;
+  a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh;
+  a.seg_st = seg_st; a.seg_sh = seg_sh; a.bt_stride = bt_stride;
+  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
+  a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size);
+  a.G = pack ? 2 * G : G;   // the plan's rows: planes of rows where two share an MFMA
+  a.g_inv = G > 1 && (G * std::min<int64_t>(qmax, INT32_MAX) + 64) < (1ll << 32) / G ? (unsigned)(((1ll << 32) + G - 1) / G) : 0u;
   a.qmax = (int)std::min<int64_t>(qmax, INT32_MAX);
-  (void)seg_st; (void)seg_sh;
-  const dim3 grid((unsigned)num_seqs, (unsigned)((num_q_heads + 3) / 4));
+  a.num_seqs = (int)num_seqs; a.hkv = (int)num_kv_heads;
+  a.max_splits = (int)num_splits;
+  a.cut_rows = num_splits > 1 ? (int)std::min<int64_t>(segm_rows, INT32_MAX) : 0;
+  a.rt = rt; a.ksplit = ks; a.waves = waves;
+  a.min_tiles = MIN_SPLIT_TILES;
+  a.coop = coop_tiles(num_splits > 1, ks);
+  a.xcd_order = tune.xcd_order ? atoi(tune.xcd_order) : 1;
+  a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
+                                       : (int)PLAN_FAST_MAX;
+  a.seg_cost = seg_cost_units(tune, 0);
+  const size_t lds = (size_t)(ks - 1) * rt * MERGE_FIELDS * WAVE * sizeof(float);
+  void (*kern)(BlockAttnArgs) = head_dim == 128 ? (pack ? block_attn_kernel<128, 2, true> : block_attn_kernel<128, 2, false>)
+                                                : (pack ? block_attn_kernel<64, 2, true> : block_attn_kernel<64, 2, false>);
+  const bool cuttable_any = num_splits > 1 && segm_rows > 0;
+  const int64_t tw = target_waves > 0 ? target_waves
+                     : cuttable_any   ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
+                                      : (int64_t)device_cus() * waves;
+  a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(tw / waves, INT32_MAX));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (head_dim == 128) hipLaunchKernelGGL(block_rows_kernel<128>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(block_rows_kernel<64>, grid, dim3(256), 0, st, a);
-  return launched(nm);
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.workers), dim3(WAVE * waves), lds, st, b);
+  const int rc = launched(nm);
+  if (rc != KVQ_OK || num_splits == 1 || a.cut_rows == 0) return rc;
+  a.G = G;
+  const dim3 rgrid((unsigned)num_seqs, (unsigned)((num_q_heads + RED_WAVES - 1) / RED_WAVES),
+                   (unsigned)std::min<int64_t>(maxq, MERGE_Z));
+  if (head_dim == 128) hipLaunchKernelGGL(split_reduce_kernel<128>, rgrid, dim3(WAVE * RED_WAVES), 0, st, a);
+  else hipLaunchKernelGGL(split_reduce_kernel<64>, rgrid, dim3(WAVE * RED_WAVES), 0, st, a);
+  return launched("block_decode_attention: merge");
 }
 
 int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
