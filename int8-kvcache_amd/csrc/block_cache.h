@@ -4,7 +4,8 @@
 //
 //   quant_block_kernel   quantize a step's new K/V into their blocks, raising scales (and requantizing) where needed
 //   read_block_kernel    ranges of the requests' keys back to bf16 rows
-//   block_rows_kernel    attention, one wavefront per (query token, q head)
+//   block_attn_kernel    attention of short queries, int8 MFMA on operands of two int8 planes
+//   block_prefill_kernel attention of long queries: prefill_body on the codes as bf16
 //
 // A cached value is code * scale; attention is that of those values and the bf16 q, without further rounding of either.
 
@@ -247,90 +248,6 @@ __global__ __launch_bounds__(256) void read_block_kernel(ReadBlockArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Attention of one (query token, q head) by one wavefront: a lane scores one of 64 keys, then the lanes own D / 64
-// channels each and add the 64 keys' values. fp32 throughout.
-// ------------------------------------------------------------------------------------------------
-struct BlockRowsArgs {
-  const uint16_t* q;
-  const int8_t* kc;
-  const int8_t* vc;
-  uint16_t* out;
-  const int* cu_q;
-  const int* seq_lens;
-  const int* block_table;
-  const int* tile_req;    // long-query calls: the rows of entry blockIdx.x (NULL: every token of the batch)
-  const int* tile_row;
-  BlockScales s;
-  int64_t q_st, q_sh, o_st, o_sh, k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, bt_stride;
-  float sm_log2;
-  int num_seqs, hkv, G, qmax, num_blocks, lbs;
-};
-
-template <int D>
-__device__ __forceinline__ void attend_row(const BlockRowsArgs& a, int r, int tok, int qlen, int t, int kvh, int head, int lane,
-                                           float* lq) {
-  const int len = a.seq_lens[r], lim = min(len, len - qlen + 1 + t);
-  const uint16_t* qp = a.q + (int64_t)(tok + t) * a.q_st + (int64_t)head * a.q_sh;
-  for (int d = lane; d < D; d += WAVE) lq[d] = __uint_as_float((uint32_t)qp[d] << 16) * a.sm_log2;
-  __builtin_amdgcn_wave_barrier();
-  const int bsm = (1 << a.lbs) - 1;
-  constexpr int CPL = D / WAVE;
-  float m = -1e30f, l = 0.f, acc[CPL];
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) acc[c] = 0.f;
-  for (int k0 = 0; k0 < lim; k0 += WAVE) {
-    const int key = min(k0 + lane, lim - 1);
-    int page = a.block_table[(int64_t)r * a.bt_stride + (key >> a.lbs)];
-    page = page >= 0 && page < a.num_blocks ? page : 0;
-    const int slot = key & bsm;
-    const int64_t si = (int64_t)page * a.s.sb + (int64_t)kvh * a.s.sh + (int64_t)(slot >> a.s.lg) * a.s.sg;
-    const float ks = a.s.ks[si], vs = a.s.vs[si];
-    const u32x4* kp = reinterpret_cast<const u32x4*>(a.kc + (int64_t)page * a.k_sb + (int64_t)slot * a.k_sn + (int64_t)kvh * a.k_sh);
-    float dot = 0.f;
-    for (int u = 0; u < D / 16; ++u) {
-      const u32x4 w = kp[u];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) dot = __builtin_fmaf((float)(int8_t)(w[e / 4] >> (8 * (e % 4))), lq[16 * u + e], dot);
-    }
-    const float sc = k0 + lane < lim ? dot * ks : -INFINITY;
-    const float mnew = __builtin_fmaxf(m, wave_max(sc));
-    const float alpha = __builtin_amdgcn_exp2f(m - mnew), p = __builtin_amdgcn_exp2f(sc - mnew);
-    m = mnew;
-    l = l * alpha + wave_sum(p);
-    const float pv = p * vs;
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) acc[c] *= alpha;
-    const int n = min(WAVE, lim - k0);
-    for (int j = 0; j < n; ++j) {
-      const int pj = __shfl(page, j, WAVE), sj = __shfl(slot, j, WAVE);
-      const float wj = __shfl(pv, j, WAVE);
-      const int8_t* vp = a.vc + (int64_t)pj * a.v_sb + (int64_t)sj * a.v_sn + (int64_t)kvh * a.v_sh + CPL * lane;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) acc[c] = __builtin_fmaf(wj, (float)vp[c], acc[c]);
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint16_t* op = a.out + (int64_t)(tok + t) * a.o_st + (int64_t)head * a.o_sh + CPL * lane;
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) op[c] = (uint16_t)bf16_rne(acc[c] * inv);
-}
-
-template <int D>
-__global__ __launch_bounds__(256) void block_rows_kernel(BlockRowsArgs a) {
-  __shared__ float lq[4][D];
-  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  if (a.tile_req) {   // entry blockIdx.x, kv head blockIdx.y, rows 4 blockIdx.z + wave
-    const int r = a.tile_req[blockIdx.x], R = a.tile_row[blockIdx.x] + blockIdx.z * 4 + wave;
-    const int tok = a.cu_q[r], qlen = a.cu_q[r + 1] - tok, t = R / a.G;
-    if (t < qlen) attend_row<D>(a, r, tok, qlen, t, blockIdx.y, blockIdx.y * a.G + R % a.G, lane, lq[wave]);
-  } else {            // request blockIdx.x, q head 4 blockIdx.y + wave
-    const int r = blockIdx.x, head = blockIdx.y * 4 + wave, tok = a.cu_q[r], qlen = a.cu_q[r + 1] - tok;
-    if (head >= a.G * a.hkv || qlen > a.qmax) return;
-    for (int t = 0; t < qlen; ++t) attend_row<D>(a, r, tok, qlen, t, head / a.G, head, lane, lq[wave]);
-  }
-}
-
-// ------------------------------------------------------------------------------------------------
 // Attention of short queries: attn_kernel's plan, pieces and tiles (int8 MFMA on the codes as they lie in the cache),
 // with operands that keep what an int8 code would lose. Per (request, kv head) and 32-key tile, log2 domain:
 //   S    = q16 . k_code            q16 = rint(q / sq), |q16| <= 16256 = 127 * 128: two int8 planes q16 = 128 hi + lo
@@ -356,7 +273,6 @@ __device__ __forceinline__ const BlockScales& fresh_scales() {
 
 constexpr float Q16_MAX = 16256.f;   // 127 * 128: the hi plane of rint(q / sq) stays an int8
 constexpr float P14_MAX = 16320.f;   // below 16383 by more than the reciprocal's error: the hi plane stays below 128
-constexpr float MIN_VSCALE = 1e-30f; // a block's V scale counts as at least this (its logarithm and reciprocal are taken)
 
 __device__ __forceinline__ int ror8(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true); }
 __device__ __forceinline__ float ror8(float x) { return __int_as_float(ror8(__float_as_int(x))); }
@@ -546,7 +462,7 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
       for (int t = 0; t < VT; ++t) vop[t] = (long)(((uint64_t)hi[t] << 32) | lo[t]);
     }
     // ---- the halves' scales ----
-    const float vfl = __builtin_fmaxf(tl.sc, MIN_VSCALE);
+    const float vfl = __builtin_fmaxf(tl.sc, MIN_BLOCK_SCALE);
     const float lg2 = __builtin_amdgcn_logf(vfl), rcp = __builtin_amdgcn_rcpf(vfl);
     auto of_lane = [](float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
     const float f[2] = {rs * of_lane(tl.sc, 0), rs * of_lane(tl.sc, 2)};
@@ -737,6 +653,15 @@ __global__ __launch_bounds__(256) void block_attn_kernel(BlockAttnArgs args) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// Attention of long queries: prefill_body's rows, tiles and ring on the codes converted to bf16 (exactly), with the
+// exponent of block_attn_kernel. Each tile's four scales come with its DMA, one instruction more per wavefront.
+// ------------------------------------------------------------------------------------------------
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256, 3) void block_prefill_kernel(PrefillArgs a) {
+  prefill_body<D, PR_SRC_I8_BLOCK, SPLIT>(a);
+}
+
+// ------------------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------------------
 // What every call on a block-scaled cache checks; 0, or the error after fail().
@@ -854,26 +779,6 @@ int check_attention(const char* nm, const void* q, int64_t q_st, int64_t q_sh, c
     return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
   return 0;
 }
-int block_rows(const char* nm, BlockRowsArgs& a, const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache,
-               int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
-               int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const float* k_scale,
-               const float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group, void* out, int64_t o_st,
-               int64_t o_sh, const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table,
-               int64_t bt_stride, int64_t num_q_heads, double softmax_scale) {
-  if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
-                                     num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q, seq_lens,
-                                     block_table, num_q_heads)) return rc;
-  a.q = (const uint16_t*)q; a.kc = k_cache; a.vc = v_cache; a.out = (uint16_t*)out;
-  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table; a.tile_req = a.tile_row = nullptr;
-  a.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
-  a.q_st = q_st; a.q_sh = q_sh; a.o_st = o_st; a.o_sh = o_sh;
-  a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh; a.bt_stride = bt_stride;
-  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
-  a.hkv = (int)num_kv_heads; a.G = (int)(num_q_heads / num_kv_heads); a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size);
-  a.num_seqs = 0; a.qmax = 0;
-  return 0;
-}
-
 }  // namespace
 
 extern "C" {
@@ -973,18 +878,37 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
   if (tile_piece && num_merge > 0 && (!merge || !part_out || !part_ml || !aligned16(merge) || !aligned16(part_out) ||
                                       !aligned16(part_ml)))
     return fail("%s: split work list needs 16-byte aligned merge list and partial buffers", nm);
-  BlockRowsArgs a;
-  if (const int rc = block_rows(nm, a, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
-                                num_kv_heads, head_dim, k_scale, v_scale, s_sb, s_sh, s_sg, group, out, o_st, o_sh, cu_seqlens_q,
-                                seq_lens, block_table, bt_stride, num_q_heads, softmax_scale)) return rc;
-  a.tile_req = tile_req;
-  a.tile_row = tile_row;
-  const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads, PR_ROWS / 4);
+  if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks,
+                                     block_size, num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q,
+                                     seq_lens, block_table, num_q_heads)) return rc;
+  // 32-bit page and slot offsets where they reach (the tile loop's address arithmetic)
+  if (k_sb < 0 || v_sb < 0 || k_sn < 0 || v_sn < 0 || k_sb > UINT32_MAX || v_sb > UINT32_MAX ||
+      block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
+    return fail("%s: page too large for 32-bit page / slot offsets", nm);
+  PrefillArgs a;
+  a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_cache; a.vc = (const uint16_t*)v_cache; a.out = (uint16_t*)out;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table; a.tile_req = tile_req; a.tile_row = tile_row;
+  a.tile_piece = tile_piece; a.tile_slot = tile_slot; a.part_out = part_out; a.part_ml = part_ml;
+  a.q_st = q_st; a.q_sh = q_sh; a.o_st = o_st; a.o_sh = o_sh;
+  a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh; a.bt_stride = bt_stride;
+  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
+  a.G = (int)(num_q_heads / num_kv_heads); a.lbs = log2i(block_size); a.num_blocks = (int)num_blocks;
+  a.kpage = (uint32_t)k_sb; a.vpage = (uint32_t)v_sb; a.krow = (uint32_t)k_sn; a.vrow = (uint32_t)v_sn;
+  a.contig = (k_sb == block_size * k_sn && v_sb == block_size * v_sn) ? 1 : 0;
+  a.ks = k_scale; a.vs = v_scale; a.ks_pc = a.vs_pc = 0;
+  a.lg = log2i(group); a.s_sb = s_sb; a.s_sh = s_sh; a.s_sg = s_sg;
+  const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  // (an entry that is one of several pieces is computed whole, by each of them with the same result)
-  if (head_dim == 128) hipLaunchKernelGGL(block_rows_kernel<128>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(block_rows_kernel<64>, grid, dim3(256), 0, st, a);
-  return launched(nm);
+  void (*kern)(PrefillArgs) = head_dim == 128 ? (tile_piece ? block_prefill_kernel<128, true> : block_prefill_kernel<128, false>)
+                                              : (tile_piece ? block_prefill_kernel<64, true> : block_prefill_kernel<64, false>);
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
+  const int rc = launched(nm);
+  if (rc != KVQ_OK || !tile_piece || num_merge == 0) return rc;
+  const dim3 mgrid((unsigned)num_merge, (unsigned)num_kv_heads, PR_ROWS / PR_MERGE_WAVES);
+  const int4* ml = reinterpret_cast<const int4*>(merge);
+  if (head_dim == 128) hipLaunchKernelGGL(prefill_merge_kernel<128>, mgrid, dim3(WAVE * PR_MERGE_WAVES), 0, st, a, ml);
+  else hipLaunchKernelGGL(prefill_merge_kernel<64>, mgrid, dim3(WAVE * PR_MERGE_WAVES), 0, st, a, ml);
+  return launched("block_prefill_attention: merge");
 }
 
 }  // extern "C"
