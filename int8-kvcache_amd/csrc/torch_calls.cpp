@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -40,6 +41,10 @@ decltype(&kvq_int8_decode_attention_ex) p_decode_ex;
 decltype(&kvq_dequant_pages) p_dequant;
 decltype(&kvq_paged_prefill_attention_ex) p_prefill;
 decltype(&kvq_int8_prefill_attention_ex) p_prefill_i8;
+decltype(&kvq_quant_block_cache) p_quant_block;
+decltype(&kvq_read_block_cache) p_read_block;
+decltype(&kvq_block_decode_attention) p_block_decode;
+decltype(&kvq_block_prefill_attention) p_block_prefill;
 
 // A tensor argument this file may read: exactly torch.Tensor (or Parameter), dense GPU memory, no wrapper
 // (functorch, functionalization, fake or subclass tensors go to the Python path).
@@ -284,6 +289,187 @@ PyObject* long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- block-scaled cache (kvq.block_cache) ----
+// A cache's views and scales: int8 [nb, bs, H, D] and float32 [nb, H, blocks per page] of one layout.
+struct BlockCache {
+  const int8_t *k, *v;
+  float *ks, *vs;
+  int64_t kb, kn, kh, vb, vn, vh, nb, bs, H, D, sb, sh, sg, group;
+  bool read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks_t, const at::Tensor& vs_t) {
+    if (!int8_cache(kc, vc) || ks_t.dim() != 3 || vs_t.dim() != 3 || ks_t.scalar_type() != at::kFloat ||
+        vs_t.scalar_type() != at::kFloat || ks_t.sizes() != vs_t.sizes() || ks_t.strides() != vs_t.strides())
+      return false;
+    nb = kc.size(0), bs = kc.size(1), H = kc.size(2), D = kc.size(3);
+    const int64_t blocks = ks_t.size(2);
+    if (ks_t.size(0) != nb || ks_t.size(1) != H || blocks < 1 || bs % blocks) return false;
+    group = bs / blocks;   // (the library refuses sizes it does not know)
+    k = (const int8_t*)kc.data_ptr(), v = (const int8_t*)vc.data_ptr();
+    ks = (float*)ks_t.data_ptr(), vs = (float*)vs_t.data_ptr();
+    kb = kc.stride(0), kn = kc.stride(1), kh = kc.stride(2), vb = vc.stride(0), vn = vc.stride(1), vh = vc.stride(2);
+    sb = ks_t.stride(0), sh = ks_t.stride(1), sg = ks_t.stride(2);
+    return true;
+  }
+};
+// the library sizes its grids for the current device: another one goes to the Python path, which switches
+bool on_current(const at::Tensor& t) { return t.device().index() == c10::hip::current_device(); }
+bool table(const at::Tensor& t, int64_t rows) {
+  return t.dim() == 2 && t.scalar_type() == at::kInt && t.stride(1) == 1 && t.size(0) >= rows;
+}
+
+// (key, value, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, seq_lens, block_table)
+PyObject* quant_block_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 9 || !p_quant_block) return DECLINED;
+    const at::Tensor* t[9];
+    for (int i = 0; i < 9; ++i)
+      if (!(t[i] = tensor(a[i]))) return DECLINED;
+    const at::Tensor &key = *t[0], &value = *t[1], &cu = *t[6], &sl = *t[7], &bt = *t[8];
+    BlockCache c;
+    if (!bf16_rows(key) || !bf16_rows(value) || !c.read(*t[2], *t[3], *t[4], *t[5]) || !index_vector(cu) || !index_vector(sl) ||
+        !one_device(key, value, *t[2], *t[3], *t[4], *t[5], cu, sl, bt) || !on_current(key))
+      return DECLINED;
+    const int64_t T = key.size(0), B = cu.size(0) - 1;
+    if (T == 0 || B <= 0 || key.sizes() != value.sizes() || key.size(1) != c.H || key.size(2) != c.D || sl.size(0) < B ||
+        !table(bt, B))
+      return DECLINED;
+    void *kp = key.data_ptr(), *vp = value.data_ptr(), *st = stream_of(key);
+    auto *cup = (const int32_t*)cu.data_ptr(), *slp = (const int32_t*)sl.data_ptr(), *btp = (const int32_t*)bt.data_ptr();
+    return launch("kvq_quant_block_cache", [&] {
+      return p_quant_block(kp, key.stride(0), key.stride(1), vp, value.stride(0), value.stride(1), T, (int8_t*)c.k, c.kb, c.kn,
+                           c.kh, (int8_t*)c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh, c.sg, c.group,
+                           cup, slp, btp, bt.stride(0), B, st);
+    });
+  });
+}
+
+// (k_cache, v_cache, k_scale, v_scale, starts, cu_seqlens_k, block_table, k_out, v_out)
+PyObject* read_block_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 9 || !p_read_block) return DECLINED;
+    const at::Tensor* t[9];
+    for (int i = 0; i < 9; ++i)
+      if (!(t[i] = tensor(a[i]))) return DECLINED;
+    const at::Tensor &start = *t[4], &cu = *t[5], &bt = *t[6], &ko = *t[7], &vo = *t[8];
+    BlockCache c;
+    if (!c.read(*t[0], *t[1], *t[2], *t[3]) || !index_vector(start) || !index_vector(cu) || !bf16_rows(ko) || !bf16_rows(vo) ||
+        !one_device(ko, vo, *t[0], *t[1], *t[2], *t[3], start, cu, bt) || !on_current(ko))
+      return DECLINED;
+    const int64_t N = ko.size(0), B = cu.size(0) - 1;
+    if (N == 0 || B <= 0 || ko.sizes() != vo.sizes() || ko.size(1) != c.H || ko.size(2) != c.D || start.size(0) < B ||
+        !table(bt, B))
+      return DECLINED;
+    void *kp = ko.data_ptr(), *vp = vo.data_ptr(), *st = stream_of(ko);
+    auto *sp = (const int32_t*)start.data_ptr(), *cup = (const int32_t*)cu.data_ptr(), *btp = (const int32_t*)bt.data_ptr();
+    return launch("kvq_read_block_cache", [&] {
+      return p_read_block(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh, c.sg,
+                          c.group, sp, cup, btp, bt.stride(0), B, kp, ko.stride(0), ko.stride(1), vp, vo.stride(0),
+                          vo.stride(1), N, st);
+    });
+  });
+}
+
+// What both attention calls take: (q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, k_scale, v_scale,
+// softmax_scale, ...)
+struct BlockAttn {
+  BlockCache c;
+  const at::Tensor *q, *out, *bt;
+  const int32_t *cu, *sl;
+  void *qp, *op, *st;
+  int64_t B, T, Hq;
+  double scale;
+  bool read(PyObject* const* a) {
+    const at::Tensor* t[9];
+    for (int i = 0; i < 9; ++i)
+      if (!(t[i] = tensor(a[i]))) return false;
+    q = t[0], out = t[3], bt = t[6];
+    if (!PyFloat_CheckExact(a[9])) return false;
+    scale = PyFloat_AS_DOUBLE(a[9]);
+    if (!bf16_rows(*q) || !bf16_rows(*out) || !c.read(*t[1], *t[2], *t[7], *t[8]) || !index_vector(*t[4]) ||
+        !index_vector(*t[5]) || !one_device(*q, *t[1], *t[2], *out, *t[4], *t[5], *bt, *t[7], *t[8]) || !on_current(*q))
+      return false;
+    B = t[4]->size(0) - 1, T = q->size(0), Hq = q->size(1);
+    if (B <= 0 || T == 0 || q->size(2) != c.D || out->size(0) < T || out->size(1) != Hq || out->size(2) != c.D ||
+        t[5]->size(0) < B || !table(*bt, B) || c.H <= 0 || Hq % c.H)
+      return false;
+    cu = (const int32_t*)t[4]->data_ptr(), sl = (const int32_t*)t[5]->data_ptr();
+    qp = q->data_ptr(), op = out->data_ptr(), st = stream_of(*q);
+    return true;
+  }
+};
+
+// (..., segm_out | None, segm_max | None, segm_sum | None, max_query_len, qmax, max_splits)
+PyObject* block_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 16 || !p_block_decode || getenv("KVQ_TARGET_WAVES")) return DECLINED;
+    BlockAttn x;
+    int64_t maxq, qmax, max_splits;
+    if (!x.read(a) || !as_int(a[13], maxq) || !as_int(a[14], qmax) || !as_int(a[15], max_splits)) return DECLINED;
+    int64_t S = 1, rows = 0, seg_st = 0, seg_sh = 0;
+    float *sop = nullptr, *smp = nullptr, *ssp = nullptr;
+    if (a[11] != Py_None) {
+      const at::Tensor *so = tensor(a[10]), *sm = tensor(a[11]), *ss = tensor(a[12]);
+      if (!so || !sm || !ss || so->dim() != 4 || sm->dim() != 3 || ss->dim() != 3 || !one_device(*x.q, *so, *sm, *ss))
+        return DECLINED;
+      S = sm->size(2), rows = sm->size(0), seg_st = sm->stride(0), seg_sh = sm->stride(1);
+      for (const at::Tensor* y : {so, sm, ss})
+        if (y->scalar_type() != at::kFloat || y->size(0) != rows || y->size(1) != x.Hq || y->size(2) != S) return DECLINED;
+      const int64_t D = x.c.D;
+      if (S > max_splits || sm->stride(2) != 1 || ss->strides() != sm->strides() || so->size(3) != D || so->stride(3) != 1 ||
+          so->stride(2) != D || so->stride(1) != seg_sh * D || so->stride(0) != seg_st * D)
+        return DECLINED;
+      sop = (float*)so->data_ptr(), smp = (float*)sm->data_ptr(), ssp = (float*)ss->data_ptr();
+    } else if (a[10] != Py_None || a[12] != Py_None) {
+      return DECLINED;
+    }
+    const BlockCache& c = x.c;
+    auto* btp = (const int32_t*)x.bt->data_ptr();
+    return launch("kvq_block_decode_attention", [&] {
+      return p_block_decode(x.qp, x.q->stride(0), x.q->stride(1), c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H,
+                            c.D, c.ks, c.vs, c.sb, c.sh, c.sg, c.group, x.op, x.out->stride(0), x.out->stride(1), x.cu, x.sl,
+                            btp, x.bt->stride(0), x.B, x.Hq, x.scale, sop, smp, ssp, seg_st, seg_sh, S, rows, 0, maxq, qmax,
+                            x.st);
+    });
+  });
+}
+
+// (..., rows_per_tile, tile_req, tile_row, tile_piece | None, tile_slot | None, merge | None, slots)
+PyObject* block_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 17 || !p_block_prefill) return DECLINED;
+    BlockAttn x;
+    int64_t rows, slots;
+    if (!x.read(a) || !as_int(a[10], rows) || !as_int(a[16], slots)) return DECLINED;
+    const at::Tensor *treq = tensor(a[11]), *trow = tensor(a[12]);
+    if (!treq || !trow || !index_vector(*treq) || !index_vector(*trow) || !one_device(*x.q, *treq, *trow)) return DECLINED;
+    const int64_t tiles = treq->size(0);
+    if (tiles == 0 || trow->size(0) != tiles) return DECLINED;
+    const int32_t *pp = nullptr, *sp = nullptr, *mp = nullptr;
+    int64_t nm = 0;
+    at::Tensor part_out, part_ml;
+    if (a[13] != Py_None) {
+      const at::Tensor *piece = tensor(a[13]), *slot = tensor(a[14]), *merge = tensor(a[15]);
+      if (!piece || !slot || !merge || !index_vector(*piece) || !index_vector(*slot) || piece->size(0) != tiles ||
+          slot->size(0) != tiles || merge->scalar_type() != at::kInt || merge->dim() != 2 || !merge->is_contiguous() ||
+          merge->size(1) != 4 || !one_device(*x.q, *piece, *slot, *merge))
+        return DECLINED;
+      pp = (const int32_t*)piece->data_ptr(), sp = (const int32_t*)slot->data_ptr(), mp = (const int32_t*)merge->data_ptr();
+      nm = merge->size(0);
+      const auto f32 = x.q->options().dtype(at::kFloat);
+      part_out = at::empty({slots, x.c.H, rows, x.c.D}, f32);
+      part_ml = at::empty({slots, x.c.H, rows, 2}, f32);
+    }
+    float *pop = pp ? (float*)part_out.data_ptr() : nullptr, *pmp = pp ? (float*)part_ml.data_ptr() : nullptr;
+    const BlockCache& c = x.c;
+    auto* btp = (const int32_t*)x.bt->data_ptr();
+    auto *rp = (const int32_t*)treq->data_ptr(), *wp = (const int32_t*)trow->data_ptr();
+    return launch("kvq_block_prefill_attention", [&] {
+      return p_block_prefill(x.qp, x.q->stride(0), x.q->stride(1), c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs,
+                             c.H, c.D, c.ks, c.vs, c.sb, c.sh, c.sg, c.group, x.op, x.out->stride(0), x.out->stride(1), x.cu,
+                             x.sl, btp, x.bt->stride(0), x.Hq, rp, wp, tiles, rows, x.scale, pp, sp, mp, nm, pop, pmp, x.st);
+    });
+  });
+}
+
 // (): the entry point of this thread's last call, as the Python path names it in its error
 PyObject* last_entry(PyObject*, PyObject*) { return PyUnicode_FromString(entry); }
 
@@ -299,6 +485,10 @@ PyObject* bind(PyObject*, PyObject* d) {
   p_dequant = (decltype(p_dequant))at_name("kvq_dequant_pages");
   p_prefill = (decltype(p_prefill))at_name("kvq_paged_prefill_attention_ex");
   p_prefill_i8 = (decltype(p_prefill_i8))at_name("kvq_int8_prefill_attention_ex");
+  p_quant_block = (decltype(p_quant_block))at_name("kvq_quant_block_cache");
+  p_read_block = (decltype(p_read_block))at_name("kvq_read_block_cache");
+  p_block_decode = (decltype(p_block_decode))at_name("kvq_block_decode_attention");
+  p_block_prefill = (decltype(p_block_prefill))at_name("kvq_block_prefill_attention");
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -310,6 +500,14 @@ PyMethodDef methods[] = {
      "kvq_int8_decode_attention on torch tensors"},
     {"long_attention", (PyCFunction)(void (*)(void))long_attention, METH_FASTCALL,
      "the long requests' attention on torch tensors"},
+    {"quant_block_cache", (PyCFunction)(void (*)(void))quant_block_cache, METH_FASTCALL,
+     "kvq_quant_block_cache on torch tensors"},
+    {"read_block_cache", (PyCFunction)(void (*)(void))read_block_cache, METH_FASTCALL,
+     "kvq_read_block_cache on torch tensors"},
+    {"block_decode_attention", (PyCFunction)(void (*)(void))block_decode_attention, METH_FASTCALL,
+     "kvq_block_decode_attention on torch tensors"},
+    {"block_long_attention", (PyCFunction)(void (*)(void))block_long_attention, METH_FASTCALL,
+     "kvq_block_prefill_attention on torch tensors"},
     {"last_entry", last_entry, METH_NOARGS, "the entry point of this thread's last call"},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -92,6 +92,9 @@ def quant_block_cache(key, value, key_cache, value_cache, scales, cu_seqlens_q, 
     block's first position is written. Infinities saturate and do not count for the scale. The pages written must belong
     to one request each."""
     name, n, num_seqs = "quant_block_cache", key.shape[0], cu_seqlens_q.shape[0] - 1
+    if ck._served(ck.ext(), name, key, value, key_cache, value_cache, scales["k_scale"], scales["v_scale"], cu_seqlens_q,
+                  seq_lens, block_table):
+        return
     _check(key.dim() == 3 and key.shape == value.shape and key.stride(2) == 1 and value.stride(2) == 1 and
            key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16,
            f"{name}: key / value must be bf16 [T, kv_heads, D] with a contiguous last dim")
@@ -100,7 +103,6 @@ def quant_block_cache(key, value, key_cache, value_cache, scales, cu_seqlens_q, 
     _check_index(name, num_seqs, block_table, cu_seqlens_q=cu_seqlens_q, seq_lens=seq_lens)
     if n == 0 or num_seqs <= 0:
         return
-    ck.ext()
     _check_cuda(name, key, value, key_cache, value_cache, scales["k_scale"], scales["v_scale"], cu_seqlens_q, seq_lens,
                 block_table)
     _call("kvq_quant_block_cache", key.device, key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
@@ -113,6 +115,9 @@ def read_block_cache(key_cache, value_cache, scales, starts, cu_seqlens_k, block
     key_out / value_out (bf16 [N, kv heads, D], N at least cu_seqlens_k[-1]; rows behind are left as they were).
     Returns (key_out, value_out)."""
     name, num_seqs = "read_block_cache", cu_seqlens_k.shape[0] - 1
+    if ck._served(ck.ext(), name, key_cache, value_cache, scales["k_scale"], scales["v_scale"], starts, cu_seqlens_k,
+                  block_table, key_out, value_out):
+        return key_out, value_out
     k, v, geom, sc = _cache_args(name, key_cache, value_cache, scales)
     for t in (key_out, value_out):
         _check(t.dim() == 3 and t.dtype == torch.bfloat16 and t.stride(2) == 1 and t.shape[1:] == key_cache.shape[2:] and
@@ -120,7 +125,6 @@ def read_block_cache(key_cache, value_cache, scales, starts, cu_seqlens_k, block
     _check_index(name, num_seqs, block_table, cu_seqlens_k=cu_seqlens_k, starts=starts)
     if key_out.shape[0] == 0 or num_seqs <= 0:
         return key_out, value_out
-    ck.ext()
     _check_cuda(name, key_cache, value_cache, scales["k_scale"], scales["v_scale"], starts, cu_seqlens_k, block_table, key_out,
                 value_out)
     _call("kvq_read_block_cache", key_cache.device, *k, *v, *geom, *sc, starts.data_ptr(), cu_seqlens_k.data_ptr(),
@@ -145,10 +149,13 @@ def block_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, blo
     the bf16 q (neither q nor the softmax's weights are rounded to 8 bits). A row that sees no key is zero. segm:
     split buffers (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces."""
     name, num_seqs = "block_decode_attention", cu_seqlens_q.shape[0] - 1
+    so, sm, ss = segm if segm is not None else (None, None, None)
+    if ck._served(ck.ext(), name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
+                  scales["v_scale"], softmax_scale, so, sm, ss, max_query_len, ck.SHORT_Q, ck.MAX_SPLITS):
+        return out
     k, v, geom, sc = _cache_args(name, k_cache, v_cache, scales)
     _check_attention(name, q, k_cache, out, cu_seqlens_q, seq_lens, block_table)
     hq, d = q.shape[1:]
-    so, sm, ss = segm if segm is not None else (None, None, None)
     split = (None, None, None, 0, 0, 1, 0)
     if sm is not None:
         S = sm.shape[2]
@@ -162,7 +169,6 @@ def block_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, blo
         split = (so.data_ptr(), sm.data_ptr(), ss.data_ptr(), sm.stride(0), sm.stride(1), S, sm.shape[0])
     if q.shape[0] == 0 or num_seqs <= 0:
         return out
-    ck.ext()
     _check_cuda(name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"], scales["v_scale"],
                 so, sm, ss)
     _call("kvq_block_decode_attention", q.device, q.data_ptr(), q.stride(0), q.stride(1), *k, *v, *geom, *sc,
@@ -176,14 +182,17 @@ def block_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block
     """Attention over a block-scaled cache for the plan's long requests (cuda_kernels.plan_long; the others' rows are left
     as they were), read straight from the pages: the formula of block_decode_attention on bf16 operands, the
     codes exact, their scales applied in fp32, the softmax's weights rounded to bf16."""
-    name = "block_long_attention"
+    name, e = "block_long_attention", ck.ext()
+    bs, h, d = k_cache.shape[1:]
+    _check(bs == plan.block_size, f"block size {bs} != plan block size {plan.block_size}")
+    work = plan.work(q.shape[1] // h, h, d, q.device)
+    if ck._served(e, name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
+                  scales["v_scale"], softmax_scale, e.prefill_rows, work.tile_req, work.tile_row, work.tile_piece,
+                  work.tile_slot, work.merge, work.slots):
+        return out
     k, v, geom, sc = _cache_args(name, k_cache, v_cache, scales)
     _check_attention(name, q, k_cache, out, cu_seqlens_q, seq_lens, block_table)
-    nb, bs, h, d = geom
-    _check(bs == plan.block_size, f"block size {bs} != plan block size {plan.block_size}")
-    e = ck.ext()
     _check_cuda(name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"], scales["v_scale"])
-    work = plan.work(q.shape[1] // h, h, d, q.device)
     n = work.tile_req.shape[0]
     split = work.split(h, e.prefill_rows, d)
     _call("kvq_block_prefill_attention", q.device, q.data_ptr(), q.stride(0), q.stride(1), *k, *v, *geom, *sc,

@@ -456,3 +456,60 @@ def test_debug_check(monkeypatch):
     c.scales["v_scale"][c.table[0, 3]] = float("inf")
     with pytest.raises(RuntimeError, match="req 0: v_scale not finite"):
         bc.block_paged_attention(*args)
+
+
+# ------------------------------------------------------------------------------------------------ native calls
+def _call_all(c, x):
+    """Every operator once on the GPU state `x`; the outputs, or what was raised."""
+    got = []
+    for f in (lambda: bc.quant_block_cache(x["k"], x["v"], c.kc, c.vc, x["scales"], x["cu"], x["lens"], c.table),
+              lambda: bc.read_block_cache(c.kc, c.vc, x["scales"], x["lens"] // 2, x["cu"], c.table, x["ko"], x["vo"]),
+              lambda: bc.block_paged_attention(x["q"], c.kc, c.vc, x["out"], x["cu"], x["lens"], c.table, x["most"], x["scale"],
+                                               x["scales"], x["plan"], x["segm"])):
+        try:
+            f()
+            got.append("served")
+        except Exception as e:  # noqa: BLE001 - compared with the other path's
+            got.append((type(e), str(e)))
+    return got, [t.clone() for t in (c.kc, c.vc, x["scales"]["k_scale"], x["ko"], x["vo"], x["out"])]
+
+
+CHANGES = {
+    "plain": lambda x: None,
+    "split": lambda x: x.update(segm=nan_segm(x["q"].shape[0], 28, 16, 128)),
+    "strided_split": lambda x: x.update(segm=tuple(t[:, :28] for t in nan_segm(x["q"].shape[0], 30, 8, 128))),
+    "packed_q": lambda x: x.update(q=torch.cat([x["q"], x["q"]], 1)[:, :28]),
+    "parameter_scales": lambda x: x.update(scales={n: torch.nn.Parameter(t, requires_grad=False) for n, t in x["scales"].items()}),
+    "scale_int": lambda x: x.update(scale=1),
+    "half": lambda x: x.update(q=x["q"].half(), k=x["k"].half(), ko=x["ko"].half()),
+    "few_outputs": lambda x: x.update(out=x["out"][:3], vo=x["vo"][:-1]),
+    "long_lengths": lambda x: x.update(lens=x["lens"].long()),
+    "odd_rows": lambda x: x.update(q=torch.zeros(x["q"].shape[0], 28, 132, dtype=torch.bfloat16, device=DEV)[..., :128],
+                                   k=torch.zeros(*x["k"].shape[:2], 132, dtype=torch.bfloat16, device=DEV)[..., :128]),
+    "cpu": lambda x: x.update(q=x["q"].cpu(), k=x["k"].cpu(), ko=x["ko"].cpu()),
+}
+
+
+@pytest.mark.parametrize("change", CHANGES)
+def test_native_calls_and_the_python_path_agree(change, monkeypatch):
+    assert ck.ext().calls is not None, "kvq._torch_calls is not built"
+    lens, q_lens = [300, 20, 64, 2000], [1, 20, 8, 300]
+    got = []
+    for native in (True, False):
+        c = filled(4, 128, 32, 16, lens)
+        n = sum(q_lens)
+        k, v = rows(n, 4, 128, 50)
+        x = {"k": k.to(DEV), "v": v.to(DEV), "scales": c.scales, "cu": i32(cumsum(q_lens)), "lens": i32(lens),
+             "ko": torch.zeros(n, 4, 128, dtype=torch.bfloat16, device=DEV),
+             "vo": torch.zeros(n, 4, 128, dtype=torch.bfloat16, device=DEV),
+             "q": torch.randn(n, 28, 128, generator=gen(1)).to(torch.bfloat16).to(DEV), "most": max(q_lens), "scale": 0.088,
+             "plan": ck.plan_long(cumsum(q_lens), lens, 32), "segm": None}
+        x["out"] = torch.zeros_like(x["q"])
+        CHANGES[change](x)
+        with monkeypatch.context() as m:
+            if not native:
+                m.setattr(ck.ext(), "calls", None)
+            got.append(_call_all(c, x))
+    (a, ta), (b, tb) = got
+    assert a == b
+    assert all(torch.equal(torch.nan_to_num(s.float()), torch.nan_to_num(t.float())) for s, t in zip(ta, tb))
