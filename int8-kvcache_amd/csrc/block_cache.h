@@ -5,21 +5,15 @@
 //   quant_block_kernel   quantize a step's new K/V into their blocks, raising scales (and requantizing) where needed
 //   read_block_kernel    ranges of the requests' keys back to bf16 rows
 //   block_attn_kernel    attention of short queries, int8 MFMA on operands of two int8 planes
-//   block_prefill_kernel attention of long queries: prefill_body on the codes as bf16
+//   block_verify_kernel, block_prefill_kernel   attention of many query rows (block_rows.h)
 //
 // A cached value is code * scale; attention is that of those values and the bf16 q, without further rounding of either.
+
+#include "block_rows.h"
 
 namespace {
 
 constexpr int BLK_MIN = 16, BLK_MAX = 128;   // positions per scale
-
-// Where the scales lie: that of (page p, head h, block b) at p * sb + h * sh + b * sg floats of ks / vs.
-struct BlockScales {
-  const float* ks;
-  const float* vs;
-  int64_t sb, sh, sg;
-  int lg;   // log2 of the positions per scale
-};
 
 // The request that holds slot u of a line on which request r starts at (cu[r] >> lg) + 2 r: as long as cu[r] counts
 // rows of consecutive positions, r's rows touch at most (rows >> lg) + 2 aligned blocks of 2^lg positions, so its
@@ -271,7 +265,6 @@ __device__ __forceinline__ const BlockScales& fresh_scales() {
   return *(const BlockScales*)(const void*)(p + offsetof(BlockAttnArgs, s));
 }
 
-constexpr float Q16_MAX = 16256.f;   // 127 * 128: the hi plane of rint(q / sq) stays an int8
 constexpr float P14_MAX = 16320.f;   // below 16383 by more than the reciprocal's error: the hi plane stays below 128
 
 __device__ __forceinline__ int ror8(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true); }
@@ -402,18 +395,14 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
     for (int s = 0; s < KSTEPS; ++s)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        uint32_t hi = 0u, lo = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = (int)__builtin_rintf(x[16 * s + 4 * w + e] * inv), h = (v + 64) >> 7;
-          hi |= (uint32_t)(h & 0xff) << (8 * e);
-          lo |= (uint32_t)((v - 128 * h) & 0xff) << (8 * e);
-        }
+        const int e = 16 * s + 4 * w;
+        int hi, lo;
+        q_planes4(x[e], x[e + 1], x[e + 2], x[e + 3], inv, hi, lo);
         if constexpr (PACK) {
-          qop[0][s][w] = n < 8 ? (int)hi : (int)lo;
+          qop[0][s][w] = n < 8 ? hi : lo;
         } else {
-          qop[0][s][w] = (int)hi;
-          qop[NP - 1][s][w] = (int)lo;
+          qop[0][s][w] = hi;
+          qop[NP - 1][s][w] = lo;
         }
       }
   }
@@ -653,12 +642,100 @@ __global__ __launch_bounds__(256) void block_attn_kernel(BlockAttnArgs args) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Attention of long queries: prefill_body's rows, tiles and ring on the codes converted to bf16 (exactly), with the
-// exponent of block_attn_kernel. Each tile's four scales come with its DMA, one instruction more per wavefront.
+// Many query rows (block_rows.h). block_verify_kernel: short queries of more rows than block_attn_kernel's tiles suit, on
+// its plan, in pieces of 64 rows. block_prefill_kernel: the work lists of long queries, 128 rows an entry.
 // ------------------------------------------------------------------------------------------------
+template <int D>
+__global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args) {
+  touch_args();
+  __shared__ __attribute__((aligned(1024))) RowsLds<D> lds;
+  const int lane = threadIdx.x & (WAVE - 1), n = lane & 15, g = lane >> 4;
+  walk_pieces(args.a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
+    const AttnArgs& a = fresh_args();
+    const BlockScales& s = fresh_scales();
+    const RowsView v{a.q, a.kc + (int64_t)kvh * a.k_sh, a.vc + (int64_t)kvh * a.v_sh, a.block_table + (int64_t)r * a.bt_stride,
+                     s.ks + (int64_t)kvh * s.sh, s.vs + (int64_t)kvh * s.sh, a.q_st, a.q_sh, a.k_sb, a.k_sn, a.v_sb, a.v_sn,
+                     s.sb, s.sg, a.sm_log2, a.G, a.num_blocks, a.lbs, s.lg};
+    attend_rows<D, 1>(v, lds, w.tok, w.qlen, w.len, kvh, 64 * rg, c0, w.len > 0 ? c1 : c0, min(w.len, c1 * PR_KEYS),
+                      [&](int, int t, int hq, bool valid, float m, float l, const f32x4 (&acc)[D / 16]) {
+      if (!valid) return;
+      const AttnArgs& o = fresh_args();
+      const int qt = w.tok + t;
+      if (nparts == 1) {
+        if (o.max_splits > 1 && qt < o.cut_rows && g == 0)
+          o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)hq * o.seg_sh] = -1.f;
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint16_t* op = o.out + (int64_t)qt * o.o_st + (int64_t)hq * o.o_sh + 4 * g;
+#pragma unroll
+        for (int tt = 0; tt < D / 16; ++tt)
+          *reinterpret_cast<u32x2*>(op + 16 * tt) = u32x2{pack_bf16x2_rne(acc[tt][0] * inv, acc[tt][1] * inv),
+                                                          pack_bf16x2_rne(acc[tt][2] * inv, acc[tt][3] * inv)};
+      } else {
+        const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)hq * o.seg_sh + part;
+        if (g == 0) {
+          o.segm_max[sidx] = m;
+          o.segm_sum[sidx] = part == nparts - 1 ? -2.f - l : l;
+        }
+        float* sp = o.segm_out + sidx * D + 4 * g;
+#pragma unroll
+        for (int tt = 0; tt < D / 16; ++tt) *reinterpret_cast<f32x4*>(sp + 16 * tt) = acc[tt];
+      }
+    });
+  });
+}
+
+struct BlockPrefillArgs {
+  PrefillArgs p;
+  BlockScales s;
+};
+
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(256, 3) void block_prefill_kernel(PrefillArgs a) {
-  prefill_body<D, PR_SRC_I8_BLOCK, SPLIT>(a);
+__global__ __launch_bounds__(256, 3) void block_prefill_kernel(BlockPrefillArgs args) {
+  __shared__ __attribute__((aligned(1024))) RowsLds<D> lds;
+  const PrefillArgs& a = args.p;
+  const BlockScales& s = args.s;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y, r = a.tile_req[blockIdx.x], row0 = a.tile_row[blockIdx.x];
+  const int tok = a.cu_q[r], Q = a.cu_q[r + 1] - tok, L = a.seq_lens[r];
+  const int t_last = min(Q - 1, (row0 + PR_ROWS - 1) / a.G);
+  int kend = max(0, min(L, L - Q + 1 + t_last)), c_lo = 0, c_hi = (kend + PR_KEYS - 1) / PR_KEYS;
+  if constexpr (SPLIT) {   // an equal share of the rows' tiles
+    const int pp = a.tile_piece[blockIdx.x], nparts = pp >> 16, part = pp & 0xffff, each = c_hi / nparts, rem = c_hi % nparts;
+    c_lo = part * each + min(part, rem);
+    c_hi = c_lo + each + (part < rem ? 1 : 0);
+    kend = min(kend, c_hi * PR_KEYS);
+  }
+  const RowsView v{a.q, (const int8_t*)a.kc + (int64_t)kvh * a.k_sh, (const int8_t*)a.vc + (int64_t)kvh * a.v_sh,
+                   a.block_table + (int64_t)r * a.bt_stride, s.ks + (int64_t)kvh * s.sh, s.vs + (int64_t)kvh * s.sh, a.q_st,
+                   a.q_sh, a.k_sb, a.k_sn, a.v_sb, a.v_sn, s.sb, s.sg, a.sm_log2, a.G, a.num_blocks, a.lbs, s.lg};
+  bool piece = false;
+  int pslot = 0;
+  attend_rows<D, PR_RB>(v, lds, tok, Q, L, kvh, row0, c_lo, c_hi, kend,
+                        [&](int rb, int t, int hq, bool valid, float m, float l, const f32x4 (&acc)[D / 16]) {
+    if constexpr (SPLIT) {
+      if (rb == 0) {   // read here, not held through the tile loop
+        int x = blockIdx.x;
+        asm volatile("" : "+s"(x));
+        piece = (a.tile_piece[x] >> 16) > 1;
+        pslot = a.tile_slot[x];
+      }
+    }
+    if (!valid) return;
+    if (SPLIT && piece) {   // the accumulators as they are: the merge divides by the whole denominator
+      const int64_t pr = ((int64_t)pslot * gridDim.y + kvh) * PR_ROWS + (wave * PR_RB + rb) * 16 + n;
+      if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = float2{m, l};
+      float* prow = a.part_out + pr * D + 4 * g;
+#pragma unroll
+      for (int tt = 0; tt < D / 16; ++tt) *reinterpret_cast<f32x4*>(prow + 16 * tt) = acc[tt];
+      return;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint16_t* op = a.out + (int64_t)(tok + t) * a.o_st + (int64_t)hq * a.o_sh + 4 * g;
+#pragma unroll
+    for (int tt = 0; tt < D / 16; ++tt)
+      *reinterpret_cast<u32x2*>(op + 16 * tt) = u32x2{pack_bf16x2_rne(acc[tt][0] * inv, acc[tt][1] * inv),
+                                                      pack_bf16x2_rne(acc[tt][2] * inv, acc[tt][3] * inv)};
+  });
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -803,7 +880,7 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
                                      seq_lens, block_table, num_q_heads)) return rc;
   if (num_splits > 1 && segm_rows > 0 && (!segm_out || !segm_max || !segm_sum || !aligned16(segm_out)))
     return fail("%s: split buffers missing or not 16-byte aligned", nm);
-  if ((int64_t)block_size * k_sn > INT32_MAX || 16 * v_sn > INT32_MAX || k_sn < 0 || v_sn < 0)
+  if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
     return fail("%s: page too large for 32-bit lane offsets", nm);
   const int G = (int)(num_q_heads / num_kv_heads);
   const int64_t maxq = std::min<int64_t>(std::max<int64_t>(max_query_len, 1), qmax), rows = (int64_t)G * maxq;
@@ -812,9 +889,10 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   const bool pack = rows <= 8;
   const int rt = (int)std::min<int64_t>(MAX_ROW_TILES, (rows + 15) / 16);
   const Tuning tune = read_tuning();
+  const bool many = rows > 32 && !(tune.rows32 && atoi(tune.rows32) == 0);
   const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
                      : num_splits == 1 || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? MAX_ROW_TILES : DEFAULT_KSPLIT;
-  const int ks = std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = rt * ks;
+  const int ks = many ? 1 : std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = many ? 4 : rt * ks;
   BlockAttnArgs b;
   b.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
   AttnArgs& a = b.a;
@@ -833,15 +911,16 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   a.num_seqs = (int)num_seqs; a.hkv = (int)num_kv_heads;
   a.max_splits = (int)num_splits;
   a.cut_rows = num_splits > 1 ? (int)std::min<int64_t>(segm_rows, INT32_MAX) : 0;
-  a.rt = rt; a.ksplit = ks; a.waves = waves;
+  a.rt = many ? 4 : rt; a.ksplit = ks; a.waves = waves;
   a.min_tiles = MIN_SPLIT_TILES;
   a.coop = coop_tiles(num_splits > 1, ks);
   a.xcd_order = tune.xcd_order ? atoi(tune.xcd_order) : 1;
   a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
                                        : (int)PLAN_FAST_MAX;
   a.seg_cost = seg_cost_units(tune, 0);
-  const size_t lds = (size_t)(ks - 1) * rt * MERGE_FIELDS * WAVE * sizeof(float);
-  void (*kern)(BlockAttnArgs) = head_dim == 128 ? (pack ? block_attn_kernel<128, 2, true> : block_attn_kernel<128, 2, false>)
+  const size_t lds = many ? 0 : (size_t)(ks - 1) * rt * MERGE_FIELDS * WAVE * sizeof(float);
+  void (*kern)(BlockAttnArgs) = many ? (head_dim == 128 ? block_verify_kernel<128> : block_verify_kernel<64>)
+                              : head_dim == 128 ? (pack ? block_attn_kernel<128, 2, true> : block_attn_kernel<128, 2, false>)
                                                 : (pack ? block_attn_kernel<64, 2, true> : block_attn_kernel<64, 2, false>);
   const bool cuttable_any = num_splits > 1 && segm_rows > 0;
   const int64_t tw = target_waves > 0 ? target_waves
@@ -881,11 +960,11 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
   if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks,
                                      block_size, num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q,
                                      seq_lens, block_table, num_q_heads)) return rc;
-  // 32-bit page and slot offsets where they reach (the tile loop's address arithmetic)
-  if (k_sb < 0 || v_sb < 0 || k_sn < 0 || v_sn < 0 || k_sb > UINT32_MAX || v_sb > UINT32_MAX ||
-      block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
-    return fail("%s: page too large for 32-bit page / slot offsets", nm);
-  PrefillArgs a;
+  if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
+    return fail("%s: page too large for 32-bit lane offsets", nm);
+  BlockPrefillArgs b;
+  b.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
+  PrefillArgs& a = b.p;
   a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_cache; a.vc = (const uint16_t*)v_cache; a.out = (uint16_t*)out;
   a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table; a.tile_req = tile_req; a.tile_row = tile_row;
   a.tile_piece = tile_piece; a.tile_slot = tile_slot; a.part_out = part_out; a.part_ml = part_ml;
@@ -893,15 +972,12 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
   a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh; a.bt_stride = bt_stride;
   a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
   a.G = (int)(num_q_heads / num_kv_heads); a.lbs = log2i(block_size); a.num_blocks = (int)num_blocks;
-  a.kpage = (uint32_t)k_sb; a.vpage = (uint32_t)v_sb; a.krow = (uint32_t)k_sn; a.vrow = (uint32_t)v_sn;
-  a.contig = (k_sb == block_size * k_sn && v_sb == block_size * v_sn) ? 1 : 0;
-  a.ks = k_scale; a.vs = v_scale; a.ks_pc = a.vs_pc = 0;
-  a.lg = log2i(group); a.s_sb = s_sb; a.s_sh = s_sh; a.s_sg = s_sg;
+  a.kpage = a.vpage = a.krow = a.vrow = 0; a.contig = 0; a.ks = a.vs = nullptr; a.ks_pc = a.vs_pc = 0;   // (prefill_body's)
   const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  void (*kern)(PrefillArgs) = head_dim == 128 ? (tile_piece ? block_prefill_kernel<128, true> : block_prefill_kernel<128, false>)
+  void (*kern)(BlockPrefillArgs) = head_dim == 128 ? (tile_piece ? block_prefill_kernel<128, true> : block_prefill_kernel<128, false>)
                                               : (tile_piece ? block_prefill_kernel<64, true> : block_prefill_kernel<64, false>);
-  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, b);
   const int rc = launched(nm);
   if (rc != KVQ_OK || !tile_piece || num_merge == 0) return rc;
   const dim3 mgrid((unsigned)num_merge, (unsigned)num_kv_heads, PR_ROWS / PR_MERGE_WAVES);

@@ -2104,10 +2104,6 @@ struct PrefillArgs {
   const float* ks;
   const float* vs;
   int ks_pc, vs_pc;
-  // a block-scaled cache: the scales of page p, head h, block b at p * s_sb + h * s_sh + b * s_sg of ks / vs, 2^lg
-  // positions per block
-  int lg;
-  int64_t s_sb, s_sh, s_sg;
 };
 
 constexpr int PR_RB = 2;                    // 16-row blocks per wavefront
@@ -2145,18 +2141,12 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rne(float a, float b) {
 // Where the K / V tiles come from: the bf16 temporary cache, or the INT8 pages themselves
 // (prefill_i8_kernel below), converted tile by tile either as dequant_pages converts them (bf16 of
 // code x scale) or as exact bf16 codes with the scales folded into q (K) and the output (V).
-// PR_SRC_I8_BLOCK: pages of a block-scaled cache, codes converted exactly, each 16-key half tile's K scale a factor of
-// its scores and its V scale an addend in the exponent (block_cache.h).
-constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2, PR_SRC_I8_BLOCK = 3;
-constexpr float MIN_BLOCK_SCALE = 1e-30f;   // a block's scale counts as at least this (the V scale's logarithm and
-                                            // reciprocal are taken; a K scale of 0 times a masked score is no number)
+constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2;
 
 template <int D, int SRC, bool SPLIT>
 __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   constexpr bool I8 = SRC != PR_SRC_BF16;
   constexpr bool FOLD = SRC == PR_SRC_I8_FOLD;
-  constexpr bool BLK = SRC == PR_SRC_I8_BLOCK;
-  constexpr bool CODES = FOLD || BLK;       // tiles hold the codes themselves
   constexpr int DS = D / 32;                // 32-channel chunks of the QK contraction
   constexpr int VT = D / 16;                // PV channel tiles
   constexpr int RB = PR_RB;
@@ -2177,15 +2167,11 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   constexpr int TILE8B = PR_KEYS * D;       // bytes per int8 K (or V) tile
   constexpr int PPM = TILE8B / 1024;        // DMA instructions per int8 matrix and tile
   constexpr int IPW8 = 2 * PPM / 4;         // per wavefront and tile, K and V together
-  constexpr int VMT = IPW8 + (BLK ? 1 : 0); // vector memory instructions per wavefront and tile
   constexpr int CPR8 = D / 16;              // 16-byte chunks per int8 key row
   constexpr int RPI8 = 1024 / D;            // int8 key rows per DMA instruction
   static_assert(NS8 >= 2 && IPW8 * 4 == 2 * PPM && RPI8 <= 16, "int8 ring");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[NB][2][TILEB];
   __shared__ __attribute__((aligned(1024))) uint8_t ring8[I8 ? NS8 : 1][2][I8 ? TILE8B : 16];
-  // BLK: the last four tiles' scales, each wavefront its own copy (no barrier): lane l of the one DMA puts that of half
-  // l / 2 % 2, K (l even) or V, at float l -- the first four are read
-  __shared__ __attribute__((aligned(16))) float sring[BLK ? 4 : 1][4][BLK ? WAVE : 4];
 
   const int kvh = blockIdx.y;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -2309,12 +2295,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     }
     linear = !__any(bad) && run_fits(pg_hi + 1, a.kpage) && run_fits(pg_hi + 1, a.vpage);
   }
-  const float* sbase = nullptr;
-  uint32_t sadr = 0;
-  if constexpr (BLK) {
-    sbase = ((lane & 1) ? a.vs : a.ks) + (int64_t)kvh * a.s_sh;
-    sadr = (uint32_t)(uintptr_t)(&sring[0][wave][0]);
-  }
   const char* klin = kh + (int64_t)pfirst * a.kpage;
   const char* vlin = vh + (int64_t)pfirst * a.vpage;
   // tile c: keys 0..15 sit in page p0 from slot (32 c) mod bs on, keys 16..31 right after them
@@ -2348,21 +2328,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       kb[1] = kh + ((uint64_t)(uint32_t)p1 * a.kpage + s1 * a.krow);
       vb[0] = vh + ((uint64_t)(uint32_t)p0 * a.vpage + s0 * a.vrow);
       vb[1] = vh + ((uint64_t)(uint32_t)p1 * a.vpage + s1 * a.vrow);
-    }
-    if constexpr (BLK) {
-      // a half past the last key takes the last key's block (its own may never have been written)
-      const int k1 = min(kb0 + 16, klast), i0 = kb0 >> a.lbs, i1 = k1 >> a.lbs;
-      int p0 = pfirst + i0, p1 = pfirst + i1;
-      if (!lin) {
-        p0 = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[i0]);
-        p1 = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[i1]);
-        p0 = (p0 >= 0 && p0 < a.num_blocks) ? p0 : 0;
-        p1 = (p1 >= 0 && p1 < a.num_blocks) ? p1 : 0;
-      }
-      const int64_t s0 = (int64_t)p0 * a.s_sb + (int64_t)((kb0 & bsm) >> a.lg) * a.s_sg;
-      const int64_t s1 = (int64_t)p1 * a.s_sb + (int64_t)((k1 & bsm) >> a.lg) * a.s_sg;
-      __builtin_amdgcn_global_load_lds((const void*)(sbase + ((lane & 2) ? s1 : s0)),
-                                       (__attribute__((address_space(3))) void*)(&sring[c & 3][wave][0]), 4, 0, 0);
     }
     if constexpr (I8) {
 #pragma unroll
@@ -2435,11 +2400,11 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // (registers for them would cost the kernel its third workgroup per CU). Channel 8 c + 4 h + e sits
   // at float (D / 2) h + 4 c + e of its matrix's D: a quarter-wavefront's 16-byte reads of the first
   // (or second) four scales of 16 chunks are 256 contiguous bytes (no bank conflicts).
-  __shared__ __attribute__((aligned(16))) float scl[I8 && !CODES ? 2 * D : 4];
+  __shared__ __attribute__((aligned(16))) float scl[I8 && !FOLD ? 2 * D : 4];
   uint32_t cra = 0, cwk = 0, cwv = 0, csa = 0;  // int8 stage 0 read, bf16 stage 0 writes, scales
   if constexpr (I8) {
     const int cc = threadIdx.x % CH, crow = threadIdx.x / CH;
-    if constexpr (!CODES) {
+    if constexpr (!FOLD) {
       for (int i = threadIdx.x; i < 2 * D; i += 256) {  // before any DMA; the prologue's barrier publishes it
         const bool v = i >= D;
         const int ch = i % D;
@@ -2468,7 +2433,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     const int RO = stage8_iofs(s8_t), WO = stage_iofs(sb_t);
     u32x2 kw[NPT], vw[NPT];
     f32x4 sk[2], sv[2];  // !FOLD: the chunk's 8 K and 8 V scales
-    if constexpr (!CODES && NPT == 2) {
+    if constexpr (!FOLD && NPT == 2) {
       asm volatile(
           "ds_read_b64 %0, %8 offset:%c10\n"
           "ds_read_b64 %1, %8 offset:%c11\n"
@@ -2484,7 +2449,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
           : "v"(ra), "v"(csa), "i"(RO), "i"(RO + CR * D), "i"(RO + TILE8B), "i"(RO + TILE8B + CR * D), "i"(2 * D),
             "i"(4 * D), "i"(6 * D)
           : "memory");
-    } else if constexpr (!CODES) {
+    } else if constexpr (!FOLD) {
       static_assert(NPT == 1, "rows per thread");
       asm volatile(
           "ds_read_b64 %0, %6 offset:%c8\n"
@@ -2520,7 +2485,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
     for (int i = 0; i < NPT; ++i) {
       u32x4 kb, vb;
-      if constexpr (CODES) {
+      if constexpr (FOLD) {
         kb = cv8(kw[i].x, kw[i].y);
         vb = cv8(vw[i].x, vw[i].y);
       } else {
@@ -2551,8 +2516,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // ---- per tile: scores (QK) and each row's largest, masked for the keys past a row's limit ----
   f32x4 sc[RB][2];
   float lmax[RB], top[RB];
-  // what turns a score of half b into the exponent: factor kf, addend lv = log2(V scale); iv = 1 / V scale
-  float kf[2] = {a.sm_log2, a.sm_log2}, lv[2] = {0.f, 0.f}, iv[2] = {1.f, 1.f};
   // K operand reads from inline assembly, each statement waiting for its own reads: as plain loads
   // the compiler makes them wait for every LDS DMA in flight (it cannot tell they read another ring
   // stage), which would empty the ring every tile
@@ -2596,18 +2559,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
                                                              0, 0, 0);
     }
     pr_prio<0>();
-    if constexpr (BLK) {
-      f32x4 s4;
-      asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(s4) : "v"(sadr + (c & 3) * 4 * WAVE * 4) : "memory");
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float k = __builtin_fmaxf(s4[2 * b], MIN_BLOCK_SCALE), v = __builtin_fmaxf(s4[2 * b + 1], MIN_BLOCK_SCALE);
-        auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
-        kf[b] = uniform(k * a.sm_log2);
-        lv[b] = uniform(__builtin_amdgcn_logf(v));
-        iv[b] = uniform(__builtin_amdgcn_rcpf(v));
-      }
-    }
     if (decltype(mask_t)::value && n0 + PR_KEYS > lim_lo) {  // a tile on the causal edge of some row
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
@@ -2616,18 +2567,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (n0 + 16 * b + 4 * g + i >= lim[rb]) sc[rb][b][i] = -INFINITY;
-    }
-    if constexpr (BLK) {   // (log2 units)
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float h[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          h[b] = __builtin_fmaf(__builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]),
-                                                __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])), kf[b], lv[b]);
-        lmax[rb] = __builtin_fmaxf(h[0], h[1]);
-      }
-      return;
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)  // this lane's largest score of the row in the tile (raw units)
@@ -2638,7 +2577,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // the row's largest score of the tile, log2 units (the 4 lanes of a row agree)
   auto row_top = [&]() {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) top[rb] = BLK ? group4_fmax(lmax[rb]) : group4_fmax(lmax[rb]) * a.sm_log2;
+    for (int rb = 0; rb < RB; ++rb) top[rb] = group4_fmax(lmax[rb]) * a.sm_log2;
   };
   // m is a reference maximum (log2 units) raised only when a score exceeds it by more than PR_SLACK:
   // P = 2^(s c - m) <= 2^PR_SLACK (exact in fp32, in range for bf16), so acc / l are rescaled in a few
@@ -2668,17 +2607,13 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     for (int rb = 0; rb < RB; ++rb) {
       float p[2][4], psum = 0.f;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if constexpr (BLK) psum = 0.f;
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if constexpr (BLK) p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], kf[b], lv[b] - m[rb]));
-          else p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], a.sm_log2, -m[rb]));
+          p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], a.sm_log2, -m[rb]));
           psum += p[b][i];
         }
-        if constexpr (BLK) l[rb] = __builtin_fmaf(psum, iv[b], l[rb]);
-      }
-      if constexpr (!BLK) l[rb] += psum;
+      l[rb] += psum;
       u32x4 pw;
       pw.x = pack_bf16x2_rne(p[0][0], p[0][1]);
       pw.y = pack_bf16x2_rne(p[0][2], p[0][3]);
@@ -2738,7 +2673,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       if constexpr (I8) {
 #pragma unroll
         for (int j = 0; j < NS8; ++j) issue(c_lo + j, j, linear);
-        wait_vm<VMT * (NS8 - 1)>();
+        wait_vm<IPW8 * (NS8 - 1)>();
         lds_barrier();
         convert(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
       } else {
@@ -2750,7 +2685,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     int scur = 0, snext = NS - 1, s8 = 0;
     auto next_tile = [&](int c, auto lin_t, auto mask_t) {
       if constexpr (I8) {
-        wait_vm<VMT * (NS8 - 2)>();  // this wavefront's share of tile c + 1 has landed
+        wait_vm<IPW8 * (NS8 - 2)>();  // this wavefront's share of tile c + 1 has landed
         lds_barrier();                // everyone's has, tile c is converted, and the other bf16 stage
                                       // (tile c - 1) and tile c's int8 stage are free again
         issue(c + NS8, s8, lin_t);
@@ -2766,7 +2701,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     auto next_tile_ct = [&](int c, auto st_t, auto lin_t) {
       constexpr int ST = decltype(st_t)::value;
       if constexpr (I8) {
-        wait_vm<VMT * (NS8 - 2)>();
+        wait_vm<IPW8 * (NS8 - 2)>();
         lds_barrier();
         issue(c + NS8, NS8 == 2 ? ST : s8, lin_t);
       } else {
@@ -2848,17 +2783,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     wait_vm<0>();
     bool jump = false;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      jump |= !(l[rb] <= PR_FAST_PSUM_MAX);
-      if constexpr (BLK) {   // (l is a sum of P over V scales: large ones leave P room to overflow the accumulators)
-        float z = 0.f;
-#pragma unroll
-        for (int tt = 0; tt < VT; ++tt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[rb][tt][i], 0.f, z);
-        jump |= z != 0.f;
-      }
-    }
+    for (int rb = 0; rb < RB; ++rb) jump |= !(l[rb] <= PR_FAST_PSUM_MAX);
     // Rare: a score far above its row's first tile somewhere in the workgroup -- redo the workgroup's
     // tiles with a reference maximum raised (and acc / l rescaled) whenever a score exceeds it by
     // 2^PR_SLACK.
