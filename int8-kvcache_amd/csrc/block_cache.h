@@ -684,6 +684,12 @@ __global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args
   });
 }
 
+// The bf16 prefill over a temporary cache of the codes (kvq_block_codes), the scales from the cache itself.
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256, 3) void block_codes_prefill_kernel(PrefillArgs a) {
+  prefill_body<D, PR_SRC_BF16_BLOCK, SPLIT>(a);
+}
+
 struct BlockPrefillArgs {
   PrefillArgs p;
   BlockScales s;
@@ -948,7 +954,8 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
                                 int64_t bt_stride, int64_t num_q_heads, const int32_t* tile_req, const int32_t* tile_row,
                                 int64_t num_tiles, int64_t rows_per_tile, double softmax_scale, const int32_t* tile_piece,
                                 const int32_t* tile_slot, const int32_t* merge, int64_t num_merge, float* part_out,
-                                float* part_ml, void* stream) {
+                                float* part_ml, const void* k_codes, const void* v_codes, int64_t num_pages,
+                                const int32_t* codes_table, int64_t ct_stride, void* stream) {
   const char* nm = "block_prefill_attention";
   if (num_tiles < 0 || num_tiles > INT32_MAX || num_merge < 0 || num_merge > INT32_MAX) return fail("%s: bad sizes", nm);
   if (num_tiles == 0) { g_err.clear(); return KVQ_OK; }
@@ -962,6 +969,10 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
                                      seq_lens, block_table, num_q_heads)) return rc;
   if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
     return fail("%s: page too large for 32-bit lane offsets", nm);
+  if (k_codes && (!v_codes || !codes_table || num_pages <= 0 || num_pages > INT32_MAX || !aligned16(k_codes) || !aligned16(v_codes)))
+    return fail("%s: bad temporary cache", nm);
+  if (k_codes && 2 * block_size * num_kv_heads * head_dim > INT32_MAX)
+    return fail("%s: page too large for 32-bit page / slot offsets", nm);
   BlockPrefillArgs b;
   b.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
   PrefillArgs& a = b.p;
@@ -973,11 +984,26 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
   a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
   a.G = (int)(num_q_heads / num_kv_heads); a.lbs = log2i(block_size); a.num_blocks = (int)num_blocks;
   a.kpage = a.vpage = a.krow = a.vrow = 0; a.contig = 0; a.ks = a.vs = nullptr; a.ks_pc = a.vs_pc = 0;   // (prefill_body's)
+  a.bs = b.s; a.s_table = block_table; a.s_bt_stride = bt_stride; a.s_blocks = (int)num_blocks;
+  if (k_codes) {   // the temporary cache's pages instead: bf16 [num_pages, block_size, H, D], contiguous
+    a.kc = (const uint16_t*)k_codes; a.vc = (const uint16_t*)v_codes;
+    a.block_table = codes_table; a.bt_stride = ct_stride; a.num_blocks = (int)num_pages;
+    a.k_sh = a.v_sh = head_dim;
+    a.k_sn = a.v_sn = num_kv_heads * head_dim;
+    a.k_sb = a.v_sb = block_size * a.k_sn;
+    a.krow = a.vrow = (uint32_t)(2 * a.k_sn);
+    a.kpage = a.vpage = (uint32_t)(2 * a.k_sb);
+    a.contig = 1;
+  }
   const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   void (*kern)(BlockPrefillArgs) = head_dim == 128 ? (tile_piece ? block_prefill_kernel<128, true> : block_prefill_kernel<128, false>)
                                               : (tile_piece ? block_prefill_kernel<64, true> : block_prefill_kernel<64, false>);
-  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, b);
+  void (*codes_kern)(PrefillArgs) = head_dim == 128
+      ? (tile_piece ? block_codes_prefill_kernel<128, true> : block_codes_prefill_kernel<128, false>)
+      : (tile_piece ? block_codes_prefill_kernel<64, true> : block_codes_prefill_kernel<64, false>);
+  if (k_codes) hipLaunchKernelGGL(codes_kern, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, b);
   const int rc = launched(nm);
   if (rc != KVQ_OK || !tile_piece || num_merge == 0) return rc;
   const dim3 mgrid((unsigned)num_merge, (unsigned)num_kv_heads, PR_ROWS / PR_MERGE_WAVES);
@@ -985,6 +1011,22 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
   if (head_dim == 128) hipLaunchKernelGGL(prefill_merge_kernel<128>, mgrid, dim3(WAVE * PR_MERGE_WAVES), 0, st, a, ml);
   else hipLaunchKernelGGL(prefill_merge_kernel<64>, mgrid, dim3(WAVE * PR_MERGE_WAVES), 0, st, a, ml);
   return launched("block_prefill_attention: merge");
+}
+
+int kvq_block_codes(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb,
+                    int64_t v_sn, int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim,
+                    void* k_out, void* v_out, const int32_t* block_table, int64_t bt_stride, const int32_t* src_req,
+                    const int32_t* src_j, int64_t num_pages, void* stream) {
+  const char* nm = "block_codes";
+  if (num_pages < 0 || num_pages > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (num_pages == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_blocks(nm, num_blocks, block_size, BLK_MIN, num_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache,
+                                  v_sb, v_sn, v_sh)) return rc;
+  if (!k_out || !v_out || !block_table || !src_req || !src_j) return fail("%s: null pointer", nm);
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  return dequant_launch<true>(nm, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size, num_heads,
+                              head_dim, k_out, v_out, block_table, bt_stride, src_req, src_j, num_pages, nullptr, 0, nullptr, 0,
+                              stream);
 }
 
 }  // extern "C"

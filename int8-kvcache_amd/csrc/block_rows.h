@@ -16,17 +16,7 @@
 // (prefill_body's scheme).
 namespace {
 
-constexpr float MIN_BLOCK_SCALE = 1e-30f;   // a block's scale counts as at least this (the V scale's logarithm and
-                                            // reciprocal are taken; a K scale of 0 times a masked score is no number)
 constexpr float Q16_MAX = 16256.f;   // 127 * 128: the hi plane of rint(q / sq) stays an int8
-
-// Where the scales lie: that of (page p, head h, block b) at p * sb + h * sh + b * sg floats of ks / vs.
-struct BlockScales {
-  const float* ks;
-  const float* vs;
-  int64_t sb, sh, sg;
-  int lg;   // log2 of the positions per scale
-};
 
 // Bytes e .. e + 3 (e = 4 w) of q as two int8 planes: v = rint(x * inv), v = 128 hi + lo
 __device__ __forceinline__ void q_planes4(float x0, float x1, float x2, float x3, float inv, int& hi_out, int& lo_out) {

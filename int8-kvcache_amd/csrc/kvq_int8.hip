@@ -43,6 +43,17 @@
 
 namespace {
 
+// The scales of a block-scaled cache (block_cache.h): that of (page p, head h, block b) at p * sb + h * sh + b * sg
+// floats of ks / vs.
+struct BlockScales {
+  const float* ks;
+  const float* vs;
+  int64_t sb, sh, sg;
+  int lg;   // log2 of the positions per scale
+};
+constexpr float MIN_BLOCK_SCALE = 1e-30f;   // a block's scale counts as at least this (the V scale's logarithm and
+                                            // reciprocal are taken; a K scale of 0 times a masked score is no number)
+
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -1997,7 +2008,8 @@ constexpr int DQ_BATCH = 16;
 // tokens of 498, 32 / 8 heads, blocks of 64 slots 30.4 -> 22.7 us, 157 of 157, 16 / 16 heads d64 19.8 -> 11.7, 1,024 of
 // 1,024 in blocks of 32 34.6 -> 33.3; 512 pages of 16 slots unchanged; slices of 16 tokens 23.8 and 12.7).
 constexpr int DQ_WG_PER_CU = 4, DQ_MIN_TOKENS = 4;
-template <int D>
+// CODES: the codes themselves as bf16 (exact), no scales (a block-scaled cache's, kvq_block_codes).
+template <int D, bool CODES = false>
 __global__ __launch_bounds__(256) void dequant_pages_kernel(
     const int8_t* __restrict__ kc, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* __restrict__ vc,
     int64_t v_sb, int64_t v_sn, int64_t v_sh, int num_blocks, int bs, int H, int heads_per_block,
@@ -2023,7 +2035,8 @@ __global__ __launch_bounds__(256) void dequant_pages_kernel(
   if (src < 0 || src >= num_blocks) src = 0;
   float sc[8];
   const float* sp = kv ? vs : ks;
-  if (kv ? vs_pc : ks_pc) {
+  if constexpr (CODES) {
+  } else if (kv ? vs_pc : ks_pc) {
     const float4 f0 = *reinterpret_cast<const float4*>(sp + h * D + d0);
     const float4 f1 = *reinterpret_cast<const float4*>(sp + h * D + d0 + 4);
     sc[0] = f0.x; sc[1] = f0.y; sc[2] = f0.z; sc[3] = f0.w; sc[4] = f1.x; sc[5] = f1.y; sc[6] = f1.z; sc[7] = f1.w;
@@ -2046,7 +2059,10 @@ __global__ __launch_bounds__(256) void dequant_pages_kernel(
     for (int i = 0; i < DQ_BATCH; ++i) {
       const int t = tb + i * tpc;
       if (t >= z1) break;
-      __builtin_nontemporal_store(dq8x(w[i].x, w[i].y, sc), reinterpret_cast<u32x4*>(obase + (int64_t)t * H * D));
+      u32x4 o;
+      if constexpr (CODES) o = cv8(w[i].x, w[i].y);
+      else o = dq8x(w[i].x, w[i].y, sc);
+      __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(obase + (int64_t)t * H * D));
     }
   }
 }
@@ -2104,6 +2120,11 @@ struct PrefillArgs {
   const float* ks;
   const float* vs;
   int ks_pc, vs_pc;
+  // PR_SRC_BF16_BLOCK: the codes' scales, by the pages of the cache that they were copied from
+  BlockScales bs;
+  const int* s_table;    // that cache's block table
+  int64_t s_bt_stride;
+  int s_blocks;          // its pages
 };
 
 constexpr int PR_RB = 2;                    // 16-row blocks per wavefront
@@ -2141,11 +2162,14 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rne(float a, float b) {
 // Where the K / V tiles come from: the bf16 temporary cache, or the INT8 pages themselves
 // (prefill_i8_kernel below), converted tile by tile either as dequant_pages converts them (bf16 of
 // code x scale) or as exact bf16 codes with the scales folded into q (K) and the output (V).
-constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2;
+// PR_SRC_BF16_BLOCK: a bf16 temporary cache of a block-scaled cache's codes, each 16-key half tile's K scale a factor of
+// its scores and its V scale an addend in the exponent (block_cache.h).
+constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2, PR_SRC_BF16_BLOCK = 3;
 
 template <int D, int SRC, bool SPLIT>
 __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
-  constexpr bool I8 = SRC != PR_SRC_BF16;
+  constexpr bool BLK = SRC == PR_SRC_BF16_BLOCK;
+  constexpr bool I8 = SRC != PR_SRC_BF16 && !BLK;
   constexpr bool FOLD = SRC == PR_SRC_I8_FOLD;
   constexpr int DS = D / 32;                // 32-channel chunks of the QK contraction
   constexpr int VT = D / 16;                // PV channel tiles
@@ -2172,6 +2196,10 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   static_assert(NS8 >= 2 && IPW8 * 4 == 2 * PPM && RPI8 <= 16, "int8 ring");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[NB][2][TILEB];
   __shared__ __attribute__((aligned(1024))) uint8_t ring8[I8 ? NS8 : 1][2][I8 ? TILE8B : 16];
+  // BLK: the scales of the last four tiles. A wavefront's DMA rows lie in one 16-key half (wavefronts 0 and 1: the first),
+  // whose K and V scale it brings too, at floats 0 and 1 of its row (lanes even and odd; the others repeat them)
+  static_assert(4 * RPI * IPW == PR_KEYS && 2 * RPI * IPW == 16, "two wavefronts to a half tile");
+  __shared__ __attribute__((aligned(16))) float sring[BLK ? 4 : 1][4][BLK ? WAVE : 4];
 
   const int kvh = blockIdx.y;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -2295,6 +2323,19 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     }
     linear = !__any(bad) && run_fits(pg_hi + 1, a.kpage) && run_fits(pg_hi + 1, a.vpage);
   }
+  // BLK: this wavefront's half tile's page in the cache of the codes, read a tile before its use (a half past the last key
+  // takes the last key's block: its own may never have been written)
+  const int* sbt = nullptr;
+  const float* sbase = nullptr;
+  int sid = 0;
+  auto skey = [&](int c) { return min(min(c, c_hi - 1) * PR_KEYS + 16 * (wave >> 1), kend - 1); };
+  auto next_sid = [&](int c) {
+    if constexpr (BLK) sid = ((const __attribute__((address_space(4))) int*)sbt)[skey(c) >> a.lbs];
+  };
+  if constexpr (BLK) {
+    sbt = a.s_table + (int64_t)r * a.s_bt_stride;
+    sbase = ((lane & 1) ? a.bs.vs : a.bs.ks) + (int64_t)kvh * a.bs.sh;
+  }
   const char* klin = kh + (int64_t)pfirst * a.kpage;
   const char* vlin = vh + (int64_t)pfirst * a.vpage;
   // tile c: keys 0..15 sit in page p0 from slot (32 c) mod bs on, keys 16..31 right after them
@@ -2302,6 +2343,14 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // lin_t: std::true_type = the pages are one run (no block-table read), false_type = read the
   // table, bool = decide at run time
   auto issue = [&](int c, int st, auto lin_t) {
+    if constexpr (BLK) {
+      int p = __builtin_amdgcn_readfirstlane(sid);
+      p = p >= 0 && p < a.s_blocks ? p : 0;
+      const float* sp = sbase + ((int64_t)p * a.bs.sb + (int64_t)((skey(c) & bsm) >> a.bs.lg) * a.bs.sg);
+      __builtin_amdgcn_global_load_lds((const void*)sp,
+                                       (__attribute__((address_space(3))) void*)(&sring[min(c, c_hi - 1) & 3][wave][0]), 4, 0, 0);
+      next_sid(c + 1);
+    }
     c = min(c, c_hi - 1);  // past the end: reload the last tile into the free stage
     const int kb0 = c * PR_KEYS, klast = max(kend - 1, 0);
     const char* kb[2];
@@ -2516,6 +2565,9 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // ---- per tile: scores (QK) and each row's largest, masked for the keys past a row's limit ----
   f32x4 sc[RB][2];
   float lmax[RB], top[RB];
+  // BLK: what turns a score of half b into the exponent: factor kf, addend lv = log2(V scale); iv = 1 / V scale
+  float kf[2], lv[2], iv[2];
+  const uint32_t sadr = (uint32_t)(uintptr_t)(&sring[0][0][0]);
   // K operand reads from inline assembly, each statement waiting for its own reads: as plain loads
   // the compiler makes them wait for every LDS DMA in flight (it cannot tell they read another ring
   // stage), which would empty the ring every tile
@@ -2559,6 +2611,19 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
                                                              0, 0, 0);
     }
     pr_prio<0>();
+    if constexpr (BLK) {
+      u32x2 s2[2];
+      asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:%c3\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(s2[0]), "=&v"(s2[1]) : "v"(sadr + (c & 3) * (4 * WAVE * 4)), "i"(2 * WAVE * 4) : "memory");
+      auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float v = __builtin_fmaxf(__uint_as_float(s2[b].y), MIN_BLOCK_SCALE);
+        kf[b] = uniform(__builtin_fmaxf(__uint_as_float(s2[b].x), MIN_BLOCK_SCALE) * a.sm_log2);
+        lv[b] = uniform(__builtin_amdgcn_logf(v));
+        iv[b] = uniform(__builtin_amdgcn_rcpf(v));
+      }
+    }
     if (decltype(mask_t)::value && n0 + PR_KEYS > lim_lo) {  // a tile on the causal edge of some row
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
@@ -2567,6 +2632,18 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (n0 + 16 * b + 4 * g + i >= lim[rb]) sc[rb][b][i] = -INFINITY;
+    }
+    if constexpr (BLK) {   // (in log2 units)
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float h[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          h[b] = __builtin_fmaf(__builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]),
+                                                __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])), kf[b], lv[b]);
+        lmax[rb] = __builtin_fmaxf(h[0], h[1]);
+      }
+      return;
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)  // this lane's largest score of the row in the tile (raw units)
@@ -2577,7 +2654,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // the row's largest score of the tile, log2 units (the 4 lanes of a row agree)
   auto row_top = [&]() {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) top[rb] = group4_fmax(lmax[rb]) * a.sm_log2;
+    for (int rb = 0; rb < RB; ++rb) top[rb] = group4_fmax(lmax[rb]) * (BLK ? 1.f : a.sm_log2);
   };
   // m is a reference maximum (log2 units) raised only when a score exceeds it by more than PR_SLACK:
   // P = 2^(s c - m) <= 2^PR_SLACK (exact in fp32, in range for bf16), so acc / l are rescaled in a few
@@ -2606,14 +2683,28 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       float p[2][4], psum = 0.f;
+      if constexpr (BLK) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b) {
+          const float e0 = lv[b] - m[rb];
+          float half = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], a.sm_log2, -m[rb]));
-          psum += p[b][i];
+          for (int i = 0; i < 4; ++i) {
+            p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], kf[b], e0));
+            half += p[b][i];
+          }
+          l[rb] = __builtin_fmaf(half, iv[b], l[rb]);
         }
-      l[rb] += psum;
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], a.sm_log2, -m[rb]));
+            psum += p[b][i];
+          }
+        l[rb] += psum;
+      }
       u32x4 pw;
       pw.x = pack_bf16x2_rne(p[0][0], p[0][1]);
       pw.y = pack_bf16x2_rne(p[0][2], p[0][3]);
@@ -2670,6 +2761,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     // its int8 stage (c % NS8), tiles counted from c_lo.
     // the first tiles' DMA; I8: NS8 tiles in flight, tile 0 converted once it has landed
     auto prologue = [&]() {
+      next_sid(c_lo);
       if constexpr (I8) {
 #pragma unroll
         for (int j = 0; j < NS8; ++j) issue(c_lo + j, j, linear);
@@ -2690,7 +2782,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
                                       // (tile c - 1) and tile c's int8 stage are free again
         issue(c + NS8, s8, lin_t);
       } else {
-        wait_vm<2 * IPW * (NS - 2)>();  // this wavefront's share of tile c has landed
+        wait_vm<(2 * IPW + (BLK ? 1 : 0)) * (NS - 2)>();  // this wavefront's share of tile c has landed
         lds_barrier();                  // everyone's share has; stage (c - 1) % NS is free again
         issue(c + NS - 1, snext, lin_t);
       }
@@ -2705,7 +2797,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
         lds_barrier();
         issue(c + NS8, NS8 == 2 ? ST : s8, lin_t);
       } else {
-        wait_vm<2 * IPW * (NS - 2)>();
+        wait_vm<(2 * IPW + (BLK ? 1 : 0)) * (NS - 2)>();
         lds_barrier();
         issue(c + NS - 1, (ST + NS - 1) % NS, lin_t);
       }
@@ -2783,7 +2875,17 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     wait_vm<0>();
     bool jump = false;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) jump |= !(l[rb] <= PR_FAST_PSUM_MAX);
+    for (int rb = 0; rb < RB; ++rb) {
+      jump |= !(l[rb] <= PR_FAST_PSUM_MAX);
+      if constexpr (BLK) {   // (l is a sum of P over V scales: those above 1 leave P room to overflow the accumulators)
+        float z = 0.f;
+#pragma unroll
+        for (int tt = 0; tt < VT; ++tt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[rb][tt][i], 0.f, z);
+        jump |= z != 0.f;
+      }
+    }
     // Rare: a score far above its row's first tile somewhere in the workgroup -- redo the workgroup's
     // tiles with a reference maximum raised (and acc / l rescaled) whenever a score exceeds it by
     // 2^PR_SLACK.
@@ -3761,6 +3863,41 @@ int decode_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_
 
 }  // namespace
 
+namespace {
+
+// dequant_pages_kernel over num_pages pages (CODES: without scales).
+template <bool CODES>
+int dequant_launch(const char* nm, const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache,
+                   int64_t v_sb, int64_t v_sn, int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                   int64_t head_dim, void* k_out, void* v_out, const int32_t* block_table, int64_t bt_stride,
+                   const int32_t* src_req, const int32_t* src_j, int64_t num_pages, const float* k_scale, int64_t k_scale_cols,
+                   const float* v_scale, int64_t v_scale_cols, void* stream) {
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  // heads per workgroup: as many as 256 threads' worth of (head, K|V, chunk) combinations; threads: the
+  // largest multiple of those combinations up to 256
+  const int cph = 2 * (int)head_dim / 8;
+  const int hpb = (int)std::min<int64_t>(num_heads, 256 / cph);
+  const int combos = hpb * cph;
+  const int threads = (256 / combos) * combos;
+  // few pages: each page's tokens over several workgroups
+  const int64_t groups = (num_heads + hpb - 1) / hpb;
+  const int64_t want = std::max<int64_t>(1, (int64_t)device_cus() * DQ_WG_PER_CU / (num_pages * groups));
+  const int64_t tokens = std::max<int64_t>(std::min<int64_t>(DQ_MIN_TOKENS, block_size), (block_size + want - 1) / want);
+  const int64_t slices = (block_size + tokens - 1) / tokens;
+  const dim3 grid((unsigned)num_pages, (unsigned)groups, (unsigned)slices);
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, dim3(threads), 0, st, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh,
+                       (int)num_blocks, (int)block_size, (int)num_heads, hpb, (int)tokens, (uint16_t*)k_out, (uint16_t*)v_out,
+                       block_table, bt_stride, src_req, src_j, k_scale, (int)(k_scale_cols > 1), v_scale,
+                       (int)(v_scale_cols > 1));
+  };
+  if (head_dim == 128) go(dequant_pages_kernel<128, CODES>);
+  else go(dequant_pages_kernel<64, CODES>);
+  return launched(nm);
+}
+
+}  // namespace
+
 extern "C" {
 
 int kvq_dequant_pages(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache,
@@ -3781,28 +3918,9 @@ int kvq_dequant_pages(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t
     return fail("dequant_pages: per-channel scale tables must be 16-byte aligned");
   if (num_pages > INT32_MAX || num_blocks > INT32_MAX) return fail("dequant_pages: too many pages");
   if (num_heads > 65535 * 4) return fail("dequant_pages: too many heads");
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  // heads per workgroup: as many as 256 threads' worth of (head, K|V, chunk) combinations; threads: the
-  // largest multiple of those combinations up to 256
-  const int cph = 2 * (int)head_dim / 8;
-  const int hpb = (int)std::min<int64_t>(num_heads, 256 / cph);
-  const int combos = hpb * cph;
-  const int threads = (256 / combos) * combos;
-  // few pages: each page's tokens over several workgroups
-  const int64_t groups = (num_heads + hpb - 1) / hpb;
-  const int64_t want = std::max<int64_t>(1, (int64_t)device_cus() * DQ_WG_PER_CU / (num_pages * groups));
-  const int64_t tokens = std::max<int64_t>(std::min<int64_t>(DQ_MIN_TOKENS, block_size), (block_size + want - 1) / want);
-  const int64_t slices = (block_size + tokens - 1) / tokens;
-  const dim3 grid((unsigned)num_pages, (unsigned)groups, (unsigned)slices);
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(threads), 0, st, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh,
-                       (int)num_blocks, (int)block_size, (int)num_heads, hpb, (int)tokens, (uint16_t*)k_out, (uint16_t*)v_out,
-                       block_table, bt_stride, src_req, src_j, k_scale, (int)(k_scale_cols > 1), v_scale,
-                       (int)(v_scale_cols > 1));
-  };
-  if (head_dim == 128) go(dequant_pages_kernel<128>);
-  else go(dequant_pages_kernel<64>);
-  return launched("dequant_pages");
+  return dequant_launch<false>("dequant_pages", k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
+                               num_heads, head_dim, k_out, v_out, block_table, bt_stride, src_req, src_j, num_pages, k_scale,
+                               k_scale_cols, v_scale, v_scale_cols, stream);
 }
 
 }  // extern "C"

@@ -45,6 +45,7 @@ decltype(&kvq_quant_block_cache) p_quant_block;
 decltype(&kvq_read_block_cache) p_read_block;
 decltype(&kvq_block_decode_attention) p_block_decode;
 decltype(&kvq_block_prefill_attention) p_block_prefill;
+decltype(&kvq_block_codes) p_block_codes;
 
 // A tensor argument this file may read: exactly torch.Tensor (or Parameter), dense GPU memory, no wrapper
 // (functorch, functionalization, fake or subclass tensors go to the Python path).
@@ -432,10 +433,11 @@ PyObject* block_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// (..., rows_per_tile, tile_req, tile_row, tile_piece | None, tile_slot | None, merge | None, slots)
+// (..., rows_per_tile, tile_req, tile_row, tile_piece | None, tile_slot | None, merge | None, slots,
+//  src_req | None, src_j | None, temporary block table | None): the last three copy the pages' codes as bf16 first
 PyObject* block_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> long {
-    if (n != 17 || !p_block_prefill) return DECLINED;
+    if (n != 20 || !p_block_prefill || !p_block_codes) return DECLINED;
     BlockAttn x;
     int64_t rows, slots;
     if (!x.read(a) || !as_int(a[10], rows) || !as_int(a[16], slots)) return DECLINED;
@@ -462,10 +464,31 @@ PyObject* block_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const BlockCache& c = x.c;
     auto* btp = (const int32_t*)x.bt->data_ptr();
     auto *rp = (const int32_t*)treq->data_ptr(), *wp = (const int32_t*)trow->data_ptr();
-    return launch("kvq_block_prefill_attention", [&] {
+    const int32_t *rqp = nullptr, *jp = nullptr, *tbp = nullptr;
+    int64_t P = 0, tbs = 0;
+    at::Tensor kt, vt;
+    if (a[17] != Py_None) {
+      const at::Tensor *sreq = tensor(a[17]), *sj = tensor(a[18]), *tbt = tensor(a[19]);
+      if (!sreq || !sj || !tbt || !index_vector(*sreq) || !index_vector(*sj) || sreq->size(0) == 0 ||
+          sj->size(0) != sreq->size(0) || !table(*tbt, 0) || !one_device(*x.q, *sreq, *sj, *tbt))
+        return DECLINED;
+      P = sreq->size(0), tbs = tbt->stride(0);
+      rqp = (const int32_t*)sreq->data_ptr(), jp = (const int32_t*)sj->data_ptr(), tbp = (const int32_t*)tbt->data_ptr();
+      kt = at::empty({P, c.bs, c.H, c.D}, x.q->options());
+      vt = at::empty({P, c.bs, c.H, c.D}, x.q->options());
+    }
+    void *ktp = P ? kt.data_ptr() : nullptr, *vtp = P ? vt.data_ptr() : nullptr;
+    return launch(P ? "kvq_block_codes" : "kvq_block_prefill_attention", [&] {
+      if (P) {
+        const int rc = p_block_codes(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, ktp, vtp, btp,
+                                     x.bt->stride(0), rqp, jp, P, x.st);
+        if (rc) return rc;
+        entry = "kvq_block_prefill_attention";
+      }
       return p_block_prefill(x.qp, x.q->stride(0), x.q->stride(1), c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs,
                              c.H, c.D, c.ks, c.vs, c.sb, c.sh, c.sg, c.group, x.op, x.out->stride(0), x.out->stride(1), x.cu,
-                             x.sl, btp, x.bt->stride(0), x.Hq, rp, wp, tiles, rows, x.scale, pp, sp, mp, nm, pop, pmp, x.st);
+                             x.sl, btp, x.bt->stride(0), x.Hq, rp, wp, tiles, rows, x.scale, pp, sp, mp, nm, pop, pmp, ktp,
+                             vtp, P, tbp, tbs, x.st);
     });
   });
 }
@@ -489,6 +512,7 @@ PyObject* bind(PyObject*, PyObject* d) {
   p_read_block = (decltype(p_read_block))at_name("kvq_read_block_cache");
   p_block_decode = (decltype(p_block_decode))at_name("kvq_block_decode_attention");
   p_block_prefill = (decltype(p_block_prefill))at_name("kvq_block_prefill_attention");
+  p_block_codes = (decltype(p_block_codes))at_name("kvq_block_codes");
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }

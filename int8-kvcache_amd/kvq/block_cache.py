@@ -180,26 +180,38 @@ def block_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, blo
 
 def block_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, plan, softmax_scale, scales):
     """Attention over a block-scaled cache for the plan's long requests (cuda_kernels.plan_long; the others' rows are left
-    as they were), read straight from the pages: the formula of block_decode_attention on bf16 operands, the
-    codes exact, their scales applied in fp32, the softmax's weights rounded to bf16."""
+    as they were): the formula of block_decode_attention on bf16 operands, the codes exact, their scales applied in fp32, the
+    softmax's weights rounded to bf16. KVQ_PREFILL_DIRECT as long_attention's: 1 (or fold) reads the int8 pages
+    themselves, 0 a temporary bf16 cache of the plan's pages' codes; unset: whichever is faster (cuda_kernels.direct_pays)."""
     name, e = "block_long_attention", ck.ext()
     bs, h, d = k_cache.shape[1:]
     _check(bs == plan.block_size, f"block size {bs} != plan block size {plan.block_size}")
     work = plan.work(q.shape[1] // h, h, d, q.device)
+    direct = os.environ.get("KVQ_PREFILL_DIRECT")
+    _check(direct in (None, "0", "1", "fold"), f"KVQ_PREFILL_DIRECT must be 0, 1 or fold, got {direct!r}")
+    src = plan.gpu(q.device) if direct == "0" or direct is None and not work.direct else (None, None, None)
     if ck._served(e, name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
                   scales["v_scale"], softmax_scale, e.prefill_rows, work.tile_req, work.tile_row, work.tile_piece,
-                  work.tile_slot, work.merge, work.slots):
+                  work.tile_slot, work.merge, work.slots, *src):
         return out
     k, v, geom, sc = _cache_args(name, k_cache, v_cache, scales)
     _check_attention(name, q, k_cache, out, cu_seqlens_q, seq_lens, block_table)
     _check_cuda(name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"], scales["v_scale"])
     n = work.tile_req.shape[0]
     split = work.split(h, e.prefill_rows, d)
+    codes = (None, None, 0, None, 0)
+    if src[0] is not None:
+        src_req, src_j, bt_tmp = src
+        kt = torch.empty((src_req.shape[0], bs, h, d), dtype=q.dtype, device=q.device)
+        vt = torch.empty_like(kt)
+        _call("kvq_block_codes", q.device, *k, *v, *geom, kt.data_ptr(), vt.data_ptr(), block_table.data_ptr(),
+              block_table.stride(0), src_req.data_ptr(), src_j.data_ptr(), src_req.shape[0])
+        codes = (kt.data_ptr(), vt.data_ptr(), kt.shape[0], bt_tmp.data_ptr(), bt_tmp.stride(0))
     _call("kvq_block_prefill_attention", q.device, q.data_ptr(), q.stride(0), q.stride(1), *k, *v, *geom, *sc,
           out.data_ptr(), out.stride(0), out.stride(1), cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
           block_table.data_ptr(), block_table.stride(0), q.shape[1], work.tile_req.data_ptr(), work.tile_row.data_ptr(),
           n, e.prefill_rows, float(softmax_scale),
-          *((None, None, None, 0, None, None) if split is None else e._split_args(split, n, h, d)))
+          *((None, None, None, 0, None, None) if split is None else e._split_args(split, n, h, d)), *codes)
     return out
 
 

@@ -38,6 +38,13 @@ def page_table(lens, bs, seed, spare=3):
     return t, nb
 
 
+@pytest.fixture(params=["0", "1"], ids=["copied", "direct"])
+def source(request, monkeypatch):
+    """What long queries read: a temporary bf16 cache of the codes, or the int8 pages themselves."""
+    monkeypatch.setenv("KVQ_PREFILL_DIRECT", request.param)
+    return request.param
+
+
 class Cache:
     """A cache on the GPU and its plain twin on the host, filled step by step through both."""
 
@@ -238,7 +245,7 @@ def test_split_buffers_of_fewer_rows():
     attend(c, 14, [1, 3, 2], lens, nan_segm(4, 14, 16, 64))
 
 
-def test_scales_that_differ_by_orders_of_magnitude():
+def test_scales_that_differ_by_orders_of_magnitude(source):
     """Blocks whose V (and K) is a million times larger or smaller than their neighbours'."""
     lens = [333, 96, 40]
     table, nb = page_table(lens, 16, 1)
@@ -255,7 +262,7 @@ def test_scales_that_differ_by_orders_of_magnitude():
 
 
 @pytest.mark.parametrize("magnitude", [1e-3, 1.0, 30.0])
-def test_peaked_and_flat_softmax(magnitude):
+def test_peaked_and_flat_softmax(magnitude, source):
     """Scores from nearly equal to hundreds apart (the running maximum jumps by far more than its slack)."""
     lens = [700, 257, 64]
     c = filled(4, 128, 32, 32, lens)
@@ -272,14 +279,14 @@ def test_peaked_and_flat_softmax(magnitude):
 
 @pytest.mark.parametrize("hq,h,d", HEADS)
 @pytest.mark.parametrize("bs,group", [(16, 16), (64, 32)])
-def test_long_queries(hq, h, d, bs, group):
+def test_long_queries(hq, h, d, bs, group, source):
     """Prompts from their start and mid-way, ending anywhere in tiles, pages and row tiles."""
     lens = [9, 40, 129, 333, 700, 64]
     c = filled(h, d, bs, group, lens, layout="vllm" if bs == 16 else "apart")
     attend(c, hq, [9, 10, 129, 57, 300, 64], lens)
 
 
-def test_long_query_few_rows_over_many_keys():
+def test_long_query_few_rows_over_many_keys(source):
     """Rows cut into pieces of keys and merged."""
     lens = [9000, 2000]
     c = filled(4, 128, 16, 16, lens)
@@ -288,7 +295,7 @@ def test_long_query_few_rows_over_many_keys():
     attend(c, 28, [20, 11], lens)
 
 
-def test_mixed_batch():
+def test_mixed_batch(source):
     lens = [1, 100, 0, 5000, 700, 2500]
     c = filled(8, 128, 32, 32, lens)
     q = [1, 1, 1, 1, 700, 333]
@@ -296,7 +303,7 @@ def test_mixed_batch():
     attend(c, 32, q, lens)
 
 
-def test_softmax_scale_and_host_bounds():
+def test_softmax_scale_and_host_bounds(source):
     """Another softmax scale; a plan made from upper bounds of the lengths."""
     lens = [100, 90]
     c = filled(4, 128, 16, 16, lens)
@@ -386,7 +393,7 @@ def test_generation_captured_and_replayed(hq, h, d, bs, group):
         R.check(sb.out, want, bound, i)
 
 
-def test_pages_past_two_and_four_gib():
+def test_pages_past_two_and_four_gib(source):
     """A cache of more than 4 GiB a side: the pages used lie at its ends and around 2 and 4 GiB."""
     h, d, bs = 8, 128, 64
     nb = (4 << 30) // (h * d * bs) + 40
@@ -495,7 +502,8 @@ def test_native_calls_and_the_python_path_agree(change, monkeypatch):
     assert ck.ext().calls is not None, "kvq._torch_calls is not built"
     lens, q_lens = [300, 20, 64, 2000], [1, 20, 8, 300]
     got = []
-    for native in (True, False):
+    for native, direct in ((True, "0"), (False, "0"), (True, "1"), (False, "1")):
+        monkeypatch.setenv("KVQ_PREFILL_DIRECT", direct)
         c = filled(4, 128, 32, 16, lens)
         n = sum(q_lens)
         k, v = rows(n, 4, 128, 50)
@@ -510,6 +518,6 @@ def test_native_calls_and_the_python_path_agree(change, monkeypatch):
             if not native:
                 m.setattr(ck.ext(), "calls", None)
             got.append(_call_all(c, x))
-    (a, ta), (b, tb) = got
-    assert a == b
-    assert all(torch.equal(torch.nan_to_num(s.float()), torch.nan_to_num(t.float())) for s, t in zip(ta, tb))
+    for (a, ta), (b, tb) in zip(got[::2], got[1::2]):
+        assert a == b
+        assert all(torch.equal(torch.nan_to_num(s.float()), torch.nan_to_num(t.float())) for s, t in zip(ta, tb))
