@@ -25,7 +25,7 @@
 #include <stdint.h>
 
 /* The version of these entry points' signatures (kvq_abi_version): changes with any of them. */
-#define KVQ_ABI_VERSION 14
+#define KVQ_ABI_VERSION 15
 
 #ifdef __cplusplus
 extern "C" {
@@ -318,17 +318,17 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
                                int64_t qmax, void* stream);
 
 /* Pages' codes as bf16 (exact) in a contiguous temporary cache [num_pages, bs, H, D], pages as kvq_dequant_pages takes
- * them. */
+ * them, and in scales_out [H, num_pages * bs / 16, 4] what the prefill below needs of each 16 slots' scales. */
 int kvq_block_codes(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb,
                     int64_t v_sn, int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim,
-                    void* k_out, void* v_out, const int32_t* block_table, int64_t bt_stride, const int32_t* src_req,
-                    const int32_t* src_j, int64_t num_pages, void* stream);
+                    const float* k_scale, const float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group,
+                    void* k_out, void* v_out, float* scales_out, const int32_t* block_table, int64_t bt_stride,
+                    const int32_t* src_req, const int32_t* src_j, int64_t num_pages, void* stream);
 
 /* The same attention for the rows of a work list, as kvq_int8_prefill_attention_ex takes it (tile_piece NULL: every
- * entry reads all of its rows' keys). k_codes / v_codes: the requests' pages as kvq_block_codes leaves them (num_pages of
- * them, codes_table [num_seqs, ..] with row stride ct_stride in place of block_table, which still finds the scales); read
- * instead of the int8 pages, whose conversion in the kernel costs more where many rows read each key. NULL: the int8
- * pages. */
+ * entry reads all of its rows' keys). k_codes / v_codes / code_scales: the requests' pages as kvq_block_codes leaves them
+ * (num_pages of them, codes_table [num_seqs, ..] with row stride ct_stride in place of block_table), read instead of the
+ * int8 pages, whose conversion in the kernel costs more where many rows read each key. NULL: the int8 pages. */
 int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
                                 int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
                                 int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
@@ -338,8 +338,8 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
                                 int64_t bt_stride, int64_t num_q_heads, const int32_t* tile_req, const int32_t* tile_row,
                                 int64_t num_tiles, int64_t rows_per_tile, double softmax_scale, const int32_t* tile_piece,
                                 const int32_t* tile_slot, const int32_t* merge, int64_t num_merge, float* part_out,
-                                float* part_ml, const void* k_codes, const void* v_codes, int64_t num_pages,
-                                const int32_t* codes_table, int64_t ct_stride, void* stream);
+                                float* part_ml, const void* k_codes, const void* v_codes, const float* code_scales,
+                                int64_t num_pages, const int32_t* codes_table, int64_t ct_stride, void* stream);
 
 /* Text of the last error on this thread ("" if none). */
 const char* kvq_last_error(void);

@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args
   });
 }
 
-// The bf16 prefill over a temporary cache of the codes (kvq_block_codes), the scales from the cache itself.
+// The bf16 prefill over a temporary cache of the codes and their scales' table (kvq_block_codes).
 template <int D, bool SPLIT>
 __global__ __launch_bounds__(256, 3) void block_codes_prefill_kernel(PrefillArgs a) {
   prefill_body<D, PR_SRC_BF16_BLOCK, SPLIT>(a);
@@ -954,8 +954,8 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
                                 int64_t bt_stride, int64_t num_q_heads, const int32_t* tile_req, const int32_t* tile_row,
                                 int64_t num_tiles, int64_t rows_per_tile, double softmax_scale, const int32_t* tile_piece,
                                 const int32_t* tile_slot, const int32_t* merge, int64_t num_merge, float* part_out,
-                                float* part_ml, const void* k_codes, const void* v_codes, int64_t num_pages,
-                                const int32_t* codes_table, int64_t ct_stride, void* stream) {
+                                float* part_ml, const void* k_codes, const void* v_codes, const float* code_scales,
+                                int64_t num_pages, const int32_t* codes_table, int64_t ct_stride, void* stream) {
   const char* nm = "block_prefill_attention";
   if (num_tiles < 0 || num_tiles > INT32_MAX || num_merge < 0 || num_merge > INT32_MAX) return fail("%s: bad sizes", nm);
   if (num_tiles == 0) { g_err.clear(); return KVQ_OK; }
@@ -969,7 +969,7 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
                                      seq_lens, block_table, num_q_heads)) return rc;
   if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
     return fail("%s: page too large for 32-bit lane offsets", nm);
-  if (k_codes && (!v_codes || !codes_table || num_pages <= 0 || num_pages > INT32_MAX || !aligned16(k_codes) || !aligned16(v_codes)))
+  if (k_codes && (!v_codes || !codes_table || !code_scales || !aligned16(code_scales) || num_pages <= 0 || num_pages > INT32_MAX || !aligned16(k_codes) || !aligned16(v_codes)))
     return fail("%s: bad temporary cache", nm);
   if (k_codes && 2 * block_size * num_kv_heads * head_dim > INT32_MAX)
     return fail("%s: page too large for 32-bit page / slot offsets", nm);
@@ -984,7 +984,7 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
   a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
   a.G = (int)(num_q_heads / num_kv_heads); a.lbs = log2i(block_size); a.num_blocks = (int)num_blocks;
   a.kpage = a.vpage = a.krow = a.vrow = 0; a.contig = 0; a.ks = a.vs = nullptr; a.ks_pc = a.vs_pc = 0;   // (prefill_body's)
-  a.bs = b.s; a.s_table = block_table; a.s_bt_stride = bt_stride; a.s_blocks = (int)num_blocks;
+  a.s_table = reinterpret_cast<const f32x4*>(code_scales);
   if (k_codes) {   // the temporary cache's pages instead: bf16 [num_pages, block_size, H, D], contiguous
     a.kc = (const uint16_t*)k_codes; a.vc = (const uint16_t*)v_codes;
     a.block_table = codes_table; a.bt_stride = ct_stride; a.num_blocks = (int)num_pages;
@@ -1015,17 +1015,20 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
 
 int kvq_block_codes(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb,
                     int64_t v_sn, int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim,
-                    void* k_out, void* v_out, const int32_t* block_table, int64_t bt_stride, const int32_t* src_req,
-                    const int32_t* src_j, int64_t num_pages, void* stream) {
+                    const float* k_scale, const float* v_scale, int64_t s_sb, int64_t s_sh, int64_t s_sg, int64_t group,
+                    void* k_out, void* v_out, float* scales_out, const int32_t* block_table, int64_t bt_stride,
+                    const int32_t* src_req, const int32_t* src_j, int64_t num_pages, void* stream) {
   const char* nm = "block_codes";
   if (num_pages < 0 || num_pages > INT32_MAX) return fail("%s: bad sizes", nm);
   if (num_pages == 0) { g_err.clear(); return KVQ_OK; }
-  if (const int rc = check_blocks(nm, num_blocks, block_size, BLK_MIN, num_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache,
+  if (const int rc = check_blocks(nm, num_blocks, block_size, group, num_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache,
                                   v_sb, v_sn, v_sh)) return rc;
-  if (!k_out || !v_out || !block_table || !src_req || !src_j) return fail("%s: null pointer", nm);
-  if (!aligned16(k_out) || !aligned16(v_out)) return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  if (!k_out || !v_out || !scales_out || !k_scale || !v_scale || !block_table || !src_req || !src_j) return fail("%s: null pointer", nm);
+  if (!aligned16(k_out) || !aligned16(v_out) || !aligned16(scales_out))
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
   return dequant_launch<true>(nm, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size, num_heads,
                               head_dim, k_out, v_out, block_table, bt_stride, src_req, src_j, num_pages, nullptr, 0, nullptr, 0,
+                              BlockCodes{block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group), reinterpret_cast<f32x4*>(scales_out)},
                               stream);
 }
 

@@ -58,6 +58,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVE = 64;
 constexpr int TILE = 32;          // keys per attention tile = P quantization tile
@@ -2008,14 +2009,18 @@ constexpr int DQ_BATCH = 16;
 // tokens of 498, 32 / 8 heads, blocks of 64 slots 30.4 -> 22.7 us, 157 of 157, 16 / 16 heads d64 19.8 -> 11.7, 1,024 of
 // 1,024 in blocks of 32 34.6 -> 33.3; 512 pages of 16 slots unchanged; slices of 16 tokens 23.8 and 12.7).
 constexpr int DQ_WG_PER_CU = 4, DQ_MIN_TOKENS = 4;
-// CODES: the codes themselves as bf16 (exact), no scales (a block-scaled cache's, kvq_block_codes).
+// CODES: the codes themselves as bf16 (exact), and the scales in a table (a block-scaled cache's, kvq_block_codes).
+struct BlockCodes {
+  BlockScales s;
+  f32x4* table;   // [H, P * block_size / 16]: what the prefill needs of each 16 slots' scales
+};
 template <int D, bool CODES = false>
 __global__ __launch_bounds__(256) void dequant_pages_kernel(
     const int8_t* __restrict__ kc, int64_t k_sb, int64_t k_sn, int64_t k_sh, const int8_t* __restrict__ vc,
     int64_t v_sb, int64_t v_sn, int64_t v_sh, int num_blocks, int bs, int H, int heads_per_block,
     int tokens_per_block, uint16_t* __restrict__ ko, uint16_t* __restrict__ vo, const int* __restrict__ bt, int64_t bt_stride,
     const int* __restrict__ src_req, const int* __restrict__ src_j, const float* __restrict__ ks, int ks_pc,
-    const float* __restrict__ vs, int vs_pc) {
+    const float* __restrict__ vs, int vs_pc, BlockCodes codes) {
   constexpr int CPK = D / 8;                      // 8-channel chunks of one K (or V) row
   constexpr int CPH = 2 * CPK;                    // combinations per head: K and V chunks
   const int p = blockIdx.x;
@@ -2033,6 +2038,19 @@ __global__ __launch_bounds__(256) void dequant_pages_kernel(
   const int j = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)src_j)[p]);
   int src = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[(int64_t)r * bt_stride + j]);
   if (src < 0 || src >= num_blocks) src = 0;
+  if constexpr (CODES) {
+    // (finite whatever lies in blocks that were never written: their keys are masked by infinite scores)
+    auto scale = [](float x) { return __builtin_fminf(__builtin_fmaxf(x, MIN_BLOCK_SCALE), 1e37f); };
+    const int nb16 = bs / 16;
+    if (blockIdx.z == 0)
+      for (int i = tid; i < nh * nb16; i += C * tpc) {
+        const int hh = h0 + i / nb16, b = i % nb16;
+        const int64_t at = (int64_t)src * codes.s.sb + (int64_t)hh * codes.s.sh + (int64_t)((16 * b) >> codes.s.lg) * codes.s.sg;
+        const float v = scale(codes.s.vs[at]);
+        codes.table[((int64_t)hh * gridDim.x + p) * nb16 + b] = f32x4{scale(codes.s.ks[at]), __builtin_amdgcn_logf(v),
+                                                                      __builtin_amdgcn_rcpf(v), 0.f};
+      }
+  }
   float sc[8];
   const float* sp = kv ? vs : ks;
   if constexpr (CODES) {
@@ -2089,7 +2107,6 @@ __global__ __launch_bounds__(256) void dequant_pages_kernel(
 // V^T operand reads the same keys: two transposing 8-byte LDS reads per channel tile.
 // ------------------------------------------------------------------------------------------------
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct PrefillArgs {
   const uint16_t* q;
@@ -2120,11 +2137,9 @@ struct PrefillArgs {
   const float* ks;
   const float* vs;
   int ks_pc, vs_pc;
-  // PR_SRC_BF16_BLOCK: the codes' scales, by the pages of the cache that they were copied from
-  BlockScales bs;
-  const int* s_table;    // that cache's block table
-  int64_t s_bt_stride;
-  int s_blocks;          // its pages
+  // PR_SRC_BF16_BLOCK: the scales of the temporary cache's codes, [Hkv, num_blocks * block_size / 16] of K scale, log2 of the
+  // V scale, 1 / V scale, 0
+  const f32x4* s_table;
 };
 
 constexpr int PR_RB = 2;                    // 16-row blocks per wavefront
@@ -2196,10 +2211,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   static_assert(NS8 >= 2 && IPW8 * 4 == 2 * PPM && RPI8 <= 16, "int8 ring");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[NB][2][TILEB];
   __shared__ __attribute__((aligned(1024))) uint8_t ring8[I8 ? NS8 : 1][2][I8 ? TILE8B : 16];
-  // BLK: the scales of the last four tiles. A wavefront's DMA rows lie in one 16-key half (wavefronts 0 and 1: the first),
-  // whose K and V scale it brings too, at floats 0 and 1 of its row (lanes even and odd; the others repeat them)
-  static_assert(4 * RPI * IPW == PR_KEYS && 2 * RPI * IPW == 16, "two wavefronts to a half tile");
-  __shared__ __attribute__((aligned(16))) float sring[BLK ? 4 : 1][4][BLK ? WAVE : 4];
 
   const int kvh = blockIdx.y;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -2323,19 +2334,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     }
     linear = !__any(bad) && run_fits(pg_hi + 1, a.kpage) && run_fits(pg_hi + 1, a.vpage);
   }
-  // BLK: this wavefront's half tile's page in the cache of the codes, read a tile before its use (a half past the last key
-  // takes the last key's block: its own may never have been written)
-  const int* sbt = nullptr;
-  const float* sbase = nullptr;
-  int sid = 0;
-  auto skey = [&](int c) { return min(min(c, c_hi - 1) * PR_KEYS + 16 * (wave >> 1), kend - 1); };
-  auto next_sid = [&](int c) {
-    if constexpr (BLK) sid = ((const __attribute__((address_space(4))) int*)sbt)[skey(c) >> a.lbs];
-  };
-  if constexpr (BLK) {
-    sbt = a.s_table + (int64_t)r * a.s_bt_stride;
-    sbase = ((lane & 1) ? a.bs.vs : a.bs.ks) + (int64_t)kvh * a.bs.sh;
-  }
   const char* klin = kh + (int64_t)pfirst * a.kpage;
   const char* vlin = vh + (int64_t)pfirst * a.vpage;
   // tile c: keys 0..15 sit in page p0 from slot (32 c) mod bs on, keys 16..31 right after them
@@ -2343,14 +2341,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // lin_t: std::true_type = the pages are one run (no block-table read), false_type = read the
   // table, bool = decide at run time
   auto issue = [&](int c, int st, auto lin_t) {
-    if constexpr (BLK) {
-      int p = __builtin_amdgcn_readfirstlane(sid);
-      p = p >= 0 && p < a.s_blocks ? p : 0;
-      const float* sp = sbase + ((int64_t)p * a.bs.sb + (int64_t)((skey(c) & bsm) >> a.bs.lg) * a.bs.sg);
-      __builtin_amdgcn_global_load_lds((const void*)sp,
-                                       (__attribute__((address_space(3))) void*)(&sring[min(c, c_hi - 1) & 3][wave][0]), 4, 0, 0);
-      next_sid(c + 1);
-    }
     c = min(c, c_hi - 1);  // past the end: reload the last tile into the free stage
     const int kb0 = c * PR_KEYS, klast = max(kend - 1, 0);
     const char* kb[2];
@@ -2565,9 +2555,26 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // ---- per tile: scores (QK) and each row's largest, masked for the keys past a row's limit ----
   f32x4 sc[RB][2];
   float lmax[RB], top[RB];
-  // BLK: what turns a score of half b into the exponent: factor kf, addend lv = log2(V scale); iv = 1 / V scale
-  float kf[2], lv[2], iv[2];
-  const uint32_t sadr = (uint32_t)(uintptr_t)(&sring[0][0][0]);
+  // BLK: a half tile's entry (K scale, log2 of the V scale, 1 / V scale, 0) of the temporary cache's table, uniform; those of
+  // the next tile are requested a tile before their use
+  const f32x4* stab = nullptr;
+  f32x4 ent[2], ent_next[2];
+  if constexpr (BLK) stab = a.s_table + (int64_t)kvh * (int64_t)a.num_blocks * ((bsm + 1) / 16);
+  auto next_entries = [&](int c) {
+    if constexpr (BLK) {
+      const int k0 = min(c, c_hi - 1) * PR_KEYS, k1 = min(k0 + 16, max(kend - 1, 0));
+      int p0 = pfirst + (k0 >> a.lbs), p1 = pfirst + (k1 >> a.lbs);
+      if (!linear) {
+        p0 = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[k0 >> a.lbs]);
+        p1 = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[k1 >> a.lbs]);
+        p0 = (p0 >= 0 && p0 < a.num_blocks) ? p0 : 0;
+        p1 = (p1 >= 0 && p1 < a.num_blocks) ? p1 : 0;
+      }
+      const auto* t = (const __attribute__((address_space(4))) f32x4*)stab;
+      ent_next[0] = t[((int64_t)p0 << (a.lbs - 4)) + ((k0 & bsm) >> 4)];
+      ent_next[1] = t[((int64_t)p1 << (a.lbs - 4)) + ((k1 & bsm) >> 4)];
+    }
+  };
   // K operand reads from inline assembly, each statement waiting for its own reads: as plain loads
   // the compiler makes them wait for every LDS DMA in flight (it cannot tell they read another ring
   // stage), which would empty the ring every tile
@@ -2576,6 +2583,11 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   auto scores = [&](auto st_t, int c, auto mask_t) {
     pr_prio<1>();
     const int n0 = c * PR_KEYS;
+    if constexpr (BLK) {
+      ent[0] = ent_next[0];
+      ent[1] = ent_next[1];
+      next_entries(c + 1);
+    }
     uint32_t ad[DS];
 #pragma unroll
     for (int s = 0; s < DS; ++s) ad[s] = kadr[s] + stage_vofs(st_t);
@@ -2611,19 +2623,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
                                                              0, 0, 0);
     }
     pr_prio<0>();
-    if constexpr (BLK) {
-      u32x2 s2[2];
-      asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:%c3\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(s2[0]), "=&v"(s2[1]) : "v"(sadr + (c & 3) * (4 * WAVE * 4)), "i"(2 * WAVE * 4) : "memory");
-      auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float v = __builtin_fmaxf(__uint_as_float(s2[b].y), MIN_BLOCK_SCALE);
-        kf[b] = uniform(__builtin_fmaxf(__uint_as_float(s2[b].x), MIN_BLOCK_SCALE) * a.sm_log2);
-        lv[b] = uniform(__builtin_amdgcn_logf(v));
-        iv[b] = uniform(__builtin_amdgcn_rcpf(v));
-      }
-    }
     if (decltype(mask_t)::value && n0 + PR_KEYS > lim_lo) {  // a tile on the causal edge of some row
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
@@ -2640,7 +2639,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
           h[b] = __builtin_fmaf(__builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]),
-                                                __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])), kf[b], lv[b]);
+                                                __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])), ent[b][0] * a.sm_log2, ent[b][1]);
         lmax[rb] = __builtin_fmaxf(h[0], h[1]);
       }
       return;
@@ -2683,17 +2682,12 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       float p[2][4], psum = 0.f;
-      if constexpr (BLK) {
+      if constexpr (BLK) {   // (the denominators below, on the matrix cores)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float e0 = lv[b] - m[rb];
-          float half = 0.f;
+          const float f = ent[b][0] * a.sm_log2, e0 = ent[b][1] - m[rb];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], kf[b], e0));
-            half += p[b][i];
-          }
-          l[rb] = __builtin_fmaf(half, iv[b], l[rb]);
+          for (int i = 0; i < 4; ++i) p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], f, e0));
         }
       } else {
 #pragma unroll
@@ -2743,6 +2737,19 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
           acc[rb][t0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rb], acc[rb][t0 + u], 0, 0, 0);
       }
     }
+    // BLK: the sums of the rounded P by half, each over its V scale: row b of the first operand picks the keys of half b, so
+    // they stand in the lanes of group 0
+    if constexpr (BLK) {
+      u32x4 pw = {n == 0 ? 0x3f803f80u : 0u, 0u, n == 1 ? 0x3f803f80u : 0u, 0u};
+      pw.y = pw.x;
+      pw.w = pw.z;
+      const bf16x8 pick = *reinterpret_cast<bf16x8*>(&pw);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pick, pop[rb], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+        l[rb] = __builtin_fmaf(sum[0], ent[0][2], __builtin_fmaf(sum[1], ent[1][2], l[rb]));
+      }
+    }
   };
 
   bool piece = false;   // one of several pieces of the rows, and its slot
@@ -2761,7 +2768,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     // its int8 stage (c % NS8), tiles counted from c_lo.
     // the first tiles' DMA; I8: NS8 tiles in flight, tile 0 converted once it has landed
     auto prologue = [&]() {
-      next_sid(c_lo);
+      next_entries(c_lo);
       if constexpr (I8) {
 #pragma unroll
         for (int j = 0; j < NS8; ++j) issue(c_lo + j, j, linear);
@@ -2782,7 +2789,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
                                       // (tile c - 1) and tile c's int8 stage are free again
         issue(c + NS8, s8, lin_t);
       } else {
-        wait_vm<(2 * IPW + (BLK ? 1 : 0)) * (NS - 2)>();  // this wavefront's share of tile c has landed
+        wait_vm<2 * IPW * (NS - 2)>();  // this wavefront's share of tile c has landed
         lds_barrier();                  // everyone's share has; stage (c - 1) % NS is free again
         issue(c + NS - 1, snext, lin_t);
       }
@@ -2797,7 +2804,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
         lds_barrier();
         issue(c + NS8, NS8 == 2 ? ST : s8, lin_t);
       } else {
-        wait_vm<(2 * IPW + (BLK ? 1 : 0)) * (NS - 2)>();
+        wait_vm<2 * IPW * (NS - 2)>();
         lds_barrier();
         issue(c + NS - 1, (ST + NS - 1) % NS, lin_t);
       }
@@ -3871,7 +3878,7 @@ int dequant_launch(const char* nm, const int8_t* k_cache, int64_t k_sb, int64_t 
                    int64_t v_sb, int64_t v_sn, int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
                    int64_t head_dim, void* k_out, void* v_out, const int32_t* block_table, int64_t bt_stride,
                    const int32_t* src_req, const int32_t* src_j, int64_t num_pages, const float* k_scale, int64_t k_scale_cols,
-                   const float* v_scale, int64_t v_scale_cols, void* stream) {
+                   const float* v_scale, int64_t v_scale_cols, const BlockCodes& codes, void* stream) {
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   // heads per workgroup: as many as 256 threads' worth of (head, K|V, chunk) combinations; threads: the
   // largest multiple of those combinations up to 256
@@ -3889,7 +3896,7 @@ int dequant_launch(const char* nm, const int8_t* k_cache, int64_t k_sb, int64_t 
     hipLaunchKernelGGL(kern, grid, dim3(threads), 0, st, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh,
                        (int)num_blocks, (int)block_size, (int)num_heads, hpb, (int)tokens, (uint16_t*)k_out, (uint16_t*)v_out,
                        block_table, bt_stride, src_req, src_j, k_scale, (int)(k_scale_cols > 1), v_scale,
-                       (int)(v_scale_cols > 1));
+                       (int)(v_scale_cols > 1), codes);
   };
   if (head_dim == 128) go(dequant_pages_kernel<128, CODES>);
   else go(dequant_pages_kernel<64, CODES>);
@@ -3920,7 +3927,7 @@ int kvq_dequant_pages(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t
   if (num_heads > 65535 * 4) return fail("dequant_pages: too many heads");
   return dequant_launch<false>("dequant_pages", k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks, block_size,
                                num_heads, head_dim, k_out, v_out, block_table, bt_stride, src_req, src_j, num_pages, k_scale,
-                               k_scale_cols, v_scale, v_scale_cols, stream);
+                               k_scale_cols, v_scale, v_scale_cols, BlockCodes{}, stream);
 }
 
 }  // extern "C"

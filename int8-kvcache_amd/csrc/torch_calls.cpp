@@ -466,7 +466,7 @@ PyObject* block_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     auto *rp = (const int32_t*)treq->data_ptr(), *wp = (const int32_t*)trow->data_ptr();
     const int32_t *rqp = nullptr, *jp = nullptr, *tbp = nullptr;
     int64_t P = 0, tbs = 0;
-    at::Tensor kt, vt;
+    at::Tensor kt, vt, st;
     if (a[17] != Py_None) {
       const at::Tensor *sreq = tensor(a[17]), *sj = tensor(a[18]), *tbt = tensor(a[19]);
       if (!sreq || !sj || !tbt || !index_vector(*sreq) || !index_vector(*sj) || sreq->size(0) == 0 ||
@@ -476,19 +476,21 @@ PyObject* block_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       rqp = (const int32_t*)sreq->data_ptr(), jp = (const int32_t*)sj->data_ptr(), tbp = (const int32_t*)tbt->data_ptr();
       kt = at::empty({P, c.bs, c.H, c.D}, x.q->options());
       vt = at::empty({P, c.bs, c.H, c.D}, x.q->options());
+      st = at::empty({c.H, P * (c.bs / 16), 4}, x.q->options().dtype(at::kFloat));
     }
     void *ktp = P ? kt.data_ptr() : nullptr, *vtp = P ? vt.data_ptr() : nullptr;
+    float* stp = P ? (float*)st.data_ptr() : nullptr;
     return launch(P ? "kvq_block_codes" : "kvq_block_prefill_attention", [&] {
       if (P) {
-        const int rc = p_block_codes(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, ktp, vtp, btp,
-                                     x.bt->stride(0), rqp, jp, P, x.st);
+        const int rc = p_block_codes(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh,
+                                     c.sg, c.group, ktp, vtp, stp, btp, x.bt->stride(0), rqp, jp, P, x.st);
         if (rc) return rc;
         entry = "kvq_block_prefill_attention";
       }
       return p_block_prefill(x.qp, x.q->stride(0), x.q->stride(1), c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs,
                              c.H, c.D, c.ks, c.vs, c.sb, c.sh, c.sg, c.group, x.op, x.out->stride(0), x.out->stride(1), x.cu,
                              x.sl, btp, x.bt->stride(0), x.Hq, rp, wp, tiles, rows, x.scale, pp, sp, mp, nm, pop, pmp, ktp,
-                             vtp, P, tbp, tbs, x.st);
+                             vtp, stp, P, tbp, tbs, x.st);
     });
   });
 }

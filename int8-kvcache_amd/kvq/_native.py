@@ -10,7 +10,7 @@ import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkvq_int8.so")
-ABI_VERSION = 14
+ABI_VERSION = 15
 ERR_LAUNCH = 2      # KVQ_ERR_LAUNCH
 
 _i64 = ctypes.c_int64
@@ -65,12 +65,12 @@ SIGNATURES = {
     "kvq_block_decode_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
                                    _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
                                    _i64, _i64, _f64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr],
-    "kvq_block_codes": [_ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64,
-                        _ptr, _ptr, _i64, _ptr],
+    "kvq_block_codes": [_ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64,
+                        _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr],
     "kvq_block_prefill_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
                                     _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
                                     _i64, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr,
-                                    _i64, _ptr, _i64, _ptr],
+                                    _ptr, _i64, _ptr, _i64, _ptr],
     "kvq_last_error": [],
     "kvq_abi_version": [],
 }

@@ -199,14 +199,15 @@ def block_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block
     _check_cuda(name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"], scales["v_scale"])
     n = work.tile_req.shape[0]
     split = work.split(h, e.prefill_rows, d)
-    codes = (None, None, 0, None, 0)
+    codes = (None, None, None, 0, None, 0)
     if src[0] is not None:
         src_req, src_j, bt_tmp = src
         kt = torch.empty((src_req.shape[0], bs, h, d), dtype=q.dtype, device=q.device)
         vt = torch.empty_like(kt)
-        _call("kvq_block_codes", q.device, *k, *v, *geom, kt.data_ptr(), vt.data_ptr(), block_table.data_ptr(),
-              block_table.stride(0), src_req.data_ptr(), src_j.data_ptr(), src_req.shape[0])
-        codes = (kt.data_ptr(), vt.data_ptr(), kt.shape[0], bt_tmp.data_ptr(), bt_tmp.stride(0))
+        st = torch.empty((h, kt.shape[0] * (bs // 16), 4), dtype=torch.float32, device=q.device)
+        _call("kvq_block_codes", q.device, *k, *v, *geom, *sc, kt.data_ptr(), vt.data_ptr(), st.data_ptr(),
+              block_table.data_ptr(), block_table.stride(0), src_req.data_ptr(), src_j.data_ptr(), src_req.shape[0])
+        codes = (kt.data_ptr(), vt.data_ptr(), st.data_ptr(), kt.shape[0], bt_tmp.data_ptr(), bt_tmp.stride(0))
     _call("kvq_block_prefill_attention", q.device, q.data_ptr(), q.stride(0), q.stride(1), *k, *v, *geom, *sc,
           out.data_ptr(), out.stride(0), out.stride(1), cu_seqlens_q.data_ptr(), seq_lens.data_ptr(),
           block_table.data_ptr(), block_table.stride(0), q.shape[1], work.tile_req.data_ptr(), work.tile_row.data_ptr(),

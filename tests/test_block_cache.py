@@ -104,7 +104,7 @@ def _c(name, **change):
             "block_decode_attention": [None, 3584, 128, *k, *v, *geom, *sc, None, 3584, 128, None, None, None, 3, 2, 28, 0.1,
                                        None, None, None, 0, 0, 1, 0, 0, 1, 8, None],
             "block_prefill_attention": [None, 3584, 128, *k, *v, *geom, *sc, None, 3584, 128, None, None, None, 3, 28, 16, 16,
-                                        1, 128, 0.1, None, None, None, 0, None, None, None, None, 0, None, 0, None]}[name]
+                                        1, 128, 0.1, None, None, None, 0, None, None, None, None, None, 0, None, 0, None]}[name]
     at = {"quant_block_cache": 15, "read_block_cache": 8, "block_decode_attention": 11, "block_prefill_attention": 11}[name]
     places = {"num_blocks": at, "block_size": at + 1, "heads": at + 2, "d": at + 3, "group": at + 9, "k_cache": at - 8,
               "k_sn": at - 6, "num_seqs": len(args) - 2, "splits": 36, "rows_per_tile": 32}
