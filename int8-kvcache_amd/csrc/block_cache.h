@@ -648,7 +648,7 @@ __global__ __launch_bounds__(256) void block_attn_kernel(BlockAttnArgs args) {
 template <int D>
 __global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args) {
   touch_args();
-  __shared__ __attribute__((aligned(1024))) RowsLds<D> lds;
+  __shared__ __attribute__((aligned(1024))) RowsLds<D, 4> lds;
   const int lane = threadIdx.x & (WAVE - 1), n = lane & 15, g = lane >> 4;
   walk_pieces(args.a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
     const AttnArgs& a = fresh_args();
@@ -656,7 +656,7 @@ __global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args
     const RowsView v{a.q, a.kc + (int64_t)kvh * a.k_sh, a.vc + (int64_t)kvh * a.v_sh, a.block_table + (int64_t)r * a.bt_stride,
                      s.ks + (int64_t)kvh * s.sh, s.vs + (int64_t)kvh * s.sh, a.q_st, a.q_sh, a.k_sb, a.k_sn, a.v_sb, a.v_sn,
                      s.sb, s.sg, a.sm_log2, a.G, a.num_blocks, a.lbs, s.lg};
-    attend_rows<D, 1>(v, lds, w.tok, w.qlen, w.len, kvh, 64 * rg, c0, w.len > 0 ? c1 : c0, min(w.len, c1 * PR_KEYS),
+    attend_rows<D, 4, 1>(v, lds, w.tok, w.qlen, w.len, kvh, 64 * rg, c0, w.len > 0 ? c1 : c0, min(w.len, c1 * PR_KEYS),
                       [&](int, int t, int hq, bool valid, float m, float l, const f32x4 (&acc)[D / 16]) {
       if (!valid) return;
       const AttnArgs& o = fresh_args();
@@ -695,9 +695,13 @@ struct BlockPrefillArgs {
   BlockScales s;
 };
 
+// D = 128: eight wavefronts of one row block each (four of two leave the tile loop short of registers).
+template <int D>
+constexpr int BLOCK_PREFILL_WAVES = D == 128 ? 8 : 4;
 template <int D, bool SPLIT>
-__global__ __launch_bounds__(256, 3) void block_prefill_kernel(BlockPrefillArgs args) {
-  __shared__ __attribute__((aligned(1024))) RowsLds<D> lds;
+__global__ __launch_bounds__(WAVE * BLOCK_PREFILL_WAVES<D>, 4) void block_prefill_kernel(BlockPrefillArgs args) {
+  constexpr int NW = BLOCK_PREFILL_WAVES<D>, RB = PR_ROWS / (16 * NW);
+  __shared__ __attribute__((aligned(1024))) RowsLds<D, NW> lds;
   const PrefillArgs& a = args.p;
   const BlockScales& s = args.s;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 15, g = lane >> 4;
@@ -716,7 +720,7 @@ __global__ __launch_bounds__(256, 3) void block_prefill_kernel(BlockPrefillArgs 
                    a.q_sh, a.k_sb, a.k_sn, a.v_sb, a.v_sn, s.sb, s.sg, a.sm_log2, a.G, a.num_blocks, a.lbs, s.lg};
   bool piece = false;
   int pslot = 0;
-  attend_rows<D, PR_RB>(v, lds, tok, Q, L, kvh, row0, c_lo, c_hi, kend,
+  attend_rows<D, NW, RB>(v, lds, tok, Q, L, kvh, row0, c_lo, c_hi, kend,
                         [&](int rb, int t, int hq, bool valid, float m, float l, const f32x4 (&acc)[D / 16]) {
     if constexpr (SPLIT) {
       if (rb == 0) {   // read here, not held through the tile loop
@@ -728,7 +732,7 @@ __global__ __launch_bounds__(256, 3) void block_prefill_kernel(BlockPrefillArgs 
     }
     if (!valid) return;
     if (SPLIT && piece) {   // the accumulators as they are: the merge divides by the whole denominator
-      const int64_t pr = ((int64_t)pslot * gridDim.y + kvh) * PR_ROWS + (wave * PR_RB + rb) * 16 + n;
+      const int64_t pr = ((int64_t)pslot * gridDim.y + kvh) * PR_ROWS + (wave * RB + rb) * 16 + n;
       if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = float2{m, l};
       float* prow = a.part_out + pr * D + 4 * g;
 #pragma unroll
@@ -1003,7 +1007,7 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
       ? (tile_piece ? block_codes_prefill_kernel<128, true> : block_codes_prefill_kernel<128, false>)
       : (tile_piece ? block_codes_prefill_kernel<64, true> : block_codes_prefill_kernel<64, false>);
   if (k_codes) hipLaunchKernelGGL(codes_kern, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, b);
+  else hipLaunchKernelGGL(kern, grid, dim3(WAVE * (head_dim == 128 ? BLOCK_PREFILL_WAVES<128> : BLOCK_PREFILL_WAVES<64>)), 0, st, b);
   const int rc = launched(nm);
   if (rc != KVQ_OK || !tile_piece || num_merge == 0) return rc;
   const dim3 mgrid((unsigned)num_merge, (unsigned)num_kv_heads, PR_ROWS / PR_MERGE_WAVES);

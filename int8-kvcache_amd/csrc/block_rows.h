@@ -1,13 +1,13 @@
 // Attention of many query rows over a block-scaled INT8 cache: the tile loop that long queries (block_prefill_kernel) and
 // verification (block_verify_kernel) share. Part of kvq_int8.hip, included by block_cache.h.
 //
-// Four wavefronts take 64 RB (token, q head) rows of one (request, kv head), RB blocks of 16 rows each, and walk 32-key
+// NW wavefronts take 16 NW RB (token, q head) rows of one (request, kv head), RB blocks of 16 rows each, and walk 32-key
 // tiles together. Per tile, in the log2 domain of block_attn_kernel:
 //   QK  S^T[key][row]  = K . Q16^T   v_mfma_i32_16x16x64_i8, q in two int8 planes: the codes feed the MFMA as they are
 //   e   = S sq scale k_scale + log2(v_scale),  P = 2^(e - m),  l += P / v_scale
 //   PV  O^T[chan][row] += V^T . P^T  v_mfma_f32_16x16x32_bf16, P rounded to bf16, V codes converted to bf16 (exactly)
 // so that O stays in the accumulators from tile to tile (an int8 product needs 3 operations per channel and row to add
-// its integers to O, which at 32 keys a tile costs more than the conversion of V by all four wavefronts). K in int8 also
+// its integers to O, which at 32 keys a tile costs more than the conversion of V by all the wavefronts). K in int8 also
 // halves the LDS reads of the QK operands, of which every wavefront needs the whole tile.
 //
 // The tile's codes and scales come by DMA into LDS rings of four slots, up to three tiles ahead; V is converted into one of
@@ -45,19 +45,19 @@ struct RowsView {
   int G, num_blocks, lbs, lg;
 };
 
-template <int D>
+template <int D, int NW>
 struct RowsLds {
   static constexpr int SLOTS = 4;
   uint8_t k8[SLOTS][PR_KEYS * D];
   uint8_t v8[SLOTS][PR_KEYS * D];
   uint8_t v16[2][PR_KEYS * 2 * D];
-  float sc[SLOTS][4][WAVE];   // [slot][wavefront]: K and V scale of the half tile that the wavefront's K or V rows lie in
+  float sc[SLOTS][NW][WAVE];   // [slot][wavefront]: K and V scale of the half tile that the wavefront's K or V rows lie in
 };
 
 // Rows row0 .. of request rows (tok, Q tokens, L keys) over tiles [c_lo, c_hi), whose last key is below kend. fin(rb, t,
 // hq, valid, m, l, acc): row block rb's result in the lane of row n, channels 16 tt + 4 g + i in acc[tt][i].
-template <int D, int RB, typename Fin>
-__device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, int tok, int Q, int L, int kvh, int row0,
+template <int D, int NW, int RB, typename Fin>
+__device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& lds, int tok, int Q, int L, int kvh, int row0,
                                             int c_lo, int c_hi, int kend, Fin&& fin) {
   constexpr int KS = D / 64;                // QK steps of 64 channels
   constexpr int VT = D / 16;                // PV channel tiles
@@ -65,23 +65,19 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
   constexpr int ROWB = 2 * D, TILEB = PR_KEYS * ROWB;
   constexpr int CHR = D / 16;               // 16-byte chunks of an int8 row
   constexpr int TILE8B = PR_KEYS * D, PPM = TILE8B / 1024;   // DMA instructions per int8 matrix and tile
-  constexpr int IPW = 2 * PPM / 4, VMT = IPW + 1;            // per wavefront and tile; with the scales
+  constexpr int IPW = 2 * PPM / NW, VMT = IPW + 1;           // per wavefront and tile; with the scales
   constexpr int RPI = 1024 / D;             // int8 rows per DMA instruction
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int n = lane & 15, g = lane >> 4;
   const int G = a.G;
   const int wrow0 = row0 + wave * 16 * RB;
   const bool active = wrow0 < Q * G;        // else the wavefront only moves and converts tiles
-  int t[RB], hq[RB], lim[RB];
-  bool valid[RB];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int R = wrow0 + 16 * rb + n;
-    t[rb] = R / G;
-    hq[rb] = kvh * G + R % G;
-    valid[rb] = t[rb] < Q;
-    lim[rb] = L - Q + 1 + t[rb];
-  }
+  // the lane's row of block rb: its token of the request (found again where it is needed, not held through the tiles)
+  auto row_of = [&](int rb) {
+    int x = wrow0 + n;
+    asm volatile("" : "+v"(x));
+    return x + 16 * rb;
+  };
   const int lim_lo = L - Q + 1 + wrow0 / G;
 
   // ---- q: two int8 planes per row, rs the factor of its integer scores ----
@@ -90,11 +86,12 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     u32x4 w[2 * KS];
-    const uint16_t* qp = a.q + (int64_t)(tok + t[rb]) * a.q_st + (int64_t)hq[rb] * a.q_sh + 16 * g;
+    const int R = row_of(rb), t = R / G;
+    const uint16_t* qp = a.q + (int64_t)(tok + t) * a.q_st + (int64_t)(kvh * G + R - t * G) * a.q_sh + 16 * g;
 #pragma unroll
     for (int u = 0; u < 2 * KS; ++u) {
       w[u] = u32x4{0u, 0u, 0u, 0u};
-      if (valid[rb]) w[u] = *reinterpret_cast<const u32x4*>(qp + 64 * (u / 2) + 8 * (u % 2));
+      if (t < Q) w[u] = *reinterpret_cast<const u32x4*>(qp + 64 * (u / 2) + 8 * (u % 2));
     }
     float amax = 0.f;
 #pragma unroll
@@ -116,17 +113,17 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
       }
   }
 
-  // ---- DMA: wavefront w's instruction i is number j = w + 4 i of the tile's 2 PPM: matrix j / PPM (K, V), key rows
+  // ---- DMA: wavefront w's instruction i is number j = w + NW i of the tile's 2 PPM: matrix j / PPM (K, V), key rows
   // RPI (j % PPM) .. + RPI - 1, lane l at byte 16 l. All of a wavefront's rows lie in one half tile (16 keys, one page, one
   // scale), of which it also brings the scales. K rows are swizzled (chunk c of row r at c ^ swz_k(r)) for the operand
   // reads below. Rows past the last key are rows of a valid page; the mask drops them. ----
-  const int part = wave % PPM, half = RPI * part >= 16 ? 1 : 0;     // (the same for each i: 4 is a multiple of PPM)
-  static_assert(4 % PPM == 0, "a wavefront's instructions share their rows");
+  const int part = wave % PPM, half = RPI * part >= 16 ? 1 : 0;     // (the same for each i: NW is a multiple of PPM)
+  static_assert(NW % PPM == 0 && IPW >= 1, "a wavefront's instructions share their rows");
   constexpr int HW1 = D == 128 ? 2 : 1;                             // a wavefront of half 1 (wavefront 0 is of half 0)
   uint32_t o8[IPW];
 #pragma unroll
   for (int i = 0; i < IPW; ++i) {
-    const int mat = (wave + 4 * i) / PPM, row = RPI * part + lane / CHR, ch = lane % CHR;
+    const int mat = (wave + NW * i) / PPM, row = RPI * part + lane / CHR, ch = lane % CHR;
     o8[i] = mat ? (uint32_t)((row % 16) * a.v_sn + 16 * ch) : (uint32_t)((row % 16) * a.k_sn + 16 * (ch ^ swz_k<CHR>(row)));
   }
   const float* sbase = (lane & 1) ? a.vs : a.ks;
@@ -139,12 +136,12 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
     c = min(c, c_hi - 1);   // past the end: the last tile again, into a free slot or over itself
     int p = __builtin_amdgcn_readfirstlane(id);
     p = p >= 0 && p < a.num_blocks ? p : 0;
-    const int slot = c & (RowsLds<D>::SLOTS - 1), o = (c * PR_KEYS + 16 * half) & bsm;
+    const int slot = c & (RowsLds<D, NW>::SLOTS - 1), o = (c * PR_KEYS + 16 * half) & bsm;
     const float* sp = sbase + ((int64_t)p * a.s_sb + (int64_t)((key_of(c) & bsm) >> a.lg) * a.s_sg);
     __builtin_amdgcn_global_load_lds((const void*)sp, (__attribute__((address_space(3))) void*)(&lds.sc[slot][wave][0]), 4, 0, 0);
 #pragma unroll
     for (int i = 0; i < IPW; ++i) {
-      const int mat = (wave + 4 * i) / PPM;   // uniform
+      const int mat = (wave + NW * i) / PPM;   // uniform
       const int8_t* b = mat ? a.vc + ((int64_t)p * a.v_sb + (int64_t)o * a.v_sn) : a.kc + ((int64_t)p * a.k_sb + (int64_t)o * a.k_sn);
       uint8_t* dst = (mat ? lds.v8[slot] : lds.k8[slot]) + 1024 * part;
       asm volatile("" : "+s"(b));
@@ -165,8 +162,8 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
   for (int tt = 0; tt < VT; ++tt) vadr[tt] = v0 + vr0 * ROWB + 16 * ((2 * tt + ((n % 4) >> 1)) ^ vswz(vr0)) + 8 * (n & 1);
 
   // ---- V codes of tile c -> bf16 stage sb: thread x takes the 8-channel chunk x % CH of rows x / CH + CR i ----
-  constexpr int CR = 256 / CH, NPT = PR_KEYS / CR;
-  static_assert(CR % CH == 0 && NPT * CR == PR_KEYS && (NPT == 1 || NPT == 2), "conversion share");
+  constexpr int CR = NW * WAVE / CH, NPT = PR_KEYS / CR;
+  static_assert((CR % CH == 0 || NPT == 1) && NPT * CR == PR_KEYS && (NPT == 1 || NPT == 2), "conversion share");
   const int cc = threadIdx.x % CH, crow = threadIdx.x / CH;
   const uint32_t cra = (uint32_t)(uintptr_t)(&lds.v8[0][0]) + crow * D + 8 * cc, cwv = v0 + crow * ROWB + 16 * (cc ^ vswz(crow));
   auto vofs = [](auto st_t) -> uint32_t {
@@ -177,20 +174,23 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
     if constexpr (std::is_same_v<decltype(st_t), int>) return 0;
     else return decltype(st_t)::value * TILEB;
   };
-  auto convert = [&](int c, auto sb_t) {
-    const uint32_t ra = cra + (c & (RowsLds<D>::SLOTS - 1)) * TILE8B, wv = cwv + vofs(sb_t);
+  u32x2 w[NPT];   // V codes to convert, read with a tile's K operands
+  auto convert = [&](auto sb_t) {
+    const uint32_t wv = cwv + vofs(sb_t);
     const int WO = iofs(sb_t);
-    u32x2 w[NPT];
-    if constexpr (NPT == 2)
-      asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:%c3\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(w[0]), "=&v"(w[NPT - 1]) : "v"(ra), "i"(CR * D) : "memory");
-    else
-      asm volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(w[0]) : "v"(ra) : "memory");
 #pragma unroll
     for (int i = 0; i < NPT; ++i) {
       const u32x4 b = cv8(w[i].x, w[i].y);
       asm volatile("ds_write_b128 %0, %1 offset:%c2" : : "v"(wv), "v"(b), "i"(WO + i * CR * ROWB) : "memory");
     }
+  };
+  auto read_codes = [&](int c) {
+    const uint32_t ra = cra + (c & (RowsLds<D, NW>::SLOTS - 1)) * TILE8B;
+    if constexpr (NPT == 2)
+      asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:%c3\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(w[0]), "=&v"(w[NPT - 1]) : "v"(ra), "i"(CR * D) : "memory");
+    else
+      asm volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(w[0]) : "v"(ra) : "memory");
   };
 
   float m[RB], l[RB];
@@ -207,27 +207,39 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
   clear();
 
   // ---- scores of tile c and what turns them into exponents: factor f (by row), addend lv = log2(V scale), iv = 1 / V
-  // scale. The LDS reads stand in assembly that waits for them alone (as plain loads they would wait for every DMA). ----
+  // scale. The LDS reads -- the V codes of tile c + 1 with them -- stand in assembly that waits for them alone (as plain
+  // loads they would wait for every DMA). ----
   float sc[RB][2][4], f[RB][2], lv[2], iv[2];
   auto scores = [&](int c, auto mask_t) {
     pr_prio<1>();
-    const int slot = c & (RowsLds<D>::SLOTS - 1), n0 = c * PR_KEYS;
-    const uint32_t ko = slot * TILE8B, so = s0 + slot * (4 * WAVE * 4);
+    const int slot = c & (RowsLds<D, NW>::SLOTS - 1), n0 = c * PR_KEYS;
+    const uint32_t ko = slot * TILE8B, so = s0 + slot * (NW * WAVE * 4);
+    const uint32_t ra = cra + ((c + 1) & (RowsLds<D, NW>::SLOTS - 1)) * TILE8B;
     i32x4 kop[2][KS];
     u32x2 s2[2];
-    if constexpr (KS == 2)
+    if constexpr (KS == 2 && NPT == 2)
       asm volatile(
-          "ds_read_b128 %0, %6\n\tds_read_b128 %1, %7\n\tds_read_b128 %2, %6 offset:%c9\n\tds_read_b128 %3, %7 offset:%c9\n\t"
-          "ds_read_b64 %4, %8\n\tds_read_b64 %5, %8 offset:%c10\n\ts_waitcnt lgkmcnt(0)"
-          : "=&v"(kop[0][0]), "=&v"(kop[0][KS - 1]), "=&v"(kop[1][0]), "=&v"(kop[1][KS - 1]), "=&v"(s2[0]), "=&v"(s2[1])
-          : "v"(kadr[0] + ko), "v"(kadr[KS - 1] + ko), "v"(so), "i"(16 * D), "i"(HW1 * WAVE * 4)
+          "ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\tds_read_b128 %2, %8 offset:%c12\n\tds_read_b128 %3, %9 offset:%c12\n\t"
+          "ds_read_b64 %4, %10\n\tds_read_b64 %5, %10 offset:%c13\n\tds_read_b64 %6, %11\n\tds_read_b64 %7, %11 offset:%c14\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(kop[0][0]), "=&v"(kop[0][KS - 1]), "=&v"(kop[1][0]), "=&v"(kop[1][KS - 1]), "=&v"(s2[0]), "=&v"(s2[1]),
+            "=&v"(w[0]), "=&v"(w[NPT - 1])
+          : "v"(kadr[0] + ko), "v"(kadr[KS - 1] + ko), "v"(so), "v"(ra), "i"(16 * D), "i"(HW1 * WAVE * 4), "i"(CR * D)
+          : "memory");
+    else if constexpr (KS == 2)
+      asm volatile(
+          "ds_read_b128 %0, %7\n\tds_read_b128 %1, %8\n\tds_read_b128 %2, %7 offset:%c11\n\tds_read_b128 %3, %8 offset:%c11\n\t"
+          "ds_read_b64 %4, %9\n\tds_read_b64 %5, %9 offset:%c12\n\tds_read_b64 %6, %10\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(kop[0][0]), "=&v"(kop[0][KS - 1]), "=&v"(kop[1][0]), "=&v"(kop[1][KS - 1]), "=&v"(s2[0]), "=&v"(s2[1]),
+            "=&v"(w[0])
+          : "v"(kadr[0] + ko), "v"(kadr[KS - 1] + ko), "v"(so), "v"(ra), "i"(16 * D), "i"(HW1 * WAVE * 4)
           : "memory");
     else
-      asm volatile(
-          "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%c6\n\tds_read_b64 %2, %5\n\tds_read_b64 %3, %5 offset:%c7\n\t"
-          "s_waitcnt lgkmcnt(0)"
-          : "=&v"(kop[0][0]), "=&v"(kop[1][0]), "=&v"(s2[0]), "=&v"(s2[1])
-          : "v"(kadr[0] + ko), "v"(so), "i"(16 * D), "i"(HW1 * WAVE * 4)
+      asm volatile(   // (NPT == 1)
+          "ds_read_b128 %0, %5\n\tds_read_b128 %1, %5 offset:%c8\n\tds_read_b64 %2, %6\n\tds_read_b64 %3, %6 offset:%c9\n\t"
+          "ds_read_b64 %4, %7\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(kop[0][0]), "=&v"(kop[1][0]), "=&v"(s2[0]), "=&v"(s2[1]), "=&v"(w[0])
+          : "v"(kadr[0] + ko), "v"(so), "v"(ra), "i"(16 * D), "i"(HW1 * WAVE * 4)
           : "memory");
 #pragma unroll
     for (int b = 0; b < 2; ++b)
@@ -255,12 +267,14 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
     }
     if (decltype(mask_t)::value && n0 + PR_KEYS > lim_lo) {  // a tile on the causal edge of some row
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
+      for (int rb = 0; rb < RB; ++rb) {
+        const int lim = L - Q + 1 + row_of(rb) / G;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (n0 + 16 * b + 4 * g + i >= lim[rb]) sc[rb][b][i] = -INFINITY;
+            if (n0 + 16 * b + 4 * g + i >= lim) sc[rb][b][i] = -INFINITY;
+      }
     }
   };
   // the row's largest exponent of the tile (the 4 lanes of a row agree)
@@ -282,13 +296,8 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const float e0 = lv[b] - m[rb];
-        float psum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], f[rb][b], e0));
-          psum += p[b][i];
-        }
-        l[rb] = __builtin_fmaf(psum, iv[b], l[rb]);
+        for (int i = 0; i < 4; ++i) p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], f[rb][b], e0));
       }
       u32x4 pw;
       pw.x = pack_bf16x2_rne(p[0][0], p[0][1]);
@@ -324,6 +333,17 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
           acc[rb][t0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rb], acc[rb][t0 + u], 0, 0, 0);
       }
     }
+    // the denominators come from the matrix cores too: row b of this operand picks the keys of half b, so that the sums of
+    // the rounded P by half stand in the lanes of group 0
+    u32x4 pw = {n == 0 ? 0x3f803f80u : 0u, 0u, n == 1 ? 0x3f803f80u : 0u, 0u};
+    pw.y = pw.x;
+    pw.w = pw.z;
+    const bf16x8 pick = *reinterpret_cast<bf16x8*>(&pw);
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pick, pop[rb], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      l[rb] = __builtin_fmaf(sum[0], iv[0], __builtin_fmaf(sum[1], iv[1], l[rb]));
+    }
   };
 
   if (c_hi > c_lo) {   // (uniform across the workgroup)
@@ -337,7 +357,8 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
       for (int j = 0; j < 3; ++j) issue(c_lo + j, id[j]);
       wait_vm<VMT * 2>();
       lds_barrier();
-      convert(c_lo, std::integral_constant<int, 0>{});
+      read_codes(c_lo);
+      convert(std::integral_constant<int, 0>{});
     };
     // tile c may be computed after this: its codes, scales and bf16 V are there for every wavefront, and so are tile c + 1's
     // codes (converted at the end of the tile); tile c + 3 is requested into the slots of tile c - 1
@@ -352,8 +373,10 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
       if (active) {
         scores(c, mask_t);
         softmax_pv(st_t);
+      } else {
+        read_codes(c + 1);
       }
-      convert(c + 1 < c_hi ? c + 1 : c, nx_t);
+      convert(nx_t);   // (past the last tile: old codes, not used)
       __builtin_amdgcn_sched_barrier(0);
     };
     const int J = min(c_hi, max(lim_lo, 0) / PR_KEYS);   // tiles below J have no key past any row's limit
@@ -364,8 +387,10 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) m[rb] = __builtin_fmaxf(row_top(rb), -1e30f);
       softmax_pv(std::integral_constant<int, 0>{});
+    } else {
+      read_codes(c_lo + 1);
     }
-    convert(c_lo + 1 < c_hi ? c_lo + 1 : c_lo, std::integral_constant<int, 1>{});
+    convert(std::integral_constant<int, 1>{});
     int c = c_lo + 1;
     const std::integral_constant<int, 0> st0;
     const std::integral_constant<int, 1> st1;
@@ -406,15 +431,20 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D>& lds, 
             for (int tt = 0; tt < VT; ++tt) acc[rb][tt] *= alpha;
           }
           softmax_pv((c - c_lo) & 1);
+        } else {
+          read_codes(c + 1);
         }
-        convert(c + 1 < c_hi ? c + 1 : c, (c + 1 - c_lo) & 1);
+        convert((c + 1 - c_lo) & 1);
       }
       wait_vm<0>();
       __syncthreads();   // (another piece may follow)
     }
   }
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) fin(rb, t[rb], hq[rb], valid[rb], m[rb], group4_sum(l[rb]), acc[rb]);
+  for (int rb = 0; rb < RB; ++rb) {
+    const int R = row_of(rb), t = R / G;
+    fin(rb, t, kvh * G + R - t * G, t < Q, m[rb], group4_sum(l[rb]), acc[rb]);
+  }
 }
 
 }  // namespace
