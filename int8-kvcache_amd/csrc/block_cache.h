@@ -18,18 +18,26 @@ constexpr int BLK_MIN = 16, BLK_MAX = 128;   // positions per scale
 // The request that holds slot u of a line on which request r starts at (cu[r] >> lg) + 2 r: as long as cu[r] counts
 // rows of consecutive positions, r's rows touch at most (rows >> lg) + 2 aligned blocks of 2^lg positions, so its
 // blocks fit before the next request's start wherever its first position lies in a block. A launch sizes its grid
-// from the row count alone. 64-way search, the lanes a probe each; every lane returns the same r.
-__device__ __forceinline__ int request_of_slot(const int* __restrict__ cu, int num_seqs, int lg, int u, int lane) {
+// from the row count alone. 64-way search, the lanes a request each at the end, whose cu[r], cu[r + 1] and of[r] come
+// with the same round trip to memory; uniform across the wavefront.
+struct SlotRequest {
+  int r, cu0, cu1, of;
+};
+__device__ __forceinline__ SlotRequest request_of_slot(const int* __restrict__ cu, const int* __restrict__ of, int num_seqs,
+                                                       int lg, int u, int lane) {
   int lo = 0, n = num_seqs;
-  while (n > 1) {
+  while (n > WAVE) {
     const int step = (n + WAVE - 1) / WAVE, r = lo + lane * step;
     const bool in = lane * step < n && (cu[r] >> lg) + 2 * r <= u;
     // (the first probe always holds: request lo starts at or before u)
-    const int k = __builtin_popcountll(__ballot(in)) - 1;
-    lo += max(k, 0) * step;
+    lo += max(__builtin_popcountll(__ballot(in)) - 1, 0) * step;
     n = min(step, num_seqs - lo);
   }
-  return __builtin_amdgcn_readfirstlane(lo);
+  const int r = lo + min(lane, n - 1);
+  const int c0 = cu[r], c1 = cu[r + 1], o = of[r];
+  const int k = max(__builtin_popcountll(__ballot(lane < n && (c0 >> lg) + 2 * r <= u)) - 1, 0);
+  return {__builtin_amdgcn_readfirstlane(lo) + k, __builtin_amdgcn_readlane(c0, k), __builtin_amdgcn_readlane(c1, k),
+          __builtin_amdgcn_readlane(o, k)};
 }
 inline int64_t block_slots(int64_t rows, int64_t num_seqs, int lg) { return (rows >> lg) + 2 * num_seqs; }
 
@@ -95,52 +103,60 @@ __global__ __launch_bounds__(WAVE * (W < 4 ? 4 : W)) void quant_block_kernel(Qua
   __shared__ float top[WPB][2];
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int item = blockIdx.x * (WPB / W) + wave / W, part = wave % W;
+  // three dependent round trips to memory, no more: the request; its rows and the page id; the block as it is
   bool live = item < a.items;
-  int h = 0, p0 = 0, first = 0, last = 0, tok0 = 0, page = 0, off = 0;
-  if (live) {
-    const int u = item / a.heads;
-    h = item - u * a.heads;
-    const int r = request_of_slot(a.cu_q, a.num_seqs, a.lg, u, lane);
-    const int tok = a.cu_q[r], q = min(a.cu_q[r + 1], a.num_tokens) - tok, len = a.seq_lens[r];
-    p0 = len - (a.cu_q[r + 1] - tok);                                     // first new position (negative ones: no slot)
-    const int blk = (max(p0, 0) >> a.lg) + u - ((tok >> a.lg) + 2 * r);   // the item's block of the request's positions
-    const int b0 = blk << a.lg;
-    first = max(max(p0, 0), b0);                                          // new positions [first, last) of the block
-    last = min(p0 + q, b0 + (1 << a.lg));
-    live = first < last;
-    if (live) {
-      page = page_at(a.block_table, a.bt_stride, r, b0 >> a.lbs);
-      live = page >= 0 && page < a.num_blocks;                            // a bad id: nothing is written
-    }
-    off = b0 & ((1 << a.lbs) - 1);                                        // the block's first slot of the page
-    tok0 = tok - p0;                                                      // token of position p: tok0 + p
-    p0 = b0;
-  }
+  int h = 0, b0 = 0, first = 0, last = 0, page = 0, off = 0;
+  int64_t tok0 = 0;
   const int row = lane / LPR, d0 = 8 * (lane % LPR);
   u32x4 kin[N], vin[N];
   u32x2 kold[N], vold[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    kin[j] = vin[j] = u32x4{0u, 0u, 0u, 0u};
+    kold[j] = vold[j] = u32x2{0u, 0u};
+  }
+  if (live) {
+    const int u = item / a.heads;
+    h = item - u * a.heads;
+    const SlotRequest q = request_of_slot(a.cu_q, a.seq_lens, a.num_seqs, a.lg, u, lane);
+    const int p0 = q.of - (q.cu1 - q.cu0);                                 // first new position (negative ones: no slot)
+    b0 = ((max(p0, 0) >> a.lg) + u - ((q.cu0 >> a.lg) + 2 * q.r)) << a.lg; // the item's block of the request's positions
+    first = max(max(p0, 0), b0);                                           // its new positions: [first, last)
+    last = min(p0 + min(q.cu1, a.num_tokens) - q.cu0, b0 + (1 << a.lg));
+    tok0 = (int64_t)q.cu0 - p0;                                            // token of position p: tok0 + p
+    live = first < last;
+    if (live) {
+      const int id = a.block_table[(int64_t)q.r * a.bt_stride + (b0 >> a.lbs)];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int p = b0 + 16 * part + row + RPL * j;
+        if (p >= first && p < last) {
+          kin[j] = *reinterpret_cast<const u32x4*>(a.key + (tok0 + p) * a.key_st + (int64_t)h * a.key_sh + d0);
+          vin[j] = *reinterpret_cast<const u32x4*>(a.value + (tok0 + p) * a.val_st + (int64_t)h * a.val_sh + d0);
+        }
+      }
+      page = __builtin_amdgcn_readfirstlane(id);
+      live = page >= 0 && page < a.num_blocks;                             // a bad id: nothing is written
+      page = live ? page : 0;
+    }
+    off = b0 & ((1 << a.lbs) - 1);                                         // the block's first slot of the page
+  }
   int8_t* kc = a.kc + (int64_t)page * a.kc_sb + (int64_t)(off + 16 * part) * a.kc_sn + (int64_t)h * a.kc_sh + d0;
   int8_t* vc = a.vc + (int64_t)page * a.vc_sb + (int64_t)(off + 16 * part) * a.vc_sn + (int64_t)h * a.vc_sh + d0;
-  const bool begun = live && first > p0;                                  // earlier positions of the request share the block
+  const bool begun = live && first > b0;                                   // earlier positions of the request share the block
   float km = 0.f, vm = 0.f, ks_old = 0.f, vs_old = 0.f;
   float* ksp = a.ks + (int64_t)page * a.s_sb + (int64_t)h * a.s_sh + (int64_t)(off >> a.lg) * a.s_sg;
   float* vsp = a.vs + (int64_t)page * a.s_sb + (int64_t)h * a.s_sh + (int64_t)(off >> a.lg) * a.s_sg;
   if (begun) {
     ks_old = *ksp;
     vs_old = *vsp;
-  }
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int i = row + RPL * j, p = p0 + 16 * part + i;
-    kin[j] = vin[j] = u32x4{0u, 0u, 0u, 0u};
-    kold[j] = vold[j] = u32x2{0u, 0u};
-    if (live && p >= first && p < last) {
-      const int64_t t = tok0 + p;
-      kin[j] = *reinterpret_cast<const u32x4*>(a.key + t * a.key_st + (int64_t)h * a.key_sh + d0);
-      vin[j] = *reinterpret_cast<const u32x4*>(a.value + t * a.val_st + (int64_t)h * a.val_sh + d0);
-    } else if (begun && p < first) {
-      kold[j] = *reinterpret_cast<const u32x2*>(kc + (int64_t)i * a.kc_sn);
-      vold[j] = *reinterpret_cast<const u32x2*>(vc + (int64_t)i * a.vc_sn);
+    for (int j = 0; j < N; ++j) {
+      const int i = row + RPL * j;
+      if (b0 + 16 * part + i < first) {
+        kold[j] = *reinterpret_cast<const u32x2*>(kc + (int64_t)i * a.kc_sn);
+        vold[j] = *reinterpret_cast<const u32x2*>(vc + (int64_t)i * a.vc_sn);
+      }
     }
   }
 #pragma unroll
@@ -172,7 +188,7 @@ __global__ __launch_bounds__(WAVE * (W < 4 ? 4 : W)) void quant_block_kernel(Qua
   const float ky = 1.f / ks, vy = 1.f / vs, kr = ks_old / ks, vr = vs_old / vs;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int i = row + RPL * j, p = p0 + 16 * part + i;
+    const int i = row + RPL * j, p = b0 + 16 * part + i;
     u32x2* kp = reinterpret_cast<u32x2*>(kc + (int64_t)i * a.kc_sn);
     u32x2* vp = reinterpret_cast<u32x2*>(vc + (int64_t)i * a.vc_sn);
     if (p >= first && p < last) {
@@ -209,8 +225,8 @@ __global__ __launch_bounds__(256) void read_block_kernel(ReadBlockArgs a) {
   const int item = blockIdx.x * 4 + wave;
   if (item >= a.items) return;
   const int u = item / a.heads, h = item - u * a.heads;
-  const int r = request_of_slot(a.cu_k, a.num_seqs, 4, u, lane);
-  const int row0 = a.cu_k[r], n = min(a.cu_k[r + 1], a.num_rows) - row0, start = a.start[r];
+  const SlotRequest q = request_of_slot(a.cu_k, a.start, a.num_seqs, 4, u, lane);
+  const int r = q.r, row0 = q.cu0, n = min(q.cu1, a.num_rows) - row0, start = q.of;
   if (start < 0) return;
   const int b0 = ((start >> 4) + u - ((row0 >> 4) + 2 * r)) << 4;
   const int first = max(start, b0), last = min(start + n, b0 + 16);

@@ -91,10 +91,11 @@ def quant_block_cache(key, value, key_cache, value_cache, scales, cu_seqlens_q, 
     never shrink while a block is being filled (positions written again after a rollback, too); they start anew when the
     block's first position is written. Infinities saturate and do not count for the scale. The pages written must belong
     to one request each."""
-    name, n, num_seqs = "quant_block_cache", key.shape[0], cu_seqlens_q.shape[0] - 1
+    name = "quant_block_cache"
     if ck._served(ck.ext(), name, key, value, key_cache, value_cache, scales["k_scale"], scales["v_scale"], cu_seqlens_q,
                   seq_lens, block_table):
         return
+    n, num_seqs = key.shape[0], cu_seqlens_q.shape[0] - 1
     _check(key.dim() == 3 and key.shape == value.shape and key.stride(2) == 1 and value.stride(2) == 1 and
            key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16,
            f"{name}: key / value must be bf16 [T, kv_heads, D] with a contiguous last dim")
@@ -114,10 +115,11 @@ def read_block_cache(key_cache, value_cache, scales, starts, cu_seqlens_k, block
     """Read keys back: positions starts[r] .. of request r become rows cu_seqlens_k[r] .. cu_seqlens_k[r + 1] - 1 of
     key_out / value_out (bf16 [N, kv heads, D], N at least cu_seqlens_k[-1]; rows behind are left as they were).
     Returns (key_out, value_out)."""
-    name, num_seqs = "read_block_cache", cu_seqlens_k.shape[0] - 1
+    name = "read_block_cache"
     if ck._served(ck.ext(), name, key_cache, value_cache, scales["k_scale"], scales["v_scale"], starts, cu_seqlens_k,
                   block_table, key_out, value_out):
         return key_out, value_out
+    num_seqs = cu_seqlens_k.shape[0] - 1
     k, v, geom, sc = _cache_args(name, key_cache, value_cache, scales)
     for t in (key_out, value_out):
         _check(t.dim() == 3 and t.dtype == torch.bfloat16 and t.stride(2) == 1 and t.shape[1:] == key_cache.shape[2:] and
@@ -148,11 +150,12 @@ def block_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, blo
     decode_attention's arguments: out rows softmax(q k^T softmax_scale) v, bottom-right causal, of the cached values and
     the bf16 q (neither q nor the softmax's weights are rounded to 8 bits). A row that sees no key is zero. segm:
     split buffers (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces."""
-    name, num_seqs = "block_decode_attention", cu_seqlens_q.shape[0] - 1
+    name = "block_decode_attention"
     so, sm, ss = segm if segm is not None else (None, None, None)
     if ck._served(ck.ext(), name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
                   scales["v_scale"], softmax_scale, so, sm, ss, max_query_len, ck.SHORT_Q, ck.MAX_SPLITS):
         return out
+    num_seqs = cu_seqlens_q.shape[0] - 1
     k, v, geom, sc = _cache_args(name, k_cache, v_cache, scales)
     _check_attention(name, q, k_cache, out, cu_seqlens_q, seq_lens, block_table)
     hq, d = q.shape[1:]
