@@ -2555,12 +2555,12 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // ---- per tile: scores (QK) and each row's largest, masked for the keys past a row's limit ----
   f32x4 sc[RB][2];
   float lmax[RB], top[RB];
-  // BLK: a half tile's entry (K scale, log2 of the V scale, 1 / V scale, 0) of the temporary cache's table, uniform; those of
-  // the next tile are requested a tile before their use
+  // BLK: a half tile's entry (K scale, log2 of the V scale, 1 / V scale, 0) of the temporary cache's table, uniform; asked
+  // for ahead of the tile's scores (a tile earlier they took 8 more scalar registers, and the loop spilled)
   const f32x4* stab = nullptr;
-  f32x4 ent[2], ent_next[2];
+  f32x4 ent[2];
   if constexpr (BLK) stab = a.s_table + (int64_t)kvh * (int64_t)a.num_blocks * ((bsm + 1) / 16);
-  auto next_entries = [&](int c) {
+  auto entries = [&](int c) {
     if constexpr (BLK) {
       const int k0 = min(c, c_hi - 1) * PR_KEYS, k1 = min(k0 + 16, max(kend - 1, 0));
       int p0 = pfirst + (k0 >> a.lbs), p1 = pfirst + (k1 >> a.lbs);
@@ -2571,8 +2571,8 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
         p1 = (p1 >= 0 && p1 < a.num_blocks) ? p1 : 0;
       }
       const auto* t = (const __attribute__((address_space(4))) f32x4*)stab;
-      ent_next[0] = t[((int64_t)p0 << (a.lbs - 4)) + ((k0 & bsm) >> 4)];
-      ent_next[1] = t[((int64_t)p1 << (a.lbs - 4)) + ((k1 & bsm) >> 4)];
+      ent[0] = t[((int64_t)p0 << (a.lbs - 4)) + ((k0 & bsm) >> 4)];
+      ent[1] = t[((int64_t)p1 << (a.lbs - 4)) + ((k1 & bsm) >> 4)];
     }
   };
   // K operand reads from inline assembly, each statement waiting for its own reads: as plain loads
@@ -2583,11 +2583,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   auto scores = [&](auto st_t, int c, auto mask_t) {
     pr_prio<1>();
     const int n0 = c * PR_KEYS;
-    if constexpr (BLK) {
-      ent[0] = ent_next[0];
-      ent[1] = ent_next[1];
-      next_entries(c + 1);
-    }
+    entries(c);
     uint32_t ad[DS];
 #pragma unroll
     for (int s = 0; s < DS; ++s) ad[s] = kadr[s] + stage_vofs(st_t);
@@ -2711,6 +2707,11 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     // waiting for its own reads: the compiler would otherwise make them wait for every LDS DMA in
     // flight (it cannot tell they read another ring stage), emptying the ring each tile.
     typedef unsigned long long u64;
+    // BLK: the addresses from channel tile 0's each time (the row's swizzle is even, so tile tt's chunk is that of tile 0 with
+    // tt's bits flipped): held in registers they would leave the tile loop short of them
+    uint32_t vbase = vadr[0];
+    if constexpr (BLK) asm volatile("" : "+v"(vbase));
+    auto va = [&](int tt) { return BLK ? (vbase ^ (32u * tt)) : vadr[tt]; };
 #pragma unroll
     for (int t0 = 0; t0 < VT; t0 += 4) {
       u64 lo[4], hi[4];
@@ -2725,7 +2726,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
           "ds_read_b64_tr_b16 %7, %11 offset:%c13\n"
           "s_waitcnt lgkmcnt(0)"
           : "=&v"(lo[0]), "=&v"(hi[0]), "=&v"(lo[1]), "=&v"(hi[1]), "=&v"(lo[2]), "=&v"(hi[2]), "=&v"(lo[3]), "=&v"(hi[3])
-          : "v"(vadr[t0] + so), "v"(vadr[t0 + 1] + so), "v"(vadr[t0 + 2] + so), "v"(vadr[t0 + 3] + so), "i"(SOI),
+          : "v"(va(t0) + so), "v"(va(t0 + 1) + so), "v"(va(t0 + 2) + so), "v"(va(t0 + 3) + so), "i"(SOI),
             "i"(SOI + 16 * ROWB)
           : "memory");
 #pragma unroll
@@ -2768,7 +2769,6 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     // its int8 stage (c % NS8), tiles counted from c_lo.
     // the first tiles' DMA; I8: NS8 tiles in flight, tile 0 converted once it has landed
     auto prologue = [&]() {
-      next_entries(c_lo);
       if constexpr (I8) {
 #pragma unroll
         for (int j = 0; j < NS8; ++j) issue(c_lo + j, j, linear);
