@@ -661,10 +661,11 @@ __global__ __launch_bounds__(256) void block_attn_kernel(BlockAttnArgs args) {
 // Many query rows (block_rows.h). block_verify_kernel: short queries of more rows than block_attn_kernel's tiles suit, on
 // its plan, in pieces of 64 rows. block_prefill_kernel: the work lists of long queries, 128 rows an entry.
 // ------------------------------------------------------------------------------------------------
-template <int D>
-__global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args) {
+constexpr int64_t BLOCK_VERIFY_ONE_GROUP = 128;   // (request, kv head) pairs of a cut batch from which one group is faster
+template <int D, int KW>
+__global__ __launch_bounds__(256 * KW, KW == 1 ? 3 : 2) void block_verify_kernel(BlockAttnArgs args) {
   touch_args();
-  __shared__ __attribute__((aligned(1024))) RowsLds<D, 4> lds;
+  __shared__ __attribute__((aligned(1024))) RowsLds<D, 4> lds[KW];
   const int lane = threadIdx.x & (WAVE - 1), n = lane & 15, g = lane >> 4;
   walk_pieces(args.a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
     const AttnArgs& a = fresh_args();
@@ -672,7 +673,7 @@ __global__ __launch_bounds__(256, 3) void block_verify_kernel(BlockAttnArgs args
     const RowsView v{a.q, a.kc + (int64_t)kvh * a.k_sh, a.vc + (int64_t)kvh * a.v_sh, a.block_table + (int64_t)r * a.bt_stride,
                      s.ks + (int64_t)kvh * s.sh, s.vs + (int64_t)kvh * s.sh, a.q_st, a.q_sh, a.k_sb, a.k_sn, a.v_sb, a.v_sn,
                      s.sb, s.sg, a.sm_log2, a.G, a.num_blocks, a.lbs, s.lg};
-    attend_rows<D, 4, 1>(v, lds, w.tok, w.qlen, w.len, kvh, 64 * rg, c0, w.len > 0 ? c1 : c0, min(w.len, c1 * PR_KEYS),
+    attend_rows<D, 4, 1, KW>(v, lds, w.tok, w.qlen, w.len, kvh, 64 * rg, c0, w.len > 0 ? c1 : c0, min(w.len, c1 * PR_KEYS),
                       [&](int, int t, int hq, bool valid, float m, float l, const f32x4 (&acc)[D / 16]) {
       if (!valid) return;
       const AttnArgs& o = fresh_args();
@@ -717,7 +718,7 @@ constexpr int BLOCK_PREFILL_WAVES = D == 128 ? 8 : 4;
 template <int D, bool SPLIT>
 __global__ __launch_bounds__(WAVE * BLOCK_PREFILL_WAVES<D>, 4) void block_prefill_kernel(BlockPrefillArgs args) {
   constexpr int NW = BLOCK_PREFILL_WAVES<D>, RB = PR_ROWS / (16 * NW);
-  __shared__ __attribute__((aligned(1024))) RowsLds<D, NW> lds;
+  __shared__ __attribute__((aligned(1024))) RowsLds<D, NW> lds[1];
   const PrefillArgs& a = args.p;
   const BlockScales& s = args.s;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 15, g = lane >> 4;
@@ -736,7 +737,7 @@ __global__ __launch_bounds__(WAVE * BLOCK_PREFILL_WAVES<D>, 4) void block_prefil
                    a.q_sh, a.k_sb, a.k_sn, a.v_sb, a.v_sn, s.sb, s.sg, a.sm_log2, a.G, a.num_blocks, a.lbs, s.lg};
   bool piece = false;
   int pslot = 0;
-  attend_rows<D, NW, RB>(v, lds, tok, Q, L, kvh, row0, c_lo, c_hi, kend,
+  attend_rows<D, NW, RB, 1>(v, lds, tok, Q, L, kvh, row0, c_lo, c_hi, kend,
                         [&](int rb, int t, int hq, bool valid, float m, float l, const f32x4 (&acc)[D / 16]) {
     if constexpr (SPLIT) {
       if (rb == 0) {   // read here, not held through the tile loop
@@ -915,10 +916,18 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   const bool pack = rows <= 8;
   const int rt = (int)std::min<int64_t>(MAX_ROW_TILES, (rows + 15) / 16);
   const Tuning tune = read_tuning();
-  const bool many = rows > 32 && !(tune.rows32 && atoi(tune.rows32) == 0);
+  // many rows (attn_rules.h) share each tile through LDS: one group of wavefronts a workgroup, three workgroups a CU, where
+  // the batch is cut into enough pieces for that (us, one and two groups: 64 x 8 tokens of 28 / 4 heads at 512 to 8,192 keys
+  // 72.0 and 78.9, 32 x 4 at 4,096 39.7 and 45.7, 64 x 8 of 32 / 8 80.4 and 87.5), else two groups that share a piece's
+  // tiles (16 x 8 at 1,000 to 3,000 27.5 and 23.3, 64 decode rows of 32 / 1 41.8 and 38.1; whole segments 64 x 8 at 4,096
+  // 103 and 77). KVQ_V32_KSPLIT sets the groups, KVQ_ROWS32=0 takes block_attn_kernel for every row count.
+  const int64_t pairs = num_seqs * num_kv_heads;
+  const bool cut = num_splits > 1 && segm_rows > 0;
+  const bool many = verify_rows(rows, pairs, cut) && !(tune.rows32 && atoi(tune.rows32) == 0);
+  const int kw = tune.v32_ksplit ? v32_key_splits(tune) : cut && pairs >= BLOCK_VERIFY_ONE_GROUP ? 1 : 2;
   const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
                      : num_splits == 1 || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? MAX_ROW_TILES : DEFAULT_KSPLIT;
-  const int ks = many ? 1 : std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = many ? 4 : rt * ks;
+  const int ks = many ? 1 : std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = many ? 4 * kw : rt * ks;
   BlockAttnArgs b;
   b.s = block_scales(k_scale, v_scale, s_sb, s_sh, s_sg, group);
   AttnArgs& a = b.a;
@@ -938,19 +947,19 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   a.max_splits = (int)num_splits;
   a.cut_rows = num_splits > 1 ? (int)std::min<int64_t>(segm_rows, INT32_MAX) : 0;
   a.rt = many ? 4 : rt; a.ksplit = ks; a.waves = waves;
-  a.min_tiles = MIN_SPLIT_TILES;
+  a.min_tiles = many ? MIN_SPLIT_TILES * kw : MIN_SPLIT_TILES;
   a.coop = coop_tiles(num_splits > 1, ks);
   a.xcd_order = tune.xcd_order ? atoi(tune.xcd_order) : 1;
   a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
                                        : (int)PLAN_FAST_MAX;
-  a.seg_cost = seg_cost_units(tune, 0);
+  a.seg_cost = seg_cost_units(tune, many ? 2 : 0);
   const size_t lds = many ? 0 : (size_t)(ks - 1) * rt * MERGE_FIELDS * WAVE * sizeof(float);
-  void (*kern)(BlockAttnArgs) = many ? (head_dim == 128 ? block_verify_kernel<128> : block_verify_kernel<64>)
+  void (*kern)(BlockAttnArgs) = many ? (head_dim == 128 ? (kw == 2 ? block_verify_kernel<128, 2> : block_verify_kernel<128, 1>)
+                                     : (kw == 2 ? block_verify_kernel<64, 2> : block_verify_kernel<64, 1>))
                               : head_dim == 128 ? (pack ? block_attn_kernel<128, 2, true> : block_attn_kernel<128, 2, false>)
                                                 : (pack ? block_attn_kernel<64, 2, true> : block_attn_kernel<64, 2, false>);
-  const bool cuttable_any = num_splits > 1 && segm_rows > 0;
   const int64_t tw = target_waves > 0 ? target_waves
-                     : cuttable_any   ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
+                     : cut            ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
                                       : (int64_t)device_cus() * waves;
   a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(tw / waves, INT32_MAX));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

@@ -10,7 +10,7 @@
 // its integers to O, which at 32 keys a tile costs more than the conversion of V by all the wavefronts). K in int8 also
 // halves the LDS reads of the QK operands, of which every wavefront needs the whole tile.
 //
-// The tile's codes and scales come by DMA into LDS rings of four slots, up to three tiles ahead; V is converted into one of
+// The tiles' codes and scales come by DMA into LDS rings of four slots, up to three tiles ahead; V is converted into one of
 // two bf16 stages, a tile ahead of its use; one barrier a tile. The first tile sets each row's reference maximum, later
 // tiles only accumulate, and a workgroup in which some row's scores then grew out of range is done again with rescaling
 // (prefill_body's scheme).
@@ -45,6 +45,7 @@ struct RowsView {
   int G, num_blocks, lbs, lg;
 };
 
+// A group's rings: the codes and scales of four tiles, V as bf16 of the one computed and the next.
 template <int D, int NW>
 struct RowsLds {
   static constexpr int SLOTS = 4;
@@ -56,8 +57,9 @@ struct RowsLds {
 
 // Rows row0 .. of request rows (tok, Q tokens, L keys) over tiles [c_lo, c_hi), whose last key is below kend. fin(rb, t,
 // hq, valid, m, l, acc): row block rb's result in the lane of row n, channels 16 tt + 4 g + i in acc[tt][i].
-template <int D, int NW, int RB, typename Fin>
-__device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& lds, int tok, int Q, int L, int kvh, int row0,
+// KW groups of NW wavefronts take the tiles in turn, each with rings of its own, and the first joins their results.
+template <int D, int NW, int RB, int KW, typename Fin>
+__device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&lds_all)[KW], int tok, int Q, int L, int kvh, int row0,
                                             int c_lo, int c_hi, int kend, Fin&& fin) {
   constexpr int KS = D / 64;                // QK steps of 64 channels
   constexpr int VT = D / 16;                // PV channel tiles
@@ -67,9 +69,14 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
   constexpr int TILE8B = PR_KEYS * D, PPM = TILE8B / 1024;   // DMA instructions per int8 matrix and tile
   constexpr int IPW = 2 * PPM / NW, VMT = IPW + 1;           // per wavefront and tile; with the scales
   constexpr int RPI = 1024 / D;             // int8 rows per DMA instruction
-  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int lane = threadIdx.x & (WAVE - 1), wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int wave = wave_all % NW, kw = wave_all / NW;
+  using Lds = RowsLds<D, NW>;
+  Lds& lds = lds_all[kw];
   const int n = lane & 15, g = lane >> 4;
   const int G = a.G;
+  const int steps = (c_hi - c_lo + KW - 1) / KW;     // every group's tiles: one past the last is not computed
+  auto tile_of = [&](int i) { return c_lo + kw + i * KW; };
   const int wrow0 = row0 + wave * 16 * RB;
   const bool active = wrow0 < Q * G;        // else the wavefront only moves and converts tiles
   // the lane's row of block rb: its token of the request (found again where it is needed, not held through the tiles)
@@ -131,22 +138,24 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
   // the id of the page that this wavefront's half of tile c lies in, read a tile before its use; half 1 past the last key
   // takes the last key's page
   auto key_of = [&](int c) { return half ? min(c * PR_KEYS + 16, kend - 1) : c * PR_KEYS; };
-  auto page_id = [&](int c) { return ((const __attribute__((address_space(4))) int*)a.bt)[key_of(min(c, c_hi - 1)) >> a.lbs]; };
-  auto issue = [&](int c, int id) {
-    c = min(c, c_hi - 1);   // past the end: the last tile again, into a free slot or over itself
+  auto page_id = [&](int i) {
+    return ((const __attribute__((address_space(4))) int*)a.bt)[key_of(min(tile_of(i), c_hi - 1)) >> a.lbs];
+  };
+  auto issue = [&](int i, int id) {
+    const int c = min(tile_of(i), c_hi - 1);   // past the end: the last tile again
     int p = __builtin_amdgcn_readfirstlane(id);
     p = p >= 0 && p < a.num_blocks ? p : 0;
-    const int slot = c & (RowsLds<D, NW>::SLOTS - 1), o = (c * PR_KEYS + 16 * half) & bsm;
+    const int slot = i & (Lds::SLOTS - 1), o = (c * PR_KEYS + 16 * half) & bsm;
     const float* sp = sbase + ((int64_t)p * a.s_sb + (int64_t)((key_of(c) & bsm) >> a.lg) * a.s_sg);
     __builtin_amdgcn_global_load_lds((const void*)sp, (__attribute__((address_space(3))) void*)(&lds.sc[slot][wave][0]), 4, 0, 0);
 #pragma unroll
-    for (int i = 0; i < IPW; ++i) {
-      const int mat = (wave + NW * i) / PPM;   // uniform
+    for (int k = 0; k < IPW; ++k) {
+      const int mat = (wave + NW * k) / PPM;   // uniform
       const int8_t* b = mat ? a.vc + ((int64_t)p * a.v_sb + (int64_t)o * a.v_sn) : a.kc + ((int64_t)p * a.k_sb + (int64_t)o * a.k_sn);
       uint8_t* dst = (mat ? lds.v8[slot] : lds.k8[slot]) + 1024 * part;
       asm volatile("" : "+s"(b));
-      asm volatile("" : "+v"(o8[i]));
-      __builtin_amdgcn_global_load_lds((const void*)(b + (uint64_t)o8[i]), (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+      asm volatile("" : "+v"(o8[k]));
+      __builtin_amdgcn_global_load_lds((const void*)(b + (uint64_t)o8[k]), (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
     }
   };
 
@@ -164,7 +173,7 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
   // ---- V codes of tile c -> bf16 stage sb: thread x takes the 8-channel chunk x % CH of rows x / CH + CR i ----
   constexpr int CR = NW * WAVE / CH, NPT = PR_KEYS / CR;
   static_assert((CR % CH == 0 || NPT == 1) && NPT * CR == PR_KEYS && (NPT == 1 || NPT == 2), "conversion share");
-  const int cc = threadIdx.x % CH, crow = threadIdx.x / CH;
+  const int cx = wave * WAVE + lane, cc = cx % CH, crow = cx / CH;
   const uint32_t cra = (uint32_t)(uintptr_t)(&lds.v8[0][0]) + crow * D + 8 * cc, cwv = v0 + crow * ROWB + 16 * (cc ^ vswz(crow));
   auto vofs = [](auto st_t) -> uint32_t {
     if constexpr (std::is_same_v<decltype(st_t), int>) return (uint32_t)(st_t * TILEB);
@@ -184,8 +193,8 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
       asm volatile("ds_write_b128 %0, %1 offset:%c2" : : "v"(wv), "v"(b), "i"(WO + i * CR * ROWB) : "memory");
     }
   };
-  auto read_codes = [&](int c) {
-    const uint32_t ra = cra + (c & (RowsLds<D, NW>::SLOTS - 1)) * TILE8B;
+  auto read_codes = [&](int i) {
+    const uint32_t ra = cra + (i & (Lds::SLOTS - 1)) * TILE8B;
     if constexpr (NPT == 2)
       asm volatile("ds_read_b64 %0, %2\n\tds_read_b64 %1, %2 offset:%c3\n\ts_waitcnt lgkmcnt(0)"
                    : "=&v"(w[0]), "=&v"(w[NPT - 1]) : "v"(ra), "i"(CR * D) : "memory");
@@ -206,15 +215,15 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
   };
   clear();
 
-  // ---- scores of tile c and what turns them into exponents: factor f (by row), addend lv = log2(V scale), iv = 1 / V
-  // scale. The LDS reads -- the V codes of tile c + 1 with them -- stand in assembly that waits for them alone (as plain
+  // ---- scores of the group's tile i and what turns them into exponents: factor f (by row), addend lv = log2(V scale), iv = 1 / V
+  // scale. The LDS reads -- the V codes of tile i + 1 with them -- stand in assembly that waits for them alone (as plain
   // loads they would wait for every DMA). ----
   float sc[RB][2][4], f[RB][2], lv[2], iv[2];
-  auto scores = [&](int c, auto mask_t) {
+  auto scores = [&](int i, auto mask_t) {
     pr_prio<1>();
-    const int slot = c & (RowsLds<D, NW>::SLOTS - 1), n0 = c * PR_KEYS;
+    const int slot = i & (Lds::SLOTS - 1), n0 = tile_of(i) * PR_KEYS;
     const uint32_t ko = slot * TILE8B, so = s0 + slot * (NW * WAVE * 4);
-    const uint32_t ra = cra + ((c + 1) & (RowsLds<D, NW>::SLOTS - 1)) * TILE8B;
+    const uint32_t ra = cra + ((i + 1) & (Lds::SLOTS - 1)) * TILE8B;
     i32x4 kop[2][KS];
     u32x2 s2[2];
     if constexpr (KS == 2 && NPT == 2)
@@ -351,55 +360,57 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
     auto prologue = [&] {
       int id[3];
 #pragma unroll
-      for (int j = 0; j < 3; ++j) id[j] = page_id(c_lo + j);
-      ahead = page_id(c_lo + 3);
+      for (int j = 0; j < 3; ++j) id[j] = page_id(j);
+      ahead = page_id(3);
 #pragma unroll
-      for (int j = 0; j < 3; ++j) issue(c_lo + j, id[j]);
+      for (int j = 0; j < 3; ++j) issue(j, id[j]);
       wait_vm<VMT * 2>();
       lds_barrier();
-      read_codes(c_lo);
+      read_codes(0);
       convert(std::integral_constant<int, 0>{});
     };
-    // tile c may be computed after this: its codes, scales and bf16 V are there for every wavefront, and so are tile c + 1's
-    // codes (converted at the end of the tile); tile c + 3 is requested into the slots of tile c - 1
-    auto next_tile = [&](int c) {
+    // tile i may be computed after this: its codes, scales and bf16 V are there for every wavefront, and so are tile i + 1's
+    // codes (converted at the end of the tile); tile i + 3 is requested into the slots of tile i - 1
+    auto next_tile = [&](int i) {
       wait_vm<VMT>();
       lds_barrier();
-      issue(c + 3, ahead);
-      ahead = page_id(c + 4);
+      issue(i + 3, ahead);
+      ahead = page_id(i + 4);
     };
-    auto tile = [&](int c, auto st_t, auto nx_t, auto mask_t) {   // bf16 stage of tile c, and of tile c + 1
-      next_tile(c);
-      if (active) {
-        scores(c, mask_t);
+    auto mine = [&](int i) { return active && (KW == 1 || tile_of(i) < c_hi); };
+    auto tile = [&](int i, auto st_t, auto nx_t, auto mask_t) {   // bf16 stage of tile i, and of tile i + 1
+      next_tile(i);
+      if (mine(i)) {
+        scores(i, mask_t);
         softmax_pv(st_t);
       } else {
-        read_codes(c + 1);
+        read_codes(i + 1);
       }
       convert(nx_t);   // (past the last tile: old codes, not used)
       __builtin_amdgcn_sched_barrier(0);
     };
-    const int J = min(c_hi, max(lim_lo, 0) / PR_KEYS);   // tiles below J have no key past any row's limit
+    // the group's tiles below J have no key past any row's limit
+    const int J = min(steps, (min(c_hi, max(lim_lo, 0) / PR_KEYS) - c_lo - kw + KW - 1) / KW);
     prologue();
-    next_tile(c_lo);
-    if (active) {
-      scores(c_lo, std::true_type{});
+    next_tile(0);
+    if (mine(0)) {
+      scores(0, std::true_type{});
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) m[rb] = __builtin_fmaxf(row_top(rb), -1e30f);
       softmax_pv(std::integral_constant<int, 0>{});
     } else {
-      read_codes(c_lo + 1);
+      read_codes(1);
     }
     convert(std::integral_constant<int, 1>{});
-    int c = c_lo + 1;
+    int i = 1;
     const std::integral_constant<int, 0> st0;
     const std::integral_constant<int, 1> st1;
-    // (J and `active` are the wavefront's own; every wavefront runs each tile's barrier and conversion once)
-    for (; c + 2 <= J; c += 2) {
-      tile(c, st1, st0, std::false_type{});
-      tile(c + 1, st0, st1, std::false_type{});
+    // (J and `active` are the wavefront's own; every wavefront runs each step's barrier and conversion once)
+    for (; i + 2 <= J; i += 2) {
+      tile(i, st1, st0, std::false_type{});
+      tile(i + 1, st0, st1, std::false_type{});
     }
-    for (; c < c_hi; ++c) tile(c, (c - c_lo) & 1, (c + 1 - c_lo) & 1, std::true_type{});
+    for (; i < steps; ++i) tile(i, i & 1, (i + 1) & 1, std::true_type{});
     wait_vm<0>();
     bool jump = false;
 #pragma unroll
@@ -410,16 +421,16 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
 #pragma unroll
       for (int tt = 0; tt < VT; ++tt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[rb][tt][i], 0.f, z);
+        for (int e = 0; e < 4; ++e) z = __builtin_fmaf(acc[rb][tt][e], 0.f, z);
       jump |= z != 0.f;
     }
     if (__syncthreads_or(jump)) {
       clear();
       prologue();
-      for (c = c_lo; c < c_hi; ++c) {
-        next_tile(c);
-        if (active) {
-          scores(c, std::true_type{});
+      for (i = 0; i < steps; ++i) {
+        next_tile(i);
+        if (mine(i)) {
+          scores(i, std::true_type{});
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
             const float top = row_top(rb);
@@ -430,20 +441,57 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW>& l
 #pragma unroll
             for (int tt = 0; tt < VT; ++tt) acc[rb][tt] *= alpha;
           }
-          softmax_pv((c - c_lo) & 1);
+          softmax_pv(i & 1);
         } else {
-          read_codes(c + 1);
+          read_codes(i + 1);
         }
-        convert((c + 1 - c_lo) & 1);
+        convert((i + 1) & 1);
       }
       wait_vm<0>();
-      __syncthreads();   // (another piece may follow)
+      __syncthreads();   // (the rings may be written again)
     }
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) l[rb] = group4_sum(l[rb]);
+  if constexpr (KW > 1) {
+    // the groups' results, through the rings of the later ones: [field][wavefront][lane]
+    static_assert(KW == 2 && sizeof(Lds) >= (4 * VT + 2) * RB * NW * WAVE * sizeof(float), "merge fits the rings");
+    float* sl = reinterpret_cast<float*>(&lds_all[1]) + wave * WAVE + lane;
+    constexpr int F = NW * WAVE;
+    if (kw == 1) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float* x = sl + rb * (4 * VT + 2) * F;
+        x[0] = m[rb];
+        x[F] = l[rb];
+#pragma unroll
+        for (int tt = 0; tt < VT; ++tt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[(2 + 4 * tt + e) * F] = acc[rb][tt][e];
+      }
+    }
+    __syncthreads();
+    if (kw == 0) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const float* x = sl + rb * (4 * VT + 2) * F;
+        const float m1 = x[0], M = __builtin_fmaxf(m[rb], m1);
+        const float w0 = __builtin_amdgcn_exp2f(m[rb] - M), w1 = __builtin_amdgcn_exp2f(m1 - M);
+        m[rb] = M;
+        l[rb] = __builtin_fmaf(w1, x[F], l[rb] * w0);
+#pragma unroll
+        for (int tt = 0; tt < VT; ++tt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[rb][tt][e] = __builtin_fmaf(w1, x[(2 + 4 * tt + e) * F], acc[rb][tt][e] * w0);
+      }
+    }
+    __syncthreads();   // (the rings may be written again)
+    if (kw) return;
   }
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int R = row_of(rb), t = R / G;
-    fin(rb, t, kvh * G + R - t * G, t < Q, m[rb], group4_sum(l[rb]), acc[rb]);
+    fin(rb, t, kvh * G + R - t * G, t < Q, m[rb], l[rb], acc[rb]);
   }
 }
 
