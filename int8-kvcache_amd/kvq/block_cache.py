@@ -20,6 +20,7 @@ Everything is enqueued on the current torch stream of the tensors' device; no ca
 KVQ_DEBUG=1 input check, so fixed-shape calls can be captured in a HIP graph.
 """
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -181,18 +182,44 @@ def block_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, blo
     return out
 
 
+class _DirectCost(NamedTuple):
+    """us by which reading the int8 pages in the kernel differs from copying their codes first, at one head_dim: a
+    least-squares fit of 240 drawn steps timed in graphs both ways."""
+    alone: float    # more per key tile of the longest workgroup, at most one workgroup a CU
+    shared: float   # the same with more
+    launch: float   # the copy's launch, and its time per million K elements (with their V)
+    pages: float
+
+
+_DIRECT = {128: _DirectCost(0.034, 0.172, 1.55, 0.90), 64: _DirectCost(0.130, 0.143, 2.17, 1.42)}
+
+
+def direct_pays(longest, workgroups, d, fill, elems):
+    """Whether the prefill of a block-scaled cache reads the int8 pages itself (block_prefill_kernel) instead of a copy of
+    `elems` K (and as many V) codes as bf16. Over the fitted steps the source taken is within 1.1 of the faster and 0.2%
+    off on average. Graph, us, copied and direct: 16 tokens of 16,384 keys (28 / 4 heads) 38.9 and 28.4, 776 of 1,390
+    (32 / 8) 51.4 and 46.4; 1,302 of 1,490 with 274 of 5,979 (28 / 4) 81 and 93, 512 of 8,192 93 and 103."""
+    c = _DIRECT.get(d, _DIRECT[128])
+    return (c.shared if workgroups > fill else c.alone) * longest < c.launch + c.pages * elems / 1e6
+
+
 def block_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, plan, softmax_scale, scales):
     """Attention over a block-scaled cache for the plan's long requests (cuda_kernels.plan_long; the others' rows are left
     as they were): the formula of block_decode_attention on bf16 operands, the codes exact, their scales applied in fp32, the
     softmax's weights rounded to bf16. KVQ_PREFILL_DIRECT as long_attention's: 1 (or fold) reads the int8 pages
-    themselves, 0 a temporary bf16 cache of the plan's pages' codes; unset: whichever is faster (cuda_kernels.direct_pays)."""
+    themselves, 0 a temporary bf16 cache of the plan's pages' codes; unset: whichever is faster (direct_pays)."""
     name, e = "block_long_attention", ck.ext()
     bs, h, d = k_cache.shape[1:]
     _check(bs == plan.block_size, f"block size {bs} != plan block size {plan.block_size}")
     work = plan.work(q.shape[1] // h, h, d, q.device)
     direct = os.environ.get("KVQ_PREFILL_DIRECT")
     _check(direct in (None, "0", "1", "fold"), f"KVQ_PREFILL_DIRECT must be 0, 1 or fold, got {direct!r}")
-    src = plan.gpu(q.device) if direct == "0" or direct is None and not work.direct else (None, None, None)
+    if direct is None:
+        if work.direct_block is None:
+            work.direct_block = direct_pays(work.longest, work.tile_req.shape[0] * h, d, ck.one_pass_fill(q.device),
+                                            plan.src_req.shape[0] * bs * h * d)
+        direct = "1" if work.direct_block else "0"
+    src = plan.gpu(q.device) if direct == "0" else (None, None, None)
     if ck._served(e, name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
                   scales["v_scale"], softmax_scale, e.prefill_rows, work.tile_req, work.tile_row, work.tile_piece,
                   work.tile_slot, work.merge, work.slots, *src):

@@ -494,8 +494,9 @@ class LongPlan:
                 lists = (lists[4], *lists[:4])   # the 16-byte merge entries first
             views = _to_device(lists, device)
             direct = direct_pays(longest, d, elems)
-            self._work[(group, hkv, d)] = (PrefillWork(*views, None, None, None, 0, direct) if len(views) == 2 else
-                                           PrefillWork(views[1], views[2], views[3], views[4], views[0], slots, direct))
+            self._work[(group, hkv, d)] = (PrefillWork(*views, None, None, None, 0, direct, longest) if len(views) == 2 else
+                                           PrefillWork(views[1], views[2], views[3], views[4], views[0], slots, direct,
+                                                       longest))
         return self._work[(group, hkv, d)]
 
 
@@ -510,6 +511,8 @@ class PrefillWork:
     merge: torch.Tensor
     slots: int
     direct: bool                # read the INT8 pages (same output bits) instead of dequantizing them first
+    longest: int = 0            # key tiles of the longest workgroup
+    direct_block: bool = None   # the same choice for a block-scaled cache, made where it is first asked for (kvq.block_cache)
 
     def split(self, hkv, rows, d):
         """The split arguments of the prefill calls with fresh partial buffers, or None."""

@@ -149,3 +149,12 @@ def test_plain_write_keeps_scales_and_grows_them():
     assert sc[1, 0, 0] == torch.tensor(2.0) / 127 and kc[1, :4, 0, 0].tolist() == [64, -32, 64, 127]
     R.write(torch.full((1, 1, 64), 0.25).to(torch.bfloat16), kc, sc, [0, 1], [5], table)
     assert sc[1, 0, 0] == torch.tensor(2.0) / 127 and kc[1, :5, 0, 0].tolist() == [64, -32, 64, 127, 16]
+
+
+def test_source_of_long_queries():
+    """Few rows over many keys read the int8 pages, many rows a copy of the codes (the measured sides of the rule)."""
+    elems = lambda keys, h, d=128: keys * h * d  # noqa: E731
+    assert bc.direct_pays(8, 256, 128, 256, elems(16384, 4))        # 16 tokens of 16,384 keys, cut
+    assert bc.direct_pays(44, 200, 128, 256, elems(1390, 8))        # 776 of 1,390, whole
+    assert not bc.direct_pays(55, 500, 128, 256, elems(8192, 4))    # 512 of 8,192, cut
+    assert not bc.direct_pays(512, 8192, 128, 256, 4 * elems(16384, 8))
