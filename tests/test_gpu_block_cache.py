@@ -197,6 +197,26 @@ def test_read_back(h, d, bs, group):
         assert bool((got[cu[-1]:] == 5.0).all())
 
 
+def test_read_back_past_the_last_level_cache():
+    """A read of more than 256 MiB (streaming loads and stores)."""
+    h, d, bs = 16, 64, 64
+    n = (258 << 20) // (6 * h * d)
+    lens = [n - 777, 777]
+    table, nb = page_table(lens, bs, 1)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    kc, vc = (torch.randint(-127, 128, (nb, bs, h, d), generator=g, device=DEV, dtype=torch.int8) for _ in range(2))
+    scales = {x: torch.rand(nb, h, 2, generator=g, device=DEV) + 0.1 for x in ("k_scale", "v_scale")}
+    k, v = (torch.zeros(n, h, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    bc.read_block_cache(kc, vc, scales, i32([0, 0]), i32(cumsum(lens)), table.to(DEV), k, v)
+    for got, cache, scale in ((k, kc, scales["k_scale"]), (v, vc, scales["v_scale"])):
+        at = 0
+        for r, m in enumerate(lens):
+            codes, s = R.values(cache, scale, table[r].to(DEV), m)
+            want = (codes.float() * s.float()[..., None]).to(torch.bfloat16).transpose(0, 1)
+            assert torch.equal(got[at:at + m], want), r
+            at += m
+
+
 # ------------------------------------------------------------------------------------------------ attention
 HEADS = [(28, 4, 128), (32, 8, 128), (14, 2, 64), (16, 16, 64), (32, 1, 128), (8, 1, 64), (9, 1, 128), (34, 2, 64)]
 
