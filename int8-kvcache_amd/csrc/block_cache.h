@@ -416,9 +416,12 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
       }
 #pragma unroll
     for (int e = 0; e < KPL; ++e) amax = __builtin_fmaxf(amax, __builtin_fabsf(x[e]));
+    float odd = 0.f;   // 0, or NaN where the row holds a NaN or an infinity: then its output does too
+#pragma unroll
+    for (int e = 0; e < KPL; ++e) odd = __builtin_fmaf(x[e], 0.f, odd);
     amax = __builtin_fmaxf(group4_fmax(amax), 1e-30f);
     const float inv = Q16_MAX / amax;
-    rs = amax / Q16_MAX * a.sm_log2;
+    rs = amax / Q16_MAX * a.sm_log2 + group4_sum(odd);
 #pragma unroll
     for (int s = 0; s < KSTEPS; ++s)
 #pragma unroll
@@ -621,6 +624,13 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
   // ---- the end of a piece: bf16 out of a whole segment, or the fp32 partial of a cut one (as finish_segment) ----
   const AttnArgs& o = fresh_args();
   const int qt = tok + rtok, head = kvh * G + rh;
+  if (l != l) {   // (a denominator that is no number would not tell the merge that the row was cut)
+    l = 1.f;
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = NAN;
+  }
   if (nparts == 1) {
     if (o.max_splits > 1 && qt < o.cut_rows && g == 0)
       o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh] = -1.f;
@@ -702,6 +712,7 @@ __global__ __launch_bounds__(256 * KW, KW == 1 ? 3 : 2) void block_verify_kernel
       } else {
         const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)hq * o.seg_sh + part;
         if (g == 0) {
+          if (l != l) l = 1.f;   // (no number would not tell the merge that the row was cut; the accumulators are none either)
           o.segm_max[sidx] = m;
           o.segm_sum[sidx] = part == nparts - 1 ? -2.f - l : l;
         }
@@ -887,7 +898,8 @@ int check_attention(const char* nm, const void* q, int64_t q_st, int64_t q_sh, c
                     int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
                     int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim, const float* k_scale,
                     const float* v_scale, int64_t group, void* out, int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q,
-                    const int32_t* seq_lens, const int32_t* block_table, int64_t num_q_heads) {
+                    const int32_t* seq_lens, const int32_t* block_table, int64_t num_q_heads, double softmax_scale) {
+  if (!(softmax_scale > 0.0) || !std::isfinite(softmax_scale)) return fail("%s: softmax_scale must be positive and finite", nm);
   if (const int rc = check_blocks(nm, num_blocks, block_size, group, num_kv_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache,
                                   v_sb, v_sn, v_sh)) return rc;
   if (num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
@@ -918,7 +930,7 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   if (num_seqs == 0) { g_err.clear(); return KVQ_OK; }
   if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks,
                                      block_size, num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q,
-                                     seq_lens, block_table, num_q_heads)) return rc;
+                                     seq_lens, block_table, num_q_heads, softmax_scale)) return rc;
   if (num_splits > 1 && segm_rows > 0 && (!segm_out || !segm_max || !segm_sum || !aligned16(segm_out)))
     return fail("%s: split buffers missing or not 16-byte aligned", nm);
   if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
@@ -1009,7 +1021,7 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
     return fail("%s: split work list needs 16-byte aligned merge list and partial buffers", nm);
   if (const int rc = check_attention(nm, q, q_st, q_sh, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn, v_sh, num_blocks,
                                      block_size, num_kv_heads, head_dim, k_scale, v_scale, group, out, o_st, o_sh, cu_seqlens_q,
-                                     seq_lens, block_table, num_q_heads)) return rc;
+                                     seq_lens, block_table, num_q_heads, softmax_scale)) return rc;
   if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
     return fail("%s: page too large for 32-bit lane offsets", nm);
   if (k_codes && (!v_codes || !codes_table || !code_scales || !aligned16(code_scales) || num_pages <= 0 || num_pages > INT32_MAX || !aligned16(k_codes) || !aligned16(v_codes)))

@@ -106,9 +106,14 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         amax = __builtin_fmaxf(amax, __builtin_fmaxf(__builtin_fabsf(bf16_lo(w[u][j])), __builtin_fabsf(bf16_hi(w[u][j]))));
+    float odd = 0.f;   // 0, or NaN where the row holds a NaN or an infinity: then its output does too
+#pragma unroll
+    for (int u = 0; u < 2 * KS; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd = __builtin_fmaf(bf16_lo(w[u][j]), 0.f, __builtin_fmaf(bf16_hi(w[u][j]), 0.f, odd));
     amax = __builtin_fmaxf(group4_fmax(amax), 1e-30f);
     const float inv = Q16_MAX / amax;
-    rs[rb] = amax / Q16_MAX * a.sm_log2;
+    rs[rb] = amax / Q16_MAX * a.sm_log2 + group4_sum(odd);
 #pragma unroll
     for (int u = 0; u < 2 * KS; ++u)
 #pragma unroll
@@ -279,10 +284,12 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
       for (int rb = 0; rb < RB; ++rb) {
         const int lim = L - Q + 1 + row_of(rb) / G;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b) {
+          f[rb][b] = f[rb][b] < 1e-37f ? 1e-37f : f[rb][b];   // (a product that underflowed times -inf is no number)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (n0 + 16 * b + 4 * g + i >= lim) sc[rb][b][i] = -INFINITY;
+        }
       }
     }
   };

@@ -27,6 +27,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -2040,14 +2041,15 @@ __global__ __launch_bounds__(256) void dequant_pages_kernel(
   if (src < 0 || src >= num_blocks) src = 0;
   if constexpr (CODES) {
     // (finite whatever lies in blocks that were never written: their keys are masked by infinite scores)
-    auto scale = [](float x) { return __builtin_fminf(__builtin_fmaxf(x, MIN_BLOCK_SCALE), 1e37f); };
+    // (and K's at least 1e-20: its product with the softmax scale times a masked score must not be 0 times infinite)
+    auto scale = [](float x, float least) { return __builtin_fminf(__builtin_fmaxf(x, least), 1e37f); };
     const int nb16 = bs / 16;
     if (blockIdx.z == 0)
       for (int i = tid; i < nh * nb16; i += C * tpc) {
         const int hh = h0 + i / nb16, b = i % nb16;
         const int64_t at = (int64_t)src * codes.s.sb + (int64_t)hh * codes.s.sh + (int64_t)((16 * b) >> codes.s.lg) * codes.s.sg;
-        const float v = scale(codes.s.vs[at]);
-        codes.table[((int64_t)hh * gridDim.x + p) * nb16 + b] = f32x4{scale(codes.s.ks[at]), __builtin_amdgcn_logf(v),
+        const float v = scale(codes.s.vs[at], MIN_BLOCK_SCALE);
+        codes.table[((int64_t)hh * gridDim.x + p) * nb16 + b] = f32x4{scale(codes.s.ks[at], 1e-20f), __builtin_amdgcn_logf(v),
                                                                       __builtin_amdgcn_rcpf(v), 0.f};
       }
   }

@@ -107,7 +107,7 @@ def _c(name, **change):
                                         1, 128, 0.1, None, None, None, 0, None, None, None, None, None, 0, None, 0, None]}[name]
     at = {"quant_block_cache": 15, "read_block_cache": 8, "block_decode_attention": 11, "block_prefill_attention": 11}[name]
     places = {"num_blocks": at, "block_size": at + 1, "heads": at + 2, "d": at + 3, "group": at + 9, "k_cache": at - 8,
-              "k_sn": at - 6, "num_seqs": len(args) - 2, "splits": 36, "rows_per_tile": 32}
+              "k_sn": at - 6, "num_seqs": len(args) - 2, "splits": 36, "rows_per_tile": 32, "scale": 30 if name == "block_decode_attention" else 33}
     for key, val in change.items():
         args[places[key]] = val
     lib = _native.load()
@@ -133,6 +133,10 @@ def test_c_entry_refusals_of_the_attention():
     assert rc == 1 and "work list tiles must be 128 rows" in err
     rc, err = _c("block_decode_attention", heads=3)
     assert rc == 1 and "bad head counts" in err
+    for name in ("block_decode_attention", "block_prefill_attention"):
+        for scale in (0.0, -0.1, float("nan"), float("inf")):
+            rc, err = _c(name, scale=scale)
+            assert rc == 1 and "softmax_scale must be positive and finite" in err
 
 
 def test_plain_write_keeps_scales_and_grows_them():

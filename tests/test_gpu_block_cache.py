@@ -347,6 +347,44 @@ def test_padded_requests_of_a_graph_batch():
     attend(c, 28, [1, 1, 0, 0], lens, nan_segm(4, 28, 16, 128))
 
 
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [8, 8, 3, 8], [40, 9, 300, 12]])
+def test_rows_that_are_no_number_stay_their_own(q_lens, split, source):
+    """A NaN or an infinity in one q row makes that row NaN and no other; rows of zeros average what they see, over zero
+    scales too (blocks never written, as in a warm-up) and where their tiles are masked."""
+    lens = [3000, 70, 400, 33]
+    c = filled(4, 128, 32, 16, lens)
+    c.scales["k_scale"][c.table[3, :2].long()] = 0
+    cu = cumsum(q_lens)
+    q = torch.randn(cu[-1], 28, 128, generator=gen(1)).to(torch.bfloat16).to(DEV)
+    q[cu[1]:cu[2], 3] = 0
+    q[cu[3]:] = 0
+    clean = q.clone()
+    bad = [(0, 5, 17, "nan"), (cu[1] - 1, 27, 127, "inf"), (cu[2], 0, 0, "-inf")]
+    for t, h, d, x in bad:
+        q[t, h, d] = float(x)
+    segm = nan_segm(cu[-1], 28, 16, 128) if split else None
+    out = torch.full_like(q, 7.0)
+    bc.block_paged_attention(q, c.kc, c.vc, out, i32(cu), i32(lens), c.table, max(q_lens), 128 ** -0.5, c.scales,
+                             ck.plan_long(cu, lens, 32), segm)
+    want, bound = R.attention(clean, c.kc, c.vc, c.scales, cu, lens, c.table, 128 ** -0.5)
+    for t, h, _, _ in bad:
+        assert bool(torch.isnan(out[t, h]).all()), (t, h)
+        out[t, h] = want[t, h].to(out.dtype)
+    R.check(out, want, bound, q_lens)
+
+
+@pytest.mark.parametrize("short_q", [1, 1_000_000])
+def test_other_short_query_limits(short_q, monkeypatch, source):
+    """KVQ_SHORT_Q's other uses: verification rows through the long path, whole prompts through the short one."""
+    monkeypatch.setattr(ck, "SHORT_Q", short_q)
+    lens = [90, 500, 33, 700]
+    c = filled(4, 128, 16, 16, lens)
+    attend(c, 28, [1, 8, 3, 1], lens)
+    attend(c, 28, [1, 300, 33, 20], lens)
+    attend(c, 28, [1, 300, 33, 20], lens, nan_segm(354, 28, 16, 128))
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("hq,h,d,bs,group", [(28, 4, 128, 16, 16), (14, 2, 64, 64, 32)])
 def test_generation_captured_and_replayed(hq, h, d, bs, group):
