@@ -196,8 +196,8 @@ _DIRECT = {128: _DirectCost(0.034, 0.172, 1.55, 0.90), 64: _DirectCost(0.130, 0.
 
 def direct_pays(longest, workgroups, d, fill, elems):
     """Whether the prefill of a block-scaled cache reads the int8 pages itself (block_prefill_kernel) instead of a copy of
-    `elems` K (and as many V) codes as bf16. Over the fitted steps the source taken is within 1.1 of the faster and 0.2%
-    off on average. Graph, us, copied and direct: 16 tokens of 16,384 keys (28 / 4 heads) 38.9 and 28.4, 776 of 1,390
+    `elems` K (and as many V) codes as bf16. Over the 240 fitted steps the source taken is within 1.1 of the faster and
+    0.2% off on average, over 240 others within 1.08 and 0.3%. Graph, us, copied and direct: 16 tokens of 16,384 keys (28 / 4 heads) 38.9 and 28.4, 776 of 1,390
     (32 / 8) 51.4 and 46.4; 1,302 of 1,490 with 274 of 5,979 (28 / 4) 81 and 93, 512 of 8,192 93 and 103."""
     c = _DIRECT.get(d, _DIRECT[128])
     return (c.shared if workgroups > fill else c.alone) * longest < c.launch + c.pages * elems / 1e6
