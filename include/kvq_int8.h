@@ -304,7 +304,7 @@ int kvq_read_block_cache(const int8_t* k_cache, int64_t kc_sb, int64_t kc_sn, in
 
 /* Attention over a block-scaled cache for requests with 1 <= q_len <= qmax:
  *   o = softmax(q . (k_code * k_scale) * softmax_scale) (v_code * v_scale),  bottom-right causal, bf16 q and out;
- * a row that sees no key is zero, one whose q holds a NaN or an infinity is NaN; softmax_scale positive. Neither q nor the softmax's weights are rounded to 8 bits. Rows, skipped requests, split
+ * a row that sees no key is zero, one whose q holds a NaN or an infinity is NaN; softmax_scale from 1e-16 to 1e16. Neither q nor the softmax's weights are rounded to 8 bits. Rows, skipped requests, split
  * buffers and the other arguments as kvq_int8_decode_attention_ex. */
 int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
                                int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,

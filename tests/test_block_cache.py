@@ -137,6 +137,49 @@ def test_c_entry_refusals_of_the_attention():
         for scale in (0.0, -0.1, float("nan"), float("inf")):
             rc, err = _c(name, scale=scale)
             assert rc == 1 and "softmax_scale must be positive and finite" in err
+        for scale in (9e-17, 1.1e16, 1e-300, 1e300):
+            rc, err = _c(name, scale=scale)
+            assert rc == 1 and "from 1e-16 to 1e+16" in err
+
+
+def _codes_prefill(**change):
+    """kvq_block_prefill_attention over a temporary cache, valid but for `change` (refused before any pointer is used)."""
+    a = dict(kc=16, codes_k=16, codes_v=16, code_scales=16, pages=8, codes_table=16, block=32, heads=4)
+    a.update(change)
+    geom, cache, sc = [8, a["block"], a["heads"], 128], [16, 4096, 128, 256], [16, 16, 16, 4, 1, 16]
+    lib = _native.load()
+    rc = lib.kvq_block_prefill_attention(16, 3584, 128, *cache, *cache, *geom, *sc, 16, 3584, 128, 16, 16, 16, 3, 28, 16, 16, 1,
+                                         128, 0.1, None, None, None, 0, None, None, a["codes_k"], a["codes_v"],
+                                         a["code_scales"], a["pages"], a["codes_table"], 3, None)
+    return rc, lib.kvq_last_error().decode()
+
+
+@pytest.mark.parametrize("change", [{"codes_v": None}, {"code_scales": None}, {"codes_table": None}, {"codes_k": 24},
+                                    {"codes_v": 24}, {"code_scales": 20}, {"pages": 0}, {"pages": -1}, {"pages": 1 << 31}])
+def test_c_entry_refusals_of_a_temporary_cache(change):
+    rc, err = _codes_prefill(**change)
+    assert rc == 1 and "bad temporary cache" in err
+
+
+def test_c_entry_refuses_a_temporary_cache_of_huge_pages():
+    rc, err = _codes_prefill(block=1 << 22)    # 2 * 2^22 * 4 * 128 bytes a page
+    assert rc == 1 and "page / slot offsets" in err
+
+
+@pytest.mark.parametrize("place,val,msg", [
+    (11, 96, "head_dim must be 64 or 128"), (9, 24, "block_size must be a power of two"), (17, 48, "positions per scale"),
+    (17, 64, "positions per scale"), (10, 0, "bad sizes"), (8, 0, "bad sizes"), (0, None, "16-byte aligned"),
+    (0, 24, "16-byte aligned"), (2, 120, "16-byte aligned"), (12, None, "null pointer"), (13, None, "null pointer"),
+    (18, None, "null pointer"), (19, None, "null pointer"), (20, None, "null pointer"), (21, None, "null pointer"),
+    (23, None, "null pointer"), (24, None, "null pointer"), (18, 24, "rows must be 16-byte aligned"),
+    (19, 24, "rows must be 16-byte aligned"), (20, 24, "rows must be 16-byte aligned"), (25, -1, "bad sizes"),
+    (25, 1 << 31, "bad sizes")])
+def test_c_entry_refusals_of_block_codes(place, val, msg):
+    args = [16, 4096, 128, 256, 16, 4096, 128, 256, 8, 32, 4, 128, 16, 16, 16, 4, 1, 16, 16, 16, 16, 16, 3, 16, 16, 2, None]
+    args[place] = val
+    lib = _native.load()
+    rc = lib.kvq_block_codes(*args)
+    assert rc == 1 and msg in lib.kvq_last_error().decode()
 
 
 def test_plain_write_keeps_scales_and_grows_them():

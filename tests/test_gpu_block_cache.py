@@ -338,6 +338,16 @@ def test_softmax_scale_and_host_bounds(source):
     R.check(out, want, bound)
 
 
+@pytest.mark.parametrize("poison", [False, True])
+@pytest.mark.parametrize("scale", [1e-16, 1e-12, 0.09])
+def test_unwritten_halves_of_a_tile_under_small_softmax_scales(scale, poison, source):
+    """The last tile of most requests ends in a half whose block was never written (scales 0 or NaN): masked, no NaN from it."""
+    lens = [70, 38, 3, 200]
+    c = filled(4, 128, 64, 16, lens, poison=poison)
+    attend(c, 28, [1, 2, 3, 2], lens, scale=scale)
+    attend(c, 28, [12, 30, 3, 140], lens, scale=scale)
+
+
 def test_padded_requests_of_a_graph_batch():
     """Requests beyond the batch's: no query tokens (cu repeats), length 0, rows of the table unset."""
     lens = [50, 700, 0, 0]
