@@ -656,7 +656,7 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
     const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh + part;
     if (g == 0) {
       o.segm_max[sidx] = m;
-      o.segm_sum[sidx] = part == nparts - 1 ? -2.f - l : l;
+      o.segm_sum[sidx] = part == nparts - 1 ? last_piece_sum(l) : l;
     }
     float* sp = o.segm_out + sidx * D + OPL * g;
 #pragma unroll
@@ -725,7 +725,7 @@ __global__ __launch_bounds__(256 * KW, KW == 1 ? 3 : 2) void block_verify_kernel
         if (g == 0) {
           if (l != l) l = 1.f;   // (no number would not tell the merge that the row was cut; the accumulators are none either)
           o.segm_max[sidx] = m;
-          o.segm_sum[sidx] = part == nparts - 1 ? -2.f - l : l;
+          o.segm_sum[sidx] = part == nparts - 1 ? last_piece_sum(l) : l;
         }
         float* sp = o.segm_out + sidx * D + 4 * g;
 #pragma unroll
@@ -1010,8 +1010,8 @@ int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   a.G = G;
   const dim3 rgrid((unsigned)num_seqs, (unsigned)((num_q_heads + RED_WAVES - 1) / RED_WAVES),
                    (unsigned)std::min<int64_t>(maxq, MERGE_Z));
-  if (head_dim == 128) hipLaunchKernelGGL(split_reduce_kernel<128>, rgrid, dim3(WAVE * RED_WAVES), 0, st, a);
-  else hipLaunchKernelGGL(split_reduce_kernel<64>, rgrid, dim3(WAVE * RED_WAVES), 0, st, a);
+  if (head_dim == 128) hipLaunchKernelGGL((split_reduce_kernel<128, true>), rgrid, dim3(WAVE * RED_WAVES), 0, st, a);
+  else hipLaunchKernelGGL((split_reduce_kernel<64, true>), rgrid, dim3(WAVE * RED_WAVES), 0, st, a);
   return launched("block_decode_attention: merge");
 }
 

@@ -41,6 +41,7 @@
 #include "../../include/kvq_int8.h"
 #include "attn_rules.h"
 #include "page_run.h"
+#include "piece_sum.h"
 
 namespace {
 
@@ -1858,12 +1859,14 @@ __global__ __launch_bounds__(WAVE * 2 * KS) void verify_kernel(AttnArgs a) {
 // channels each. The piece count is read from the denominators (the last piece's is stored as
 // -2 - l, a row that was not cut has -1 in slot 0 and was written by the attention kernel), so the
 // merge needs neither the plan nor any buffer beyond the split buffers of the call.
+// BLOCK: the block-scaled cache's pieces, whose denominators may be far below 1e-30 (piece_sum.h); a row that saw no key is
+// zero.
 constexpr int RED_WAVES = 4;
 constexpr int MERGE_Z = 64;   // largest z extent of split_reduce_kernel's grid
 // pieces of a row fetched together with its denominators (c3: 59.4 -> 59.0 us same card, c4 unchanged;
 // 4 pieces: 61.4 us -- the extra reads of rows with fewer pieces cost more than the round trip saves)
 constexpr int MERGE_SPEC = 2;
-template <int D>
+template <int D, bool BLOCK>
 __device__ __forceinline__ void merge_row(const AttnArgs& a, int tok, int t, int h, int lane) {
   // denominators as the attention kernel left them: piece-0 slot -1 = not cut (already written);
   // otherwise pieces 0..S-2 hold l >= 0 and the last piece -2 - l
@@ -1887,17 +1890,17 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, int tok, int t, int
   for (int j = 0; j < MERGE_SPEC; ++j)
 #pragma unroll
     for (int e = 0; e < CPL; ++e) asm volatile("" : "+v"(v0[j][e]));
-  const unsigned long long neg = __ballot(enc < 0.f);
+  const unsigned long long neg = __ballot(BLOCK ? is_last_piece(enc) : enc < 0.f);
   if (neg == 0ull) return;
   const int last = __builtin_ctzll(neg);
   if (last == 0) return;  // not cut
   const int S = last + 1;
-  const float ls = lane < last ? enc : (lane == last ? -2.f - enc : 0.f);
+  const float ls = lane < last ? enc : (lane == last ? (BLOCK ? piece_sum(enc) : -2.f - enc) : 0.f);
   const float ms = lane < S ? mraw : -INFINITY;
   const float M = wave_max(ms);
   const float wt = lane < S ? __builtin_amdgcn_exp2f(ms - M) : 0.f;
   const float den = wave_sum(wt * ls);
-  const float inv = 1.f / __builtin_fmaxf(den, 1e-30f);
+  const float inv = BLOCK ? (den > 0.f ? 1.f / den : 0.f) : 1.f / __builtin_fmaxf(den, 1e-30f);
   float num[CPL];
 #pragma unroll
   for (int e = 0; e < CPL; ++e) num[e] = 0.f;
@@ -1940,7 +1943,7 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, int tok, int t, int
 }
 // Grid (request, group of RED_WAVES q heads, z): block z merges query tokens z, z + gridDim.z, ... of
 // its request, so every short request's rows are covered whatever max_query_len the caller reported.
-template <int D>
+template <int D, bool BLOCK = false>
 __global__ __launch_bounds__(WAVE * RED_WAVES) void split_reduce_kernel(AttnArgs a) {
   const int lane = threadIdx.x & (WAVE - 1);
   const int seq = blockIdx.x;
@@ -1948,7 +1951,7 @@ __global__ __launch_bounds__(WAVE * RED_WAVES) void split_reduce_kernel(AttnArgs
   const int tok = a.cu_q[seq], qlen = a.cu_q[seq + 1] - tok;
   if (h >= a.G * a.hkv || qlen <= 0 || qlen > a.qmax) return;
   const int rows = min(qlen, a.cut_rows - tok);  // tokens past the split buffers' rows were not cut
-  for (int t = blockIdx.z; t < rows; t += gridDim.z) merge_row<D>(a, tok, t, h, lane);
+  for (int t = blockIdx.z; t < rows; t += gridDim.z) merge_row<D, BLOCK>(a, tok, t, h, lane);
 }
 
 // ------------------------------------------------------------------------------------------------

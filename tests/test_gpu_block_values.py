@@ -1,0 +1,83 @@
+"""The block-scaled cache's attention where its arithmetic could give way: values of extreme sizes, rows whose attention
+lies almost whole on one key, q rows that hold an infinity, scales of blocks never written. Against 64 bits.
+
+A bf16 output is off by at most 2^-8 of each value; by 2^-8 sqrt(1/3) 0.736 = 1.66e-3 of a row's norm for values spread evenly
+over a binade's logarithm (the mean of 1 / x^2 there is 0.541 = 0.736^2). bf16 weights add the same in quadrature: 2.35e-3.
+What else is rounded is far below: q to 2^-15 of its row's largest (1e-4 of a weight for the rows here), sums in fp32."""
+import pytest
+import torch
+from conftest import nan_like, nan_segm
+
+import block_ref as R
+from kvq import block_cache as bc
+from kvq import cuda_kernels as ck
+from test_gpu_block_cache import DEV, Cache, cumsum, gen, i32, page_table, rows, source  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+SHORT = 2.0 ** -9      # of the rows' norm: short queries, a bf16 output's rounding (1.66e-3) and 17% of it
+MANY = 3e-3            # many query rows: bf16 weights too (2.35e-3), and 28%
+
+
+def written(k, v, lens, bs=16, group=16, scale_fill=0.0, seed=1):
+    h, d = k.shape[1:]
+    table, nb = page_table(lens, bs, seed)
+    c = Cache(h, d, bs, group, nb, scale_fill=scale_fill)
+    bc.quant_block_cache(k.to(torch.bfloat16).to(DEV), v.to(torch.bfloat16).to(DEV), c.kc, c.vc, c.scales, i32(cumsum(lens)),
+                         i32(lens), table.to(DEV))
+    c.table = table.to(DEV)
+    return c
+
+
+def call(c, q, q_lens, lens, segm=None):
+    cu = cumsum(q_lens)
+    out = nan_like(q)
+    bc.block_paged_attention(q, c.kc, c.vc, out, i32(cu), i32(lens), c.table, max(q_lens), c.geom[1] ** -0.5, c.scales,
+                             ck.plan_long(cu, lens, c.geom[2]), segm)
+    return out
+
+
+def off(got, want):
+    """Largest error of a request's rows, of their norm (rows: [.., D]; the norm over all of them)."""
+    assert torch.isfinite(got.float()).all()
+    return float((got.double() - want).norm() / want.norm())
+
+
+def exact(c, q, q_lens, lens):
+    return R.attention(q, c.kc, c.vc, c.scales, cumsum(q_lens), lens, c.table, c.geom[1] ** -0.5)[0]
+
+
+def check(c, q, q_lens, lens, limit, segm=None, what=()):
+    """Each request's rows within `limit` of their norm."""
+    got, want, cu = call(c, q, q_lens, lens, segm), exact(c, q, q_lens, lens), cumsum(q_lens)
+    for r in range(len(q_lens)):
+        e = off(got[cu[r]:cu[r + 1]], want[cu[r]:cu[r + 1]])
+        assert e <= limit, (what, r, e)
+
+
+# ------------------------------------------------------------------------------------------------ cut rows
+@pytest.mark.parametrize("where,size", [(w, s) for w in ("all", "the last keys") for s in (1e4, 1e6, 1e9, 1e20)] + [("all", 1e36)])
+@pytest.mark.parametrize("q_lens", [[1, 1], [2, 1], [8, 5]])
+def test_cut_rows_of_large_values(where, size, q_lens):
+    """A denominator is a sum of P / (V scale), of order 1 / (V scale) where V is large: rows cut into pieces keep it, the
+    last piece's as every other's, and agree with the rows run whole."""
+    lens = [6000, 2500]
+    k, v = rows(sum(lens), 4, 128, 2)
+    big = torch.full((sum(lens),), size) if where == "all" else torch.cat([
+        torch.where(torch.arange(n) >= n - 900, size, 1.0) for n in lens])
+    c = written(k.float(), v.float() * big[:, None, None], lens)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    limit = SHORT if max(q_lens) < 8 else MANY
+    check(c, q, q_lens, lens, limit, None, "whole")
+    check(c, q, q_lens, lens, limit, nan_segm(sum(q_lens), 28, 16, 128), "cut")
+
+
+@pytest.mark.parametrize("q_lens", [[1], [8]])
+def test_cut_rows_without_keys_in_their_last_pieces(q_lens):
+    """Verification rows of contexts that end a few keys into a piece: a row that sees nothing of the last piece (its
+    denominator there is 0) is still merged, and so is one whose request has one tile more than its pieces."""
+    for n in (4097, 4098, 4128, 4101):
+        k, v = rows(n, 4, 128, 5)
+        c = written(k.float(), v.float() * 1e5, [n])
+        q = torch.randn(sum(q_lens), 28, 128, generator=gen(4)).to(torch.bfloat16).to(DEV)
+        for splits in (2, 16, 64):
+            check(c, q, q_lens, [n], SHORT if q_lens == [1] else MANY, nan_segm(sum(q_lens), 28, splits, 128), (n, splits))
