@@ -4,12 +4,15 @@
 //
 //   quant_block_kernel   quantize a step's new K/V into their blocks, raising scales (and requantizing) where needed
 //   read_block_kernel    ranges of the requests' keys back to bf16 rows
-//   block_attn_kernel    attention of short queries, int8 MFMA on operands of two int8 planes
+//   block_attn_kernel    attention of short queries: scores on int8 MFMA, q in two int8 planes; bf16 MFMA for the values
 //   block_verify_kernel, block_prefill_kernel   attention of many query rows (block_rows.h)
 //
-// A cached value is code * scale; attention is that of those values and the bf16 q. The codes are exact throughout; q is a
-// 15-bit integer of a per-row scale where K stays int8, and bf16 as given where K's codes are bf16; the softmax's weights are
-// 14-bit integers of a scale per tile (block_attn_kernel) or bf16 (many rows).
+// A cached value is code * scale; attention is that of those values and the bf16 q. The codes are exact throughout. Rounded:
+//   q        to a 15-bit integer of its row's largest where K stays int8 (block_attn_kernel, block_rows.h): 2^-15 of the largest
+//            a channel, where K's codes are off by 2^-8 of theirs; bf16 as given where K's codes are copied as bf16
+//   weights  to a sum of two bf16 (block_attn_kernel: 2^-14 of each, error against 64 bits 1.66e-3, the bf16 output's) or to
+//            one (many rows: 2^-8, 2.0 to 2.3e-3; a second MFMA for every product there). Each weight keeps its own exponent:
+//            as integers of a tile's scale the keys beside two of 90% of a row's attention and no V were 1.3 to 4.7% of it off.
 
 #include "block_rows.h"
 
@@ -276,20 +279,21 @@ __global__ __launch_bounds__(256) void read_block_kernel(ReadBlockArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Attention of short queries: attn_kernel's plan, pieces and tiles (int8 MFMA on the codes as they lie in the cache),
+// Attention of short queries: attn_kernel's plan, pieces and tiles (int8 MFMA on the K codes as they lie in the cache),
 // with operands that keep what an int8 code would lose. Per (request, kv head) and 32-key tile, log2 domain:
 //   S    = q16 . k_code            q16 = rint(q / sq), |q16| <= 16256 = 127 * 128: two int8 planes q16 = 128 hi + lo
 //   e    = S sq scale k_scale + log2(v_scale)      the V scale rides in the exponent, so that one maximum serves both
 //   P    = 2^(e - m)               m: the row's reference maximum of e;  l += P / v_scale
-//   O   += (P14 . v_code) ps       P14 = rint(P / ps), ps = the tile's largest P / 16320: two planes again
-// so the scales cost one multiplication (K) and one addition (V) per 16-key half tile, not one per element, and the
-// products are exact integers. A half tile lies in one block (blocks are 16 positions or more).
-// PACK: at most 8 (token, q head) rows per kv head: the hi planes are the MFMA's columns 0 .. 7, the lo planes columns
-// 8 .. 15, so both planes cost one MFMA each, as a single int8 plane of 16 rows does; lanes n and n + 8 hold the same
-// row and exchange their half of S by a 16-lane rotation. Otherwise 16 rows and two MFMAs per product.
+//   O   += V^T . (Phi + Plo)       v_mfma_f32_16x16x32_bf16: V's codes as bf16 (exact), Phi = P truncated to bf16, Plo the rest
+// so the scales cost one multiplication (K) and one addition (V) per 16-key half tile, not one per element, and O stays in
+// the accumulators. A half tile lies in one block (blocks are 16 positions or more). A V code costs its lane one conversion
+// and half a pack, as much as an integer product's transposing of V and adding of its sums to O.
+// PACK: at most 8 (token, q head) rows per kv head: the hi parts (of q, of P) are the MFMA's columns 0 .. 7, the lo parts
+// columns 8 .. 15, so both cost one MFMA, as one part of 16 rows does; lanes n and n + 8 hold the same row and exchange
+// their half of S by a 16-lane rotation, and their halves of O at the end. Otherwise 16 rows and two MFMAs per product.
 // Bound by memory for long contexts: 128 requests of 32,768 keys (28 / 4 heads x 128) 4.3 GB in 638 to 659 us, 6.5 to 6.75
 // TB/s. 96 of 1 to 32,768 keys 101 us with the merge, 534 MB: fixed costs per piece. One of 4,096 13 us: the launches and one
-// wave of pieces. Two wavefronts a SIMD; three (168 registers) took 119 us on the ragged batch.
+// wave of pieces.
 // ------------------------------------------------------------------------------------------------
 struct BlockAttnArgs {
   AttnArgs a;   // (first: fresh_args)
@@ -302,16 +306,12 @@ __device__ __forceinline__ const BlockScales& fresh_scales() {
   return *(const BlockScales*)(const void*)(p + offsetof(BlockAttnArgs, s));
 }
 
-constexpr float P14_MAX = 16320.f;   // below 16383 by more than the reciprocal's error: the hi plane stays below 128
-
 __device__ __forceinline__ int ror8(int x) { return __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true); }
 __device__ __forceinline__ float ror8(float x) { return __int_as_float(ror8(__float_as_int(x))); }
 
-// Four 14-bit integers (in the low mantissa bits of t) as the bytes of one plane, keys in the order 0, 2, 1, 3 (the V
-// operand's too): bits [SH, SH + 7) of each. sh: 7 (hi plane) or 0 (lo).
-__device__ __forceinline__ uint32_t plane4(uint32_t w01, uint32_t w23, int sh) {
-  const uint32_t a = w01 >> sh, b = w23 << (8 - sh);
-  return ((a & 0x00ff00ffu) | (b & ~0x00ff00ffu)) & 0x7f7f7f7fu;
+// the upper halves of two fp32: a pair of bf16 (exact where they hold 8 significant bits, else truncated)
+__device__ __forceinline__ uint32_t bf16x2_upper(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 
 template <int D, int PF, bool PACK>
@@ -447,11 +447,13 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
       }
   }
   const int lim = rtok < qlen ? L - qlen + 1 + rtok : L;
-  const int sh = n < 8 ? 7 : 0;            // PACK: this lane's plane
+  const int sh = n < 8 ? 7 : 0;            // PACK: this lane's plane of S
+  const uint32_t drop = PACK && n < 8 ? 0u : 0xffff0000u;   // its part of P: what is left without these bits
 
-  float m = -1e30f, l = 0.f, acc[VT][4];
+  float m = -1e30f, l = 0.f;
+  f32x4 acc[VT];
 #pragma unroll
-  for (int t = 0; t < VT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+  for (int t = 0; t < VT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   auto compute = [&](auto masked_t, const Tile& tl, int c) {
     constexpr bool MASKED = decltype(masked_t)::value;
@@ -477,18 +479,6 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
           sc[b][i] = (z[0][i] << 7) + z[NP - 1][i];
         }
       }
-    }
-    // ---- V^T operands, the keys of a lane's 4-key runs in the order 0, 2, 1, 3 ----
-    long vop[VT];
-    {
-      uint32_t lo[VT], hi[VT];
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        transpose4x4(r.v[0][w], r.v[2][w], r.v[1][w], r.v[3][w], lo[4 * w], lo[4 * w + 1], lo[4 * w + 2], lo[4 * w + 3]);
-        transpose4x4(r.v[4][w], r.v[6][w], r.v[5][w], r.v[7][w], hi[4 * w], hi[4 * w + 1], hi[4 * w + 2], hi[4 * w + 3]);
-      }
-#pragma unroll
-      for (int t = 0; t < VT; ++t) vop[t] = (long)(((uint64_t)hi[t] << 32) | lo[t]);
     }
     // ---- the halves' scales ----
     const float vfl = __builtin_fmaxf(tl.sc, MIN_BLOCK_SCALE);
@@ -516,50 +506,45 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
     const float mnew = raise ? tmax : m;
     const float alpha = __builtin_amdgcn_exp2f(m - mnew);
     m = mnew;
-    const float ps = __builtin_fmaxf(__builtin_amdgcn_exp2f(tmax - mnew) * (1.f / P14_MAX), 1e-30f);
-    const float ri = __builtin_amdgcn_rcpf(ps);
-    uint32_t w[2][2];
-    float sum[2];
+    float p[2][4], sum[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float e0 = lv[b] - mnew;
-      uint32_t t[4];
       sum[b] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf((float)sc[b][i], f[b], e0));
-        if (MASKED) p = ok[b][i] ? p : 0.f;
-        sum[b] += p;
-        t[i] = __float_as_uint(__builtin_fmaf(p, ri, QC_MAGIC));
+        p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf((float)sc[b][i], f[b], e0));
+        if (MASKED) p[b][i] = ok[b][i] ? p[b][i] : 0.f;
+        sum[b] += p[b][i];
       }
-      w[b][0] = __builtin_amdgcn_perm(t[1], t[0], 0x05040100u);   // keys 1 : 0
-      w[b][1] = __builtin_amdgcn_perm(t[3], t[2], 0x05040100u);   // keys 3 : 2
     }
     l = __builtin_fmaf(sum[0], iv[0], __builtin_fmaf(sum[1], iv[1], l * alpha));
     if (__any(raise)) {
 #pragma unroll
-      for (int t = 0; t < VT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] *= alpha;
+      for (int t = 0; t < VT; ++t) acc[t] *= alpha;
     }
-    // ---- PV: O^T[channel][row] += (V^T . P^T) ps ----
-    long pop[NP];
+    // ---- PV: O^T[channel][row] += V^T . (Phi + Plo)^T, the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i ----
+    bf16x8 pop[NP];
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int s = PACK ? sh : p == 0 ? 7 : 0;
-      pop[p] = (long)(((uint64_t)plane4(w[1][0], w[1][1], s) << 32) | plane4(w[0][0], w[0][1], s));
+    for (int k = 0; k < NP; ++k) {
+      float x[2][4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[b][i] = NP == 2 && k == 0 ? p[b][i] : p[b][i] - __uint_as_float(__float_as_uint(p[b][i]) & drop);
+      u32x4 w = {bf16x2_upper(x[0][0], x[0][1]), bf16x2_upper(x[0][2], x[0][3]), bf16x2_upper(x[1][0], x[1][1]),
+                 bf16x2_upper(x[1][2], x[1][3])};
+      pop[k] = *reinterpret_cast<bf16x8*>(&w);
     }
-    const float psl = PACK && sh ? ps * 128.f : ps;
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
-      i32x4 z[NP];
+      auto code = [&](int j) { return (float)(int8_t)(r.v[j][t / 4] >> (8 * (t % 4))); };
+      u32x4 w = {bf16x2_upper(code(0), code(1)), bf16x2_upper(code(2), code(3)), bf16x2_upper(code(4), code(5)),
+                 bf16x2_upper(code(6), code(7))};
+      const bf16x8 vop = *reinterpret_cast<bf16x8*>(&w);
 #pragma unroll
-      for (int p = 0; p < NP; ++p) z[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(vop[t], pop[p], i32x4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int zi = PACK ? z[0][i] : (z[0][i] << 7) + z[NP - 1][i];
-        acc[t][i] = __builtin_fmaf((float)zi, psl, acc[t][i]);
-      }
+      for (int k = 0; k < NP; ++k) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[k], acc[t], 0, 0, 0);
     }
   };
 
@@ -668,8 +653,14 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
   }
 }
 
+// Two wavefronts a SIMD at head_dim 128, though the 163 registers that PACK needs leave room for three: those cut a batch into
+// more pieces for nothing (the ragged batch 102 -> 118 us, 32 requests of 4,000 to 8,192 keys 42.4 -> 47.0), and with pieces
+// for two but room for three the CUs that an earlier kernel leaves first take more than their share (48 decode rows behind
+// two prompts' prefill 86.8 -> 89.2 us in all).
+template <int D>
+constexpr int BLOCK_ATTN_WAVES = D == 128 ? 2 : 8;
 template <int D, int PF, bool PACK>
-__global__ __launch_bounds__(256) void block_attn_kernel(BlockAttnArgs args) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, BLOCK_ATTN_WAVES<D>))) void block_attn_kernel(BlockAttnArgs args) {
   touch_args();
   const AttnArgs& a = args.a;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);

@@ -81,3 +81,50 @@ def test_cut_rows_without_keys_in_their_last_pieces(q_lens):
         q = torch.randn(sum(q_lens), 28, 128, generator=gen(4)).to(torch.bfloat16).to(DEV)
         for splits in (2, 16, 64):
             check(c, q, q_lens, [n], SHORT if q_lens == [1] else MANY, nan_segm(sum(q_lens), 28, splits, 128), (n, splits))
+
+
+# ------------------------------------------------------------------------------------------------ dominating keys
+def sink(n, hq, h, d, q_rows, share, own, seed):
+    """K, V [n, h, d] and q [q_rows, hq, d]: key 0 (and key 40, if there is one) takes `share` of each row's attention, with a
+    V of `own` times the others'."""
+    g = gen(seed)
+    u = torch.nn.functional.normalize(torch.randn(h, d, generator=g), dim=-1)
+    k, v = torch.randn(n, h, d, generator=g), torch.randn(n, h, d, generator=g)
+    k -= (k * u).sum(-1, keepdim=True) * u
+    q = torch.randn(q_rows, h, hq // h, d, generator=g)
+    q += (8.0 - (q * u[:, None]).sum(-1, keepdim=True)) * u[:, None]                 # q . u = 8 for every row
+    top = torch.log(torch.tensor(float(n))) + 0.5 + torch.log(torch.tensor(share / (1 - share)))   # beside scores of N(0, 1)
+    for i in (0, 40):
+        if i < n:
+            k[i] = u * (top * d ** 0.5 / 8.0)
+            v[i] *= own
+    return k, v, q.reshape(q_rows, hq, d)
+
+
+@pytest.mark.parametrize("share,own", [(0.5, 0.0), (0.9, 0.02), (0.9, 0.0), (0.99, 0.0), (0.9999, 0.0)])
+@pytest.mark.parametrize("hq,h,d", [(28, 4, 128), (14, 2, 64), (9, 1, 128)])
+@pytest.mark.parametrize("query", [1, 2, 8, 20])
+@pytest.mark.parametrize("n", [300, 4096])
+def test_a_key_that_takes_most_of_a_row(share, own, hq, h, d, query, n, source):
+    """The keys beside a dominating one keep their weights' precision: what is left of the output where the dominating
+    key's own V is small is theirs, in its tile as in others."""
+    k, v, q = sink(n, hq, h, d, query, share, own, 7)
+    c = written(k, v, [n])
+    q = q.to(torch.bfloat16).to(DEV)
+    limit = SHORT if query * hq // h <= 16 else MANY
+    check(c, q, [query], [n], limit, None, "whole")
+    check(c, q, [query], [n], limit, nan_segm(query, hq, 16, d), "cut")
+
+
+@pytest.mark.parametrize("query", [1, 2, 8, 20])
+def test_a_loud_block_beside_quiet_ones(query, source):
+    """Blocks of a tile whose V scales differ by 1e5, where the loud block's keys hold no value in most channels."""
+    n = 512
+    k, v, q = sink(n, 28, 4, 128, query, 0.01, 1.0, 8)
+    v[torch.arange(n) // 16 % 2 == 0, :, 1:] = 0
+    v[torch.arange(n) // 16 % 2 == 0, :, 0] *= 1e5
+    c = written(k, v, [n])
+    q = q.to(torch.bfloat16).to(DEV)
+    got, want = call(c, q, [query], [n]), exact(c, q, [query], [n])
+    assert off(got[..., 1:], want[..., 1:]) <= (SHORT if query < 8 else MANY)
+    assert off(got[..., :1], want[..., :1]) <= (SHORT if query < 8 else MANY)
