@@ -282,8 +282,8 @@ __global__ __launch_bounds__(256) void read_block_kernel(ReadBlockArgs a) {
 // Attention of short queries: attn_kernel's plan, pieces and tiles (int8 MFMA on the K codes as they lie in the cache),
 // with operands that keep what an int8 code would lose. Per (request, kv head) and 32-key tile, log2 domain:
 //   S    = q16 . k_code            q16 = rint(q / sq), |q16| <= 16256 = 127 * 128: two int8 planes q16 = 128 hi + lo
-//   e    = S sq scale k_scale + log2(v_scale)      the V scale rides in the exponent, so that one maximum serves both
-//   P    = 2^(e - m)               m: the row's reference maximum of e;  l += P / v_scale
+//   e    = S sq scale k_scale      m: the row's largest e plus BLOCK_REF, raised where it lags by more than 8
+//   P    = 2^(e - m + log2(v_scale))               the V scale rides in the exponent;  l += P / v_scale
 //   O   += V^T . (Phi + Plo)       v_mfma_f32_16x16x32_bf16: V's codes as bf16 (exact), Phi = P truncated to bf16, Plo the rest
 // so the scales cost one multiplication (K) and one addition (V) per 16-key half tile, not one per element, and O stays in
 // the accumulators. A half tile lies in one block (blocks are 16 positions or more). A V code costs its lane one conversion
@@ -481,7 +481,7 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
       }
     }
     // ---- the halves' scales ----
-    const float vfl = __builtin_fmaxf(tl.sc, MIN_BLOCK_SCALE);
+    const float vfl = __builtin_fmaxf(tl.sc, MIN_V_SCALE);
     const float lg2 = __builtin_amdgcn_logf(vfl), rcp = __builtin_amdgcn_rcpf(vfl);
     auto of_lane = [](float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
     const float f[2] = {rs * of_lane(tl.sc, 0), rs * of_lane(tl.sc, 2)};
@@ -498,10 +498,10 @@ __device__ __forceinline__ void attend_blocks(int seq, int tok, int qlen, int se
         mx = ok[b][i] ? max(mx, sc[b][i]) : mx;
       }
       // (a dot product never reaches INT32_MIN: it marks a half without a visible key)
-      const float tb = __builtin_fmaf((float)mx, f[b], lv[b]);
+      const float tb = (float)mx * f[b];
       tmax = (MASKED && mx == INT32_MIN) ? tmax : __builtin_fmaxf(tmax, tb);
     }
-    tmax = group4_fmax(tmax);
+    tmax = group4_fmax(tmax) + BLOCK_REF;    // the reference that this tile asks for
     const bool raise = tmax > m + ATTN_SLACK;
     const float mnew = raise ? tmax : m;
     const float alpha = __builtin_amdgcn_exp2f(m - mnew);

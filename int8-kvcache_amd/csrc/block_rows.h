@@ -4,7 +4,7 @@
 // NW wavefronts take 16 NW RB (token, q head) rows of one (request, kv head), RB blocks of 16 rows each, and walk 32-key
 // tiles together. Per tile, in the log2 domain of block_attn_kernel:
 //   QK  S^T[key][row]  = K . Q16^T   v_mfma_i32_16x16x64_i8, q in two int8 planes: the codes feed the MFMA as they are
-//   e   = S sq scale k_scale + log2(v_scale),  P = 2^(e - m),  l += P / v_scale
+//   e   = S sq scale k_scale,  P = 2^(e - m + log2(v_scale)),  l += P / v_scale
 //   PV  O^T[chan][row] += V^T . P^T  v_mfma_f32_16x16x32_bf16, P rounded to bf16, V codes converted to bf16 (exactly)
 // so that O stays in the accumulators from tile to tile (an int8 product needs 3 operations per channel and row to add
 // its integers to O, which at 32 keys a tile costs more than the conversion of V by all the wavefronts). K in int8 also
@@ -220,7 +220,7 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
   };
   clear();
 
-  // ---- scores of the group's tile i and what turns them into exponents: factor f (by row), addend lv = log2(V scale), iv = 1 / V
+  // ---- scores of the group's tile i and what turns them into P: factor f (by row), addend lv = log2(V scale), iv = 1 / V
   // scale. The LDS reads -- the V codes of tile i + 1 with them -- stand in assembly that waits for them alone (as plain
   // loads they would wait for every DMA). ----
   float sc[RB][2][4], f[RB][2], lv[2], iv[2];
@@ -273,7 +273,7 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
     for (int b = 0; b < 2; ++b) {
       auto uniform = [](float x) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x))); };
       const float k = uniform(__builtin_fmaxf(__uint_as_float(s2[b].x), MIN_BLOCK_SCALE));
-      const float v = __builtin_fmaxf(__uint_as_float(s2[b].y), MIN_BLOCK_SCALE);
+      const float v = __builtin_fmaxf(__uint_as_float(s2[b].y), MIN_V_SCALE);
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) f[rb][b] = rs[rb] * k;
       lv[b] = uniform(__builtin_amdgcn_logf(v));
@@ -293,14 +293,13 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
       }
     }
   };
-  // the row's largest exponent of the tile (the 4 lanes of a row agree)
+  // the reference of the row's largest score in the tile (the 4 lanes of a row agree)
   auto row_top = [&](int rb) {
     float h[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b)
-      h[b] = __builtin_fmaf(__builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]),
-                                            __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])), f[rb][b], lv[b]);
-    return group4_fmax(__builtin_fmaxf(h[0], h[1]));
+      h[b] = __builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]), __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])) * f[rb][b];
+    return group4_fmax(__builtin_fmaxf(h[0], h[1])) + BLOCK_REF;
   };
   auto softmax_pv = [&](auto st_t) {
     const uint32_t so = vofs(st_t);
@@ -422,7 +421,7 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
     bool jump = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-      // P stays in range while a lane's denominator does; V scales above 1 leave P room to overflow the accumulators
+      // weights stay in range while a lane's denominator does; times large V scales they may overflow the accumulators
       jump |= !(l[rb] <= PR_FAST_PSUM_MAX);
       float z = 0.f;
 #pragma unroll

@@ -53,8 +53,12 @@ struct BlockScales {
   int64_t sb, sh, sg;
   int lg;   // log2 of the positions per scale
 };
-constexpr float MIN_BLOCK_SCALE = 1e-30f;   // a block's scale counts as at least this (the V scale's logarithm and
-                                            // reciprocal are taken; a K scale of 0 times a masked score is no number)
+constexpr float MIN_BLOCK_SCALE = 1e-30f;   // a K scale counts as at least this (0 times a masked score is no number)
+constexpr float MIN_V_SCALE = 0x1p-40f;     // and a V scale as this (9.1e-13; the write's smallest is 1e-8)
+// The attention's reference m is a row's largest score plus BLOCK_REF (log2 units): a weight 2^(score - m) is at most 2^-24 (m
+// may lag by 8), so that P = weight * V scale and a million keys' sum of P * code stay below 2^124 for bf16's largest values
+// (V scales of 2^121), and at the smallest V scale a weight of 2^-54 of the largest is still there.
+constexpr float BLOCK_REF = 32.f;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -1859,8 +1863,7 @@ __global__ __launch_bounds__(WAVE * 2 * KS) void verify_kernel(AttnArgs a) {
 // channels each. The piece count is read from the denominators (the last piece's is stored as
 // -2 - l, a row that was not cut has -1 in slot 0 and was written by the attention kernel), so the
 // merge needs neither the plan nor any buffer beyond the split buffers of the call.
-// BLOCK: the block-scaled cache's pieces, whose denominators may be far below 1e-30 (piece_sum.h); a row that saw no key is
-// zero.
+// BLOCK: the block-scaled cache's pieces (piece_sum.h); a row that saw no key is zero.
 constexpr int RED_WAVES = 4;
 constexpr int MERGE_Z = 64;   // largest z extent of split_reduce_kernel's grid
 // pieces of a row fetched together with its denominators (c3: 59.4 -> 59.0 us same card, c4 unchanged;
@@ -2051,7 +2054,7 @@ __global__ __launch_bounds__(256) void dequant_pages_kernel(
       for (int i = tid; i < nh * nb16; i += C * tpc) {
         const int hh = h0 + i / nb16, b = i % nb16;
         const int64_t at = (int64_t)src * codes.s.sb + (int64_t)hh * codes.s.sh + (int64_t)((16 * b) >> codes.s.lg) * codes.s.sg;
-        const float v = scale(codes.s.vs[at], MIN_BLOCK_SCALE);
+        const float v = scale(codes.s.vs[at], MIN_V_SCALE);
         codes.table[((int64_t)hh * gridDim.x + p) * nb16 + b] = f32x4{scale(codes.s.ks[at], 1e-20f), __builtin_amdgcn_logf(v),
                                                                       __builtin_amdgcn_rcpf(v), 0.f};
       }
@@ -2183,7 +2186,7 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rne(float a, float b) {
 // (prefill_i8_kernel below), converted tile by tile either as dequant_pages converts them (bf16 of
 // code x scale) or as exact bf16 codes with the scales folded into q (K) and the output (V).
 // PR_SRC_BF16_BLOCK: a bf16 temporary cache of a block-scaled cache's codes, each 16-key half tile's K scale a factor of
-// its scores and its V scale an addend in the exponent (block_cache.h).
+// its scores and its V scale's log2 an addend of P's exponent (block_cache.h).
 constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2, PR_SRC_BF16_BLOCK = 3;
 
 template <int D, int SRC, bool SPLIT>
@@ -2639,8 +2642,8 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
         float h[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          h[b] = __builtin_fmaf(__builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]),
-                                                __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])), ent[b][0] * a.sm_log2, ent[b][1]);
+          h[b] = __builtin_fmaxf(__builtin_fmaxf(sc[rb][b][0], sc[rb][b][1]), __builtin_fmaxf(sc[rb][b][2], sc[rb][b][3])) *
+                 (ent[b][0] * a.sm_log2);
         lmax[rb] = __builtin_fmaxf(h[0], h[1]);
       }
       return;
@@ -2651,10 +2654,10 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
                                  __builtin_fmaxf(__builtin_fmaxf(sc[rb][0][3], sc[rb][1][0]), __builtin_fmaxf(
                                      __builtin_fmaxf(sc[rb][1][1], sc[rb][1][2]), sc[rb][1][3])));
   };
-  // the row's largest score of the tile, log2 units (the 4 lanes of a row agree)
+  // the row's largest score of the tile, log2 units (the 4 lanes of a row agree); BLK: the reference that follows from it
   auto row_top = [&]() {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) top[rb] = group4_fmax(lmax[rb]) * (BLK ? 1.f : a.sm_log2);
+    for (int rb = 0; rb < RB; ++rb) top[rb] = BLK ? group4_fmax(lmax[rb]) + BLOCK_REF : group4_fmax(lmax[rb]) * a.sm_log2;
   };
   // m is a reference maximum (log2 units) raised only when a score exceeds it by more than PR_SLACK:
   // P = 2^(s c - m) <= 2^PR_SLACK (exact in fp32, in range for bf16), so acc / l are rescaled in a few
@@ -2889,7 +2892,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       jump |= !(l[rb] <= PR_FAST_PSUM_MAX);
-      if constexpr (BLK) {   // (l is a sum of P over V scales: those above 1 leave P room to overflow the accumulators)
+      if constexpr (BLK) {   // (l is a sum of weights: times large V scales they may still overflow the accumulators)
         float z = 0.f;
 #pragma unroll
         for (int tt = 0; tt < VT; ++tt)

@@ -5,9 +5,9 @@
 
 #include "page_run.h"   // KVQ_HOST_DEVICE
 
-// The sign bit marks the last piece, a zero's too, and nothing is added to the number: a denominator is a sum of P / (V
-// scale), anything from 1e-37 (bf16's largest values) on. Slot 0 of a row that was not cut is marked as well (-1); a cut
-// row has two pieces or more. (The static cache's kernels store -2 - l: there l is about 1 or more; a sum of 1e-7 would be lost.)
+// The sign bit marks the last piece, a zero's too, and nothing is added to the number: the largest weight of a denominator
+// is 2^-32 (BLOCK_REF). Slot 0 of a row that was not cut is marked as well (-1); a cut row has two pieces or more. (The static
+// cache's kernels store -2 - l: there l is about 1 or more; 2^-32 would be lost.)
 KVQ_HOST_DEVICE float last_piece_sum(float l) { return -l; }
 KVQ_HOST_DEVICE bool is_last_piece(float stored) { return __builtin_signbit(stored); }
 KVQ_HOST_DEVICE float piece_sum(float stored) { return __builtin_fabsf(stored); }

@@ -58,8 +58,8 @@ def check(c, q, q_lens, lens, limit, segm=None, what=()):
 @pytest.mark.parametrize("where,size", [(w, s) for w in ("all", "the last keys") for s in (1e4, 1e6, 1e9, 1e20)] + [("all", 1e36)])
 @pytest.mark.parametrize("q_lens", [[1, 1], [2, 1], [8, 5]])
 def test_cut_rows_of_large_values(where, size, q_lens):
-    """A denominator is a sum of P / (V scale), of order 1 / (V scale) where V is large: rows cut into pieces keep it, the
-    last piece's as every other's, and agree with the rows run whole."""
+    """Rows cut into pieces keep their denominators whatever the V scales are, the last piece's as every other's, and agree
+    with the rows run whole."""
     lens = [6000, 2500]
     k, v = rows(sum(lens), 4, 128, 2)
     big = torch.full((sum(lens),), size) if where == "all" else torch.cat([
@@ -128,3 +128,43 @@ def test_a_loud_block_beside_quiet_ones(query, source):
     got, want = call(c, q, [query], [n]), exact(c, q, [query], [n])
     assert off(got[..., 1:], want[..., 1:]) <= (SHORT if query < 8 else MANY)
     assert off(got[..., :1], want[..., :1]) <= (SHORT if query < 8 else MANY)
+
+
+# ------------------------------------------------------------------------------------------------ V scales far apart
+@pytest.mark.parametrize("size", [1e20, 1e30, 1e33, 1e37])
+@pytest.mark.parametrize("q_lens", [[1, 1], [2, 1], [8, 8], [40, 30]])
+def test_blocks_of_zeros_beside_the_largest_values(size, q_lens, source):
+    """A block of zeros has the smallest V scale, 1e-8, and its keys' weights count in the denominator whatever the scales of
+    the others are: up to bf16's largest values beside it."""
+    lens = [700, 1500]
+    k, v = rows(sum(lens), 4, 128, 6)
+    at = torch.cat([torch.arange(n) for n in lens])
+    v = v.float() * torch.where(at // 16 % 3 == 1, size, 0.0)[:, None, None]
+    c = written(k.float() * 0.2, v.clamp(-3e38, 3e38), lens)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    limit = SHORT if max(q_lens) < 8 else MANY
+    check(c, q, q_lens, lens, limit, None, "whole")
+    check(c, q, q_lens, lens, limit, nan_segm(sum(q_lens), 28, 16, 128), "cut")
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1], [2, 1], [8, 5], [40, 30]])
+def test_the_largest_values_behind_ones_of_order_one(q_lens, source):
+    """The last 900 keys' V around 1e36, the others' around 1, rows whole and cut."""
+    lens = [6000, 2500]
+    k, v = rows(sum(lens), 4, 128, 2)
+    big = torch.cat([torch.where(torch.arange(n) >= n - 900, 1e36, 1.0) for n in lens])
+    c = written(k.float(), v.float() * big[:, None, None], lens)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    limit = SHORT if max(q_lens) < 8 else MANY
+    check(c, q, q_lens, lens, limit, None, "whole")
+    check(c, q, q_lens, lens, limit, nan_segm(sum(q_lens), 28, 16, 128), "cut")
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1], [8, 8], [40, 30]])
+def test_values_of_the_smallest_scale(q_lens, source):
+    """V around 1e-7: every block's scale is the smallest."""
+    lens = [700, 1500]
+    k, v = rows(sum(lens), 4, 128, 6)
+    c = written(k.float(), v.float() * 1e-7, lens)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    check(c, q, q_lens, lens, SHORT if max(q_lens) < 8 else MANY)
