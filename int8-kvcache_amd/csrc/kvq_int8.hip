@@ -2931,12 +2931,24 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    const float lr = group4_sum(l[rb]);
+    float lr = group4_sum(l[rb]);
+    // BLK: 0, or NaN where the row sees a key and its q holds a NaN or an infinity: then its output is NaN too (all of its
+    // scores may have been -inf, which reads as a row without keys)
+    float odd = 0.f;
+    if constexpr (BLK) {
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) odd = __builtin_fmaf((float)qop[rb][s][e], 0.f, odd);
+      odd = lim[rb] > 0 ? group4_sum(odd) : 0.f;
+      lr += odd;
+    }
     if (!valid[rb]) continue;
     float inv = lr > 0.f ? 1.f / lr : 0.f;
+    if constexpr (BLK) inv += odd;
     float* prow = nullptr;
     if (SPLIT && piece) {
-      inv = 1.f;   // a piece leaves its accumulators as they are: the merge divides by the whole denominator
+      inv = BLK ? 1.f + odd : 1.f;   // a piece leaves its accumulators as they are: the merge divides by the whole denominator
       const int64_t pr = ((int64_t)pslot * gridDim.y + kvh) * PR_ROWS + (wave * RB + rb) * 16 + n;
       if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = float2{m[rb], lr};
       prow = a.part_out + pr * D + 4 * g;

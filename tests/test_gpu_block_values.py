@@ -168,3 +168,30 @@ def test_values_of_the_smallest_scale(q_lens, source):
     c = written(k.float(), v.float() * 1e-7, lens)
     q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
     check(c, q, q_lens, lens, SHORT if max(q_lens) < 8 else MANY)
+
+
+# ------------------------------------------------------------------------------------------------ rows that are no number
+@pytest.mark.parametrize("value", ["inf", "-inf", "nan"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("q_lens", [[1, 1], [2, 3], [8, 8], [40, 20]])
+def test_an_infinity_over_keys_of_one_sign(value, sign, q_lens, source):
+    """q holds an infinity in a channel whose cached K has one sign, so that every score may be -inf: the row is NaN, not
+    zeros (which say that it saw no key), where it sees one key and where it sees all; its neighbours are as they were."""
+    lens = [q_lens[0], 9000]                       # the first request from its start: its first row sees one key
+    k, v = rows(sum(lens), 4, 128, 9)
+    k = k.float()
+    k[..., 5] = sign * (1.0 + k[..., 5].abs())
+    c = written(k, v.float(), lens)
+    cu = cumsum(q_lens)
+    q = torch.randn(cu[-1], 28, 128, generator=gen(1)).to(torch.bfloat16).to(DEV)
+    bad = [(0, 3), (0, 27), (cu[1] - 1, 9), (cu[1], 0), (cu[2] - 1, 14)]
+    for segm in (None, nan_segm(cu[-1], 28, 16, 128)):
+        want = call(c, q, q_lens, lens, segm)
+        odd = q.clone()
+        for t, h in bad:
+            odd[t, h, 5] = float(value)
+        got = call(c, odd, q_lens, lens, segm)
+        for t, h in bad:
+            assert bool(torch.isnan(got[t, h]).all()), (t, h)
+            got[t, h] = want[t, h]
+        assert off(got, want.double()) <= 2.0 ** -8     # (a tile done again may round otherwise)
