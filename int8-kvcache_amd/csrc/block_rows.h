@@ -497,6 +497,11 @@ __device__ __forceinline__ void attend_rows(const RowsView& a, RowsLds<D, NW> (&
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int R = row_of(rb), t = R / G;
+    if (L - Q + 1 + t <= 0) {   // a row that sees no key, zero whatever its q holds
+      l[rb] = 0.f;
+#pragma unroll
+      for (int tt = 0; tt < VT; ++tt) acc[rb][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     fin(rb, t, kvh * G + R - t * G, t < Q, m[rb], l[rb], acc[rb]);
   }
 }

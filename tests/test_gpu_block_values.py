@@ -195,3 +195,32 @@ def test_an_infinity_over_keys_of_one_sign(value, sign, q_lens, source):
             assert bool(torch.isnan(got[t, h]).all()), (t, h)
             got[t, h] = want[t, h]
         assert off(got, want.double()) <= 2.0 ** -8     # (a tile done again may round otherwise)
+
+
+@pytest.mark.parametrize("q_lens", [[1, 2], [8, 8], [40, 20]])
+def test_a_row_without_keys_is_zero_whatever_its_q(q_lens, source):
+    """Requests of fewer keys than query tokens (and of none): the rows that see nothing are zero, also where q holds a NaN."""
+    lens = [0 if q_lens[0] == 1 else 5, q_lens[1] - 1]
+    k, v = rows(sum(lens), 4, 128, 9)
+    c = written(k.float(), v.float(), lens)
+    cu = cumsum(q_lens)
+    q = torch.randn(cu[-1], 28, 128, generator=gen(1)).to(torch.bfloat16).to(DEV)
+    unseen = [(0, 3), (cu[1], 9)]
+    for t, h in unseen:
+        q[t, h, 7] = float("nan")
+    for segm in (None, nan_segm(cu[-1], 28, 16, 128)):
+        got = call(c, q, q_lens, lens, segm)
+        for t, h in unseen:
+            assert not bool(got[t, h].any()), (t, h)
+        assert torch.isfinite(got.float()).all()
+
+
+@pytest.mark.parametrize("fill", [float("inf"), float("nan"), -1.0, 3e38])
+@pytest.mark.parametrize("q_lens", [[1, 2, 3, 2], [8, 8, 3, 8], [12, 30, 3, 140]])
+def test_scales_of_unwritten_blocks_are_not_read(fill, q_lens, source):
+    """Scale buffers that were never cleared: what lies in the blocks behind a request's last key changes nothing."""
+    lens = [70, 38, 3, 200]
+    k, v = rows(sum(lens), 4, 128, 9)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(1)).to(torch.bfloat16).to(DEV)
+    got = [call(written(k.float(), v.float(), lens, 64, 16, scale_fill=x), q, q_lens, lens) for x in (0.0, fill)]
+    assert torch.isfinite(got[0].float()).all() and torch.equal(got[0].view(torch.int16), got[1].view(torch.int16))
