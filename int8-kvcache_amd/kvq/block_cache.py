@@ -218,7 +218,8 @@ def block_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block
         if work.direct_block is None:
             work.direct_block = direct_pays(work.longest, work.tile_req.shape[0] * h, d, ck.one_pass_fill(q.device),
                                             plan.src_req.shape[0] * bs * h * d)
-        direct = "1" if work.direct_block else "0"
+        # (a capture that finds the pages' lists missing reads the pages themselves: nothing can be copied inside it)
+        direct = "1" if work.direct_block or (plan._gpu is None and ck._capturing(q.device)) else "0"
     src = plan.gpu(q.device) if direct == "0" else (None, None, None)
     if ck._served(e, name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
                   scales["v_scale"], softmax_scale, e.prefill_rows, work.tile_req, work.tile_row, work.tile_piece,

@@ -470,15 +470,15 @@ class LongPlan:
         """The prefill call's work list on the device (PrefillWork): `tiles`, the longest rows' keys cut into
         pieces where that pays (split_rows), and whether the call reads the INT8 pages itself. Built on the
         host, copied once per plan and shape; a capture that finds it missing but `tiles` made takes those, whole
-        rows in two kernels, as nothing can be copied inside it."""
+        rows in two kernels (of a block-scaled cache: from whichever source is faster), as nothing can be copied inside it."""
         if self._work is None:
             self._work = {}
         if (group, hkv, d) not in self._work:
             rows = ext().prefill_rows
-            if self._tiles and (group, rows) in self._tiles and _capturing(device):
-                return PrefillWork(*self._tiles[group, rows], None, None, None, 0, False)
             req, row, keys = self._row_tiles(group, rows)
             tiles = np.maximum((keys + PREFILL_TILE - 1) // PREFILL_TILE, 1)
+            if self._tiles and (group, rows) in self._tiles and _capturing(device):
+                return PrefillWork(*self._tiles[group, rows], None, None, None, 0, False, int(tiles.max(initial=0)))
             held = self.long_qlen * group                                # a request's last entry may be part full
             count = (held + rows - 1) // rows
             valid = np.ones(req.shape[0])
@@ -511,7 +511,7 @@ class PrefillWork:
     merge: torch.Tensor
     slots: int
     direct: bool                # read the INT8 pages (same output bits) instead of dequantizing them first
-    longest: int = 0            # key tiles of the longest workgroup
+    longest: int                # key tiles of the longest workgroup
     direct_block: bool = None   # the same choice for a block-scaled cache, made where it is first asked for (kvq.block_cache)
 
     def split(self, hkv, rows, d):

@@ -224,3 +224,31 @@ def test_scales_of_unwritten_blocks_are_not_read(fill, q_lens, source):
     q = torch.randn(sum(q_lens), 28, 128, generator=gen(1)).to(torch.bfloat16).to(DEV)
     got = [call(written(k.float(), v.float(), lens, 64, 16, scale_fill=x), q, q_lens, lens) for x in (0.0, fill)]
     assert torch.isfinite(got[0].float()).all() and torch.equal(got[0].view(torch.int16), got[1].view(torch.int16))
+
+
+# ------------------------------------------------------------------------------------------------ captured without lists
+@pytest.mark.parametrize("copies", [True, False])
+def test_capture_after_the_plans_own_copies(copies, monkeypatch):
+    """A program that made a plan's device copies itself (tiles, and the pages' lists or not) and then captures its first
+    call: replays follow the inputs and agree with an eager call."""
+    monkeypatch.delenv("KVQ_PREFILL_DIRECT", raising=False)
+    n, d = 2000, 128
+    k, v = rows(n, 4, d, 3)
+    c = written(k.float(), v.float(), [n])
+    q = torch.randn(1500, 28, d, generator=gen(1)).to(torch.bfloat16).to(DEV)
+    cu, sl = i32([0, 1500]), i32([n])
+    plan = ck.plan_long([0, 1500], [n], 16)
+    plan.tiles(7, DEV)
+    if copies:
+        plan.gpu(DEV)
+    out = nan_like(q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bc.block_long_attention(q, c.kc, c.vc, out, cu, sl, c.table, plan, d ** -0.5, c.scales)
+    for i in range(3):
+        q.normal_()
+        out.fill_(float("nan"))
+        graph.replay()
+        want = bc.block_long_attention(q, c.kc, c.vc, nan_like(q), cu, sl, c.table, plan, d ** -0.5, c.scales)
+        assert off(out, want.double()) <= MANY, i
