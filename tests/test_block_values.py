@@ -39,3 +39,28 @@ def test_source_of_a_capture_without_a_work_list(query, keys, copied, copies, mo
     bc.block_long_attention(q, kc, vc, q, cu, lens, torch.zeros(1, 4, dtype=torch.int32), plan, 0.1, bc.block_scales(4, 16, 4, 16, "cpu"))
     (src,) = ran
     assert len(src) == 3 and (src[0] is not None) == (copied and copies)
+
+
+@pytest.mark.parametrize("group", [16, 64])
+@pytest.mark.parametrize("step", [1, 3, 64])
+def test_a_cached_value_and_the_row_that_went_in(group, step):
+    """However a prompt is cut into steps, a cached value is off its bf16 row by at most half a step of the scale it was
+    quantized with and half a step of each larger one its block took since."""
+    n, h, d, bs = 150, 2, 64, 64
+    g = torch.Generator().manual_seed(step)
+    x = (torch.randn(n, h, d, generator=g) * (0.2 + 3 * torch.rand(n, 1, 1, generator=g))).to(torch.bfloat16)
+    cache, _ = R.new_cache(4, bs, h, d, "apart")
+    scale, table = torch.zeros(4, h, bs // group), torch.tensor([[2, 0, 3]])
+    off, held = torch.zeros(n, h), 0
+    while held < n:
+        m = min(step, n - held)
+        _, before = R.values(cache, scale, table[0], n)
+        R.write(x[held:held + m], cache, scale, [0, m], [held + m], table)
+        held += m
+        codes, s = R.values(cache, scale, table[0], n)
+        grew = (s != before).t()                                    # [n, H]: new rows, and those behind whom a scale grew
+        grew[held - m:held] = True
+        off += torch.where(grew, s.t() / 2, torch.zeros_like(off)).float()
+        off[held:] = 0
+    got = (codes * s[..., None]).transpose(0, 1)
+    assert bool(((got - x.double()).abs() <= off.double()[..., None] * (1 + 1e-4)).all())
