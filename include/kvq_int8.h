@@ -304,8 +304,11 @@ int kvq_read_block_cache(const int8_t* k_cache, int64_t kc_sb, int64_t kc_sn, in
 
 /* Attention over a block-scaled cache for requests with 1 <= q_len <= qmax:
  *   o = softmax(q . (k_code * k_scale) * softmax_scale) (v_code * v_scale),  bottom-right causal, bf16 q and out;
- * a row that sees no key is zero, one whose q holds a NaN or an infinity is NaN; softmax_scale from 1e-16 to 1e16. Neither q nor the softmax's weights are rounded to 8 bits. Rows, skipped requests, split
- * buffers and the other arguments as kvq_int8_decode_attention_ex. */
+ * a row that sees no key is zero, another whose q holds a NaN or an infinity is NaN; softmax_scale from 1e-16 to 1e16. The
+ * codes are exact, a V scale counts as at least 2^-40 (the write's least is 1e-8). Rounded: each channel of q to a multiple of
+ * its row's largest / 16,256; the weights to 2^-14 of each where at most 16 (token, q head) rows share a kv head, and by
+ * attn_rules.h up to 32, else to bf16 (2^-8 of each). Rows, skipped requests, split buffers and the other arguments as
+ * kvq_int8_decode_attention_ex (segm_sum's last piece is marked by its sign). */
 int kvq_block_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
                                int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
                                int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,
@@ -328,7 +331,8 @@ int kvq_block_codes(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k
 /* The same attention for the rows of a work list, as kvq_int8_prefill_attention_ex takes it (tile_piece NULL: every
  * entry reads all of its rows' keys). k_codes / v_codes / code_scales: the requests' pages as kvq_block_codes leaves them
  * (num_pages of them, codes_table [num_seqs, ..] with row stride ct_stride in place of block_table), read instead of the
- * int8 pages, whose conversion in the kernel costs more where many rows read each key. NULL: the int8 pages. */
+ * int8 pages, whose conversion in the kernel costs more where many rows read each key; q is then taken as it is. NULL: the
+ * int8 pages. Weights are rounded to bf16 either way. */
 int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const int8_t* k_cache, int64_t k_sb,
                                 int64_t k_sn, int64_t k_sh, const int8_t* v_cache, int64_t v_sb, int64_t v_sn,
                                 int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads,

@@ -12,7 +12,7 @@
 //            a channel, where K's codes are off by 2^-8 of theirs; bf16 as given where K's codes are copied as bf16
 //   weights  to a sum of two bf16 (block_attn_kernel: 2^-14 of each, error against 64 bits 1.66e-3, the bf16 output's) or to
 //            one (many rows: 2^-8, 2.0 to 2.3e-3; a second MFMA for every product there). Each weight keeps its own exponent:
-//            as integers of a tile's scale the keys beside two of 90% of a row's attention and no V were 1.3 to 4.7% of it off.
+//            as integers of a tile's scale the keys beside two of 95% of a row's attention and no V were 1.3 to 4.7% off.
 
 #include "block_rows.h"
 
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256) void read_block_kernel(ReadBlockArgs a) {
 // PACK: at most 8 (token, q head) rows per kv head: the hi parts (of q, of P) are the MFMA's columns 0 .. 7, the lo parts
 // columns 8 .. 15, so both cost one MFMA, as one part of 16 rows does; lanes n and n + 8 hold the same row and exchange
 // their half of S by a 16-lane rotation, and their halves of O at the end. Otherwise 16 rows and two MFMAs per product.
-// Bound by memory for long contexts: 128 requests of 32,768 keys (28 / 4 heads x 128) 4.3 GB in 638 to 659 us, 6.5 to 6.75
+// Bound by memory for long contexts: 128 requests of 32,768 keys (28 / 4 heads x 128) 4.3 GB in 636 to 662 us, 6.5 to 6.77
 // TB/s. 96 of 1 to 32,768 keys 101 us with the merge, 534 MB: fixed costs per piece. One of 4,096 13 us: the launches and one
 // wave of pieces.
 // ------------------------------------------------------------------------------------------------
@@ -682,8 +682,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, BLOCK_AT
 // ------------------------------------------------------------------------------------------------
 // Many query rows (block_rows.h). block_verify_kernel: short queries of more rows than block_attn_kernel's tiles suit, on
 // its plan, in pieces of 64 rows. block_prefill_kernel: the work lists of long queries, 128 rows an entry.
-// 64 requests of 8 tokens, 512 to 8,192 keys (28 / 4 heads x 128): 48 us + 8.6 of the merge, 162 MB; the vector units are busy
-// 48% of the cycles and the wavefronts wait for 31% of theirs. 700 + 333 tokens (block_prefill_kernel, cut): 43 us + 7.4.
+// 64 requests of 8 tokens, 512 to 8,192 keys (28 / 4 heads x 128): 46 us + 8.5 of the merge, 162 MB; the vector units are busy
+// 48% of the cycles and the wavefronts wait for 31% of theirs. Not at a limit of its own: each wavefront reads the whole tile
+// from LDS for 16 rows, and all of them convert V behind one barrier. 700 + 333 tokens (block_prefill_kernel, cut): 43 us + 7.5.
 // ------------------------------------------------------------------------------------------------
 constexpr int64_t BLOCK_VERIFY_ONE_GROUP = 128;   // (request, kv head) pairs of a cut batch from which one group is faster
 template <int D, int KW>
@@ -726,8 +727,8 @@ __global__ __launch_bounds__(256 * KW, KW == 1 ? 3 : 2) void block_verify_kernel
   });
 }
 
-// The bf16 prefill over a temporary cache of the codes and their scales' table (kvq_block_codes). 2 x 8,192 tokens of 28 / 4
-// heads x 128 947 us, 1.16 PFLOP/s, the matrix cores busy 59% of the cycles (profiled alone; with the copy, 21 us, 967 to
+// The bf16 prefill over a temporary cache of the codes and their scales' table (kvq_block_codes). 2 x 8,192 tokens of 32 / 8
+// heads x 128 941 us, 1.17 PFLOP/s, the matrix cores busy 59% of the cycles (profiled alone; with the copy, 21 us, 963 to
 // 1,028 us a call).
 template <int D, bool SPLIT>
 __global__ __launch_bounds__(256, 3) void block_codes_prefill_kernel(PrefillArgs a) {

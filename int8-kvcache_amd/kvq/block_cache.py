@@ -149,8 +149,10 @@ def block_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, blo
                            max_query_len=1):
     """Attention over a block-scaled cache for the requests with at most SHORT_Q query tokens (others are skipped), with
     decode_attention's arguments: out rows softmax(q k^T softmax_scale) v, bottom-right causal, of the cached values and
-    the bf16 q (neither q nor the softmax's weights are rounded to 8 bits). A row that sees no key is zero. segm:
-    split buffers (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces."""
+    the bf16 q. Rounded: each channel of q to a multiple of its row's largest / 16,256; the weights to 2^-14 of each for up to
+    16 (token, q head) rows per kv head (32 where the call is not cut), to bf16 (2^-8) for more. A row that sees no key is
+    zero, another with a NaN or an infinity in q NaN. segm: split buffers (cuda_kernels.split_buffers), which allow a
+    (request, kv head) to be cut into pieces."""
     name = "block_decode_attention"
     so, sm, ss = segm if segm is not None else (None, None, None)
     if ck._served(ck.ext(), name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],
@@ -205,8 +207,8 @@ def direct_pays(longest, workgroups, d, fill, elems):
 
 def block_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, plan, softmax_scale, scales):
     """Attention over a block-scaled cache for the plan's long requests (cuda_kernels.plan_long; the others' rows are left
-    as they were): the formula of block_decode_attention on bf16 operands, the codes exact, their scales applied in fp32, the
-    softmax's weights rounded to bf16. KVQ_PREFILL_DIRECT as long_attention's: 1 (or fold) reads the int8 pages
+    as they were): the formula of block_decode_attention, the codes exact, their scales applied in fp32, the softmax's
+    weights rounded to bf16 (and q as there, where the int8 pages are read). KVQ_PREFILL_DIRECT as long_attention's: 1 (or fold) reads the int8 pages
     themselves, 0 a temporary bf16 cache of the plan's pages' codes; unset: whichever is faster (direct_pays)."""
     name, e = "block_long_attention", ck.ext()
     bs, h, d = k_cache.shape[1:]

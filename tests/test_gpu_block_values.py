@@ -85,8 +85,8 @@ def test_cut_rows_without_keys_in_their_last_pieces(q_lens):
 
 # ------------------------------------------------------------------------------------------------ dominating keys
 def sink(n, hq, h, d, q_rows, share, own, seed):
-    """K, V [n, h, d] and q [q_rows, hq, d]: key 0 (and key 40, if there is one) takes `share` of each row's attention, with a
-    V of `own` times the others'."""
+    """K, V [n, h, d] and q [q_rows, hq, d]: keys 0 and 40 each take `share` of a row's attention beside the other keys, with V
+    of `own` times theirs."""
     g = gen(seed)
     u = torch.nn.functional.normalize(torch.randn(h, d, generator=g), dim=-1)
     k, v = torch.randn(n, h, d, generator=g), torch.randn(n, h, d, generator=g)
