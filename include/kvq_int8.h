@@ -305,7 +305,7 @@ int kvq_read_block_cache(const int8_t* k_cache, int64_t kc_sb, int64_t kc_sn, in
 /* Attention over a block-scaled cache for requests with 1 <= q_len <= qmax:
  *   o = softmax(q . (k_code * k_scale) * softmax_scale) (v_code * v_scale),  bottom-right causal, bf16 q and out;
  * a row that sees no key is zero, another whose q holds a NaN or an infinity is NaN; softmax_scale from 1e-16 to 1e16. The
- * codes are exact, a V scale counts as at least 2^-40 (the write's least is 1e-8). Rounded: each channel of q to a multiple of
+ * codes are exact, a V scale counts as at least 2^-70 (the write's least is 1e-8). Rounded: each channel of q to a multiple of
  * its row's largest / 16,256; the weights to 2^-14 of each where at most 16 (token, q head) rows share a kv head, and by
  * attn_rules.h up to 32, else to bf16 (2^-8 of each). Rows, skipped requests, split buffers and the other arguments as
  * kvq_int8_decode_attention_ex (segm_sum's last piece is marked by its sign). */

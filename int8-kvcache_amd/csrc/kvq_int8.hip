@@ -54,10 +54,11 @@ struct BlockScales {
   int lg;   // log2 of the positions per scale
 };
 constexpr float MIN_BLOCK_SCALE = 1e-30f;   // a K scale counts as at least this (0 times a masked score is no number)
-constexpr float MIN_V_SCALE = 0x1p-40f;     // and a V scale as this (9.1e-13; the write's smallest is 1e-8)
+constexpr float MIN_V_SCALE = 0x1p-70f;     // and a V scale as this (8.5e-22; the write's smallest is 1e-8)
 // The attention's reference m is a row's largest score plus BLOCK_REF (log2 units): a weight 2^(score - m) is at most 2^-24 (m
 // may lag by 8), so that P = weight * V scale and a million keys' sum of P * code stay below 2^124 for bf16's largest values
-// (V scales of 2^121), and at the smallest V scale a weight of 2^-54 of the largest is still there.
+// (V scales of 2^121); P stays a normal number down to weights of 2^-67 of the largest at the write's smallest V scale, of
+// 2^-24 at MIN_V_SCALE.
 constexpr float BLOCK_REF = 32.f;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));

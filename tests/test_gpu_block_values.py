@@ -252,3 +252,19 @@ def test_capture_after_the_plans_own_copies(copies, monkeypatch):
         graph.replay()
         want = bc.block_long_attention(q, c.kc, c.vc, nan_like(q), cu, sl, c.table, plan, d ** -0.5, c.scales)
         assert off(out, want.double()) <= MANY, i
+
+
+# ------------------------------------------------------------------------------------------------ scales made elsewhere
+@pytest.mark.parametrize("q_lens", [[1, 1], [2, 1], [8, 8], [40, 30]])
+def test_scales_far_below_the_writes(q_lens, source):
+    """Scales that another program made: V's of 1e-18 as any other; of 0 (a cache that was cleared, not written) the values
+    are zero, to what the smallest scale that counts leaves of 127 codes."""
+    lens = [700, 1500]
+    k, v = rows(sum(lens), 4, 128, 6)
+    c = written(k.float(), v.float(), lens)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    c.scales["v_scale"].fill_(1e-18)
+    for segm in (None, nan_segm(sum(q_lens), 28, 16, 128)):
+        check(c, q, q_lens, lens, SHORT if max(q_lens) < 8 else MANY, segm)
+    c.scales["v_scale"].zero_()
+    assert float(call(c, q, q_lens, lens).abs().max()) <= 128 * 2.0 ** -70
