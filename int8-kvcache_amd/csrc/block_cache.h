@@ -728,7 +728,7 @@ __global__ __launch_bounds__(256 * KW, KW == 1 ? 3 : 2) void block_verify_kernel
 }
 
 // The bf16 prefill over a temporary cache of the codes and their scales' table (kvq_block_codes). 2 x 8,192 tokens of 32 / 8
-// heads x 128 941 us, 1.17 PFLOP/s, the matrix cores busy 59% of the cycles (profiled alone; with the copy, 21 us, 963 to
+// heads x 128 941 us, 1.17 PFLOP/s, the matrix cores busy 59% of the cycles (profiled alone; with the copy, 21 us, 960 to
 // 1,028 us a call).
 template <int D, bool SPLIT>
 __global__ __launch_bounds__(256, 3) void block_codes_prefill_kernel(PrefillArgs a) {

@@ -268,3 +268,25 @@ def test_scales_far_below_the_writes(q_lens, source):
         check(c, q, q_lens, lens, SHORT if max(q_lens) < 8 else MANY, segm)
     c.scales["v_scale"].zero_()
     assert float(call(c, q, q_lens, lens).abs().max()) <= 128 * 2.0 ** -70
+
+
+@pytest.mark.parametrize("bs,group", [(128, 128), (256, 128), (64, 64), (32, 16)])
+@pytest.mark.parametrize("order", [(2, 1, 0), (1, 0, 2), (0, 2, 1)])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [8, 3, 8], [40, 200, 9]])
+def test_scales_in_any_order(bs, group, order, q_lens, source):
+    """Scales of another memory order than [pages, heads, blocks], with the largest blocks and pages: the outputs are those of
+    scales side by side, bit for bit."""
+    lens = [700, 257, 1300]
+    k, v = rows(sum(lens), 4, 128, 6)
+    c = written(k.float(), v.float(), lens, bs, group)
+    q = torch.randn(sum(q_lens), 28, 128, generator=gen(3)).to(torch.bfloat16).to(DEV)
+    back = [i for i, _ in sorted(enumerate(order), key=lambda x: x[1])]
+    for segm in (None, nan_segm(sum(q_lens), 28, 16, 128)):
+        want = call(c, q, q_lens, lens, segm)
+        check(c, q, q_lens, lens, SHORT if max(q_lens) < 8 else MANY, segm)
+        kept = c.scales
+        c.scales = {n: s.permute(order).contiguous().permute(back) for n, s in kept.items()}
+        assert c.scales["k_scale"].stride() != kept["k_scale"].stride()
+        got = call(c, q, q_lens, lens, segm)
+        c.scales = kept
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
