@@ -25,7 +25,7 @@
 #include <stdint.h>
 
 /* The version of these entry points' signatures (kvq_abi_version): changes with any of them. */
-#define KVQ_ABI_VERSION 15
+#define KVQ_ABI_VERSION 16
 
 #ifdef __cplusplus
 extern "C" {
@@ -344,6 +344,103 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
                                 const int32_t* tile_slot, const int32_t* merge, int64_t num_merge, float* part_out,
                                 float* part_ml, const void* k_codes, const void* v_codes, const float* code_scales,
                                 int64_t num_pages, const int32_t* codes_table, int64_t ct_stride, void* stream);
+
+/* ---- 4-bit cache, no counterpart in the reference ----
+ * A cached value is an e2m1 code (0, 1/2, 1, 3/2, 2, 3, 4, 6 or their negatives) times 2^(byte - 127), one exponent byte for
+ * each 32 channels of a row (page, slot, head), K's and V's apart. Caches are bytes [nb, bs, H, D / 2], strides (sb, sn, sh, 1)
+ * in bytes, multiples of 16, channel 2 c in the low half of byte c; exponent bytes k_scale / v_scale [nb, H, bs, D / 32],
+ * strides (s_sb, s_sh, D / 32, 1), 16-byte aligned as well. Tables and lengths as above; head_dim 64 or 128. An exponent byte
+ * that the write does not make (above 252: 255 would be no number) may give any value for its own row, and counts nowhere else. */
+
+/* Quantize rows into slots: for t < num_tokens whose slot is in [0, nb * bs), others are skipped. Of a group's 32 values x, with
+ * top = max |x| (finite x):  e = floor(log2 top) - 2, one more where top 2^-e > 7, from -100 to 125; byte e + 127; codes the
+ * nearest of x 2^-e, ties to the even code, at most 6 (infinities too); a NaN is 0. Bit-reproducible. */
+int kvq_quant_fp4_cache(const void* key, int64_t key_st, int64_t key_sh, const void* value, int64_t val_st, int64_t val_sh,
+                        uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, uint8_t* v_cache, int64_t vc_sb,
+                        int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                        int64_t head_dim, uint8_t* k_scale, uint8_t* v_scale, int64_t s_sb, int64_t s_sh,
+                        const int64_t* slot_mapping, int64_t num_tokens, void* stream);
+
+/* Read ranges of keys back as bf16 (exact), with kvq_read_block_cache's ranges and rows. */
+int kvq_read_fp4_cache(const uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, const uint8_t* v_cache,
+                       int64_t vc_sb, int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                       int64_t head_dim, const uint8_t* k_scale, const uint8_t* v_scale, int64_t s_sb, int64_t s_sh,
+                       const int32_t* starts, const int32_t* cu_seqlens_k, const int32_t* block_table, int64_t bt_stride,
+                       int64_t num_seqs, void* k_out, int64_t ko_st, int64_t ko_sh, void* v_out, int64_t vo_st, int64_t vo_sh,
+                       int64_t num_rows, void* stream);
+
+/* Pages as bf16 (exact) in a contiguous temporary cache [num_pages, bs, H, D], pages as kvq_dequant_pages takes them, and in
+ * scales_out [H, num_pages * bs / 16, 4] the table that the prefill below reads beside them. */
+int kvq_fp4_pages(const uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, const uint8_t* v_cache, int64_t vc_sb,
+                  int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim,
+                  const uint8_t* k_scale, const uint8_t* v_scale, int64_t s_sb, int64_t s_sh, void* k_out, void* v_out,
+                  float* scales_out, const int32_t* block_table, int64_t bt_stride, const int32_t* src_req,
+                  const int32_t* src_j, int64_t num_pages, void* stream);
+
+/* The attention below for the rows of a work list, as kvq_paged_prefill_attention_ex takes it (tile_piece NULL: every entry
+ * reads all of its rows' keys), over pages that kvq_fp4_pages left (pages_table [num_seqs, ..], row stride pt_stride). q is
+ * taken as it is, the weights are rounded to bf16. */
+int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k_pages, const void* v_pages,
+                              const float* page_scales, int64_t num_pages, int64_t block_size, int64_t num_kv_heads,
+                              int64_t head_dim, void* out, int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q,
+                              const int32_t* seq_lens, const int32_t* pages_table, int64_t pt_stride, int64_t num_q_heads,
+                              const int32_t* tile_req, const int32_t* tile_row, int64_t num_tiles, int64_t rows_per_tile,
+                              double softmax_scale, const int32_t* tile_piece, const int32_t* tile_slot, const int32_t* merge,
+                              int64_t num_merge, float* part_out, float* part_ml, void* stream);
+
+/* Attention over a 4-bit cache for requests with 1 <= q_len <= qmax: o = softmax(q k^T softmax_scale) v, bottom-right causal,
+ * bf16 q and out; a row that sees no key is zero, another whose q holds a NaN or an infinity is NaN. Cached values are exact.
+ * Rounded: the weights, to 2^-16 of each where at most 8 (token, q head) rows share a kv head, else to bf16 (2^-8). lse (fp32 [T, Hq], row stride lse_st, or NULL): the rows' natural
+ * log-sum-exp, -inf where no key is seen. softmax_scale from 1e-16 to 1e16. Rows, skipped requests, split buffers and the other
+ * arguments as kvq_block_decode_attention. */
+int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,
+                             int64_t k_sh, const uint8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                             int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                             const uint8_t* k_scale, const uint8_t* v_scale, int64_t s_sb, int64_t s_sh, void* out,
+                             int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                             const int32_t* block_table, int64_t bt_stride, int64_t num_seqs, int64_t num_q_heads,
+                             double softmax_scale, float* segm_out, float* segm_max, float* segm_sum, int64_t seg_st,
+                             int64_t seg_sh, int64_t num_splits, int64_t segm_rows, float* lse, int64_t lse_st,
+                             int64_t target_waves, int64_t max_query_len, int64_t qmax, void* stream);
+
+/* Add the attention weights of a step's rows to running sums: for requests with 1 <= q_len <= qmax and j < w_cols,
+ *   weights[r, h, j] += sum over r's tokens and h's q heads that see key j of exp(q . k_j softmax_scale - lse)
+ * weights fp32 [B, Hkv, w_cols], strides (w_sr, w_sh, 1); lse as kvq_fp4_decode_attention leaves it, rows whose lse is not
+ * finite add nothing. Row r of weights belongs to request r alone. Bit-reproducible. */
+int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,
+                        int64_t k_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                        const uint8_t* k_scale, int64_t s_sb, int64_t s_sh, const float* lse, int64_t lse_st, float* weights,
+                        int64_t w_sr, int64_t w_sh, int64_t w_cols, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                        const int32_t* block_table, int64_t bt_stride, int64_t num_seqs, int64_t num_q_heads,
+                        double softmax_scale, int64_t max_query_len, int64_t qmax, void* stream);
+
+/* Evict: of request r's n = seq_lens[r] keys (at most its bt_cols pages' slots), each kv head keeps m = keep[r] (at most
+ * kept_cols, at least 0): the last min(recent, m) and, of those before, the ones of the largest weights (ties to the lowest
+ * position, a NaN the largest; 0 from w_cols on). Their rows move to positions 0 .. m - 1 in order, their weights with them;
+ * weights[r, h, m .. n - 1] become 0. kept[r, h, i] (int32, strides (kp_sr, kp_sh, 1)): the position that row i held before;
+ * new_lens[r] = min(n, m). Where n <= m nothing moves (kept[r, h, i] = i). Entries of kept from new_lens[r] on and cache rows
+ * from there on are left as they are. The pages of a call's requests must be theirs alone. Page ids outside [0, nb) read as page
+ * 0, and are not written. Bit-reproducible. */
+int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, uint8_t* v_cache, int64_t v_sb, int64_t v_sn,
+                  int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, uint8_t* k_scale,
+                  uint8_t* v_scale, int64_t s_sb, int64_t s_sh, float* weights, int64_t w_sr, int64_t w_sh, int64_t w_cols,
+                  const int32_t* seq_lens, const int32_t* keep, int64_t recent, const int32_t* block_table, int64_t bt_stride,
+                  int64_t bt_cols, int64_t num_seqs, int32_t* kept, int64_t kp_sr, int64_t kp_sh, int64_t kept_cols,
+                  int32_t* new_lens, void* stream);
+
+/* RMS norm of each head's query and key rows and their rotation by position, for t < num_tokens and positions[t] in
+ * [0, num_positions) (other tokens' output rows are left as they are):
+ *   y = x / sqrt(mean(x^2) + eps) * weight;   (a, b) -> (a cos - b sin, b cos + a sin)
+ * for the pairs of the first rotary_dim channels: (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved. q / k and their
+ * outputs bf16 [T, H, D], strides (st, sh, 1), an output may be its input; positions int32 or int64 (position_bits); table
+ * [num_positions, rotary_dim] (row stride t_st) fp32 or bf16: rotary_dim / 2 cosines, then as many sines; weights [D] fp32 or
+ * bf16, both NULL: no norm. fp32 throughout, one rounding. rotary_dim a multiple of 16. No counterpart in the reference. */
+int kvq_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* q_out,
+                  int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int64_t num_tokens,
+                  int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, const void* positions, int64_t position_bits,
+                  const void* table, int64_t t_st, int64_t num_positions, int64_t rotary_dim, int64_t table_bf16,
+                  const void* q_weight, const void* k_weight, int64_t weight_bf16, double eps, int64_t interleaved,
+                  void* stream);
 
 /* Text of the last error on this thread ("" if none). */
 const char* kvq_last_error(void);

@@ -1,0 +1,376 @@
+// Eviction from a 4-bit cache by accumulated attention weight. Part of kvq_int8.hip (included at its end, after fp4_cache.h).
+//
+//   key_weights_kernel   adds what each cached key gets of a step's rows to its running sum
+//   evict_kernel         chooses each request's and kv head's keys and moves them to the front of its pages
+#pragma once
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// w[r, h, j] += sum over the request's rows i (query tokens x the kv head's q heads) that see key j of 2^(s_ij - lse_i)
+// The scores are fp4_attn_kernel's; K alone is read. Pieces of key tiles by attn_kernel's plan (rt is all of a request's row
+// tiles, so a key's sum has one owner in a call: nothing is atomic, the result does not depend on the order of workgroups);
+// a piece's tiles go round the workgroup's wavefronts. A wavefront holds RT row tiles' planes; more rows take another round
+// over the piece's tiles, whose keys' sums the same lanes then add to again.
+// ------------------------------------------------------------------------------------------------
+struct KeyWeightArgs {
+  AttnArgs a;   // (first: fresh_args)
+  Fp4Scales s;
+  const float* lse;
+  float* w;
+  int64_t lse_st, w_sr, w_sh;
+  int cols;
+};
+static_assert(offsetof(KeyWeightArgs, a) == 0, "AttnArgs lead the kernel arguments");
+
+// sum over each 16 lanes
+__device__ __forceinline__ float sum_row(float x) {
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));   // row_ror:8
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, true));   // row_ror:4
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x122, 0xf, 0xf, true));   // row_ror:2
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x121, 0xf, 0xf, true));   // row_ror:1
+}
+
+constexpr int KW_WAVES = 4;
+template <int D, int RT>
+__global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightArgs args) {
+  touch_args();
+  constexpr int SB = D / FP4_GROUP;
+  const AttnArgs& a = args.a;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int n = lane & 15, g = lane >> 4;
+  walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int, int c0, int c1, int, int) {
+    const int L = __builtin_amdgcn_readfirstlane(w.len), qlen = __builtin_amdgcn_readfirstlane(w.qlen);
+    const int tok = __builtin_amdgcn_readfirstlane(w.tok);
+    if (L <= 0) return;
+    const int G = a.G, bs = 1 << a.lbs;
+    const int* bt = a.block_table + (int64_t)r * a.bt_stride;
+    const uint8_t* kbase = (const uint8_t*)a.kc + (int64_t)kvh * a.k_sh + n * (int)a.k_sn + (D / 8) * g;
+    const uint8_t* sbase = args.s.k + (int64_t)kvh * args.s.sh + n * SB + g * (D / 4) / FP4_GROUP;
+    float* wrow = args.w + (int64_t)r * args.w_sr + (int64_t)kvh * args.w_sh;
+    for (int row0 = 0; row0 < qlen * G; row0 += 16 * RT) {
+      Fp4Query<D> q[RT];
+      float f[RT], l2[RT];
+      int lim[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int R = row0 + 16 * t + n, rtok = div_group(a, R), rh = R - rtok * G;
+        const bool real = rtok < qlen;
+        const int64_t at = tok + min(rtok, qlen - 1);
+        q[t].make(a.q + at * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, real, g);
+        const float l = args.lse[at * args.lse_st + kvh * G + rh];
+        // a row whose log-sum-exp is no finite number adds nothing: it saw no key, or its weights are none
+        const bool in = real && __builtin_fabsf(l) < INFINITY;
+        f[t] = a.sm_log2;
+        l2[t] = l * 1.4426950408889634f;
+        lim[t] = in ? L - qlen + 1 + rtok : 0;
+      }
+      struct Tile {
+        uint32_t k[2][D / 32];
+        uint8_t ks[2];
+      };
+      auto load = [&](Tile& x, int c) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int key = min(c * TILE + 16 * b, (L - 1) & ~15);
+          const int p = page_at(bt, 0, 0, key >> a.lbs), pg = p >= 0 && p < a.num_blocks ? p : 0, of = key & (bs - 1);
+          load_k16<D>(x.k[b], kbase + (int64_t)pg * a.k_sb + (int64_t)of * a.k_sn);
+          x.ks[b] = sbase[(int64_t)pg * args.s.sb + of * SB];
+        }
+      };
+      Tile x;
+      for (int c = c0 + wave; c < c1; c += KW_WAVES) {
+        load(x, c);
+        // lanes n < 8 own key 16 (n / 4) + 4 g + n % 4 of the tile
+        const int own = c * TILE + 16 * (n >> 2) + 4 * g + (n & 3);
+        const bool mine = n < 8 && own < min(L, args.cols);
+        float sum[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const f32x4 z = fp4_scores<D>(x.k[b], x.ks[b], q[t]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], f[t], -l2[t]));
+              sum[4 * b + i] += c * TILE + 16 * b + 4 * g + i < lim[t] ? p : 0.f;
+            }
+          }
+        float add = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float s = sum_row(sum[i]);
+          add = n == i ? s : add;
+        }
+        if (mine) wrow[own] += add;
+      }
+    }
+  });
+}
+
+// ------------------------------------------------------------------------------------------------
+// One workgroup per (request, kv head) with n keys of which it may hold m = keep < n. Kept: the last min(recent, m), and of the
+// rest those of the m - recent largest sums, ties to the lowest position.
+//   select   the sum at which the count is reached, by three histograms of 12, 12 and 8 bits of its ordered bits
+//   list     the kept positions in order: a wavefront's share of the positions is counted, then written behind those before it
+//   move     row i takes the row of the i-th kept position, which is i or later: rows are read into registers, in order, a
+//            batch at a time, and written after a barrier, so that nothing is overwritten that is still to be read
+// ------------------------------------------------------------------------------------------------
+struct EvictArgs {
+  uint8_t* kc;
+  uint8_t* vc;
+  Fp4Scales s;
+  float* w;
+  const int* seq_lens;
+  const int* keep;
+  const int* block_table;
+  int* kept;
+  int* new_lens;
+  int64_t k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, w_sr, w_sh, bt_stride, kp_sr, kp_sh;
+  int heads, num_blocks, lbs, cols, bt_cols, kept_cols, recent;
+};
+constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / WAVE;
+constexpr int EV_BINS = 4096;
+constexpr int EV_ROWS = 4;   // rows that a thread holds of a batch
+
+// order of the sums as unsigned numbers: NaN the largest, -0 as 0
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
+}
+
+template <int D>
+__global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
+  constexpr int SB = D / FP4_GROUP, CH = D / 32;   // exponent bytes, 16-byte chunks of a row's codes
+  __shared__ uint32_t bins[EV_BINS];
+  __shared__ uint32_t wsum[EV_WAVES], wsum2[EV_WAVES];
+  __shared__ uint32_t found[3];
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int r = blockIdx.x / a.heads, h = blockIdx.x - r * a.heads;
+  const int* bt = a.block_table + (int64_t)r * a.bt_stride;
+  const int n = min(max(a.seq_lens[r], 0), (int)min((int64_t)a.bt_cols << a.lbs, (int64_t)INT32_MAX));
+  const int m = min(max(a.keep[r], 0), a.kept_cols), len = min(n, m);
+  int* kept = a.kept + (int64_t)r * a.kp_sr + (int64_t)h * a.kp_sh;
+  float* w = a.w + (int64_t)r * a.w_sr + (int64_t)h * a.w_sh;
+  if (h == 0 && tid == 0) a.new_lens[r] = len;
+  if (n <= m) {   // all of them stay where they are
+    for (int i = tid; i < n; i += EV_THREADS) kept[i] = i;
+    return;
+  }
+  const int recent = min(a.recent, m), c = n - recent, need = m - recent;   // candidates: positions 0 .. c - 1; need < c
+  auto sum_at = [&](int i) { return i < a.cols ? w[i] : 0.f; };
+  // ---- select ----
+  uint32_t edge = 0xffffffffu;   // keys above it are kept, and `ties` of those equal to it
+  int ties = 0;
+  if (need > 0) {
+    uint32_t prefix = 0;
+    int left = need;   // still to be found at or below the current bin
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 20 : pass == 1 ? 8 : 0, nb = pass == 2 ? 256 : EV_BINS;
+      const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xfff00000u : 0xffffff00u;
+      for (int i = tid; i < nb; i += EV_THREADS) bins[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < c; i += EV_THREADS) {
+        const uint32_t key = ordered(sum_at(i));
+        if ((key & mask) == prefix) atomicAdd(&bins[(key >> shift) & (nb - 1)], 1u);
+      }
+      __syncthreads();
+      // the bin, counted from the largest, where the count reaches `left`
+      const int per = nb / EV_THREADS > 0 ? nb / EV_THREADS : 1;   // bins per thread, from the top
+      uint32_t own = 0;
+      const int top = nb - 1 - tid * per;
+      if (top >= 0)
+        for (int i = 0; i < per; ++i) own += bins[top - i];
+      uint32_t incl = (uint32_t)wave_incl_sum((int)own);
+      if (lane == WAVE - 1) wsum[wave] = incl;
+      __syncthreads();
+      for (int k = 0; k < wave; ++k) incl += wsum[k];
+      if (top >= 0 && (int)incl >= left && (int)(incl - own) < left) {
+        uint32_t before = incl - own;
+        int b = top;
+        while ((int)(before + bins[b]) < left) before += bins[b--];
+        found[0] = (uint32_t)b;
+        found[1] = before;
+      }
+      __syncthreads();
+      prefix |= found[0] << shift;
+      left -= (int)found[1];
+      __syncthreads();
+    }
+    edge = prefix;
+    ties = left;
+  }
+  // ---- list: wavefront k has the positions [k, k + 1) * share ----
+  const int share = ((n + EV_WAVES - 1) / EV_WAVES + WAVE - 1) / WAVE * WAVE;
+  const int from = min(wave * share, n), to = min(from + share, n);
+  auto above = [&](int i, uint32_t key) { return i >= c || (need > 0 && key > edge); };
+  auto equal = [&](int i, uint32_t key) { return i < c && need > 0 && key == edge; };
+  uint32_t cnt = 0, eq = 0;
+  for (int i0 = from; i0 < to; i0 += WAVE) {
+    const int i = i0 + lane;
+    const uint32_t key = i < min(to, c) ? ordered(sum_at(i)) : 0u;
+    cnt += __builtin_popcountll(__ballot(i < to && above(i, key)));
+    eq += __builtin_popcountll(__ballot(i < to && equal(i, key)));
+  }
+  if (lane == 0) {
+    wsum[wave] = cnt;
+    wsum2[wave] = eq;
+  }
+  __syncthreads();
+  uint32_t at = 0, eq_at = 0;
+  for (int k = 0; k < wave; ++k) {
+    at += wsum[k];
+    eq_at += wsum2[k];
+  }
+  for (int i0 = from; i0 < to; i0 += WAVE) {
+    const int i = i0 + lane;
+    const uint32_t key = i < min(to, c) ? ordered(sum_at(i)) : 0u;
+    const uint64_t ab = __ballot(i < to && above(i, key)), em = __ballot(i < to && equal(i, key));
+    const uint64_t below = (1ull << lane) - 1;
+    const uint32_t e = eq_at + __builtin_popcountll(em & below);   // ties before this position
+    const bool tie = (em >> lane & 1) && (int)e < ties;
+    const uint32_t to_at = at + __builtin_popcountll(ab & below) + min(e, (uint32_t)ties);
+    if ((ab >> lane & 1) || tie) kept[to_at] = i;
+    at += __builtin_popcountll(ab);
+    eq_at += __builtin_popcountll(em);
+  }
+  __threadfence_block();
+  __syncthreads();
+  // ---- move ----
+  auto page = [&](int i) { return bt[i >> a.lbs]; };
+  auto good = [&](int p) { return p >= 0 && p < a.num_blocks; };
+  const int bs = 1 << a.lbs;
+  constexpr int LPR = 2 * CH, RPB = EV_THREADS / LPR;   // lanes per row (K's chunks, then V's), rows per batch step
+  const int ch = tid % LPR, row = tid / LPR;
+  const bool v = ch >= CH;
+  uint8_t* cache = v ? a.vc + (int64_t)h * a.v_sh : a.kc + (int64_t)h * a.k_sh;
+  const int64_t sb = v ? a.v_sb : a.k_sb, sn = v ? a.v_sn : a.k_sn;
+  uint8_t* scale = (v ? a.s.v : a.s.k) + (int64_t)h * a.s.sh;
+  for (int b0 = 0; b0 < m; b0 += RPB * EV_ROWS) {
+    i32x4 code[EV_ROWS];
+    uint32_t byte[EV_ROWS];
+    float sum[EV_ROWS];
+    int src[EV_ROWS];
+#pragma unroll
+    for (int u = 0; u < EV_ROWS; ++u) {
+      const int i = b0 + u * RPB + row;
+      src[u] = i < m ? kept[i] : -1;
+      byte[u] = 0;
+      sum[u] = 0.f;
+      code[u] = i32x4{0, 0, 0, 0};
+      if (src[u] > i) {
+        const int p = page(src[u]);
+        const int64_t pg = good(p) ? p : 0;
+        const int of = src[u] & (bs - 1);
+        code[u] = *reinterpret_cast<const i32x4*>(cache + pg * sb + of * sn + 16 * (ch % CH));
+        byte[u] = scale[pg * a.s.sb + of * SB + ch % CH];
+        if (ch == 0) sum[u] = sum_at(src[u]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < EV_ROWS; ++u) {
+      const int i = b0 + u * RPB + row;
+      if (src[u] <= i) continue;
+      const int p = page(i);
+      if (ch == 0 && i < a.cols) w[i] = sum[u];
+      if (!good(p)) continue;
+      const int of = i & (bs - 1);
+      *reinterpret_cast<i32x4*>(cache + (int64_t)p * sb + of * sn + 16 * (ch % CH)) = code[u];
+      scale[(int64_t)p * a.s.sb + of * SB + ch % CH] = (uint8_t)byte[u];
+    }
+    __syncthreads();
+  }
+  for (int i = m + tid; i < min(n, a.cols); i += EV_THREADS) w[i] = 0.f;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,
+                        int64_t k_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                        const uint8_t* k_scale, int64_t s_sb, int64_t s_sh, const float* lse, int64_t lse_st, float* weights,
+                        int64_t w_sr, int64_t w_sh, int64_t w_cols, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                        const int32_t* block_table, int64_t bt_stride, int64_t num_seqs, int64_t num_q_heads,
+                        double softmax_scale, int64_t max_query_len, int64_t qmax, void* stream) {
+  const char* nm = "fp4_key_weights";
+  if (num_seqs < 0 || num_seqs > INT32_MAX / 4 || max_query_len < 0 || qmax < 1 || w_cols < 0) return fail("%s: bad sizes", nm);
+  if (num_seqs == 0 || w_cols == 0) { g_err.clear(); return KVQ_OK; }
+  if (!(softmax_scale >= MIN_SOFTMAX_SCALE && softmax_scale <= MAX_SOFTMAX_SCALE))
+    return fail("%s: softmax_scale must be positive and finite, from %g to %g", nm, MIN_SOFTMAX_SCALE, MAX_SOFTMAX_SCALE);
+  if (const int rc = check_fp4(nm, num_blocks, block_size, num_kv_heads, head_dim, k_cache, k_sb, k_sn, k_sh, k_cache, k_sb,
+                               k_sn, k_sh, k_scale, k_scale, s_sb, s_sh)) return rc;
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
+    return fail("%s: bad head counts Hq=%lld Hkv=%lld", nm, (long long)num_q_heads, (long long)num_kv_heads);
+  if (!q || !lse || !weights || !cu_seqlens_q || !seq_lens || !block_table) return fail("%s: null pointer", nm);
+  if (!aligned16(q) || (q_st | q_sh) % 8) return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  const int G = (int)(num_q_heads / num_kv_heads);
+  const int64_t most = std::min<int64_t>(qmax, INT32_MAX / 4);
+  if (G * most > INT32_MAX / 4) return fail("%s: too many rows for one kv head", nm);
+  const int64_t rows = (int64_t)G * std::min<int64_t>(std::max<int64_t>(max_query_len, 1), most);
+  const Tuning tune = read_tuning();
+  KeyWeightArgs b;
+  b.s = Fp4Scales{const_cast<uint8_t*>(k_scale), nullptr, s_sb, s_sh};
+  b.lse = lse; b.w = weights; b.lse_st = lse_st; b.w_sr = w_sr; b.w_sh = w_sh;
+  b.cols = (int)std::min<int64_t>(w_cols, INT32_MAX);
+  AttnArgs& a = b.a;
+  memset(&a, 0, sizeof(a));
+  a.q = (const uint16_t*)q; a.kc = (const int8_t*)k_cache;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table;
+  a.q_st = q_st; a.q_sh = q_sh; a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.bt_stride = bt_stride;
+  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
+  a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size); a.G = G;
+  a.g_inv = G > 1 && (G * most + 64) < (1ll << 32) / G ? (unsigned)(((1ll << 32) + G - 1) / G) : 0u;
+  a.qmax = (int)most;
+  a.num_seqs = (int)num_seqs; a.hkv = (int)num_kv_heads;
+  a.max_splits = 1 << 20; a.cut_rows = INT32_MAX;   // (nothing is kept per piece: any number of them)
+  a.rt = (int)((G * most + 15) / 16);               // all of a request's row tiles in one group
+  a.ksplit = 1; a.waves = KW_WAVES; a.min_tiles = KW_WAVES; a.coop = 1;
+  a.xcd_order = tune.xcd_order ? atoi(tune.xcd_order) : 1;
+  a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
+                                       : (int)PLAN_FAST_MAX;
+  a.seg_cost = seg_cost_units(tune, 0);
+  void (*kern)(KeyWeightArgs) = head_dim == 128
+      ? (rows <= 16 ? key_weights_kernel<128, 1> : rows <= 32 ? key_weights_kernel<128, 2> : key_weights_kernel<128, 4>)
+      : (rows <= 16 ? key_weights_kernel<64, 1> : rows <= 32 ? key_weights_kernel<64, 2> : key_weights_kernel<64, 4>);
+  a.workers = (int)std::max<int64_t>(1, (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * KW_WAVES, 0) / KW_WAVES);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.workers), dim3(WAVE * KW_WAVES), 0, st, b);
+  return launched(nm);
+}
+
+int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, uint8_t* v_cache, int64_t v_sb, int64_t v_sn,
+                  int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, uint8_t* k_scale,
+                  uint8_t* v_scale, int64_t s_sb, int64_t s_sh, float* weights, int64_t w_sr, int64_t w_sh, int64_t w_cols,
+                  const int32_t* seq_lens, const int32_t* keep, int64_t recent, const int32_t* block_table, int64_t bt_stride,
+                  int64_t bt_cols, int64_t num_seqs, int32_t* kept, int64_t kp_sr, int64_t kp_sh, int64_t kept_cols,
+                  int32_t* new_lens, void* stream) {
+  const char* nm = "fp4_evict";
+  if (num_seqs < 0 || w_cols < 0 || w_cols > INT32_MAX || bt_cols < 0 || bt_cols > INT32_MAX || kept_cols < 0 ||
+      kept_cols > INT32_MAX || recent < 0)
+    return fail("%s: bad sizes", nm);
+  if (num_seqs == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_fp4(nm, num_blocks, block_size, num_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb, v_sn,
+                               v_sh, k_scale, v_scale, s_sb, s_sh)) return rc;
+  if (!seq_lens || !keep || !new_lens || (bt_cols && !block_table) || (w_cols && !weights) || (kept_cols && !kept))
+    return fail("%s: null pointer", nm);
+  if (num_seqs > INT32_MAX / num_heads) return fail("%s: too many requests and heads for one call", nm);
+  EvictArgs a;
+  a.kc = k_cache; a.vc = v_cache; a.s = Fp4Scales{k_scale, v_scale, s_sb, s_sh}; a.w = weights;
+  a.seq_lens = seq_lens; a.keep = keep; a.block_table = block_table; a.kept = kept; a.new_lens = new_lens;
+  a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh; a.w_sr = w_sr; a.w_sh = w_sh;
+  a.bt_stride = bt_stride; a.kp_sr = kp_sr; a.kp_sh = kp_sh;
+  a.heads = (int)num_heads; a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size); a.cols = (int)w_cols;
+  a.bt_cols = (int)bt_cols; a.kept_cols = (int)kept_cols; a.recent = (int)std::min<int64_t>(recent, INT32_MAX);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(num_seqs * num_heads));
+  if (head_dim == 128) hipLaunchKernelGGL(evict_kernel<128>, grid, dim3(EV_THREADS), 0, st, a);
+  else hipLaunchKernelGGL(evict_kernel<64>, grid, dim3(EV_THREADS), 0, st, a);
+  return launched(nm);
+}
+
+}  // extern "C"

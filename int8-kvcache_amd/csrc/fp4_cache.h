@@ -1,0 +1,845 @@
+// The 4-bit cache: e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives), two to a byte, the even channel's in the low
+// half, and one exponent byte for each 32 channels of a row (page, slot, head), K and V apart; a cached value is
+// code * 2^(byte - 127), exact in bf16; one instruction converts two of them. A row's scales are its own, so
+// rows are written, moved and dropped one by one. Part of kvq_int8.hip (included at its end: it shares the helpers above it).
+//
+//   quant_fp4_kernel   quantize a step's new K/V rows into their slots
+//   read_fp4_kernel    ranges of the requests' keys back to bf16 rows
+//   fp4_pages_kernel   pages back to a contiguous bf16 cache, for the prefill
+//   fp4_attn_kernel    attention of short queries
+#pragma once
+
+namespace {
+
+constexpr int FP4_GROUP = 32;             // channels per exponent byte
+constexpr int FP4_MIN_E = 27, FP4_MAX_E = 252;   // the exponent bytes that the write makes: 2^-100 .. 2^125
+
+// a cache's exponent bytes: those of (page p, head h, slot n) are D / 32 bytes at p * sb + h * sh + n * D / 32
+struct Fp4Scales {
+  uint8_t* k;
+  uint8_t* v;
+  int64_t sb, sh;
+};
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+// 8 codes -> 8 bf16, times 2^(byte - 127) (byte << 23 as a float's bits; exact, the smallest products as subnormals)
+__device__ __forceinline__ u32x4 fp4_to_bf16(uint32_t w, uint32_t byte) {
+  const float s = __uint_as_float(byte << 23);
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3))};
+}
+// exponent bytes that no write makes (a buffer that was never cleared) still give finite values
+__device__ __forceinline__ uint32_t fp4_finite(uint32_t byte) { return min(byte, (uint32_t)FP4_MAX_E); }
+
+// ------------------------------------------------------------------------------------------------
+// Quantize rows into their slots. For the 32 values x of a group, t = max |x| (finite x):
+//   e = floor(log2 t) - 2, one more where t 2^-e > 7, between -100 and 125;   code = the nearest of x 2^-e, ties to even, at
+//   most 6: what lies above 6 is off by no more than the half step from 4 to 6
+// infinities become 6, NaN 0. A lane holds 8 channels, so a group is 4 lanes and its maximum two exchanges within them.
+// ------------------------------------------------------------------------------------------------
+struct QuantFp4Args {
+  const uint16_t* key;
+  const uint16_t* value;
+  uint8_t* kc;
+  uint8_t* vc;
+  const int64_t* slots;
+  Fp4Scales s;
+  int64_t key_st, key_sh, val_st, val_sh, kc_sb, kc_sn, kc_sh, vc_sb, vc_sn, vc_sh, num_slots;
+  int num_tokens, heads, lbs;
+};
+
+__device__ __forceinline__ float max_quad(float x) {   // over each 4 lanes
+  x = __builtin_fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, true)));
+  return __builtin_fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, true)));
+}
+// a lane's 8 codes; byte: the group's exponent byte
+__device__ __forceinline__ uint32_t fp4_codes8(u32x4 w, uint32_t& byte) {
+  const float t = max_quad(absmax8(w));
+  const int e = (int)((__float_as_uint(t) + 0x1fffffu) >> 23) - 2;   // a mantissa above 1.75 carries
+  byte = (uint32_t)min(max(e, FP4_MIN_E), FP4_MAX_E);
+  const float m = __uint_as_float((254u - byte) << 23);
+  uint32_t codes = 0;
+  auto clean = [&](float x) { return x == x ? x * m : 0.f; };
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, clean(bf16_lo(w[0])), clean(bf16_hi(w[0])), 1.f, 0);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, clean(bf16_lo(w[1])), clean(bf16_hi(w[1])), 1.f, 1);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, clean(bf16_lo(w[2])), clean(bf16_hi(w[2])), 1.f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, clean(bf16_lo(w[3])), clean(bf16_hi(w[3])), 1.f, 3);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void quant_fp4_kernel(QuantFp4Args a) {
+  constexpr int LPR = D / 8;              // lanes per row
+  constexpr int RPB = 256 / LPR;          // (token, head) rows per workgroup
+  const int64_t item = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
+  const int t = (int)(item / a.heads), h = (int)(item - (int64_t)t * a.heads), c = threadIdx.x % LPR;
+  if (t >= a.num_tokens) return;
+  const int64_t slot = a.slots[t];
+  const u32x4 kw = *reinterpret_cast<const u32x4*>(a.key + t * a.key_st + h * a.key_sh + 8 * c);
+  const u32x4 vw = *reinterpret_cast<const u32x4*>(a.value + t * a.val_st + h * a.val_sh + 8 * c);
+  if (slot < 0 || slot >= a.num_slots) return;
+  const int64_t page = slot >> a.lbs;
+  const int off = (int)(slot & ((1 << a.lbs) - 1));
+  uint32_t kb, vb;
+  const uint32_t kq = fp4_codes8(kw, kb), vq = fp4_codes8(vw, vb);
+  *reinterpret_cast<uint32_t*>(a.kc + page * a.kc_sb + off * a.kc_sn + h * a.kc_sh + 4 * c) = kq;
+  *reinterpret_cast<uint32_t*>(a.vc + page * a.vc_sb + off * a.vc_sn + h * a.vc_sh + 4 * c) = vq;
+  if (c % 4 == 0) {
+    const int64_t at = page * a.s.sb + h * a.s.sh + off * (D / FP4_GROUP) + c / 4;
+    a.s.k[at] = (uint8_t)kb;
+    a.s.v[at] = (uint8_t)vb;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Read ranges of keys back: request r's positions start[r] .. are rows cu_k[r] .. cu_k[r + 1] - 1 of k_out / v_out. One
+// wavefront takes one aligned run of 16 positions (one page) of one head, as read_block_kernel does.
+// ------------------------------------------------------------------------------------------------
+struct ReadFp4Args {
+  const uint8_t* kc;
+  const uint8_t* vc;
+  uint16_t* ko;
+  uint16_t* vo;
+  const int* start;
+  const int* cu_k;
+  const int* block_table;
+  Fp4Scales s;
+  int64_t kc_sb, kc_sn, kc_sh, vc_sb, vc_sn, vc_sh, ko_st, ko_sh, vo_st, vo_sh, bt_stride;
+  int num_seqs, num_rows, heads, num_blocks, lbs, items;
+};
+
+template <int D, bool NT>
+__global__ __launch_bounds__(256) void read_fp4_kernel(ReadFp4Args a) {
+  constexpr int LPR = D / 8, RPL = WAVE / LPR, N = 16 / RPL, SB = D / FP4_GROUP;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int item = blockIdx.x * 4 + wave;
+  if (item >= a.items) return;
+  const int u = item / a.heads, h = item - u * a.heads;
+  const SlotRequest q = request_of_slot(a.cu_k, a.start, a.num_seqs, 4, u, lane);
+  const int r = q.r, row0 = q.cu0, n = min(q.cu1, a.num_rows) - row0, start = q.of;
+  if (start < 0) return;
+  const int b0 = ((start >> 4) + u - ((row0 >> 4) + 2 * r)) << 4;
+  const int first = max(start, b0), last = min(start + n, b0 + 16);
+  if (first >= last) return;
+  int page = page_at(a.block_table, a.bt_stride, r, b0 >> a.lbs);
+  page = page >= 0 && page < a.num_blocks ? page : 0;
+  const int off = b0 & ((1 << a.lbs) - 1);
+  const int row = lane / LPR, c = lane % LPR;
+  const int64_t si = (int64_t)page * a.s.sb + (int64_t)h * a.s.sh + (int64_t)off * SB + c / 4;
+  const uint8_t* kc = a.kc + (int64_t)page * a.kc_sb + (int64_t)off * a.kc_sn + (int64_t)h * a.kc_sh + 4 * c;
+  const uint8_t* vc = a.vc + (int64_t)page * a.vc_sb + (int64_t)off * a.vc_sn + (int64_t)h * a.vc_sh + 4 * c;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int i = row + RPL * j, p = b0 + i;
+    if (p < first || p >= last) continue;
+    const int64_t t = row0 + p - start;
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(kc + (int64_t)i * a.kc_sn);
+    const uint32_t* vp = reinterpret_cast<const uint32_t*>(vc + (int64_t)i * a.vc_sn);
+    const uint32_t kb = fp4_finite(a.s.k[si + i * SB]), vb = fp4_finite(a.s.v[si + i * SB]);
+    u32x4* ko = reinterpret_cast<u32x4*>(a.ko + t * a.ko_st + (int64_t)h * a.ko_sh + 8 * c);
+    u32x4* vo = reinterpret_cast<u32x4*>(a.vo + t * a.vo_st + (int64_t)h * a.vo_sh + 8 * c);
+    if constexpr (NT) {
+      const uint32_t k = __builtin_nontemporal_load(kp), v = __builtin_nontemporal_load(vp);
+      __builtin_nontemporal_store(fp4_to_bf16(k, kb), ko);
+      __builtin_nontemporal_store(fp4_to_bf16(v, vb), vo);
+    } else {
+      *ko = fp4_to_bf16(*kp, kb);
+      *vo = fp4_to_bf16(*vp, vb);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Pages back to a contiguous bf16 cache [P, block_size, H, D] (as dequant_pages_kernel leaves it): page p is
+// block_table[src_req[p], src_j[p]]. A lane converts 8 channels of one (slot, head), K or V by blockIdx.z; lanes in the order
+// of the output. The prefill over it is the block-scaled cache's, whose weights leave room for large values: every scale 1.
+// ------------------------------------------------------------------------------------------------
+struct Fp4PagesArgs {
+  const uint8_t* kc;
+  const uint8_t* vc;
+  uint16_t* ko;
+  uint16_t* vo;
+  f32x4* table;   // [H, P * block_size / 16]
+  const int* block_table;
+  const int* src_req;
+  const int* src_j;
+  Fp4Scales s;
+  int64_t kc_sb, kc_sn, kc_sh, vc_sb, vc_sn, vc_sh, bt_stride;
+  int heads, num_blocks, bs;
+};
+template <int D>
+__global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
+  constexpr int LPR = D / 8;
+  const int p = blockIdx.x;
+  const int r = __builtin_amdgcn_readfirstlane(a.src_req[p]), j = __builtin_amdgcn_readfirstlane(a.src_j[p]);
+  int page = __builtin_amdgcn_readfirstlane(a.block_table[(int64_t)r * a.bt_stride + j]);
+  page = page >= 0 && page < a.num_blocks ? page : 0;
+  const bool v = blockIdx.z != 0;
+  const uint8_t* cache = v ? a.vc + (int64_t)page * a.vc_sb : a.kc + (int64_t)page * a.kc_sb;
+  const int64_t sn = v ? a.vc_sn : a.kc_sn, sh = v ? a.vc_sh : a.kc_sh;
+  const uint8_t* scale = (v ? a.s.v : a.s.k) + (int64_t)page * a.s.sb;
+  if (!v) {
+    const int nb16 = a.bs / 16, entries = a.heads * nb16;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < entries; i += 256 * gridDim.y)
+      a.table[((int64_t)(i / nb16) * gridDim.x + p) * nb16 + i % nb16] = f32x4{1.f, 0.f, 1.f, 0.f};
+  }
+  u32x4* out = reinterpret_cast<u32x4*>((v ? a.vo : a.ko) + (int64_t)p * a.bs * a.heads * D);
+  const int n = a.bs * a.heads * LPR;
+  for (int i = blockIdx.y * 256 + threadIdx.x; i < n; i += 256 * gridDim.y) {
+    const int c = i % LPR, at = i / LPR, t = at / a.heads, h = at - t * a.heads;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + t * sn + h * sh + 4 * c);
+    out[i] = fp4_to_bf16(w, fp4_finite(scale[h * a.s.sh + t * (D / FP4_GROUP) + c / 4]));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Attention of short queries: attn_kernel's plan and pieces. Per (request, kv head) and 32-key tile, log2 domain:
+//   S    = K . q^T     v_mfma_f32_16x16x32_bf16: a lane's 32 (D = 64: 16) channels of a key lie in one group, so a conversion
+//                      makes two codes and their exponent two bf16 operands, exactly; q as it is
+//   e    = S scale     m: the row's largest e plus BLOCK_REF, raised where it lags by more than 8
+//   P    = 2^(e - m),  l += P
+//   O   += V^T . P     v_mfma_f32_16x16x32_bf16: V's values as bf16 (exact), P as one bf16 (2^-8) or, PACK, as two (2^-16)
+// PACK: at most 8 (token, q head) rows per kv head: they are the columns 0 .. 7 and again 8 .. 15, where P's lower parts go.
+// (The scaled MFMA takes the codes without a conversion, but sums products of 8-bit floats to 2^-13 of the largest of each few:
+// scores were 7e-4 off.)
+// Weights are kept below 2^-24 (BLOCK_REF), so that a sum over a million keys of V's largest values (6 2^125) stays finite.
+// ------------------------------------------------------------------------------------------------
+struct Fp4AttnArgs {
+  AttnArgs a;   // (first: fresh_args)
+  Fp4Scales s;
+  float* lse;   // [tokens, q heads], or NULL
+  int64_t lse_st;
+};
+static_assert(offsetof(Fp4AttnArgs, a) == 0 && sizeof(AttnArgs) % 8 == 0, "AttnArgs lead the kernel arguments");
+__device__ __forceinline__ const Fp4AttnArgs& fresh_fp4() {
+  auto* p = (const __attribute__((address_space(4))) void*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Fp4AttnArgs*)p;
+}
+constexpr float LN2 = 0.6931471805599453f;
+
+template <int D>
+struct Fp4Tile {
+  uint32_t k[2][D / 32];            // keys 16 b + n, channels (D / 4) g ..: a word of 8 for each step of the product
+  uint8_t ks[2];                    // their exponent bytes
+  uint32_t v[8];                    // keys 16 (j / 4) + 4 g + j % 4, channels (D / 16) n ..
+  uint32_t vs[2][D / 32];           // exponent bytes of keys 16 b + 4 g .. + 3
+};
+
+// 16 query rows as the MFMA's second operand: lane (n, g) holds row n's channels (D / 4) g + 8 s .. + 7 in step s.
+template <int D>
+struct Fp4Query {
+  bf16x8 op[D / 32];
+  float odd;   // 0, or NaN where the row holds a NaN or an infinity: then its output is NaN too
+  __device__ __forceinline__ void make(const uint16_t* row, bool real, int g) {
+    odd = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      u32x4 w = {0u, 0u, 0u, 0u};
+      if (real) w = *reinterpret_cast<const u32x4*>(row + (D / 4) * g + 8 * s);
+      op[s] = *reinterpret_cast<bf16x8*>(&w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) odd = __builtin_fmaf(bf16_lo(w[j]), 0.f, __builtin_fmaf(bf16_hi(w[j]), 0.f, odd));
+    }
+    odd = group4_sum(odd);
+  }
+};
+// S^T[key][row] of 16 keys: lane (n, g) holds row n's keys 4 g + i
+template <int D>
+__device__ __forceinline__ f32x4 fp4_scores(const uint32_t (&k)[D / 32], uint32_t byte, const Fp4Query<D>& q) {
+  f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    const u32x4 w = fp4_to_bf16(k[s], byte);
+    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&w), q.op[s], z, 0, 0, 0);
+  }
+  return z;
+}
+// the lane's words of 16 keys' codes
+template <int D>
+__device__ __forceinline__ void load_k16(uint32_t (&k)[D / 32], const uint8_t* p) {
+  if constexpr (D == 128) {
+    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+#pragma unroll
+    for (int s = 0; s < 4; ++s) k[s] = w[s];
+  } else {
+    const u32x2 w = ldv(reinterpret_cast<const u32x2*>(p));
+    k[0] = w.x;
+    k[1] = w.y;
+  }
+}
+
+template <int D, int PF, bool PACK>
+__device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqlen, int kvh, int row0, int c_begin, int c_end,
+                                           int ks, int KS, int rtile, int part, int nparts, float* lds, int lane) {
+  const Fp4AttnArgs& args = fresh_fp4();
+  const AttnArgs& a = args.a;
+  constexpr int RT = PACK ? 8 : 16;        // rows of this wavefront's tile
+  constexpr int VT = D / 16, OPL = D / 4, SB = D / FP4_GROUP;
+  const int G = PACK ? a.G >> 1 : a.G;     // (PACK: the plan counts plane rows, two a row)
+  const bool active = row0 < qlen * G;
+  const int num_blocks = a.num_blocks, lbs = a.lbs;
+  const int64_t k_sb = a.k_sb, k_sn = a.k_sn, v_sb = a.v_sb, v_sn = a.v_sn, s_sb = args.s.sb;
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tok = __builtin_amdgcn_readfirstlane(tok);
+  qlen = __builtin_amdgcn_readfirstlane(qlen);
+  kvh = __builtin_amdgcn_readfirstlane(kvh);
+  row0 = __builtin_amdgcn_readfirstlane(row0);
+  c_begin = __builtin_amdgcn_readfirstlane(c_begin);
+  c_end = __builtin_amdgcn_readfirstlane(c_end);
+  part = __builtin_amdgcn_readfirstlane(part);
+  nparts = __builtin_amdgcn_readfirstlane(nparts);
+  ks = __builtin_amdgcn_readfirstlane(ks);
+  KS = __builtin_amdgcn_readfirstlane(KS);
+  const int n = lane & 15, g = lane >> 4;
+  const int L = __builtin_amdgcn_readfirstlane(seqlen);
+  if (L <= 0 || !active) c_end = c_begin;
+  const int nt = c_begin + ks < c_end ? (c_end - c_begin - ks + KS - 1) / KS : 0;
+  auto tile = [&](int j) { return c_begin + ks + j * KS; };
+  const int* bt = a.block_table + (int64_t)seq * a.bt_stride;
+  const int bs = 1 << lbs;
+  auto div_g = [&](int x) { return G == 1 ? x : a.g_inv ? (int)__umulhi((unsigned)x, a.g_inv) : x / G; };
+
+  const int R = row0 + (n & (RT - 1)), rtok = div_g(R), rh = R - rtok * G;
+  const int lim_lo = L - qlen + 1 + __builtin_amdgcn_readfirstlane(div_g(row0));
+  const uint8_t* kbase = (const uint8_t*)a.kc + (int64_t)kvh * a.k_sh;
+  const uint8_t* vbase = (const uint8_t*)a.vc + (int64_t)kvh * a.v_sh;
+  const uint8_t* ksb = args.s.k + (int64_t)kvh * args.s.sh;
+  const uint8_t* vsb = args.s.v + (int64_t)kvh * args.s.sh;
+  const int koff = n * (int)k_sn + (D / 8) * g, ksoff = n * SB + g * (D / 4) / FP4_GROUP;
+  const int voff = 4 * g * (int)v_sn + n * (VT / 2);
+  const int vsn = (int)v_sn;
+  const int vshift = 8 * (n * VT / FP4_GROUP);
+
+  auto page_of = [&](int key) -> int {
+    const int idx = __builtin_amdgcn_readfirstlane(key >> lbs);
+    const int p = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[idx]);
+    return (p >= 0 && p < num_blocks) ? p : 0;
+  };
+  auto load = [&](Fp4Tile<D>& r, int c) {
+    const int n0 = c * TILE, n1 = n0 + 16;
+    const int p0 = page_of(n0);
+    const int p1 = n1 < L ? page_of(n1) : p0;
+    const int o0 = n0 & (bs - 1), o1 = n1 < L ? (n1 & (bs - 1)) : o0;
+    const int pg[2] = {p0, p1}, of[2] = {o0, o1};
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const uint8_t* kb = kbase + (int64_t)pg[b] * k_sb + (int64_t)of[b] * k_sn;
+      const uint8_t* vb = vbase + (int64_t)pg[b] * v_sb + (int64_t)of[b] * v_sn;
+      const int64_t so = (int64_t)pg[b] * s_sb + of[b] * SB;
+      load_k16<D>(r.k[b], kb + koff);
+      r.ks[b] = __builtin_nontemporal_load(ksb + so + ksoff);
+      if constexpr (D == 128) {
+        const u32x4 s = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vsb + so + 4 * g * SB));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.vs[b][i] = s[i];
+      } else {
+        const u32x2 s = ldv(reinterpret_cast<const u32x2*>(vsb + so + 4 * g * SB));
+        r.vs[b][0] = s.x;
+        r.vs[b][1] = s.y;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (D == 128) r.v[4 * b + i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb + voff + i * vsn));
+        else r.v[4 * b + i] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(vb + voff + i * vsn));
+      }
+    }
+  };
+
+  Fp4Tile<D> ring[PF];
+  if (nt > 0) {
+#pragma unroll
+    for (int j = 0; j < PF - 1; ++j) load(ring[j], tile(min(j, nt - 1)));
+  }
+  Fp4Query<D> q;
+  q.make(a.q + (int64_t)(tok + min(rtok, qlen - 1)) * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, rtok < qlen, g);
+  const float rs = a.sm_log2 + q.odd;
+  const int lim = rtok < qlen ? L - qlen + 1 + rtok : L;
+  const uint32_t drop = PACK && n < 8 ? 0u : 0xffff0000u;   // PACK: this lane's part of P is what is left without these bits
+
+  float m = -1e30f, l = 0.f;
+  f32x4 acc[VT];
+#pragma unroll
+  for (int t = 0; t < VT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](auto masked_t, const Fp4Tile<D>& r, int c) {
+    constexpr bool MASKED = decltype(masked_t)::value;
+    const int n0 = c * TILE;
+    // ---- scores; key of (b, i) = n0 + 16 b + 4 g + i ----
+    f32x4 z[2];
+    bool ok[2][4];
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      z[b] = fp4_scores<D>(r.k[b], r.ks[b], q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ok[b][i] = MASKED ? n0 + 16 * b + 4 * g + i < lim : true;
+        tmax = ok[b][i] ? __builtin_fmaxf(tmax, z[b][i]) : tmax;
+      }
+    }
+    // ---- online softmax ----
+    tmax = __builtin_fmaf(group4_fmax(tmax), rs, BLOCK_REF);   // the reference that this tile asks for
+    const bool raise = tmax > m + ATTN_SLACK;
+    const float mnew = raise ? tmax : m;
+    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+    m = mnew;
+    float p[2][4];
+    l *= alpha;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[b][i], rs, -mnew));
+        if (MASKED) p[b][i] = ok[b][i] ? p[b][i] : 0.f;
+        l += p[b][i];
+      }
+    if (__any(raise)) {
+#pragma unroll
+      for (int t = 0; t < VT; ++t) acc[t] *= alpha;
+    }
+    // ---- PV: O^T[channel][row] += V^T . P^T, the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i ----
+    u32x4 pw;
+    if constexpr (PACK) {
+      float x[2][4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[b][i] = p[b][i] - __uint_as_float(__float_as_uint(p[b][i]) & drop);
+      pw = u32x4{bf16x2_upper(x[0][0], x[0][1]), bf16x2_upper(x[0][2], x[0][3]), bf16x2_upper(x[1][0], x[1][1]),
+                 bf16x2_upper(x[1][2], x[1][3])};
+    } else {
+      pw = u32x4{pack_bf16x2_rne(p[0][0], p[0][1]), pack_bf16x2_rne(p[0][2], p[0][3]), pack_bf16x2_rne(p[1][0], p[1][1]),
+                 pack_bf16x2_rne(p[1][2], p[1][3])};
+    }
+    const bf16x8 pop = *reinterpret_cast<bf16x8*>(&pw);
+    float vsc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // (D = 64: two keys' bytes to a word)
+      const uint32_t w = D == 128 ? r.vs[j / 4][j % 4] >> vshift : r.vs[j / 4][j % 4 / 2] >> (vshift + 16 * (j % 2));
+      vsc[j] = __uint_as_float((w & 0xffu) << 23);
+      // whatever lies behind the last key is finite: it meets weights of 0
+      if (MASKED) vsc[j] = n0 + 16 * (j / 4) + 4 * g + j % 4 < L ? vsc[j] : 0.f;
+    }
+    auto pairs = [&](auto byte_t) {   // the channels 2 B and 2 B + 1 of the lane's
+      constexpr int B = decltype(byte_t)::value;
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r.v[j], vsc[j], B));
+      u32x4 even, odd;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+        odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+      }
+      acc[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), pop, acc[2 * B], 0, 0, 0);
+      acc[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), pop, acc[2 * B + 1], 0, 0, 0);
+    };
+    pairs(std::integral_constant<int, 0>{});
+    pairs(std::integral_constant<int, 1>{});
+    if constexpr (D == 128) {
+      pairs(std::integral_constant<int, 2>{});
+      pairs(std::integral_constant<int, 3>{});
+    }
+  };
+
+  // the ring of attn_kernel: PF - 1 tiles in flight, loads past the end re-read the last tile
+  if (nt > 0) {
+    const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
+    const int j_full = min(nt, full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0);
+    int j0 = 0;
+    for (; j0 + PF <= j_full; j0 += PF) {
+#pragma unroll
+      for (int jj = 0; jj < PF; ++jj) {
+        load(ring[(jj + PF - 1) % PF], tile(min(j0 + jj + PF - 1, nt - 1)));
+        compute(std::false_type{}, ring[jj], tile(j0 + jj));
+      }
+    }
+    for (; j0 < nt; j0 += PF) {
+#pragma unroll
+      for (int jj = 0; jj < PF; ++jj) {
+        const int j = j0 + jj;
+        if (j >= nt) break;
+        load(ring[(jj + PF - 1) % PF], tile(min(j + PF - 1, nt - 1)));
+        compute(std::true_type{}, ring[jj], tile(j));
+      }
+    }
+  }
+
+  // ---- epilogue: lane (n, g) holds channels (D/4) g + (D/16) i + t of its row in acc[t][i] ----
+  l = group4_sum(l);
+  if constexpr (PACK) {   // both planes of a row: lanes n and n + 8 end with the same sums
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] += ror8(acc[t][i]);
+  }
+  if (KS > 1) {   // attn_kernel's merge of the key splits
+    static_assert(VT * 4 + 2 <= MERGE_FIELDS, "merge slot too small");
+    auto slot = [&](int k) { return lds + (size_t)((k - 1) * a.rt + rtile) * MERGE_FIELDS * WAVE + lane; };
+    if (ks > 0 && active) {
+      float* sl = slot(ks);
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sl[(4 * t + i) * WAVE] = acc[t][i];
+      sl[(4 * VT) * WAVE] = m;
+      sl[(4 * VT + 1) * WAVE] = l;
+    }
+    __syncthreads();
+    if (ks == 0 && active) {
+      float M = m;
+      for (int k = 1; k < KS; ++k) M = __builtin_fmaxf(M, slot(k)[(4 * VT) * WAVE]);
+      const float w0 = __builtin_amdgcn_exp2f(m - M);
+      l *= w0;
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] *= w0;
+      for (int k = 1; k < KS; ++k) {
+        const float* src = slot(k);
+        const float wk = __builtin_amdgcn_exp2f(src[(4 * VT) * WAVE] - M);
+        l = __builtin_fmaf(wk, src[(4 * VT + 1) * WAVE], l);
+#pragma unroll
+        for (int t = 0; t < VT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(wk, src[(4 * t + i) * WAVE], acc[t][i]);
+      }
+      m = M;
+    }
+    __syncthreads();
+  }
+  if (ks > 0 || !active || rtok >= qlen || (PACK && n >= 8)) return;
+  // ---- the end of a piece: bf16 out of a whole segment, or the fp32 partial of a cut one (as attend_blocks) ----
+  const Fp4AttnArgs& f = fresh_fp4();
+  const AttnArgs& o = f.a;
+  const int qt = tok + rtok, head = kvh * G + rh;
+  float lse = __builtin_fmaf(m, LN2, __builtin_amdgcn_logf(l) * LN2);
+  if (l != l) {   // (a denominator that is no number would not tell the merge that the row was cut)
+    lse = NAN;
+    l = 1.f;
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = NAN;
+  }
+  if (nparts == 1) {
+    if (g == 0) {
+      if (o.max_splits > 1 && qt < o.cut_rows) o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh] = -1.f;
+      if (f.lse) f.lse[(int64_t)qt * f.lse_st + head] = lse;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint32_t w[OPL / 2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < VT; t += 2) w[(VT * i + t) / 2] = pack_bf16x2(acc[t][i] * inv, acc[t + 1][i] * inv);
+    u32x4* op = reinterpret_cast<u32x4*>(o.out + (int64_t)qt * o.o_st + (int64_t)head * o.o_sh + OPL * g);
+#pragma unroll
+    for (int u = 0; u < OPL / 8; ++u) op[u] = u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+  } else {
+    const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh + part;
+    if (g == 0) {
+      o.segm_max[sidx] = m;
+      o.segm_sum[sidx] = part == nparts - 1 ? last_piece_sum(l) : l;
+    }
+    float* sp = o.segm_out + sidx * D + OPL * g;
+#pragma unroll
+    for (int u = 0; u < OPL / 4; ++u) {
+      const int c0 = 4 * u;
+      reinterpret_cast<float4*>(sp)[u] = float4{acc[(c0 + 0) % VT][(c0 + 0) / VT], acc[(c0 + 1) % VT][(c0 + 1) / VT],
+                                                acc[(c0 + 2) % VT][(c0 + 2) / VT], acc[(c0 + 3) % VT][(c0 + 3) / VT]};
+    }
+  }
+}
+
+template <int D, int PF, bool PACK>
+__global__ __launch_bounds__(256) void fp4_attn_kernel(Fp4AttnArgs args) {
+  touch_args();
+  const AttnArgs& a = args.a;
+  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int rt = a.rt, ksplit = a.ksplit, kspl = div_row_tiles(wave, rt), rtile = wave - kspl * rt;
+  extern __shared__ float merge_lds[];
+  int solo = 0;
+  walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
+    const int row0 = (rg * rt + rtile) * (PACK ? 8 : 16);
+    if (ksplit > 1 && c1 - c0 >= a.coop) {
+      attend_fp4<D, PF, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, kspl, ksplit, rtile, part, nparts, merge_lds, lane);
+    } else {
+      if (solo % ksplit == kspl)
+        attend_fp4<D, PF, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, 0, 1, rtile, part, nparts, merge_lds, lane);
+      ++solo;
+    }
+  });
+}
+
+// split_reduce_kernel, with the rows' log-sum-exp
+template <int D>
+__global__ __launch_bounds__(WAVE * RED_WAVES) void fp4_reduce_kernel(AttnArgs a, float* lse, int64_t lse_st) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  const int seq = blockIdx.x;
+  const int h = blockIdx.y * RED_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int tok = a.cu_q[seq], qlen = a.cu_q[seq + 1] - tok;
+  if (h >= a.G * a.hkv || qlen <= 0 || qlen > a.qmax) return;
+  const int rows = min(qlen, a.cut_rows - tok);
+  for (int t = blockIdx.z; t < rows; t += gridDim.z)
+    merge_row<D, true>(a, tok, t, h, lane, lse ? lse + (int64_t)(tok + t) * lse_st + h : nullptr);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------------
+// What every call on a 4-bit cache checks; 0, or the error after fail().
+int check_fp4(const char* nm, int64_t num_blocks, int64_t block_size, int64_t heads, int64_t head_dim, const void* kc,
+              int64_t k_sb, int64_t k_sn, int64_t k_sh, const void* vc, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+              const void* ks, const void* vs, int64_t s_sb, int64_t s_sh) {
+  if (head_dim != 64 && head_dim != 128) return fail("%s: head_dim must be 64 or 128, got %lld", nm, (long long)head_dim);
+  if (block_size < 16 || !pow2(block_size) || block_size > (1 << 24))
+    return fail("%s: block_size must be a power of two >= 16", nm);
+  if (heads <= 0 || heads > 65535 || num_blocks <= 0 || num_blocks > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (!kc || !vc || !ks || !vs) return fail("%s: null pointer", nm);
+  if (!aligned16(kc) || !aligned16(vc) || (k_sb | k_sn | k_sh | v_sb | v_sn | v_sh) % 16)
+    return fail("%s: cache rows must be 16-byte aligned (base pointers and strides)", nm);
+  if (!aligned16(ks) || !aligned16(vs) || (s_sb | s_sh) % 16)
+    return fail("%s: scales must be 16-byte aligned (base pointers and strides)", nm);
+  if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
+    return fail("%s: page too large for 32-bit lane offsets", nm);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kvq_quant_fp4_cache(const void* key, int64_t key_st, int64_t key_sh, const void* value, int64_t val_st, int64_t val_sh,
+                        uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, uint8_t* v_cache, int64_t vc_sb,
+                        int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                        int64_t head_dim, uint8_t* k_scale, uint8_t* v_scale, int64_t s_sb, int64_t s_sh,
+                        const int64_t* slot_mapping, int64_t num_tokens, void* stream) {
+  const char* nm = "quant_fp4_cache";
+  if (num_tokens < 0 || num_tokens > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (num_tokens == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_fp4(nm, num_blocks, block_size, num_heads, head_dim, k_cache, kc_sb, kc_sn, kc_sh, v_cache, vc_sb,
+                               vc_sn, vc_sh, k_scale, v_scale, s_sb, s_sh)) return rc;
+  if (!key || !value || !slot_mapping) return fail("%s: null pointer", nm);
+  if (!aligned16(key) || !aligned16(value) || (key_st | key_sh | val_st | val_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  QuantFp4Args a;
+  a.key = (const uint16_t*)key; a.value = (const uint16_t*)value; a.kc = k_cache; a.vc = v_cache; a.slots = slot_mapping;
+  a.s = Fp4Scales{k_scale, v_scale, s_sb, s_sh};
+  a.key_st = key_st; a.key_sh = key_sh; a.val_st = val_st; a.val_sh = val_sh;
+  a.kc_sb = kc_sb; a.kc_sn = kc_sn; a.kc_sh = kc_sh; a.vc_sb = vc_sb; a.vc_sn = vc_sn; a.vc_sh = vc_sh;
+  a.num_slots = num_blocks * block_size;
+  a.num_tokens = (int)num_tokens; a.heads = (int)num_heads; a.lbs = log2i(block_size);
+  const int64_t rpb = 256 / (head_dim / 8), blocks = (num_tokens * num_heads + rpb - 1) / rpb;
+  if (blocks > INT32_MAX) return fail("%s: too many tokens and heads for one call", nm);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (head_dim == 128) hipLaunchKernelGGL(quant_fp4_kernel<128>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(quant_fp4_kernel<64>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  return launched(nm);
+}
+
+int kvq_read_fp4_cache(const uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, const uint8_t* v_cache,
+                       int64_t vc_sb, int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
+                       int64_t head_dim, const uint8_t* k_scale, const uint8_t* v_scale, int64_t s_sb, int64_t s_sh,
+                       const int32_t* starts, const int32_t* cu_seqlens_k, const int32_t* block_table, int64_t bt_stride,
+                       int64_t num_seqs, void* k_out, int64_t ko_st, int64_t ko_sh, void* v_out, int64_t vo_st, int64_t vo_sh,
+                       int64_t num_rows, void* stream) {
+  const char* nm = "read_fp4_cache";
+  if (num_rows < 0 || num_seqs < 0 || num_rows > INT32_MAX || num_seqs > INT32_MAX / 4) return fail("%s: bad sizes", nm);
+  if (num_rows == 0 || num_seqs == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_fp4(nm, num_blocks, block_size, num_heads, head_dim, k_cache, kc_sb, kc_sn, kc_sh, v_cache, vc_sb,
+                               vc_sn, vc_sh, k_scale, v_scale, s_sb, s_sh)) return rc;
+  if (!k_out || !v_out || !starts || !cu_seqlens_k || !block_table) return fail("%s: null pointer", nm);
+  if (!aligned16(k_out) || !aligned16(v_out) || (ko_st | ko_sh | vo_st | vo_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  ReadFp4Args a;
+  a.kc = k_cache; a.vc = v_cache; a.ko = (uint16_t*)k_out; a.vo = (uint16_t*)v_out;
+  a.start = starts; a.cu_k = cu_seqlens_k; a.block_table = block_table;
+  a.s = Fp4Scales{const_cast<uint8_t*>(k_scale), const_cast<uint8_t*>(v_scale), s_sb, s_sh};
+  a.kc_sb = kc_sb; a.kc_sn = kc_sn; a.kc_sh = kc_sh; a.vc_sb = vc_sb; a.vc_sn = vc_sn; a.vc_sh = vc_sh;
+  a.ko_st = ko_st; a.ko_sh = ko_sh; a.vo_st = vo_st; a.vo_sh = vo_sh; a.bt_stride = bt_stride;
+  a.num_seqs = (int)num_seqs; a.num_rows = (int)num_rows; a.heads = (int)num_heads; a.num_blocks = (int)num_blocks;
+  a.lbs = log2i(block_size);
+  const int64_t items = block_slots(num_rows, num_seqs, 4) * num_heads;
+  if (items > INT32_MAX - 3) return fail("%s: too many rows and heads for one call", nm);
+  a.items = (int)items;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const bool nt = 5 * num_rows * num_heads * head_dim > READ_NT_BYTES;
+  void (*kern)(ReadFp4Args) = head_dim == 128 ? (nt ? read_fp4_kernel<128, true> : read_fp4_kernel<128, false>)
+                                              : (nt ? read_fp4_kernel<64, true> : read_fp4_kernel<64, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, a);
+  return launched(nm);
+}
+
+int kvq_fp4_pages(const uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, const uint8_t* v_cache, int64_t vc_sb,
+                  int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim,
+                  const uint8_t* k_scale, const uint8_t* v_scale, int64_t s_sb, int64_t s_sh, void* k_out, void* v_out,
+                  float* scales_out, const int32_t* block_table, int64_t bt_stride, const int32_t* src_req,
+                  const int32_t* src_j, int64_t num_pages, void* stream) {
+  const char* nm = "fp4_pages";
+  if (num_pages < 0 || num_pages > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (num_pages == 0) { g_err.clear(); return KVQ_OK; }
+  if (const int rc = check_fp4(nm, num_blocks, block_size, num_heads, head_dim, k_cache, kc_sb, kc_sn, kc_sh, v_cache, vc_sb,
+                               vc_sn, vc_sh, k_scale, v_scale, s_sb, s_sh)) return rc;
+  if (!k_out || !v_out || !scales_out || !block_table || !src_req || !src_j) return fail("%s: null pointer", nm);
+  if (!aligned16(k_out) || !aligned16(v_out) || !aligned16(scales_out))
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  if (2 * block_size * num_heads * head_dim > INT32_MAX) return fail("%s: page too large for 32-bit lane offsets", nm);
+  Fp4PagesArgs a;
+  a.kc = k_cache; a.vc = v_cache; a.ko = (uint16_t*)k_out; a.vo = (uint16_t*)v_out;
+  a.table = reinterpret_cast<f32x4*>(scales_out); a.block_table = block_table; a.src_req = src_req; a.src_j = src_j;
+  a.s = Fp4Scales{const_cast<uint8_t*>(k_scale), const_cast<uint8_t*>(v_scale), s_sb, s_sh};
+  a.kc_sb = kc_sb; a.kc_sn = kc_sn; a.kc_sh = kc_sh; a.vc_sb = vc_sb; a.vc_sn = vc_sn; a.vc_sh = vc_sh; a.bt_stride = bt_stride;
+  a.heads = (int)num_heads; a.num_blocks = (int)num_blocks; a.bs = (int)block_size;
+  // few pages: each page over several workgroups
+  const int64_t chunks = (block_size * num_heads * head_dim / 8 + 255) / 256;
+  const int64_t slices = std::min<int64_t>(std::min<int64_t>(chunks, 65535), std::max<int64_t>(1, (int64_t)device_cus() * 8 / (2 * num_pages)));
+  const dim3 grid((unsigned)num_pages, (unsigned)slices, 2);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (head_dim == 128) hipLaunchKernelGGL(fp4_pages_kernel<128>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(fp4_pages_kernel<64>, grid, dim3(256), 0, st, a);
+  return launched(nm);
+}
+
+int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k_pages, const void* v_pages,
+                              const float* page_scales, int64_t num_pages, int64_t block_size, int64_t num_kv_heads,
+                              int64_t head_dim, void* out, int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q,
+                              const int32_t* seq_lens, const int32_t* pages_table, int64_t pt_stride, int64_t num_q_heads,
+                              const int32_t* tile_req, const int32_t* tile_row, int64_t num_tiles, int64_t rows_per_tile,
+                              double softmax_scale, const int32_t* tile_piece, const int32_t* tile_slot, const int32_t* merge,
+                              int64_t num_merge, float* part_out, float* part_ml, void* stream) {
+  const char* nm = "fp4_prefill_attention";
+  if (num_tiles < 0 || num_tiles > INT32_MAX || num_merge < 0 || num_merge > INT32_MAX) return fail("%s: bad sizes", nm);
+  if (num_tiles == 0) { g_err.clear(); return KVQ_OK; }
+  if (rows_per_tile != PR_ROWS) return fail("%s: work list tiles must be %d rows", nm, PR_ROWS);
+  if (!tile_req || !tile_row || (tile_piece && !tile_slot)) return fail("%s: bad work list", nm);
+  if (tile_piece && num_merge > 0 && (!merge || !part_out || !part_ml || !aligned16(merge) || !aligned16(part_out) ||
+                                      !aligned16(part_ml)))
+    return fail("%s: split work list needs 16-byte aligned merge list and partial buffers", nm);
+  if (!(softmax_scale >= MIN_SOFTMAX_SCALE && softmax_scale <= MAX_SOFTMAX_SCALE))
+    return fail("%s: softmax_scale must be positive and finite, from %g to %g", nm, MIN_SOFTMAX_SCALE, MAX_SOFTMAX_SCALE);
+  if (const int rc = check_fp4(nm, num_pages, block_size, num_kv_heads, head_dim, k_pages, 0, 0, 0, v_pages, 0, 0, 0, page_scales,
+                               page_scales, 0, 0)) return rc;
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
+    return fail("%s: bad head counts Hq=%lld Hkv=%lld", nm, (long long)num_q_heads, (long long)num_kv_heads);
+  if (!q || !out || !cu_seqlens_q || !seq_lens || !pages_table) return fail("%s: null pointer", nm);
+  if (!aligned16(q) || !aligned16(out) || (q_st | q_sh | o_st | o_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  if (2 * block_size * num_kv_heads * head_dim > INT32_MAX)
+    return fail("%s: page too large for 32-bit page / slot offsets", nm);
+  PrefillArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_pages; a.vc = (const uint16_t*)v_pages; a.out = (uint16_t*)out;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = pages_table; a.tile_req = tile_req; a.tile_row = tile_row;
+  a.tile_piece = tile_piece; a.tile_slot = tile_slot; a.part_out = part_out; a.part_ml = part_ml;
+  a.q_st = q_st; a.q_sh = q_sh; a.o_st = o_st; a.o_sh = o_sh; a.bt_stride = pt_stride;
+  a.k_sh = a.v_sh = head_dim;
+  a.k_sn = a.v_sn = num_kv_heads * head_dim;
+  a.k_sb = a.v_sb = block_size * a.k_sn;
+  a.krow = a.vrow = (uint32_t)(2 * a.k_sn);
+  a.kpage = a.vpage = (uint32_t)(2 * a.k_sb);
+  a.contig = 1;
+  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
+  a.G = (int)(num_q_heads / num_kv_heads); a.lbs = log2i(block_size); a.num_blocks = (int)num_pages;
+  a.s_table = reinterpret_cast<const f32x4*>(page_scales);
+  const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  void (*kern)(PrefillArgs) = head_dim == 128
+      ? (tile_piece ? block_codes_prefill_kernel<128, true> : block_codes_prefill_kernel<128, false>)
+      : (tile_piece ? block_codes_prefill_kernel<64, true> : block_codes_prefill_kernel<64, false>);
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
+  const int rc = launched(nm);
+  if (rc != KVQ_OK || !tile_piece || num_merge == 0) return rc;
+  const dim3 mgrid((unsigned)num_merge, (unsigned)num_kv_heads, PR_ROWS / PR_MERGE_WAVES);
+  const int4* ml = reinterpret_cast<const int4*>(merge);
+  if (head_dim == 128) hipLaunchKernelGGL(prefill_merge_kernel<128>, mgrid, dim3(WAVE * PR_MERGE_WAVES), 0, st, a, ml);
+  else hipLaunchKernelGGL(prefill_merge_kernel<64>, mgrid, dim3(WAVE * PR_MERGE_WAVES), 0, st, a, ml);
+  return launched("fp4_prefill_attention: merge");
+}
+
+int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,
+                             int64_t k_sh, const uint8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
+                             int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
+                             const uint8_t* k_scale, const uint8_t* v_scale, int64_t s_sb, int64_t s_sh, void* out,
+                             int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                             const int32_t* block_table, int64_t bt_stride, int64_t num_seqs, int64_t num_q_heads,
+                             double softmax_scale, float* segm_out, float* segm_max, float* segm_sum, int64_t seg_st,
+                             int64_t seg_sh, int64_t num_splits, int64_t segm_rows, float* lse, int64_t lse_st,
+                             int64_t target_waves, int64_t max_query_len, int64_t qmax, void* stream) {
+  const char* nm = "fp4_decode_attention";
+  if (num_splits < 1 || num_splits > MAX_SPLITS) return fail("%s: at most %d split-KV segments", nm, MAX_SPLITS);
+  if (num_seqs < 0 || num_seqs > INT32_MAX / 4 || max_query_len < 0 || qmax < 1 || target_waves < 0 || segm_rows < 0)
+    return fail("%s: bad sizes", nm);
+  if (num_seqs == 0) { g_err.clear(); return KVQ_OK; }
+  if (!(softmax_scale >= MIN_SOFTMAX_SCALE && softmax_scale <= MAX_SOFTMAX_SCALE))
+    return fail("%s: softmax_scale must be positive and finite, from %g to %g", nm, MIN_SOFTMAX_SCALE, MAX_SOFTMAX_SCALE);
+  if (const int rc = check_fp4(nm, num_blocks, block_size, num_kv_heads, head_dim, k_cache, k_sb, k_sn, k_sh, v_cache, v_sb,
+                               v_sn, v_sh, k_scale, v_scale, s_sb, s_sh)) return rc;
+  if (num_q_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
+    return fail("%s: bad head counts Hq=%lld Hkv=%lld", nm, (long long)num_q_heads, (long long)num_kv_heads);
+  if (!q || !out || !cu_seqlens_q || !seq_lens || !block_table) return fail("%s: null pointer", nm);
+  if (!aligned16(q) || !aligned16(out) || (q_st | q_sh | o_st | o_sh) % 8)
+    return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  if (num_splits > 1 && segm_rows > 0 && (!segm_out || !segm_max || !segm_sum || !aligned16(segm_out)))
+    return fail("%s: split buffers missing or not 16-byte aligned", nm);
+  const int G = (int)(num_q_heads / num_kv_heads);
+  const int64_t maxq = std::min<int64_t>(std::max<int64_t>(max_query_len, 1), qmax), rows = (int64_t)G * maxq;
+  if (rows > INT32_MAX / 4) return fail("%s: grid too large", nm);
+  // the row tile: 8 rows, both planes in one MFMA, where that holds all of a request's rows; else 16
+  const bool pack = rows <= 8;
+  const int rt = (int)std::min<int64_t>(MAX_ROW_TILES, (rows + 15) / 16);
+  const Tuning tune = read_tuning();
+  const bool cut = num_splits > 1 && segm_rows > 0;
+  const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
+                     : num_splits == 1 || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? MAX_ROW_TILES : DEFAULT_KSPLIT;
+  const int ks = std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = rt * ks;
+  Fp4AttnArgs b;
+  b.s = Fp4Scales{const_cast<uint8_t*>(k_scale), const_cast<uint8_t*>(v_scale), s_sb, s_sh};
+  b.lse = lse; b.lse_st = lse_st;
+  AttnArgs& a = b.a;
+  a.q = (const uint16_t*)q; a.kc = (const int8_t*)k_cache; a.vc = (const int8_t*)v_cache; a.out = (uint16_t*)out;
+  a.segm_out = segm_out; a.segm_max = segm_max; a.segm_sum = segm_sum;
+  a.cu_q = cu_seqlens_q; a.seq_lens = seq_lens; a.block_table = block_table;
+  a.ks = a.vs = nullptr; a.ks_pc = a.vs_pc = 0;
+  a.q_st = q_st; a.q_sh = q_sh; a.o_st = o_st; a.o_sh = o_sh;
+  a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh;
+  a.seg_st = seg_st; a.seg_sh = seg_sh; a.bt_stride = bt_stride;
+  a.sm_log2 = (float)(softmax_scale * 1.4426950408889634);
+  a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size);
+  a.G = pack ? 2 * G : G;   // the plan's rows: planes of rows where two share an MFMA
+  a.g_inv = G > 1 && (G * std::min<int64_t>(qmax, INT32_MAX) + 64) < (1ll << 32) / G ? (unsigned)(((1ll << 32) + G - 1) / G) : 0u;
+  a.qmax = (int)std::min<int64_t>(qmax, INT32_MAX);
+  a.num_seqs = (int)num_seqs; a.hkv = (int)num_kv_heads;
+  a.max_splits = (int)num_splits;
+  a.cut_rows = num_splits > 1 ? (int)std::min<int64_t>(segm_rows, INT32_MAX) : 0;
+  a.rt = rt; a.ksplit = ks; a.waves = waves;
+  a.min_tiles = MIN_SPLIT_TILES;
+  a.coop = coop_tiles(num_splits > 1, ks);
+  a.xcd_order = tune.xcd_order ? atoi(tune.xcd_order) : 1;
+  a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
+                                       : (int)PLAN_FAST_MAX;
+  a.seg_cost = seg_cost_units(tune, 0);
+  const size_t lds = (size_t)(ks - 1) * rt * MERGE_FIELDS * WAVE * sizeof(float);
+  void (*kern)(Fp4AttnArgs) = head_dim == 128 ? (pack ? fp4_attn_kernel<128, 3, true> : fp4_attn_kernel<128, 3, false>)
+                                              : (pack ? fp4_attn_kernel<64, 3, true> : fp4_attn_kernel<64, 3, false>);
+  const int64_t tw = target_waves > 0 ? target_waves
+                     : cut            ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
+                                      : (int64_t)device_cus() * waves;
+  a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(tw / waves, INT32_MAX));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(kern, dim3((unsigned)a.workers), dim3(WAVE * waves), lds, st, b);
+  const int rc = launched(nm);
+  if (rc != KVQ_OK || num_splits == 1 || a.cut_rows == 0) return rc;
+  a.G = G;
+  const dim3 rgrid((unsigned)num_seqs, (unsigned)((num_q_heads + RED_WAVES - 1) / RED_WAVES),
+                   (unsigned)std::min<int64_t>(maxq, MERGE_Z));
+  if (head_dim == 128) hipLaunchKernelGGL(fp4_reduce_kernel<128>, rgrid, dim3(WAVE * RED_WAVES), 0, st, a, lse, lse_st);
+  else hipLaunchKernelGGL(fp4_reduce_kernel<64>, rgrid, dim3(WAVE * RED_WAVES), 0, st, a, lse, lse_st);
+  return launched("fp4_decode_attention: merge");
+}
+
+}  // extern "C"

@@ -1864,14 +1864,15 @@ __global__ __launch_bounds__(WAVE * 2 * KS) void verify_kernel(AttnArgs a) {
 // channels each. The piece count is read from the denominators (the last piece's is stored as
 // -2 - l, a row that was not cut has -1 in slot 0 and was written by the attention kernel), so the
 // merge needs neither the plan nor any buffer beyond the split buffers of the call.
-// BLOCK: the block-scaled cache's pieces (piece_sum.h); a row that saw no key is zero.
+// BLOCK: the block-scaled and the 4-bit cache's pieces (piece_sum.h); a row that saw no key is zero. lse: where the row's
+// log-sum-exp goes (NaN where its values are).
 constexpr int RED_WAVES = 4;
 constexpr int MERGE_Z = 64;   // largest z extent of split_reduce_kernel's grid
 // pieces of a row fetched together with its denominators (c3: 59.4 -> 59.0 us same card, c4 unchanged;
 // 4 pieces: 61.4 us -- the extra reads of rows with fewer pieces cost more than the round trip saves)
 constexpr int MERGE_SPEC = 2;
 template <int D, bool BLOCK>
-__device__ __forceinline__ void merge_row(const AttnArgs& a, int tok, int t, int h, int lane) {
+__device__ __forceinline__ void merge_row(const AttnArgs& a, int tok, int t, int h, int lane, float* lse = nullptr) {
   // denominators as the attention kernel left them: piece-0 slot -1 = not cut (already written);
   // otherwise pieces 0..S-2 hold l >= 0 and the last piece -2 - l
   const int64_t base = (int64_t)(tok + t) * a.seg_st + (int64_t)h * a.seg_sh;
@@ -1944,6 +1945,7 @@ __device__ __forceinline__ void merge_row(const AttnArgs& a, int tok, int t, int
   } else {
     op[0] = (uint16_t)bf16_rne(num[0] * inv);
   }
+  if (lse && lane == 0) *lse = num[0] != num[0] ? NAN : (M + __builtin_amdgcn_logf(den)) * 0.6931471805599453f;
 }
 // Grid (request, group of RED_WAVES q heads, z): block z merges query tokens z, z + gridDim.z, ... of
 // its request, so every short request's rows are covered whatever max_query_len the caller reported.
@@ -3954,3 +3956,6 @@ int kvq_dequant_pages(const int8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t
 }  // extern "C"
 
 #include "block_cache.h"
+#include "fp4_cache.h"
+#include "evict.h"
+#include "rope.h"

@@ -46,6 +46,14 @@ decltype(&kvq_read_block_cache) p_read_block;
 decltype(&kvq_block_decode_attention) p_block_decode;
 decltype(&kvq_block_prefill_attention) p_block_prefill;
 decltype(&kvq_block_codes) p_block_codes;
+decltype(&kvq_quant_fp4_cache) p_quant_fp4;
+decltype(&kvq_read_fp4_cache) p_read_fp4;
+decltype(&kvq_fp4_pages) p_fp4_pages;
+decltype(&kvq_fp4_prefill_attention) p_fp4_prefill;
+decltype(&kvq_fp4_decode_attention) p_fp4_decode;
+decltype(&kvq_fp4_key_weights) p_key_weights;
+decltype(&kvq_fp4_evict) p_evict;
+decltype(&kvq_norm_rope) p_norm_rope;
 
 // A tensor argument this file may read: exactly torch.Tensor (or Parameter), dense GPU memory, no wrapper
 // (functorch, functionalization, fake or subclass tensors go to the Python path).
@@ -495,6 +503,298 @@ PyObject* block_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- 4-bit cache (kvq.fp4_cache) ----
+// A cache's views and exponent bytes: uint8 [nb, bs, H, D / 2] and [nb, H, bs, D / 32].
+struct Fp4Cache {
+  uint8_t *k, *v, *ks, *vs;
+  int64_t kb, kn, kh, vb, vn, vh, nb, bs, H, D, sb, sh;
+  bool read(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks_t, const at::Tensor& vs_t) {
+    if (kc.dim() != 4 || kc.scalar_type() != at::kByte || vc.scalar_type() != at::kByte || vc.sizes() != kc.sizes() ||
+        kc.stride(3) != 1 || vc.stride(3) != 1)
+      return false;
+    nb = kc.size(0), bs = kc.size(1), H = kc.size(2), D = 2 * kc.size(3);
+    if (bs < 16 || (bs & (bs - 1))) return false;
+    for (const at::Tensor* s : {&ks_t, &vs_t})
+      if (s->dim() != 4 || s->scalar_type() != at::kByte || s->size(0) != nb || s->size(1) != H || s->size(2) != bs ||
+          s->size(3) != D / 32 || s->stride(3) != 1 || s->stride(2) != D / 32 || s->strides() != ks_t.strides())
+        return false;
+    k = (uint8_t*)kc.data_ptr(), v = (uint8_t*)vc.data_ptr(), ks = (uint8_t*)ks_t.data_ptr(), vs = (uint8_t*)vs_t.data_ptr();
+    kb = kc.stride(0), kn = kc.stride(1), kh = kc.stride(2), vb = vc.stride(0), vn = vc.stride(1), vh = vc.stride(2);
+    sb = ks_t.stride(0), sh = ks_t.stride(1);
+    return true;
+  }
+};
+bool bf16_rows_of(const at::Tensor& t, int64_t heads, int64_t d) { return bf16_rows(t) && t.size(1) == heads && t.size(2) == d; }
+bool lse_rows(const at::Tensor& t, int64_t rows, int64_t heads) {
+  return t.dim() == 2 && t.scalar_type() == at::kFloat && t.stride(1) == 1 && t.size(0) >= rows && t.size(1) == heads;
+}
+
+// (key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+PyObject* quant_fp4_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 7 || !p_quant_fp4) return DECLINED;
+    const at::Tensor* t[7];
+    for (int i = 0; i < 7; ++i)
+      if (!(t[i] = tensor(a[i]))) return DECLINED;
+    const at::Tensor &key = *t[0], &value = *t[1], &slots = *t[6];
+    Fp4Cache c;
+    if (!c.read(*t[2], *t[3], *t[4], *t[5]) || !bf16_rows_of(key, c.H, c.D) || !bf16_rows(value) || key.sizes() != value.sizes() ||
+        slots.dim() != 1 || slots.scalar_type() != at::kLong || slots.stride(0) != 1 || slots.size(0) == 0 ||
+        slots.size(0) > key.size(0) || !one_device(key, value, *t[2], *t[3], *t[4], *t[5], slots) || !on_current(key))
+      return DECLINED;
+    const int64_t T = slots.size(0);
+    void *kp = key.data_ptr(), *vp = value.data_ptr(), *st = stream_of(key);
+    auto* sp = (const int64_t*)slots.data_ptr();
+    return launch("kvq_quant_fp4_cache", [&] {
+      return p_quant_fp4(kp, key.stride(0), key.stride(1), vp, value.stride(0), value.stride(1), c.k, c.kb, c.kn, c.kh, c.v, c.vb,
+                         c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh, sp, T, st);
+    });
+  });
+}
+
+// (k_cache, v_cache, k_scale, v_scale, starts, cu_seqlens_k, block_table, k_out, v_out)
+PyObject* read_fp4_cache(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 9 || !p_read_fp4) return DECLINED;
+    const at::Tensor* t[9];
+    for (int i = 0; i < 9; ++i)
+      if (!(t[i] = tensor(a[i]))) return DECLINED;
+    const at::Tensor &start = *t[4], &cu = *t[5], &bt = *t[6], &ko = *t[7], &vo = *t[8];
+    Fp4Cache c;
+    if (!c.read(*t[0], *t[1], *t[2], *t[3]) || !index_vector(start) || !index_vector(cu) || !bf16_rows_of(ko, c.H, c.D) ||
+        !bf16_rows(vo) || ko.sizes() != vo.sizes() || !one_device(ko, vo, *t[0], *t[1], *t[2], *t[3], start, cu, bt) ||
+        !on_current(ko))
+      return DECLINED;
+    const int64_t N = ko.size(0), B = cu.size(0) - 1;
+    if (N == 0 || B <= 0 || start.size(0) < B || !table(bt, B)) return DECLINED;
+    void *kp = ko.data_ptr(), *vp = vo.data_ptr(), *st = stream_of(ko);
+    auto *sp = (const int32_t*)start.data_ptr(), *cup = (const int32_t*)cu.data_ptr(), *btp = (const int32_t*)bt.data_ptr();
+    return launch("kvq_read_fp4_cache", [&] {
+      return p_read_fp4(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh, sp, cup, btp,
+                        bt.stride(0), B, kp, ko.stride(0), ko.stride(1), vp, vo.stride(0), vo.stride(1), N, st);
+    });
+  });
+}
+
+// What both attention calls take: (q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, k_scale, v_scale,
+// softmax_scale, ...)
+struct Fp4Attn {
+  Fp4Cache c;
+  const at::Tensor *q, *out, *bt;
+  const int32_t *cu, *sl;
+  void *qp, *op, *st;
+  int64_t B, T, Hq;
+  double scale;
+  bool read(PyObject* const* a) {
+    const at::Tensor* t[9];
+    for (int i = 0; i < 9; ++i)
+      if (!(t[i] = tensor(a[i]))) return false;
+    q = t[0], out = t[3], bt = t[6];
+    if (!PyFloat_CheckExact(a[9])) return false;
+    scale = PyFloat_AS_DOUBLE(a[9]);
+    if (!bf16_rows(*q) || !c.read(*t[1], *t[2], *t[7], *t[8]) || !index_vector(*t[4]) || !index_vector(*t[5]) ||
+        !one_device(*q, *t[1], *t[2], *out, *t[4], *t[5], *bt, *t[7], *t[8]) || !on_current(*q))
+      return false;
+    B = t[4]->size(0) - 1, T = q->size(0), Hq = q->size(1);
+    if (B <= 0 || T == 0 || q->size(2) != c.D || !bf16_rows_of(*out, Hq, c.D) || out->size(0) < T || t[5]->size(0) < B ||
+        !table(*bt, B) || c.H <= 0 || Hq % c.H)
+      return false;
+    cu = (const int32_t*)t[4]->data_ptr(), sl = (const int32_t*)t[5]->data_ptr();
+    qp = q->data_ptr(), op = out->data_ptr(), st = stream_of(*q);
+    return true;
+  }
+};
+
+// (..., segm_out | None, segm_max | None, segm_sum | None, max_query_len, qmax, max_splits, lse | None)
+PyObject* fp4_decode_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 17 || !p_fp4_decode || getenv("KVQ_TARGET_WAVES")) return DECLINED;
+    Fp4Attn x;
+    int64_t maxq, qmax, max_splits;
+    if (!x.read(a) || !as_int(a[13], maxq) || !as_int(a[14], qmax) || !as_int(a[15], max_splits)) return DECLINED;
+    int64_t S = 1, rows = 0, seg_st = 0, seg_sh = 0, lse_st = 0;
+    float *sop = nullptr, *smp = nullptr, *ssp = nullptr, *lp = nullptr;
+    if (a[11] != Py_None) {
+      const at::Tensor *so = tensor(a[10]), *sm = tensor(a[11]), *ss = tensor(a[12]);
+      if (!so || !sm || !ss || so->dim() != 4 || sm->dim() != 3 || ss->dim() != 3 || !one_device(*x.q, *so, *sm, *ss))
+        return DECLINED;
+      S = sm->size(2), rows = sm->size(0), seg_st = sm->stride(0), seg_sh = sm->stride(1);
+      for (const at::Tensor* y : {so, sm, ss})
+        if (y->scalar_type() != at::kFloat || y->size(0) != rows || y->size(1) != x.Hq || y->size(2) != S) return DECLINED;
+      const int64_t D = x.c.D;
+      if (S > max_splits || sm->stride(2) != 1 || ss->strides() != sm->strides() || so->size(3) != D || so->stride(3) != 1 ||
+          so->stride(2) != D || so->stride(1) != seg_sh * D || so->stride(0) != seg_st * D)
+        return DECLINED;
+      sop = (float*)so->data_ptr(), smp = (float*)sm->data_ptr(), ssp = (float*)ss->data_ptr();
+    } else if (a[10] != Py_None || a[12] != Py_None) {
+      return DECLINED;
+    }
+    if (a[16] != Py_None) {
+      const at::Tensor* lse = tensor(a[16]);
+      if (!lse || !lse_rows(*lse, x.T, x.Hq) || !one_device(*x.q, *lse)) return DECLINED;
+      lp = (float*)lse->data_ptr(), lse_st = lse->stride(0);
+    }
+    const Fp4Cache& c = x.c;
+    auto* btp = (const int32_t*)x.bt->data_ptr();
+    return launch("kvq_fp4_decode_attention", [&] {
+      return p_fp4_decode(x.qp, x.q->stride(0), x.q->stride(1), c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D,
+                          c.ks, c.vs, c.sb, c.sh, x.op, x.out->stride(0), x.out->stride(1), x.cu, x.sl, btp, x.bt->stride(0), x.B,
+                          x.Hq, x.scale, sop, smp, ssp, seg_st, seg_sh, S, rows, lp, lse_st, 0, maxq, qmax, x.st);
+    });
+  });
+}
+
+// (..., rows_per_tile, tile_req, tile_row, tile_piece | None, tile_slot | None, merge | None, slots, src_req, src_j,
+//  temporary block table)
+PyObject* fp4_long_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 20 || !p_fp4_pages || !p_fp4_prefill) return DECLINED;
+    Fp4Attn x;
+    int64_t rows, slots;
+    if (!x.read(a) || !as_int(a[10], rows) || !as_int(a[16], slots)) return DECLINED;
+    const at::Tensor *treq = tensor(a[11]), *trow = tensor(a[12]);
+    if (!treq || !trow || !index_vector(*treq) || !index_vector(*trow) || !one_device(*x.q, *treq, *trow)) return DECLINED;
+    const int64_t tiles = treq->size(0);
+    if (tiles == 0 || trow->size(0) != tiles) return DECLINED;
+    const int32_t *pp = nullptr, *sp = nullptr, *mp = nullptr;
+    int64_t nm = 0;
+    at::Tensor part_out, part_ml;
+    if (a[13] != Py_None) {
+      const at::Tensor *piece = tensor(a[13]), *slot = tensor(a[14]), *merge = tensor(a[15]);
+      if (!piece || !slot || !merge || !index_vector(*piece) || !index_vector(*slot) || piece->size(0) != tiles ||
+          slot->size(0) != tiles || merge->scalar_type() != at::kInt || merge->dim() != 2 || !merge->is_contiguous() ||
+          merge->size(1) != 4 || !one_device(*x.q, *piece, *slot, *merge))
+        return DECLINED;
+      pp = (const int32_t*)piece->data_ptr(), sp = (const int32_t*)slot->data_ptr(), mp = (const int32_t*)merge->data_ptr();
+      nm = merge->size(0);
+      const auto f32 = x.q->options().dtype(at::kFloat);
+      part_out = at::empty({slots, x.c.H, rows, x.c.D}, f32);
+      part_ml = at::empty({slots, x.c.H, rows, 2}, f32);
+    }
+    float *pop = pp ? (float*)part_out.data_ptr() : nullptr, *pmp = pp ? (float*)part_ml.data_ptr() : nullptr;
+    const Fp4Cache& c = x.c;
+    auto* btp = (const int32_t*)x.bt->data_ptr();
+    auto *rp = (const int32_t*)treq->data_ptr(), *wp = (const int32_t*)trow->data_ptr();
+    const at::Tensor *sreq = tensor(a[17]), *sj = tensor(a[18]), *tbt = tensor(a[19]);
+    if (!sreq || !sj || !tbt || !index_vector(*sreq) || !index_vector(*sj) || sreq->size(0) == 0 ||
+        sj->size(0) != sreq->size(0) || !table(*tbt, 0) || !one_device(*x.q, *sreq, *sj, *tbt))
+      return DECLINED;
+    const int64_t P = sreq->size(0), tbs = tbt->stride(0);
+    auto *rqp = (const int32_t*)sreq->data_ptr(), *jp = (const int32_t*)sj->data_ptr(), *tbp = (const int32_t*)tbt->data_ptr();
+    const at::Tensor kt = at::empty({P, c.bs, c.H, c.D}, x.q->options()), vt = at::empty({P, c.bs, c.H, c.D}, x.q->options());
+    const at::Tensor st = at::empty({c.H, P * (c.bs / 16), 4}, x.q->options().dtype(at::kFloat));
+    void *ktp = kt.data_ptr(), *vtp = vt.data_ptr();
+    auto* stp = (float*)st.data_ptr();
+    return launch("kvq_fp4_pages", [&] {
+      const int rc = p_fp4_pages(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh, ktp,
+                                 vtp, stp, btp, x.bt->stride(0), rqp, jp, P, x.st);
+      if (rc) return rc;
+      entry = "kvq_fp4_prefill_attention";
+      return p_fp4_prefill(x.qp, x.q->stride(0), x.q->stride(1), ktp, vtp, stp, P, c.bs, c.H, c.D, x.op, x.out->stride(0),
+                           x.out->stride(1), x.cu, x.sl, tbp, tbs, x.Hq, rp, wp, tiles, rows, x.scale, pp, sp, mp, nm, pop, pmp,
+                           x.st);
+    });
+  });
+}
+
+// (q, k_cache, k_scale, lse, weights, cu_seqlens_q, seq_lens, block_table, softmax_scale, max_query_len, qmax)
+PyObject* add_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 11 || !p_key_weights) return DECLINED;
+    const at::Tensor* t[8];
+    for (int i = 0; i < 8; ++i)
+      if (!(t[i] = tensor(a[i]))) return DECLINED;
+    const at::Tensor &q = *t[0], &kc = *t[1], &ks = *t[2], &lse = *t[3], &w = *t[4], &cu = *t[5], &sl = *t[6], &bt = *t[7];
+    if (!PyFloat_CheckExact(a[8])) return DECLINED;
+    const double scale = PyFloat_AS_DOUBLE(a[8]);
+    int64_t maxq, qmax;
+    Fp4Cache c;
+    if (!as_int(a[9], maxq) || !as_int(a[10], qmax) || !c.read(kc, kc, ks, ks) || !bf16_rows(q) || !index_vector(cu) ||
+        !index_vector(sl) || !one_device(q, kc, ks, lse, w, cu, sl, bt) || !on_current(q))
+      return DECLINED;
+    const int64_t B = cu.size(0) - 1, T = q.size(0), Hq = q.size(1);
+    if (B <= 0 || T == 0 || q.size(2) != c.D || c.H <= 0 || Hq % c.H || sl.size(0) < B || !table(bt, B) || !lse_rows(lse, T, Hq) ||
+        w.dim() != 3 || w.scalar_type() != at::kFloat || w.stride(2) != 1 || w.size(0) < B || w.size(1) != c.H || w.size(2) == 0)
+      return DECLINED;
+    void *qp = q.data_ptr(), *st = stream_of(q);
+    auto* lp = (const float*)lse.data_ptr();
+    auto* wp = (float*)w.data_ptr();
+    auto *cup = (const int32_t*)cu.data_ptr(), *slp = (const int32_t*)sl.data_ptr(), *btp = (const int32_t*)bt.data_ptr();
+    return launch("kvq_fp4_key_weights", [&] {
+      return p_key_weights(qp, q.stride(0), q.stride(1), c.k, c.kb, c.kn, c.kh, c.nb, c.bs, c.H, c.D, c.ks, c.sb, c.sh, lp,
+                           lse.stride(0), wp, w.stride(0), w.stride(1), w.size(2), cup, slp, btp, bt.stride(0), B, Hq, scale, maxq,
+                           qmax, st);
+    });
+  });
+}
+
+// (k_cache, v_cache, k_scale, v_scale, weights, seq_lens, keep, recent, block_table, kept, new_lens)
+PyObject* evict_keys(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 11 || !p_evict) return DECLINED;
+    const at::Tensor* t[11];
+    for (int i = 0; i < 11; ++i)
+      if (i != 7 && !(t[i] = tensor(a[i]))) return DECLINED;
+    const at::Tensor &kc = *t[0], &vc = *t[1], &w = *t[4], &sl = *t[5], &keep = *t[6], &bt = *t[8], &kept = *t[9], &nl = *t[10];
+    int64_t recent;
+    Fp4Cache c;
+    if (!as_int(a[7], recent) || recent < 0 || !c.read(kc, vc, *t[2], *t[3]) || !index_vector(sl) || !index_vector(keep) ||
+        !index_vector(nl) || !one_device(kc, vc, *t[2], *t[3], w, sl, keep, bt, kept, nl) || !on_current(kc))
+      return DECLINED;
+    const int64_t B = sl.size(0);
+    if (B == 0 || keep.size(0) < B || nl.size(0) < B || !table(bt, B) || w.dim() != 3 || w.scalar_type() != at::kFloat ||
+        w.stride(2) != 1 || w.size(0) < B || w.size(1) != c.H || kept.dim() != 3 || kept.scalar_type() != at::kInt ||
+        kept.stride(2) != 1 || kept.size(0) < B || kept.size(1) != c.H)
+      return DECLINED;
+    void* st = stream_of(kc);
+    auto* wp = (float*)w.data_ptr();
+    auto *slp = (const int32_t*)sl.data_ptr(), *kp = (const int32_t*)keep.data_ptr(), *btp = (const int32_t*)bt.data_ptr();
+    auto *op = (int32_t*)kept.data_ptr(), *np = (int32_t*)nl.data_ptr();
+    return launch("kvq_fp4_evict", [&] {
+      return p_evict(c.k, c.kb, c.kn, c.kh, c.v, c.vb, c.vn, c.vh, c.nb, c.bs, c.H, c.D, c.ks, c.vs, c.sb, c.sh, wp, w.stride(0),
+                     w.stride(1), w.size(2), slp, kp, recent, btp, bt.stride(0), bt.size(1), B, op, kept.stride(0), kept.stride(1),
+                     kept.size(2), np, st);
+    });
+  });
+}
+
+// (q, k, positions, cos_sin, q_weight | None, k_weight | None, eps, interleaved, q_out, k_out)
+PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> long {
+    if (n != 10 || !p_norm_rope || !PyFloat_CheckExact(a[6]) || !PyBool_Check(a[7])) return DECLINED;
+    const at::Tensor *qt = tensor(a[0]), *kt = tensor(a[1]), *pt = tensor(a[2]), *tt = tensor(a[3]), *qot = tensor(a[8]),
+                     *kot = tensor(a[9]);
+    if (!qt || !kt || !pt || !tt || !qot || !kot) return DECLINED;
+    const at::Tensor &q = *qt, &k = *kt, &pos = *pt, &tab = *tt, &qo = *qot, &ko = *kot;
+    if (!bf16_rows(q) || !bf16_rows(k) || !bf16_rows(qo) || !bf16_rows(ko) || qo.sizes() != q.sizes() || ko.sizes() != k.sizes() ||
+        k.size(0) != q.size(0) || k.size(2) != q.size(2) || q.size(0) == 0 || pos.dim() != 1 || pos.size(0) != q.size(0) ||
+        (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || !pos.is_contiguous() || tab.dim() != 2 ||
+        (tab.scalar_type() != at::kFloat && tab.scalar_type() != at::kBFloat16) || tab.stride(1) != 1 ||
+        !one_device(q, k, pos, tab, qo, ko) || !on_current(q))
+      return DECLINED;
+    const void *qw = nullptr, *kw = nullptr;
+    bool wide = false;
+    if (a[4] != Py_None || a[5] != Py_None) {
+      const at::Tensor *x = tensor(a[4]), *y = tensor(a[5]);
+      if (!x || !y || x->dim() != 1 || x->size(0) != q.size(2) || x->sizes() != y->sizes() || x->scalar_type() != y->scalar_type() ||
+          (x->scalar_type() != at::kFloat && x->scalar_type() != at::kBFloat16) || !x->is_contiguous() || !y->is_contiguous() ||
+          !one_device(q, *x, *y))
+        return DECLINED;
+      qw = x->data_ptr(), kw = y->data_ptr(), wide = x->scalar_type() == at::kFloat;
+    }
+    const double eps = PyFloat_AS_DOUBLE(a[6]);
+    const bool inter = a[7] == Py_True;
+    void *qp = q.data_ptr(), *kp = k.data_ptr(), *qop = qo.data_ptr(), *kop = ko.data_ptr(), *st = stream_of(q);
+    const void *pp = pos.data_ptr(), *tp = tab.data_ptr();
+    return launch("kvq_norm_rope", [&] {
+      return p_norm_rope(qp, q.stride(0), q.stride(1), kp, k.stride(0), k.stride(1), qop, qo.stride(0), qo.stride(1), kop,
+                         ko.stride(0), ko.stride(1), q.size(0), q.size(1), k.size(1), q.size(2), pp,
+                         pos.scalar_type() == at::kLong ? 64 : 32, tp, tab.stride(0), tab.size(0), tab.size(1),
+                         tab.scalar_type() == at::kBFloat16, qw, kw, !wide, eps, inter, st);
+    });
+  });
+}
+
 // (): the entry point of this thread's last call, as the Python path names it in its error
 PyObject* last_entry(PyObject*, PyObject*) { return PyUnicode_FromString(entry); }
 
@@ -515,6 +815,14 @@ PyObject* bind(PyObject*, PyObject* d) {
   p_block_decode = (decltype(p_block_decode))at_name("kvq_block_decode_attention");
   p_block_prefill = (decltype(p_block_prefill))at_name("kvq_block_prefill_attention");
   p_block_codes = (decltype(p_block_codes))at_name("kvq_block_codes");
+  p_quant_fp4 = (decltype(p_quant_fp4))at_name("kvq_quant_fp4_cache");
+  p_read_fp4 = (decltype(p_read_fp4))at_name("kvq_read_fp4_cache");
+  p_fp4_pages = (decltype(p_fp4_pages))at_name("kvq_fp4_pages");
+  p_fp4_prefill = (decltype(p_fp4_prefill))at_name("kvq_fp4_prefill_attention");
+  p_fp4_decode = (decltype(p_fp4_decode))at_name("kvq_fp4_decode_attention");
+  p_key_weights = (decltype(p_key_weights))at_name("kvq_fp4_key_weights");
+  p_evict = (decltype(p_evict))at_name("kvq_fp4_evict");
+  p_norm_rope = (decltype(p_norm_rope))at_name("kvq_norm_rope");
   if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
@@ -534,6 +842,20 @@ PyMethodDef methods[] = {
      "kvq_block_decode_attention on torch tensors"},
     {"block_long_attention", (PyCFunction)(void (*)(void))block_long_attention, METH_FASTCALL,
      "kvq_block_prefill_attention on torch tensors"},
+    {"quant_fp4_cache", (PyCFunction)(void (*)(void))quant_fp4_cache, METH_FASTCALL,
+     "kvq_quant_fp4_cache on torch tensors"},
+    {"read_fp4_cache", (PyCFunction)(void (*)(void))read_fp4_cache, METH_FASTCALL,
+     "kvq_read_fp4_cache on torch tensors"},
+    {"fp4_decode_attention", (PyCFunction)(void (*)(void))fp4_decode_attention, METH_FASTCALL,
+     "kvq_fp4_decode_attention on torch tensors"},
+    {"fp4_long_attention", (PyCFunction)(void (*)(void))fp4_long_attention, METH_FASTCALL,
+     "the long requests' attention over a 4-bit cache on torch tensors"},
+    {"add_key_weights", (PyCFunction)(void (*)(void))add_key_weights, METH_FASTCALL,
+     "kvq_fp4_key_weights on torch tensors"},
+    {"evict_keys", (PyCFunction)(void (*)(void))evict_keys, METH_FASTCALL,
+     "kvq_fp4_evict on torch tensors"},
+    {"norm_rope", (PyCFunction)(void (*)(void))norm_rope, METH_FASTCALL,
+     "kvq_norm_rope on torch tensors"},
     {"last_entry", last_entry, METH_NOARGS, "the entry point of this thread's last call"},
     {nullptr, nullptr, 0, nullptr}};
 

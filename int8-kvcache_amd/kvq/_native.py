@@ -10,7 +10,7 @@ import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkvq_int8.so")
-ABI_VERSION = 15
+ABI_VERSION = 16
 ERR_LAUNCH = 2      # KVQ_ERR_LAUNCH
 
 _i64 = ctypes.c_int64
@@ -71,6 +71,25 @@ SIGNATURES = {
                                     _i64, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64,
                                     _i64, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr,
                                     _ptr, _i64, _ptr, _i64, _ptr],
+    "kvq_quant_fp4_cache": [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64,
+                            _i64, _i64, _i64, _ptr, _ptr, _i64, _i64, _ptr, _i64, _ptr],
+    "kvq_read_fp4_cache": [_ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64,
+                           _i64, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr],
+    "kvq_fp4_pages": [_ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64,
+                      _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr],
+    "kvq_fp4_prefill_attention": [_ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr,
+                                  _ptr, _ptr, _i64, _i64, _ptr, _ptr, _i64, _i64, _f64, _ptr, _ptr, _ptr, _i64, _ptr,
+                                  _ptr, _ptr],
+    "kvq_fp4_decode_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                                 _i64, _ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64,
+                                 _f64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr],
+    "kvq_fp4_key_weights": [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr,
+                            _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _f64, _i64, _i64, _ptr],
+    "kvq_fp4_evict": [_ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64, _i64,
+                      _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr,
+                      _ptr],
+    "kvq_norm_rope": [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64,
+                      _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64, _f64, _i64, _ptr],
     "kvq_last_error": [],
     "kvq_abi_version": [],
 }
