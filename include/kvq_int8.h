@@ -348,7 +348,7 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
 /* ---- 4-bit cache, no counterpart in the reference ----
  * A cached value is an e2m1 code (0, 1/2, 1, 3/2, 2, 3, 4, 6 or their negatives) times 2^(byte - 127), one exponent byte for
  * each 32 channels of a row (page, slot, head), K's and V's apart. Caches are bytes [nb, bs, H, D / 2], strides (sb, sn, sh, 1)
- * in bytes, multiples of 16, channel 2 c in the low half of byte c; exponent bytes k_scale / v_scale [nb, H, bs, D / 32],
+ * in bytes, multiples of 16, pages below 4 GiB apart, channel 2 c in the low half of byte c; exponent bytes k_scale / v_scale [nb, H, bs, D / 32],
  * strides (s_sb, s_sh, D / 32, 1), 16-byte aligned as well. Tables and lengths as above; head_dim 64 or 128. An exponent byte
  * that the write does not make (above 252: 255 would be no number) may give any value for its own row, and counts nowhere else. */
 
@@ -390,7 +390,7 @@ int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const v
 
 /* Attention over a 4-bit cache for requests with 1 <= q_len <= qmax: o = softmax(q k^T softmax_scale) v, bottom-right causal,
  * bf16 q and out; a row that sees no key is zero, another whose q holds a NaN or an infinity is NaN. Cached values are exact.
- * Rounded: the weights, to 2^-16 of each where at most 8 (token, q head) rows share a kv head, else to bf16 (2^-8). lse (fp32 [T, Hq], row stride lse_st, or NULL): the rows' natural
+ * Rounded: the weights, to bf16 (2^-8 of each). lse (fp32 [T, Hq], row stride lse_st, or NULL): the rows' natural
  * log-sum-exp, -inf where no key is seen. softmax_scale from 1e-16 to 1e16. Rows, skipped requests, split buffers and the other
  * arguments as kvq_block_decode_attention. */
 int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,

@@ -45,8 +45,9 @@ __global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightA
     if (L <= 0) return;
     const int G = a.G, bs = 1 << a.lbs;
     const int* bt = a.block_table + (int64_t)r * a.bt_stride;
-    const uint8_t* kbase = (const uint8_t*)a.kc + (int64_t)kvh * a.k_sh + n * (int)a.k_sn + (D / 8) * g;
-    const uint8_t* sbase = args.s.k + (int64_t)kvh * args.s.sh + n * SB + g * (D / 4) / FP4_GROUP;
+    const uint8_t* kbase = (const uint8_t*)a.kc + (int64_t)kvh * a.k_sh;
+    const uint8_t* sbase = args.s.k + (int64_t)kvh * args.s.sh;
+    const uint32_t koff = n * (int)a.k_sn + (D / 8) * g, soff = n * SB + g * (D / 4) / FP4_GROUP;
     float* wrow = args.w + (int64_t)r * args.w_sr + (int64_t)kvh * args.w_sh;
     for (int row0 = 0; row0 < qlen * G; row0 += 16 * RT) {
       Fp4Query<D> q[RT];
@@ -57,7 +58,8 @@ __global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightA
         const int R = row0 + 16 * t + n, rtok = div_group(a, R), rh = R - rtok * G;
         const bool real = rtok < qlen;
         const int64_t at = tok + min(rtok, qlen - 1);
-        q[t].make(a.q + at * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, real, g);
+        q[t].load(a.q + at * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, real, g);
+        q[t].make();
         const float l = args.lse[at * args.lse_st + kvh * G + rh];
         // a row whose log-sum-exp is no finite number adds nothing: it saw no key, or its weights are none
         const bool in = real && __builtin_fabsf(l) < INFINITY;
@@ -74,8 +76,8 @@ __global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightA
         for (int b = 0; b < 2; ++b) {
           const int key = min(c * TILE + 16 * b, (L - 1) & ~15);
           const int p = page_at(bt, 0, 0, key >> a.lbs), pg = p >= 0 && p < a.num_blocks ? p : 0, of = key & (bs - 1);
-          load_k16<D>(x.k[b], kbase + (int64_t)pg * a.k_sb + (int64_t)of * a.k_sn);
-          x.ks[b] = sbase[(int64_t)pg * args.s.sb + of * SB];
+          load_k16<D>(x.k[b], page_base(kbase, pg, (uint32_t)a.k_sb), koff, of * (uint32_t)a.k_sn);
+          x.ks[b] = load_at<uint8_t>(page_base(sbase, pg, (uint32_t)args.s.sb), soff, of * SB);
         }
       };
       Tile x;

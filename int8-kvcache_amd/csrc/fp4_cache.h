@@ -200,8 +200,11 @@ __global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
 //                      makes two codes and their exponent two bf16 operands, exactly; q as it is
 //   e    = S scale     m: the row's largest e plus BLOCK_REF, raised where it lags by more than 8
 //   P    = 2^(e - m),  l += P
-//   O   += V^T . P     v_mfma_f32_16x16x32_bf16: V's values as bf16 (exact), P as one bf16 (2^-8) or, PACK, as two (2^-16)
-// PACK: at most 8 (token, q head) rows per kv head: they are the columns 0 .. 7 and again 8 .. 15, where P's lower parts go.
+//   O   += V^T . P     v_mfma_f32_16x16x32_bf16: V's values as bf16 (exact), P rounded to bf16 (2^-8 of each weight)
+// A conversion leaves two channels of a key side by side; the product sums over what is side by side. Not PACK: v_perm pairs
+// keys of a channel, two for four values. PACK (at most 8 (token, q head) rows per kv head): the rows are the columns 0 .. 7 and
+// again 8 .. 15, and the product runs over (key, channel of the pair): P stands beside zeros, in columns 0 .. 7 for the even
+// channel and in 8 .. 15 for the odd one. No value moves, and the accumulators are half as many.
 // (The scaled MFMA takes the codes without a conversion, but sums products of 8-bit floats to 2^-13 of the largest of each few:
 // scores were 7e-4 off.)
 // Weights are kept below 2^-24 (BLOCK_REF), so that a sum over a million keys of V's largest values (6 2^125) stays finite.
@@ -211,6 +214,7 @@ struct Fp4AttnArgs {
   Fp4Scales s;
   float* lse;   // [tokens, q heads], or NULL
   int64_t lse_st;
+  int apart;    // K and V rows are not side by side
 };
 static_assert(offsetof(Fp4AttnArgs, a) == 0 && sizeof(AttnArgs) % 8 == 0, "AttnArgs lead the kernel arguments");
 __device__ __forceinline__ const Fp4AttnArgs& fresh_fp4() {
@@ -220,28 +224,41 @@ __device__ __forceinline__ const Fp4AttnArgs& fresh_fp4() {
 }
 constexpr float LN2 = 0.6931471805599453f;
 
-template <int D>
-struct Fp4Tile {
-  uint32_t k[2][D / 32];            // keys 16 b + n, channels (D / 4) g ..: a word of 8 for each step of the product
-  uint8_t ks[2];                    // their exponent bytes
-  uint32_t v[8];                    // keys 16 (j / 4) + 4 g + j % 4, channels (D / 16) n ..
-  uint32_t vs[2][D / 32];           // exponent bytes of keys 16 b + 4 g .. + 3
-};
+// A wavefront's ring of tiles in LDS. A slot holds two halves of 16 keys, each its rows' K and V codes in 16-byte chunks (chunk
+// p of row r: K's first, then V's), then the rows' exponent bytes, K's and V's (and 256 bytes in all, what a DMA of 4 bytes a lane
+// writes).
+constexpr int fp4_chunks(int d) { return d / 16; }                             // chunks of a row, K's and V's
+constexpr int fp4_codes(int d) { return 16 * 16 * fp4_chunks(d); }             // bytes of a half's codes
+constexpr int fp4_half(int d) { return fp4_codes(d) + 256; }
+constexpr int fp4_slot(int d) { return 2 * fp4_half(d); }
+constexpr int fp4_accs(int d, bool pack) { return pack ? d / 32 : d / 16; }
+// what a lane hands over in the merge of key splits: accumulators, maximum, denominator
+constexpr int fp4_merge_fields(int d, bool pack) { return 4 * fp4_accs(d, pack) + 2; }
+// Wavefronts of a workgroup: what its registers and LDS leave room for. Segments that are not cut are shared by all of them.
+constexpr int FP4_WAVES = 8;
+constexpr int FP4_SLOTS = 4;
+constexpr int FP4_DMA_AUX = 2;   // streaming: K and V are read once
 
 // 16 query rows as the MFMA's second operand: lane (n, g) holds row n's channels (D / 4) g + 8 s .. + 7 in step s.
 template <int D>
 struct Fp4Query {
+  u32x4 raw[D / 32];
   bf16x8 op[D / 32];
   float odd;   // 0, or NaN where the row holds a NaN or an infinity: then its output is NaN too
-  __device__ __forceinline__ void make(const uint16_t* row, bool real, int g) {
+  __device__ __forceinline__ void load(const uint16_t* row, bool real, int g) {
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      raw[s] = u32x4{0u, 0u, 0u, 0u};
+      if (real) raw[s] = *reinterpret_cast<const u32x4*>(row + (D / 4) * g + 8 * s);
+    }
+  }
+  __device__ __forceinline__ void make() {
     odd = 0.f;
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) {
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (real) w = *reinterpret_cast<const u32x4*>(row + (D / 4) * g + 8 * s);
-      op[s] = *reinterpret_cast<bf16x8*>(&w);
+      op[s] = *reinterpret_cast<bf16x8*>(&raw[s]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) odd = __builtin_fmaf(bf16_lo(w[j]), 0.f, __builtin_fmaf(bf16_hi(w[j]), 0.f, odd));
+      for (int j = 0; j < 4; ++j) odd = __builtin_fmaf(bf16_lo(raw[s][j]), 0.f, __builtin_fmaf(bf16_hi(raw[s][j]), 0.f, odd));
     }
     odd = group4_sum(odd);
   }
@@ -257,31 +274,60 @@ __device__ __forceinline__ f32x4 fp4_scores(const uint32_t (&k)[D / 32], uint32_
   }
   return z;
 }
+// A streaming load of each lane's own `off` from a base that the wavefront shares, through a buffer descriptor: the base and
+// `uni` stay in scalar registers, a lane's part is 32 bits (as 64-bit addresses they took two vector registers and an addition
+// a load: 14 of a tile's 160 vector instructions).
+template <typename T>
+__device__ __forceinline__ T load_at(const uint8_t* base, uint32_t off, uint32_t uni) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, INT32_MAX, QC_RSRC_WORD3);
+  if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(r, off, uni, QC_LOAD_AUX));
+  else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(r, off, uni, QC_LOAD_AUX));
+  else if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, uni, QC_LOAD_AUX));
+  else if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, uni, QC_LOAD_AUX));
+  else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b8(r, off, uni, QC_LOAD_AUX));
+}
+// page p of `base`: strides are below 4 GiB (check_fp4)
+__device__ __forceinline__ const uint8_t* page_base(const uint8_t* base, int p, uint32_t stride) {
+  return base + (uint64_t)(uint32_t)p * stride;
+}
 // the lane's words of 16 keys' codes
 template <int D>
-__device__ __forceinline__ void load_k16(uint32_t (&k)[D / 32], const uint8_t* p) {
+__device__ __forceinline__ void load_k16(uint32_t (&k)[D / 32], const uint8_t* base, uint32_t off, uint32_t uni) {
   if constexpr (D == 128) {
-    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    const u32x4 w = load_at<u32x4>(base, off, uni);
 #pragma unroll
     for (int s = 0; s < 4; ++s) k[s] = w[s];
   } else {
-    const u32x2 w = ldv(reinterpret_cast<const u32x2*>(p));
+    const u32x2 w = load_at<u32x2>(base, off, uni);
     k[0] = w.x;
     k[1] = w.y;
   }
 }
 
-template <int D, int PF, bool PACK>
+// Where chunk p of row r of a half stands in LDS, in chunks. A DMA writes 64 chunks in the order of its lanes; which chunk a lane
+// asks for is free. K and V rows side by side in memory (vLLM's views): a DMA takes 8 (D = 64: 16) whole rows, so that it asks for
+// lines of 128 bytes (half lines, K's and V's in turn, stream at 5.9 TB/s, whole ones at 6.8). Apart: K's rows, then V's. The
+// chunks of a row are swapped by the row (exclusive or), so that the reads below meet few banks twice.
+template <int D>
+__device__ __forceinline__ int fp4_place(bool apart, int r, int p) {
+  constexpr int CH = fp4_chunks(D), H = CH / 2;
+  return apart ? (p / H) * 16 * H + r * H + ((p % H) ^ ((r * H / 4) & (H - 1))) : r * CH + (p ^ (r & (CH - 1)));
+}
+
+template <int D, bool PACK>
 __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqlen, int kvh, int row0, int c_begin, int c_end,
-                                           int ks, int KS, int rtile, int part, int nparts, float* lds, int lane) {
+                                           int ks, int KS, int rtile, int part, int nparts, uint8_t* lds, int lane) {
   const Fp4AttnArgs& args = fresh_fp4();
   const AttnArgs& a = args.a;
   constexpr int RT = PACK ? 8 : 16;        // rows of this wavefront's tile
-  constexpr int VT = D / 16, OPL = D / 4, SB = D / FP4_GROUP;
-  const int G = PACK ? a.G >> 1 : a.G;     // (PACK: the plan counts plane rows, two a row)
+  constexpr int VT = D / 16, NA = fp4_accs(D, PACK), SB = D / FP4_GROUP;
+  constexpr int S = FP4_SLOTS, SLOT = fp4_slot(D), HALF = fp4_half(D), CODES = fp4_codes(D), CH = fp4_chunks(D);
+  constexpr int DMAS = CODES / 1024, OPS = 2 * (DMAS + 1);   // DMAs of a half's codes; vector memory operations of a tile
+  static_assert(S * OPS < 64, "vmcnt range");
+  const int G = PACK ? a.G >> 1 : a.G;     // (PACK: the plan counts 16 columns a tile, two a row)
   const bool active = row0 < qlen * G;
   const int num_blocks = a.num_blocks, lbs = a.lbs;
-  const int64_t k_sb = a.k_sb, k_sn = a.k_sn, v_sb = a.v_sb, v_sn = a.v_sn, s_sb = args.s.sb;
+  const uint32_t c_sb = (uint32_t)a.k_sb, c_sn = (uint32_t)a.k_sn, s_sb = (uint32_t)args.s.sb;
   seq = __builtin_amdgcn_readfirstlane(seq);
   tok = __builtin_amdgcn_readfirstlane(tok);
   qlen = __builtin_amdgcn_readfirstlane(qlen);
@@ -304,76 +350,153 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 
   const int R = row0 + (n & (RT - 1)), rtok = div_g(R), rh = R - rtok * G;
   const int lim_lo = L - qlen + 1 + __builtin_amdgcn_readfirstlane(div_g(row0));
-  const uint8_t* kbase = (const uint8_t*)a.kc + (int64_t)kvh * a.k_sh;
-  const uint8_t* vbase = (const uint8_t*)a.vc + (int64_t)kvh * a.v_sh;
-  const uint8_t* ksb = args.s.k + (int64_t)kvh * args.s.sh;
-  const uint8_t* vsb = args.s.v + (int64_t)kvh * args.s.sh;
-  const int koff = n * (int)k_sn + (D / 8) * g, ksoff = n * SB + g * (D / 4) / FP4_GROUP;
-  const int voff = 4 * g * (int)v_sn + n * (VT / 2);
-  const int vsn = (int)v_sn;
-  const int vshift = 8 * (n * VT / FP4_GROUP);
+  Fp4Query<D> q;
+  if (nt > 0) q.load(a.q + (int64_t)(tok + min(rtok, qlen - 1)) * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, rtok < qlen, g);
 
-  auto page_of = [&](int key) -> int {
-    const int idx = __builtin_amdgcn_readfirstlane(key >> lbs);
-    const int p = __builtin_amdgcn_readfirstlane(((const __attribute__((address_space(4))) int*)bt)[idx]);
-    return (p >= 0 && p < num_blocks) ? p : 0;
+  // ---- what each lane's DMAs ask for, beside a page and slot, and where it reads ----
+  const bool apart = args.apart;
+  const uint8_t* src[DMAS];
+#pragma unroll
+  for (int u = 0; u < DMAS; ++u) {
+    const int at = 64 * u + lane;   // the place this lane's chunk goes to: fp4_place the other way round
+    constexpr int H = CH / 2;
+    int r, p;
+    if (apart) {
+      r = at / H % 16;
+      p = at / (16 * H) * H + ((at % H) ^ ((r * H / 4) & (H - 1)));
+    } else {
+      r = at / CH;
+      p = (at % CH) ^ (r & (CH - 1));
+    }
+    src[u] = (const uint8_t*)(p < H ? a.kc + (int64_t)kvh * a.k_sh : a.vc + (int64_t)kvh * a.v_sh) + (uint64_t)(r * c_sn) + 16 * (p % H);
+  }
+  // exponent bytes: 4 SB words of K's, as many of V's, then both again
+  const uint8_t* ssrc = ((lane / (4 * SB)) % 2 ? args.s.v : args.s.k) + (int64_t)kvh * args.s.sh + 4 * (lane % (4 * SB));
+  const uint32_t base = (uint32_t)(uintptr_t)lds;
+  uint32_t kadr, vadr[4];
+  {
+    const int ch = g * (D / 8);   // byte of the row's K
+    kadr = base + 16 * fp4_place<D>(apart, n, ch / 16) + ch % 16;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int ch = n * (VT / 2);
+    vadr[i] = base + 16 * fp4_place<D>(apart, 4 * g + i, CH / 2 + ch / 16) + ch % 16;
+  }
+  const uint32_t ksadr = base + CODES + n * SB + g * (D / 4) / FP4_GROUP, vsadr = base + CODES + 16 * SB + 4 * g * SB;
+  const uint32_t vrot = 8 * (n * VT / FP4_GROUP) + 9;   // brings the byte of the lane's V channels to bits 23 .. 30
+
+  // a tile's two page ids are asked for one tile ahead
+  auto half_key = [&](int j, int b) { return min(tile(min(j, nt - 1)) * TILE + 16 * b, (L - 1) & ~15); };
+  int next[2] = {0, 0};
+  auto fetch = [&](int j) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      next[b] = ((const __attribute__((address_space(4))) int*)bt)[__builtin_amdgcn_readfirstlane(half_key(j, b) >> lbs)];
   };
-  auto load = [&](Fp4Tile<D>& r, int c) {
-    const int n0 = c * TILE, n1 = n0 + 16;
-    const int p0 = page_of(n0);
-    const int p1 = n1 < L ? page_of(n1) : p0;
-    const int o0 = n0 & (bs - 1), o1 = n1 < L ? (n1 & (bs - 1)) : o0;
-    const int pg[2] = {p0, p1}, of[2] = {o0, o1};
+  auto load = [&](int slot, int j) {   // tile j, whose page ids are here
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      const uint8_t* kb = kbase + (int64_t)pg[b] * k_sb + (int64_t)of[b] * k_sn;
-      const uint8_t* vb = vbase + (int64_t)pg[b] * v_sb + (int64_t)of[b] * v_sn;
-      const int64_t so = (int64_t)pg[b] * s_sb + of[b] * SB;
-      load_k16<D>(r.k[b], kb + koff);
-      r.ks[b] = __builtin_nontemporal_load(ksb + so + ksoff);
-      if constexpr (D == 128) {
-        const u32x4 s = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vsb + so + 4 * g * SB));
+      const int id = __builtin_amdgcn_readfirstlane(next[b]), p = (unsigned)id < (unsigned)num_blocks ? id : 0;
+      const uint32_t of = half_key(j, b) & (bs - 1);
+      const uint64_t co = (uint64_t)(uint32_t)p * c_sb + of * c_sn, so = (uint64_t)(uint32_t)p * s_sb + of * SB;
+      uint8_t* dst = lds + slot * SLOT + b * HALF;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.vs[b][i] = s[i];
-      } else {
-        const u32x2 s = ldv(reinterpret_cast<const u32x2*>(vsb + so + 4 * g * SB));
-        r.vs[b][0] = s.x;
-        r.vs[b][1] = s.y;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (D == 128) r.v[4 * b + i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vb + voff + i * vsn));
-        else r.v[4 * b + i] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(vb + voff + i * vsn));
-      }
+      for (int u = 0; u < DMAS; ++u)
+        __builtin_amdgcn_global_load_lds((const void*)(src[u] + co), (__attribute__((address_space(3))) void*)(dst + 1024 * u), 16, 0, FP4_DMA_AUX);
+      __builtin_amdgcn_global_load_lds((const void*)(ssrc + so), (__attribute__((address_space(3))) void*)(dst + CODES), 4, 0, FP4_DMA_AUX);
     }
   };
 
-  Fp4Tile<D> ring[PF];
   if (nt > 0) {
+    fetch(0);
 #pragma unroll
-    for (int j = 0; j < PF - 1; ++j) load(ring[j], tile(min(j, nt - 1)));
+    for (int j = 0; j < S - 1; ++j)
+      if (j < nt) {
+        load(j, j);
+        fetch(j + 1);
+      }
+    q.make();
+  } else {
+    q.odd = 0.f;
   }
-  Fp4Query<D> q;
-  q.make(a.q + (int64_t)(tok + min(rtok, qlen - 1)) * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, rtok < qlen, g);
   const float rs = a.sm_log2 + q.odd;
   const int lim = rtok < qlen ? L - qlen + 1 + rtok : L;
-  const uint32_t drop = PACK && n < 8 ? 0u : 0xffff0000u;   // PACK: this lane's part of P is what is left without these bits
+  const uint32_t pshift = PACK && n >= 8 ? 16 : 0;   // PACK: where the column's weights stand beside zeros
 
   float m = -1e30f, l = 0.f;
-  f32x4 acc[VT];
+  f32x4 acc[NA];
 #pragma unroll
-  for (int t = 0; t < VT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NA; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](auto masked_t, const Fp4Tile<D>& r, int c) {
+  // tile j in `slot`; vm: this wavefront's vector memory operations behind the tile's own (the reads' statements wait for
+  // themselves: the compiler sees neither the DMAs nor that they are done)
+  auto compute = [&](auto masked_t, auto vm_t, auto slot_t, int j) {
     constexpr bool MASKED = decltype(masked_t)::value;
-    const int n0 = c * TILE;
+    constexpr int VM = decltype(vm_t)::value, AT = decltype(slot_t)::value * SLOT;
+    const int n0 = tile(j) * TILE;
+    uint32_t kw[2][D / 32], ksw[2], v[8], vs[2][D / 32];
+    if constexpr (D == 128) {
+      u32x4 k0, k1;
+      asm volatile("s_waitcnt vmcnt(%c6)\n\tds_read_b128 %0, %4 offset:%c7\n\tds_read_b128 %1, %4 offset:%c8\n\t"
+                   "ds_read_u8 %2, %5 offset:%c7\n\tds_read_u8 %3, %5 offset:%c8\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(k0), "=&v"(k1), "=&v"(ksw[0]), "=&v"(ksw[1]) : "v"(kadr), "v"(ksadr), "n"(VM), "n"(AT), "n"(AT + HALF) : "memory");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        kw[0][i] = k0[i];
+        kw[1][i] = k1[i];
+      }
+    } else {
+      u32x2 k0, k1;
+      asm volatile("s_waitcnt vmcnt(%c6)\n\tds_read_b64 %0, %4 offset:%c7\n\tds_read_b64 %1, %4 offset:%c8\n\t"
+                   "ds_read_u8 %2, %5 offset:%c7\n\tds_read_u8 %3, %5 offset:%c8\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(k0), "=&v"(k1), "=&v"(ksw[0]), "=&v"(ksw[1]) : "v"(kadr), "v"(ksadr), "n"(VM), "n"(AT), "n"(AT + HALF) : "memory");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        kw[0][i] = k0[i];
+        kw[1][i] = k1[i];
+      }
+    }
     // ---- scores; key of (b, i) = n0 + 16 b + 4 g + i ----
     f32x4 z[2];
     bool ok[2][4];
     float tmax = -INFINITY;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      z[b] = fp4_scores<D>(r.k[b], r.ks[b], q);
+      z[b] = fp4_scores<D>(kw[b], ksw[b], q);
+    }
+    if constexpr (D == 128) {   // (while the products run)
+      u32x4 x0, x1;
+      asm volatile("ds_read_b32 %0, %10 offset:%c15\n\tds_read_b32 %1, %11 offset:%c15\n\tds_read_b32 %2, %12 offset:%c15\n\t"
+                   "ds_read_b32 %3, %13 offset:%c15\n\tds_read_b32 %4, %10 offset:%c16\n\tds_read_b32 %5, %11 offset:%c16\n\t"
+                   "ds_read_b32 %6, %12 offset:%c16\n\tds_read_b32 %7, %13 offset:%c16\n\tds_read_b128 %8, %14 offset:%c15\n\t"
+                   "ds_read_b128 %9, %14 offset:%c16\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
+                     "=&v"(x0), "=&v"(x1)
+                   : "v"(vadr[0]), "v"(vadr[1]), "v"(vadr[2]), "v"(vadr[3]), "v"(vsadr), "n"(AT), "n"(AT + HALF) : "memory");
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vs[0][i] = x0[i];
+        vs[1][i] = x1[i];
+      }
+    } else {
+      u32x2 x0, x1;
+      asm volatile("ds_read_u16 %0, %10 offset:%c15\n\tds_read_u16 %1, %11 offset:%c15\n\tds_read_u16 %2, %12 offset:%c15\n\t"
+                   "ds_read_u16 %3, %13 offset:%c15\n\tds_read_u16 %4, %10 offset:%c16\n\tds_read_u16 %5, %11 offset:%c16\n\t"
+                   "ds_read_u16 %6, %12 offset:%c16\n\tds_read_u16 %7, %13 offset:%c16\n\tds_read_b64 %8, %14 offset:%c15\n\t"
+                   "ds_read_b64 %9, %14 offset:%c16\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
+                     "=&v"(x0), "=&v"(x1)
+                   : "v"(vadr[0]), "v"(vadr[1]), "v"(vadr[2]), "v"(vadr[3]), "v"(vsadr), "n"(AT), "n"(AT + HALF) : "memory");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        vs[0][i] = x0[i];
+        vs[1][i] = x1[i];
+      }
+    }
+    fetch(j + S);   // (here: the statements above wait for every scalar load as well)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         ok[b][i] = MASKED ? n0 + 16 * b + 4 * g + i < lim : true;
@@ -398,122 +521,138 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       }
     if (__any(raise)) {
 #pragma unroll
-      for (int t = 0; t < VT; ++t) acc[t] *= alpha;
+      for (int t = 0; t < NA; ++t) acc[t] *= alpha;
     }
-    // ---- PV: O^T[channel][row] += V^T . P^T, the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i ----
-    u32x4 pw;
+    // ---- PV: O^T[channel][row] += V^T . P^T ----
+    float vsc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // the lane's byte as an exponent: the conversion reads no other bits of its scale (D = 64: two keys' bytes to a word)
+      const uint32_t w = D == 128 ? vs[e / 4][e % 4] : vs[e / 4][e % 4 / 2];
+      vsc[e] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, D == 128 || e % 2 == 0 ? vrot : vrot + 16));
+      // whatever lies behind the last key is finite: it meets weights of 0
+      if (MASKED) vsc[e] = n0 + 16 * (e / 4) + 4 * g + e % 4 < L ? vsc[e] : 0.f;
+    }
     if constexpr (PACK) {
-      float x[2][4];
+      u32x4 pw[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[b][i] = p[b][i] - __uint_as_float(__float_as_uint(p[b][i]) & drop);
-      pw = u32x4{bf16x2_upper(x[0][0], x[0][1]), bf16x2_upper(x[0][2], x[0][3]), bf16x2_upper(x[1][0], x[1][1]),
-                 bf16x2_upper(x[1][2], x[1][3])};
-    } else {
-      pw = u32x4{pack_bf16x2_rne(p[0][0], p[0][1]), pack_bf16x2_rne(p[0][2], p[0][3]), pack_bf16x2_rne(p[1][0], p[1][1]),
-                 pack_bf16x2_rne(p[1][2], p[1][3])};
-    }
-    const bf16x8 pop = *reinterpret_cast<bf16x8*>(&pw);
-    float vsc[8];
+        for (int i = 0; i < 4; ++i) pw[b][i] = pack_bf16x2_rne(p[b][i], 0.f) << pshift;
+      auto pair = [&](auto byte_t) {   // the channels 2 B and 2 B + 1 of the lane's
+        constexpr int B = decltype(byte_t)::value;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // (D = 64: two keys' bytes to a word)
-      const uint32_t w = D == 128 ? r.vs[j / 4][j % 4] >> vshift : r.vs[j / 4][j % 4 / 2] >> (vshift + 16 * (j % 2));
-      vsc[j] = __uint_as_float((w & 0xffu) << 23);
-      // whatever lies behind the last key is finite: it meets weights of 0
-      if (MASKED) vsc[j] = n0 + 16 * (j / 4) + 4 * g + j % 4 < L ? vsc[j] : 0.f;
-    }
-    auto pairs = [&](auto byte_t) {   // the channels 2 B and 2 B + 1 of the lane's
-      constexpr int B = decltype(byte_t)::value;
-      uint32_t w[8];
+        for (int b = 0; b < 2; ++b) {
+          u32x4 w;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(r.v[j], vsc[j], B));
-      u32x4 even, odd;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
-        odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+          for (int i = 0; i < 4; ++i)
+            w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[4 * b + i], vsc[4 * b + i], B));
+          acc[B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&w), *reinterpret_cast<bf16x8*>(&pw[b]),
+                                                           acc[B], 0, 0, 0);
+        }
+      };
+      pair(std::integral_constant<int, 0>{});
+      pair(std::integral_constant<int, 1>{});
+      if constexpr (D == 128) {
+        pair(std::integral_constant<int, 2>{});
+        pair(std::integral_constant<int, 3>{});
       }
-      acc[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), pop, acc[2 * B], 0, 0, 0);
-      acc[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), pop, acc[2 * B + 1], 0, 0, 0);
-    };
-    pairs(std::integral_constant<int, 0>{});
-    pairs(std::integral_constant<int, 1>{});
-    if constexpr (D == 128) {
-      pairs(std::integral_constant<int, 2>{});
-      pairs(std::integral_constant<int, 3>{});
+    } else {
+      u32x4 pw = {pack_bf16x2_rne(p[0][0], p[0][1]), pack_bf16x2_rne(p[0][2], p[0][3]), pack_bf16x2_rne(p[1][0], p[1][1]),
+                  pack_bf16x2_rne(p[1][2], p[1][3])};
+      const bf16x8 pop = *reinterpret_cast<bf16x8*>(&pw);   // the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i
+      auto pair = [&](auto byte_t) {
+        constexpr int B = decltype(byte_t)::value;
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[e], vsc[e], B));
+        u32x4 even, odd;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          even[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100u);
+          odd[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
+        }
+        acc[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), pop, acc[2 * B], 0, 0, 0);
+        acc[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), pop, acc[2 * B + 1], 0, 0, 0);
+      };
+      pair(std::integral_constant<int, 0>{});
+      pair(std::integral_constant<int, 1>{});
+      if constexpr (D == 128) {
+        pair(std::integral_constant<int, 2>{});
+        pair(std::integral_constant<int, 3>{});
+      }
     }
   };
 
-  // the ring of attn_kernel: PF - 1 tiles in flight, loads past the end re-read the last tile
+  // S - 1 tiles in flight. The last ones have fewer behind them: they wait for all.
   if (nt > 0) {
     const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
-    const int j_full = min(nt, full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0);
+    const int j_full = min(nt - (S - 1), full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0);
     int j0 = 0;
-    for (; j0 + PF <= j_full; j0 += PF) {
-#pragma unroll
-      for (int jj = 0; jj < PF; ++jj) {
-        load(ring[(jj + PF - 1) % PF], tile(min(j0 + jj + PF - 1, nt - 1)));
-        compute(std::false_type{}, ring[jj], tile(j0 + jj));
-      }
+    for (; j0 + S <= j_full; j0 += S) {
+      auto step = [&](auto s_t) {
+        constexpr int s = decltype(s_t)::value;
+        load((s + S - 1) % S, j0 + s + S - 1);
+        compute(std::false_type{}, std::integral_constant<int, (S - 1) * OPS>{}, s_t, j0 + s);
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+      if constexpr (S > 2) step(std::integral_constant<int, 2 % S>{});
+      if constexpr (S > 3) step(std::integral_constant<int, 3 % S>{});
     }
-    for (; j0 < nt; j0 += PF) {
-#pragma unroll
-      for (int jj = 0; jj < PF; ++jj) {
-        const int j = j0 + jj;
-        if (j >= nt) break;
-        load(ring[(jj + PF - 1) % PF], tile(min(j + PF - 1, nt - 1)));
-        compute(std::true_type{}, ring[jj], tile(j));
-      }
+    for (; j0 < nt; j0 += S) {
+      auto step = [&](auto s_t) {
+        constexpr int s = decltype(s_t)::value;
+        const int j = j0 + s;
+        if (j >= nt) return;
+        if (j + S - 1 < nt) {
+          load((s + S - 1) % S, j + S - 1);
+          compute(std::true_type{}, std::integral_constant<int, (S - 1) * OPS>{}, s_t, j);
+        } else {
+          compute(std::true_type{}, std::integral_constant<int, 0>{}, s_t, j);
+        }
+      };
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+      if constexpr (S > 2) step(std::integral_constant<int, 2 % S>{});
+      if constexpr (S > 3) step(std::integral_constant<int, 3 % S>{});
     }
   }
 
-  // ---- epilogue: lane (n, g) holds channels (D/4) g + (D/16) i + t of its row in acc[t][i] ----
+  // ---- the key splits' merge, half of them into the other half at a time ----
   l = group4_sum(l);
-  if constexpr (PACK) {   // both planes of a row: lanes n and n + 8 end with the same sums
+  if (KS > 1) {
+    // (each wavefront hands over in its own ring, which is done with)
+    static_assert(fp4_merge_fields(D, PACK) * WAVE * 4 <= S * SLOT, "merge fields in the ring");
+    auto mem = [&](int k) { return reinterpret_cast<float*>(lds + (k - ks) * a.rt * S * SLOT) + lane; };
+    for (int half = KS, width = KS; width > 1; width = half) {
+      half = (width + 1) / 2;
+      if (active && ks >= half && ks < width) {
+        float* to = mem(ks);
 #pragma unroll
-    for (int t = 0; t < VT; ++t)
+        for (int t = 0; t < NA; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] += ror8(acc[t][i]);
-  }
-  if (KS > 1) {   // attn_kernel's merge of the key splits
-    static_assert(VT * 4 + 2 <= MERGE_FIELDS, "merge slot too small");
-    auto slot = [&](int k) { return lds + (size_t)((k - 1) * a.rt + rtile) * MERGE_FIELDS * WAVE + lane; };
-    if (ks > 0 && active) {
-      float* sl = slot(ks);
-#pragma unroll
-      for (int t = 0; t < VT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sl[(4 * t + i) * WAVE] = acc[t][i];
-      sl[(4 * VT) * WAVE] = m;
-      sl[(4 * VT + 1) * WAVE] = l;
-    }
-    __syncthreads();
-    if (ks == 0 && active) {
-      float M = m;
-      for (int k = 1; k < KS; ++k) M = __builtin_fmaxf(M, slot(k)[(4 * VT) * WAVE]);
-      const float w0 = __builtin_amdgcn_exp2f(m - M);
-      l *= w0;
-#pragma unroll
-      for (int t = 0; t < VT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] *= w0;
-      for (int k = 1; k < KS; ++k) {
-        const float* src = slot(k);
-        const float wk = __builtin_amdgcn_exp2f(src[(4 * VT) * WAVE] - M);
-        l = __builtin_fmaf(wk, src[(4 * VT + 1) * WAVE], l);
-#pragma unroll
-        for (int t = 0; t < VT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(wk, src[(4 * t + i) * WAVE], acc[t][i]);
+          for (int i = 0; i < 4; ++i) to[(4 * t + i) * WAVE] = acc[t][i];
+        to[(4 * NA) * WAVE] = m;
+        to[(4 * NA + 1) * WAVE] = l;
       }
-      m = M;
+      __syncthreads();
+      if (active && ks + half < width) {
+        const float* from = mem(ks + half);
+        const float mo = from[(4 * NA) * WAVE], M = __builtin_fmaxf(m, mo);
+        const float w0 = __builtin_amdgcn_exp2f(m - M), w1 = __builtin_amdgcn_exp2f(mo - M);
+        l = __builtin_fmaf(w1, from[(4 * NA + 1) * WAVE], l * w0);
+#pragma unroll
+        for (int t = 0; t < NA; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(w1, from[(4 * t + i) * WAVE], acc[t][i] * w0);
+        m = M;
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
-  if (ks > 0 || !active || rtok >= qlen || (PACK && n >= 8)) return;
-  // ---- the end of a piece: bf16 out of a whole segment, or the fp32 partial of a cut one (as attend_blocks) ----
+  if (ks > 0 || !active || rtok >= qlen) return;
+  // ---- the end of a piece: bf16 out of a whole segment, or the fp32 partial of a cut one ----
   const Fp4AttnArgs& f = fresh_fp4();
   const AttnArgs& o = f.a;
   const int qt = tok + rtok, head = kvh * G + rh;
@@ -522,57 +661,75 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
     lse = NAN;
     l = 1.f;
 #pragma unroll
-    for (int t = 0; t < VT; ++t)
+    for (int t = 0; t < NA; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[t][i] = NAN;
   }
+  // x: the lane's consecutive channels from ch on. Not PACK: acc[t][i] is channel (D/4) g + (D/16) i + t. PACK: acc[t][i] is
+  // channel (D/4) g + (D/16) i + 2 t, or the one behind it in columns 8 .. 15: the row's two lanes exchange, and take i < 2
+  // and i >= 2.
+  constexpr int OPL = PACK ? D / 8 : D / 4;
+  float x[OPL];
+  int ch = (D / 4) * g;
+  if constexpr (PACK) {
+    const bool hi = n >= 8;
+    ch += hi ? D / 8 : 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int t = 0; t < NA; ++t) {
+        const float give = hi ? acc[t][i] : acc[t][i + 2], got = ror8(give), mine = hi ? acc[t][i + 2] : acc[t][i];
+        x[VT * i + 2 * t] = hi ? got : mine;
+        x[VT * i + 2 * t + 1] = hi ? mine : got;
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < VT; ++t) x[VT * i + t] = acc[t][i];
+  }
+  const bool first = g == 0 && (!PACK || n < 8);
   if (nparts == 1) {
-    if (g == 0) {
+    if (first) {
       if (o.max_splits > 1 && qt < o.cut_rows) o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh] = -1.f;
       if (f.lse) f.lse[(int64_t)qt * f.lse_st + head] = lse;
     }
     const float inv = l > 0.f ? 1.f / l : 0.f;
     uint32_t w[OPL / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int t = 0; t < VT; t += 2) w[(VT * i + t) / 2] = pack_bf16x2(acc[t][i] * inv, acc[t + 1][i] * inv);
-    u32x4* op = reinterpret_cast<u32x4*>(o.out + (int64_t)qt * o.o_st + (int64_t)head * o.o_sh + OPL * g);
+    for (int e = 0; e < OPL / 2; ++e) w[e] = pack_bf16x2(x[2 * e] * inv, x[2 * e + 1] * inv);
+    u32x4* op = reinterpret_cast<u32x4*>(o.out + (int64_t)qt * o.o_st + (int64_t)head * o.o_sh + ch);
 #pragma unroll
     for (int u = 0; u < OPL / 8; ++u) op[u] = u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
   } else {
     const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh + part;
-    if (g == 0) {
+    if (first) {
       o.segm_max[sidx] = m;
       o.segm_sum[sidx] = part == nparts - 1 ? last_piece_sum(l) : l;
     }
-    float* sp = o.segm_out + sidx * D + OPL * g;
+    float* sp = o.segm_out + sidx * D + ch;
 #pragma unroll
-    for (int u = 0; u < OPL / 4; ++u) {
-      const int c0 = 4 * u;
-      reinterpret_cast<float4*>(sp)[u] = float4{acc[(c0 + 0) % VT][(c0 + 0) / VT], acc[(c0 + 1) % VT][(c0 + 1) / VT],
-                                                acc[(c0 + 2) % VT][(c0 + 2) / VT], acc[(c0 + 3) % VT][(c0 + 3) / VT]};
-    }
+    for (int u = 0; u < OPL / 4; ++u)
+      reinterpret_cast<float4*>(sp)[u] = float4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
   }
 }
 
-template <int D, int PF, bool PACK>
-__global__ __launch_bounds__(256) void fp4_attn_kernel(Fp4AttnArgs args) {
+template <int D, bool PACK>
+__global__ __launch_bounds__(WAVE * FP4_WAVES) __attribute__((amdgpu_waves_per_eu(1, 2))) void fp4_attn_kernel(Fp4AttnArgs args) {
   touch_args();
   const AttnArgs& a = args.a;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int rt = a.rt, ksplit = a.ksplit, kspl = div_row_tiles(wave, rt), rtile = wave - kspl * rt;
-  extern __shared__ float merge_lds[];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t fp4_lds[];
+  uint8_t* ring = fp4_lds + wave * FP4_SLOTS * fp4_slot(D);
   int solo = 0;
   walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
     const int row0 = (rg * rt + rtile) * (PACK ? 8 : 16);
-    if (ksplit > 1 && c1 - c0 >= a.coop) {
-      attend_fp4<D, PF, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, kspl, ksplit, rtile, part, nparts, merge_lds, lane);
-    } else {
-      if (solo % ksplit == kspl)
-        attend_fp4<D, PF, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, 0, 1, rtile, part, nparts, merge_lds, lane);
-      ++solo;
-    }
+    // (a piece for all key splits, or a short one for one of them: one call, the code is long)
+    const bool all = ksplit > 1 && c1 - c0 >= a.coop;
+    if (all || solo % ksplit == kspl)
+      attend_fp4<D, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, all ? kspl : 0, all ? ksplit : 1, rtile, part, nparts, ring, lane);
+    if (!all) ++solo;
   });
 }
 
@@ -607,6 +764,7 @@ int check_fp4(const char* nm, int64_t num_blocks, int64_t block_size, int64_t he
     return fail("%s: scales must be 16-byte aligned (base pointers and strides)", nm);
   if (k_sn < 0 || v_sn < 0 || block_size * k_sn > INT32_MAX || block_size * v_sn > INT32_MAX)
     return fail("%s: page too large for 32-bit lane offsets", nm);
+  if ((k_sb | v_sb | s_sb) >> 32) return fail("%s: pages 4 GiB apart or more", nm);
   return 0;
 }
 
@@ -786,20 +944,23 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
     return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
   if (num_splits > 1 && segm_rows > 0 && (!segm_out || !segm_max || !segm_sum || !aligned16(segm_out)))
     return fail("%s: split buffers missing or not 16-byte aligned", nm);
+  if (k_sb != v_sb || k_sn != v_sn) return fail("%s: K and V caches must have the same page and slot strides", nm);
   const int G = (int)(num_q_heads / num_kv_heads);
   const int64_t maxq = std::min<int64_t>(std::max<int64_t>(max_query_len, 1), qmax), rows = (int64_t)G * maxq;
   if (rows > INT32_MAX / 4) return fail("%s: grid too large", nm);
-  // the row tile: 8 rows, both planes in one MFMA, where that holds all of a request's rows; else 16
+  // the row tile: 8 rows where that holds all of a request's rows; else 16
   const bool pack = rows <= 8;
   const int rt = (int)std::min<int64_t>(MAX_ROW_TILES, (rows + 15) / 16);
   const Tuning tune = read_tuning();
   const bool cut = num_splits > 1 && segm_rows > 0;
+  const int most = cut ? MAX_ROW_TILES : FP4_WAVES;
   const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
-                     : num_splits == 1 || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? MAX_ROW_TILES : DEFAULT_KSPLIT;
-  const int ks = std::max(1, std::min(ks_max, MAX_ROW_TILES / rt)), waves = rt * ks;
+                     : !cut || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? most : DEFAULT_KSPLIT;
+  const int ks = std::max(1, std::min(ks_max, most / rt)), waves = rt * ks;
   Fp4AttnArgs b;
   b.s = Fp4Scales{const_cast<uint8_t*>(k_scale), const_cast<uint8_t*>(v_scale), s_sb, s_sh};
   b.lse = lse; b.lse_st = lse_st;
+  b.apart = !(v_cache == k_cache + head_dim / 2 && k_sh == v_sh);
   AttnArgs& a = b.a;
   a.q = (const uint16_t*)q; a.kc = (const int8_t*)k_cache; a.vc = (const int8_t*)v_cache; a.out = (uint16_t*)out;
   a.segm_out = segm_out; a.segm_max = segm_max; a.segm_sum = segm_sum;
@@ -823,9 +984,9 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
                                        : (int)PLAN_FAST_MAX;
   a.seg_cost = seg_cost_units(tune, 0);
-  const size_t lds = (size_t)(ks - 1) * rt * MERGE_FIELDS * WAVE * sizeof(float);
-  void (*kern)(Fp4AttnArgs) = head_dim == 128 ? (pack ? fp4_attn_kernel<128, 3, true> : fp4_attn_kernel<128, 3, false>)
-                                              : (pack ? fp4_attn_kernel<64, 3, true> : fp4_attn_kernel<64, 3, false>);
+  const size_t lds = (size_t)waves * FP4_SLOTS * fp4_slot((int)head_dim);
+  void (*kern)(Fp4AttnArgs) = head_dim == 128 ? (pack ? fp4_attn_kernel<128, true> : fp4_attn_kernel<128, false>)
+                                              : (pack ? fp4_attn_kernel<64, true> : fp4_attn_kernel<64, false>);
   const int64_t tw = target_waves > 0 ? target_waves
                      : cut            ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
                                       : (int64_t)device_cus() * waves;
