@@ -70,43 +70,52 @@ __global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightA
       struct Tile {
         uint32_t k[2][D / 32];
         uint8_t ks[2];
+        float w;      // the running sum of the lane's key (lanes n < 8: key 16 (n / 4) + 4 g + n % 4 of the tile)
       };
+      const int own = 16 * (n >> 2) + 4 * g + (n & 3), count = n < 8 ? min(L, args.cols) : 0;
       auto load = [&](Tile& x, int c) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const int key = min(c * TILE + 16 * b, (L - 1) & ~15);
-          const int p = page_at(bt, 0, 0, key >> a.lbs), pg = p >= 0 && p < a.num_blocks ? p : 0, of = key & (bs - 1);
+          const int p = page_at(bt, 0, 0, key >> a.lbs), pg = (unsigned)p < (unsigned)a.num_blocks ? p : 0, of = key & (bs - 1);
           load_k16<D>(x.k[b], page_base(kbase, pg, (uint32_t)a.k_sb), koff, of * (uint32_t)a.k_sn);
           x.ks[b] = load_at<uint8_t>(page_base(sbase, pg, (uint32_t)args.s.sb), soff, of * SB);
         }
+        x.w = c * TILE + own < count ? wrow[c * TILE + own] : 0.f;
       };
-      Tile x;
-      for (int c = c0 + wave; c < c1; c += KW_WAVES) {
-        load(x, c);
-        // lanes n < 8 own key 16 (n / 4) + 4 g + n % 4 of the tile
-        const int own = c * TILE + 16 * (n >> 2) + 4 * g + (n & 3);
-        const bool mine = n < 8 && own < min(L, args.cols);
+      auto add = [&](const Tile& x, int c) {
         float sum[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+        f32x4 z[RT][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) fp4_scores<D, RT>(x.k[b], x.ks[b], q, b, z);
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const f32x4 z = fp4_scores<D>(x.k[b], x.ks[b], q[t]);
+          for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i], f[t], -l2[t]));
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][b][i], f[t], -l2[t]));
               sum[4 * b + i] += c * TILE + 16 * b + 4 * g + i < lim[t] ? p : 0.f;
             }
-          }
-        float add = 0.f;
+        float mine = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float s = sum_row(sum[i]);
-          add = n == i ? s : add;
+          mine = n == i ? s : mine;
         }
-        if (mine) wrow[own] += add;
+        if (c * TILE + own < count) wrow[c * TILE + own] = x.w + mine;
+      };
+      Tile ring[2];
+      int c = c0 + wave;
+      if (c < c1) load(ring[0], c);
+      for (; c < c1; c += 2 * KW_WAVES) {
+        if (c + KW_WAVES < c1) load(ring[1], c + KW_WAVES);
+        add(ring[0], c);
+        if (c + KW_WAVES >= c1) break;
+        if (c + 2 * KW_WAVES < c1) load(ring[0], c + 2 * KW_WAVES);
+        add(ring[1], c + KW_WAVES);
       }
     }
   });
@@ -115,8 +124,10 @@ __global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightA
 // ------------------------------------------------------------------------------------------------
 // One workgroup per (request, kv head) with n keys of which it may hold m = keep < n. Kept: the last min(recent, m), and of the
 // rest those of the m - recent largest sums, ties to the lowest position.
-//   select   the sum at which the count is reached, by three histograms of 12, 12 and 8 bits of its ordered bits
-//   list     the kept positions in order: a wavefront's share of the positions is counted, then written behind those before it
+//   select   the sum at which the count is reached, by histograms of 12, 12 and 8 bits of its ordered bits; done as soon as a bin
+//            is taken whole, with sums that differ after the second
+//   list     the kept positions in order: a wavefront compares its share of the positions, 64 at a time, and lane u keeps the
+//            64 answers of the u-th; so counts, ties and places are a scan over lanes and one over wavefronts
 //   move     row i takes the row of the i-th kept position, which is i or later: rows are read into registers, in order, a
 //            batch at a time, and written after a barrier, so that nothing is overwritten that is still to be read
 // ------------------------------------------------------------------------------------------------
@@ -135,7 +146,11 @@ struct EvictArgs {
 };
 constexpr int EV_THREADS = 1024, EV_WAVES = EV_THREADS / WAVE;
 constexpr int EV_BINS = 4096;
-constexpr int EV_ROWS = 4;   // rows that a thread holds of a batch
+constexpr int EV_ROWS = 4;      // rows that a thread holds of a batch
+constexpr int EV_AHEAD = 8;     // sums that a thread asks for at once
+constexpr int EV_LIST = 4096;   // kept positions that are in LDS as well
+constexpr int EV_PAGES = 4096;  // page ids that are in LDS as well
+constexpr int EV_BLOCKS = WAVE; // blocks of 64 positions whose answers a wavefront holds
 
 // order of the sums as unsigned numbers: NaN the largest, -0 as 0
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -147,7 +162,8 @@ template <int D>
 __global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
   constexpr int SB = D / FP4_GROUP, CH = D / 32;   // exponent bytes, 16-byte chunks of a row's codes
   __shared__ uint32_t bins[EV_BINS];
-  __shared__ uint32_t wsum[EV_WAVES], wsum2[EV_WAVES];
+  __shared__ int list[EV_LIST], pages[EV_PAGES];
+  __shared__ uint32_t wsum[2][EV_WAVES];
   __shared__ uint32_t found[3];
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int r = blockIdx.x / a.heads, h = blockIdx.x - r * a.heads;
@@ -161,88 +177,141 @@ __global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
     for (int i = tid; i < n; i += EV_THREADS) kept[i] = i;
     return;
   }
+  const int used = min((n + (1 << a.lbs) - 1) >> a.lbs, EV_PAGES);
+  for (int i = tid; i < used; i += EV_THREADS) pages[i] = bt[i];
   const int recent = min(a.recent, m), c = n - recent, need = m - recent;   // candidates: positions 0 .. c - 1; need < c
+  // the lanes' sums at from + lane: a descriptor that ends with them, so that what lies behind reads as 0
+  const auto desc = __builtin_amdgcn_make_buffer_rsrc(w, 0, 4 * min(c, a.cols), QC_RSRC_WORD3);
   auto sum_at = [&](int i) { return i < a.cols ? w[i] : 0.f; };
+  // f(number of the block, its first position, the lane's key) for the blocks of 64 positions from, from + step, .. below end,
+  // several loads under way; whole wavefronts
+  auto walk = [&](int from, int end, int step, auto&& f) {
+    for (int i0 = from, k = 0; i0 < end; i0 += EV_AHEAD * step, k += EV_AHEAD) {
+      float x[EV_AHEAD];
+#pragma unroll
+      for (int u = 0; u < EV_AHEAD; ++u)
+        x[u] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(desc, 4 * (i0 + u * step + lane), 0, 0));
+#pragma unroll
+      for (int u = 0; u < EV_AHEAD; ++u)
+        if (i0 + u * step < end) f(k + u, i0 + u * step, ordered(x[u]));
+    }
+  };
+  // sum of the wavefronts' numbers before this one's
+  auto before = [&](uint32_t x, int k) {
+    if (lane == 0) wsum[k][wave] = x;
+    __syncthreads();
+    const int incl = wave_incl_sum(lane < EV_WAVES ? (int)wsum[k][lane] : 0);
+    return wave ? (uint32_t)__builtin_amdgcn_readlane(incl, wave - 1) : 0u;
+  };
   // ---- select ----
   uint32_t edge = 0xffffffffu;   // keys above it are kept, and `ties` of those equal to it
   int ties = 0;
   if (need > 0) {
     uint32_t prefix = 0;
     int left = need;   // still to be found at or below the current bin
+    bool whole = false;
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 20 : pass == 1 ? 8 : 0, nb = pass == 2 ? 256 : EV_BINS;
       const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xfff00000u : 0xffffff00u;
       for (int i = tid; i < nb; i += EV_THREADS) bins[i] = 0;
       __syncthreads();
-      for (int i = tid; i < c; i += EV_THREADS) {
-        const uint32_t key = ordered(sum_at(i));
-        if ((key & mask) == prefix) atomicAdd(&bins[(key >> shift) & (nb - 1)], 1u);
-      }
+      walk(wave * WAVE, c, EV_THREADS, [&](int, int i0, uint32_t key) {
+        const bool in = i0 + lane < c && (key & mask) == prefix;
+        const uint64_t all = __ballot(in);
+        if (all == 0) return;
+        // (many alike, zeros of keys that were never looked at: one addition for those of the first lane's bin)
+        const int bin = (key >> shift) & (nb - 1), lead = __builtin_ctzll(all), one = __builtin_amdgcn_readlane(bin, lead);
+        const uint64_t same = __ballot(in && bin == one);
+        if (lane == lead) atomicAdd(&bins[bin], (uint32_t)__builtin_popcountll(same));
+        else if (in && bin != one) atomicAdd(&bins[bin], 1u);
+      });
       __syncthreads();
-      // the bin, counted from the largest, where the count reaches `left`
-      const int per = nb / EV_THREADS > 0 ? nb / EV_THREADS : 1;   // bins per thread, from the top
+      // the bin, counted from the largest, where the count reaches `left`: a thread has `per` bins
+      const int per = nb / EV_THREADS > 0 ? nb / EV_THREADS : 1, top = nb - 1 - tid * per;
       uint32_t own = 0;
-      const int top = nb - 1 - tid * per;
       if (top >= 0)
         for (int i = 0; i < per; ++i) own += bins[top - i];
       uint32_t incl = (uint32_t)wave_incl_sum((int)own);
-      if (lane == WAVE - 1) wsum[wave] = incl;
-      __syncthreads();
-      for (int k = 0; k < wave; ++k) incl += wsum[k];
+      incl += before((uint32_t)__builtin_amdgcn_readlane((int)incl, WAVE - 1), pass & 1);
       if (top >= 0 && (int)incl >= left && (int)(incl - own) < left) {
-        uint32_t before = incl - own;
+        uint32_t done = incl - own;
         int b = top;
-        while ((int)(before + bins[b]) < left) before += bins[b--];
+        while ((int)(done + bins[b]) < left) done += bins[b--];
         found[0] = (uint32_t)b;
-        found[1] = before;
+        found[1] = done;
+        found[2] = bins[b];
       }
       __syncthreads();
       prefix |= found[0] << shift;
       left -= (int)found[1];
-      __syncthreads();
+      whole = (uint32_t)left == found[2];
+      if (whole) break;
     }
-    edge = prefix;
-    ties = left;
+    // a bin taken whole: every key from its first on; one number alone (the last pass): `left` of its ties
+    edge = whole ? prefix - 1 : prefix;   // (prefix is not 0: a key is at least ordered(-inf))
+    ties = whole ? 0 : left;
   }
-  // ---- list: wavefront k has the positions [k, k + 1) * share ----
-  const int share = ((n + EV_WAVES - 1) / EV_WAVES + WAVE - 1) / WAVE * WAVE;
-  const int from = min(wave * share, n), to = min(from + share, n);
-  auto above = [&](int i, uint32_t key) { return i >= c || (need > 0 && key > edge); };
-  auto equal = [&](int i, uint32_t key) { return i < c && need > 0 && key == edge; };
+  // ---- list: wavefront k has the candidates [k, k + 1) * share ----
+  const int share = ((c + EV_WAVES - 1) / EV_WAVES + WAVE - 1) / WAVE * WAVE;
+  const int from = min(wave * share, c), to = min(from + share, c);
+  uint64_t ab = 0, em = 0;   // lane u's: which positions of block u are above the edge, or at it
+  auto compare = [&](int i0, int end) {
+    ab = em = 0;
+    walk(i0, end, WAVE, [&](int k, int p0, uint32_t key) {
+      const bool in = p0 + lane < end;
+      const uint64_t x = __ballot(in && key > edge), y = ties ? __ballot(in && key == edge) : 0ull;
+      ab = lane == k ? x : ab;
+      em = lane == k ? y : em;
+    });
+  };
+  constexpr int SPAN = EV_BLOCKS * WAVE;   // positions whose answers fit
   uint32_t cnt = 0, eq = 0;
-  for (int i0 = from; i0 < to; i0 += WAVE) {
-    const int i = i0 + lane;
-    const uint32_t key = i < min(to, c) ? ordered(sum_at(i)) : 0u;
-    cnt += __builtin_popcountll(__ballot(i < to && above(i, key)));
-    eq += __builtin_popcountll(__ballot(i < to && equal(i, key)));
-  }
-  if (lane == 0) {
-    wsum[wave] = cnt;
-    wsum2[wave] = eq;
-  }
-  __syncthreads();
-  uint32_t at = 0, eq_at = 0;
-  for (int k = 0; k < wave; ++k) {
-    at += wsum[k];
-    eq_at += wsum2[k];
-  }
-  for (int i0 = from; i0 < to; i0 += WAVE) {
-    const int i = i0 + lane;
-    const uint32_t key = i < min(to, c) ? ordered(sum_at(i)) : 0u;
-    const uint64_t ab = __ballot(i < to && above(i, key)), em = __ballot(i < to && equal(i, key));
-    const uint64_t below = (1ull << lane) - 1;
-    const uint32_t e = eq_at + __builtin_popcountll(em & below);   // ties before this position
-    const bool tie = (em >> lane & 1) && (int)e < ties;
-    const uint32_t to_at = at + __builtin_popcountll(ab & below) + min(e, (uint32_t)ties);
-    if ((ab >> lane & 1) || tie) kept[to_at] = i;
-    at += __builtin_popcountll(ab);
-    eq_at += __builtin_popcountll(em);
+  if (need > 0)
+    for (int i0 = from; i0 < to; i0 += SPAN) {
+      compare(i0, min(i0 + SPAN, to));
+      cnt += __builtin_popcountll(ab);
+      eq += __builtin_popcountll(em);
+    }
+  cnt = (uint32_t)__builtin_amdgcn_readlane(wave_incl_sum((int)cnt), WAVE - 1);
+  eq = (uint32_t)__builtin_amdgcn_readlane(wave_incl_sum((int)eq), WAVE - 1);
+  __syncthreads();   // (the last pass's numbers have been read)
+  uint32_t at = before(cnt, 0), eq_at = before(eq, 1);
+  at += min(eq_at, (uint32_t)ties);
+  if (need > 0)
+    for (int i0 = from; i0 < to; i0 += SPAN) {
+      const int end = min(i0 + SPAN, to);
+      if (to - from > SPAN) compare(i0, end);   // (else they are here)
+      // of the positions at the edge, those before the `ties`-th
+      const int e = __builtin_popcountll(em), e_incl = wave_incl_sum(e);
+      int take = min(max(ties - (int)eq_at - (e_incl - e), 0), e);
+      uint64_t rest = em;
+      if (take < e)
+        for (; take > 0; --take) rest &= rest - 1;
+      else
+        rest = 0;
+      const uint64_t chosen = ab | (em & ~rest);
+      const int num = __builtin_popcountll(chosen), incl = wave_incl_sum(num), first = (int)at + incl - num;
+      for (int u = 0; u * WAVE < end - i0; ++u) {
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)chosen, u), hi = __builtin_amdgcn_readlane((int)(uint32_t)(chosen >> 32), u);
+        const int slot = __builtin_amdgcn_readlane(first, u) + (int)__builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+        if ((lane < 32 ? lo >> lane : hi >> (lane - 32)) & 1) {
+          const int i = i0 + u * WAVE + lane;
+          kept[slot] = i;
+          if (slot < EV_LIST) list[slot] = i;
+        }
+      }
+      at += (uint32_t)__builtin_amdgcn_readlane(incl, WAVE - 1);
+      eq_at += (uint32_t)__builtin_amdgcn_readlane(e_incl, WAVE - 1);
+    }
+  for (int i = tid; i < recent; i += EV_THREADS) {
+    kept[need + i] = c + i;
+    if (need + i < EV_LIST) list[need + i] = c + i;
   }
   __threadfence_block();
   __syncthreads();
   // ---- move ----
-  auto page = [&](int i) { return bt[i >> a.lbs]; };
+  auto page = [&](int i) { return (i >> a.lbs) < EV_PAGES ? pages[i >> a.lbs] : bt[i >> a.lbs]; };
   auto good = [&](int p) { return p >= 0 && p < a.num_blocks; };
   const int bs = 1 << a.lbs;
   constexpr int LPR = 2 * CH, RPB = EV_THREADS / LPR;   // lanes per row (K's chunks, then V's), rows per batch step
@@ -259,7 +328,7 @@ __global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
 #pragma unroll
     for (int u = 0; u < EV_ROWS; ++u) {
       const int i = b0 + u * RPB + row;
-      src[u] = i < m ? kept[i] : -1;
+      src[u] = i >= m ? -1 : i < EV_LIST ? list[i] : kept[i];
       byte[u] = 0;
       sum[u] = 0.f;
       code[u] = i32x4{0, 0, 0, 0};
@@ -360,6 +429,7 @@ int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, ui
                                v_sh, k_scale, v_scale, s_sb, s_sh)) return rc;
   if (!seq_lens || !keep || !new_lens || (bt_cols && !block_table) || (w_cols && !weights) || (kept_cols && !kept))
     return fail("%s: null pointer", nm);
+  if (bt_cols > (1 << 28) / block_size) return fail("%s: tables of more than 2^28 slots", nm);   // (32-bit byte offsets)
   if (num_seqs > INT32_MAX / num_heads) return fail("%s: too many requests and heads for one call", nm);
   EvictArgs a;
   a.kc = k_cache; a.vc = v_cache; a.s = Fp4Scales{k_scale, v_scale, s_sb, s_sh}; a.w = weights;

@@ -263,16 +263,18 @@ struct Fp4Query {
     odd = group4_sum(odd);
   }
 };
-// S^T[key][row] of 16 keys: lane (n, g) holds row n's keys 4 g + i
-template <int D>
-__device__ __forceinline__ f32x4 fp4_scores(const uint32_t (&k)[D / 32], uint32_t byte, const Fp4Query<D>& q) {
-  f32x4 z = {0.f, 0.f, 0.f, 0.f};
+// S^T[key][row] of 16 keys and NR row tiles: lane (n, g) holds row n's keys 4 g + i. The keys are converted once.
+template <int D, int NR>
+__device__ __forceinline__ void fp4_scores(const uint32_t (&k)[D / 32], uint32_t byte, const Fp4Query<D> (&q)[NR], int b, f32x4 (&z)[NR][2]) {
+#pragma unroll
+  for (int t = 0; t < NR; ++t) z[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
     const u32x4 w = fp4_to_bf16(k[s], byte);
-    z = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&w), q.op[s], z, 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+      z[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&w), q[t].op[s], z[t][b], 0, 0, 0);
   }
-  return z;
 }
 // A streaming load of each lane's own `off` from a base that the wavefront shares, through a buffer descriptor: the base and
 // `uni` stay in scalar registers, a lane's part is 32 bits (as 64-bit addresses they took two vector registers and an addition
@@ -314,12 +316,14 @@ __device__ __forceinline__ int fp4_place(bool apart, int r, int p) {
   return apart ? (p / H) * 16 * H + r * H + ((p % H) ^ ((r * H / 4) & (H - 1))) : r * CH + (p ^ (r & (CH - 1)));
 }
 
-template <int D, bool PACK>
+// One wavefront's share of a piece: NR row tiles from row0 on, key tiles c_begin + ks, c_begin + ks + KS, .. below c_end.
+template <int D, bool PACK, int NR>
 __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqlen, int kvh, int row0, int c_begin, int c_end,
-                                           int ks, int KS, int rtile, int part, int nparts, uint8_t* lds, int lane) {
+                                           int ks, int KS, int part, int nparts, uint8_t* lds, int lane) {
   const Fp4AttnArgs& args = fresh_fp4();
   const AttnArgs& a = args.a;
-  constexpr int RT = PACK ? 8 : 16;        // rows of this wavefront's tile
+  constexpr int RT = PACK ? 8 : 16;        // rows of a tile
+  static_assert(!PACK || NR == 1, "at most 8 rows are one tile");
   constexpr int VT = D / 16, NA = fp4_accs(D, PACK), SB = D / FP4_GROUP;
   constexpr int S = FP4_SLOTS, SLOT = fp4_slot(D), HALF = fp4_half(D), CODES = fp4_codes(D), CH = fp4_chunks(D);
   constexpr int DMAS = CODES / 1024, OPS = 2 * (DMAS + 1);   // DMAs of a half's codes; vector memory operations of a tile
@@ -348,10 +352,20 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   const int bs = 1 << lbs;
   auto div_g = [&](int x) { return G == 1 ? x : a.g_inv ? (int)__umulhi((unsigned)x, a.g_inv) : x / G; };
 
-  const int R = row0 + (n & (RT - 1)), rtok = div_g(R), rh = R - rtok * G;
+  int rtok[NR], rh[NR];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    const int R = row0 + RT * t + (n & (RT - 1));
+    rtok[t] = div_g(R);
+    rh[t] = R - rtok[t] * G;
+  }
   const int lim_lo = L - qlen + 1 + __builtin_amdgcn_readfirstlane(div_g(row0));
-  Fp4Query<D> q;
-  if (nt > 0) q.load(a.q + (int64_t)(tok + min(rtok, qlen - 1)) * a.q_st + (int64_t)(kvh * G + rh) * a.q_sh, rtok < qlen, g);
+  Fp4Query<D> q[NR];
+  if (nt > 0) {
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+      q[t].load(a.q + (int64_t)(tok + min(rtok[t], qlen - 1)) * a.q_st + (int64_t)(kvh * G + rh[t]) * a.q_sh, rtok[t] < qlen, g);
+  }
 
   // ---- what each lane's DMAs ask for, beside a page and slot, and where it reads ----
   const bool apart = args.apart;
@@ -416,18 +430,25 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
         load(j, j);
         fetch(j + 1);
       }
-    q.make();
-  } else {
-    q.odd = 0.f;
-  }
-  const float rs = a.sm_log2 + q.odd;
-  const int lim = rtok < qlen ? L - qlen + 1 + rtok : L;
-  const uint32_t pshift = PACK && n >= 8 ? 16 : 0;   // PACK: where the column's weights stand beside zeros
-
-  float m = -1e30f, l = 0.f;
-  f32x4 acc[NA];
 #pragma unroll
-  for (int t = 0; t < NA; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NR; ++t) q[t].make();
+  } else {
+#pragma unroll
+    for (int t = 0; t < NR; ++t) q[t].odd = 0.f;
+  }
+  float rs[NR], m[NR], l[NR];
+  int lim[NR];
+  f32x4 acc[NR][NA];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    rs[t] = a.sm_log2 + q[t].odd;
+    lim[t] = rtok[t] < qlen ? L - qlen + 1 + rtok[t] : L;
+    m[t] = -1e30f;
+    l[t] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NA; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t pshift = PACK && n >= 8 ? 16 : 0;   // PACK: where the column's weights stand beside zeros
 
   // tile j in `slot`; vm: this wavefront's vector memory operations behind the tile's own (the reads' statements wait for
   // themselves: the compiler sees neither the DMAs nor that they are done)
@@ -458,13 +479,9 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       }
     }
     // ---- scores; key of (b, i) = n0 + 16 b + 4 g + i ----
-    f32x4 z[2];
-    bool ok[2][4];
-    float tmax = -INFINITY;
+    f32x4 z[NR][2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      z[b] = fp4_scores<D>(kw[b], ksw[b], q);
-    }
+    for (int b = 0; b < 2; ++b) fp4_scores<D, NR>(kw[b], ksw[b], q, b, z);
     if constexpr (D == 128) {   // (while the products run)
       u32x4 x0, x1;
       asm volatile("ds_read_b32 %0, %10 offset:%c15\n\tds_read_b32 %1, %11 offset:%c15\n\tds_read_b32 %2, %12 offset:%c15\n\t"
@@ -495,33 +512,37 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       }
     }
     fetch(j + S);   // (here: the statements above wait for every scalar load as well)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ok[b][i] = MASKED ? n0 + 16 * b + 4 * g + i < lim : true;
-        tmax = ok[b][i] ? __builtin_fmaxf(tmax, z[b][i]) : tmax;
-      }
-    }
     // ---- online softmax ----
-    tmax = __builtin_fmaf(group4_fmax(tmax), rs, BLOCK_REF);   // the reference that this tile asks for
-    const bool raise = tmax > m + ATTN_SLACK;
-    const float mnew = raise ? tmax : m;
-    const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-    m = mnew;
-    float p[2][4];
-    l *= alpha;
+    float p[NR][2][4];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int t = 0; t < NR; ++t) {
+      bool ok[2][4];
+      float tmax = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[b][i], rs, -mnew));
-        if (MASKED) p[b][i] = ok[b][i] ? p[b][i] : 0.f;
-        l += p[b][i];
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          ok[b][i] = MASKED ? n0 + 16 * b + 4 * g + i < lim[t] : true;
+          tmax = ok[b][i] ? __builtin_fmaxf(tmax, z[t][b][i]) : tmax;
+        }
+      tmax = __builtin_fmaf(group4_fmax(tmax), rs[t], BLOCK_REF);   // the reference that this tile asks for
+      const bool raise = tmax > m[t] + ATTN_SLACK;
+      const float mnew = raise ? tmax : m[t];
+      const float alpha = __builtin_amdgcn_exp2f(m[t] - mnew);
+      m[t] = mnew;
+      l[t] *= alpha;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[t][b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[t][b][i], rs[t], -mnew));
+          if (MASKED) p[t][b][i] = ok[b][i] ? p[t][b][i] : 0.f;
+          l[t] += p[t][b][i];
+        }
+      if (__any(raise)) {
+#pragma unroll
+        for (int c = 0; c < NA; ++c) acc[t][c] *= alpha;
       }
-    if (__any(raise)) {
-#pragma unroll
-      for (int t = 0; t < NA; ++t) acc[t] *= alpha;
     }
     // ---- PV: O^T[channel][row] += V^T . P^T ----
     float vsc[8];
@@ -538,7 +559,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pw[b][i] = pack_bf16x2_rne(p[b][i], 0.f) << pshift;
+        for (int i = 0; i < 4; ++i) pw[b][i] = pack_bf16x2_rne(p[0][b][i], 0.f) << pshift;
       auto pair = [&](auto byte_t) {   // the channels 2 B and 2 B + 1 of the lane's
         constexpr int B = decltype(byte_t)::value;
 #pragma unroll
@@ -547,8 +568,8 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[4 * b + i], vsc[4 * b + i], B));
-          acc[B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&w), *reinterpret_cast<bf16x8*>(&pw[b]),
-                                                           acc[B], 0, 0, 0);
+          acc[0][B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&w), *reinterpret_cast<bf16x8*>(&pw[b]),
+                                                              acc[0][B], 0, 0, 0);
         }
       };
       pair(std::integral_constant<int, 0>{});
@@ -558,9 +579,13 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
         pair(std::integral_constant<int, 3>{});
       }
     } else {
-      u32x4 pw = {pack_bf16x2_rne(p[0][0], p[0][1]), pack_bf16x2_rne(p[0][2], p[0][3]), pack_bf16x2_rne(p[1][0], p[1][1]),
-                  pack_bf16x2_rne(p[1][2], p[1][3])};
-      const bf16x8 pop = *reinterpret_cast<bf16x8*>(&pw);   // the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i
+      bf16x8 pop[NR];   // the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        u32x4 pw = {pack_bf16x2_rne(p[t][0][0], p[t][0][1]), pack_bf16x2_rne(p[t][0][2], p[t][0][3]),
+                    pack_bf16x2_rne(p[t][1][0], p[t][1][1]), pack_bf16x2_rne(p[t][1][2], p[t][1][3])};
+        pop[t] = *reinterpret_cast<bf16x8*>(&pw);
+      }
       auto pair = [&](auto byte_t) {
         constexpr int B = decltype(byte_t)::value;
         uint32_t w[8];
@@ -572,8 +597,11 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
           even[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100u);
           odd[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
         }
-        acc[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), pop, acc[2 * B], 0, 0, 0);
-        acc[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), pop, acc[2 * B + 1], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+          acc[t][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), pop[t], acc[t][2 * B], 0, 0, 0);
+          acc[t][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), pop[t], acc[t][2 * B + 1], 0, 0, 0);
+        }
       };
       pair(std::integral_constant<int, 0>{});
       pair(std::integral_constant<int, 1>{});
@@ -620,115 +648,125 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   }
 
   // ---- the key splits' merge, half of them into the other half at a time ----
-  l = group4_sum(l);
+#pragma unroll
+  for (int t = 0; t < NR; ++t) l[t] = group4_sum(l[t]);
   if (KS > 1) {
     // (each wavefront hands over in its own ring, which is done with)
-    static_assert(fp4_merge_fields(D, PACK) * WAVE * 4 <= S * SLOT, "merge fields in the ring");
-    auto mem = [&](int k) { return reinterpret_cast<float*>(lds + (k - ks) * a.rt * S * SLOT) + lane; };
+    constexpr int FIELDS = fp4_merge_fields(D, PACK);
+    static_assert(NR * FIELDS * WAVE * 4 <= S * SLOT, "merge fields in the ring");
+    auto mem = [&](int k) { return reinterpret_cast<float*>(lds + (k - ks) * (a.rt / NR) * S * SLOT) + lane; };
     for (int half = KS, width = KS; width > 1; width = half) {
       half = (width + 1) / 2;
       if (active && ks >= half && ks < width) {
         float* to = mem(ks);
 #pragma unroll
-        for (int t = 0; t < NA; ++t)
+        for (int t = 0; t < NR; ++t, to += FIELDS * WAVE) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) to[(4 * t + i) * WAVE] = acc[t][i];
-        to[(4 * NA) * WAVE] = m;
-        to[(4 * NA + 1) * WAVE] = l;
+          for (int c = 0; c < NA; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[(4 * c + i) * WAVE] = acc[t][c][i];
+          to[(4 * NA) * WAVE] = m[t];
+          to[(4 * NA + 1) * WAVE] = l[t];
+        }
       }
       __syncthreads();
       if (active && ks + half < width) {
         const float* from = mem(ks + half);
-        const float mo = from[(4 * NA) * WAVE], M = __builtin_fmaxf(m, mo);
-        const float w0 = __builtin_amdgcn_exp2f(m - M), w1 = __builtin_amdgcn_exp2f(mo - M);
-        l = __builtin_fmaf(w1, from[(4 * NA + 1) * WAVE], l * w0);
 #pragma unroll
-        for (int t = 0; t < NA; ++t)
+        for (int t = 0; t < NR; ++t, from += FIELDS * WAVE) {
+          const float mo = from[(4 * NA) * WAVE], M = __builtin_fmaxf(m[t], mo);
+          const float w0 = __builtin_amdgcn_exp2f(m[t] - M), w1 = __builtin_amdgcn_exp2f(mo - M);
+          l[t] = __builtin_fmaf(w1, from[(4 * NA + 1) * WAVE], l[t] * w0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(w1, from[(4 * t + i) * WAVE], acc[t][i] * w0);
-        m = M;
+          for (int c = 0; c < NA; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][c][i] = __builtin_fmaf(w1, from[(4 * c + i) * WAVE], acc[t][c][i] * w0);
+          m[t] = M;
+        }
       }
       __syncthreads();
     }
   }
-  if (ks > 0 || !active || rtok >= qlen) return;
+  if (ks > 0 || !active) return;
   // ---- the end of a piece: bf16 out of a whole segment, or the fp32 partial of a cut one ----
   const Fp4AttnArgs& f = fresh_fp4();
   const AttnArgs& o = f.a;
-  const int qt = tok + rtok, head = kvh * G + rh;
-  float lse = __builtin_fmaf(m, LN2, __builtin_amdgcn_logf(l) * LN2);
-  if (l != l) {   // (a denominator that is no number would not tell the merge that the row was cut)
-    lse = NAN;
-    l = 1.f;
 #pragma unroll
-    for (int t = 0; t < NA; ++t)
+  for (int t = 0; t < NR; ++t) {
+    // x: the lane's consecutive channels from ch on. Not PACK: acc[c][i] is channel (D/4) g + (D/16) i + c. PACK: acc[c][i] is
+    // channel (D/4) g + (D/16) i + 2 c, or the one behind it in columns 8 .. 15: the row's two lanes exchange, and take i < 2
+    // and i >= 2.
+    constexpr int OPL = PACK ? D / 8 : D / 4;
+    float x[OPL];
+    int ch = (D / 4) * g;
+    if constexpr (PACK) {
+      const bool hi = n >= 8;
+      ch += hi ? D / 8 : 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = NAN;
-  }
-  // x: the lane's consecutive channels from ch on. Not PACK: acc[t][i] is channel (D/4) g + (D/16) i + t. PACK: acc[t][i] is
-  // channel (D/4) g + (D/16) i + 2 t, or the one behind it in columns 8 .. 15: the row's two lanes exchange, and take i < 2
-  // and i >= 2.
-  constexpr int OPL = PACK ? D / 8 : D / 4;
-  float x[OPL];
-  int ch = (D / 4) * g;
-  if constexpr (PACK) {
-    const bool hi = n >= 8;
-    ch += hi ? D / 8 : 0;
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int c = 0; c < NA; ++c) {
+          const float give = hi ? acc[t][c][i] : acc[t][c][i + 2], got = ror8(give), mine = hi ? acc[t][c][i + 2] : acc[t][c][i];
+          x[VT * i + 2 * c] = hi ? got : mine;
+          x[VT * i + 2 * c + 1] = hi ? mine : got;
+        }
+    } else {
 #pragma unroll
-      for (int t = 0; t < NA; ++t) {
-        const float give = hi ? acc[t][i] : acc[t][i + 2], got = ror8(give), mine = hi ? acc[t][i + 2] : acc[t][i];
-        x[VT * i + 2 * t] = hi ? got : mine;
-        x[VT * i + 2 * t + 1] = hi ? mine : got;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < VT; ++c) x[VT * i + c] = acc[t][c][i];
+    }
+    if (rtok[t] >= qlen) continue;
+    const int qt = tok + rtok[t], head = kvh * G + rh[t];
+    float lse = __builtin_fmaf(m[t], LN2, __builtin_amdgcn_logf(l[t]) * LN2);
+    if (l[t] != l[t]) {   // (a denominator that is no number would not tell the merge that the row was cut)
+      lse = NAN;
+      l[t] = 1.f;
+#pragma unroll
+      for (int e = 0; e < OPL; ++e) x[e] = NAN;
+    }
+    const bool first = g == 0 && (!PACK || n < 8);
+    if (nparts == 1) {
+      if (first) {
+        if (o.max_splits > 1 && qt < o.cut_rows) o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh] = -1.f;
+        if (f.lse) f.lse[(int64_t)qt * f.lse_st + head] = lse;
       }
-  } else {
+      const float inv = l[t] > 0.f ? 1.f / l[t] : 0.f;
+      uint32_t w[OPL / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int e = 0; e < OPL / 2; ++e) w[e] = pack_bf16x2_rne(x[2 * e] * inv, x[2 * e + 1] * inv);
+      u32x4* op = reinterpret_cast<u32x4*>(o.out + (int64_t)qt * o.o_st + (int64_t)head * o.o_sh + ch);
 #pragma unroll
-      for (int t = 0; t < VT; ++t) x[VT * i + t] = acc[t][i];
-  }
-  const bool first = g == 0 && (!PACK || n < 8);
-  if (nparts == 1) {
-    if (first) {
-      if (o.max_splits > 1 && qt < o.cut_rows) o.segm_sum[(int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh] = -1.f;
-      if (f.lse) f.lse[(int64_t)qt * f.lse_st + head] = lse;
+      for (int u = 0; u < OPL / 8; ++u) op[u] = u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
+    } else {
+      const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh + part;
+      if (first) {
+        o.segm_max[sidx] = m[t];
+        o.segm_sum[sidx] = part == nparts - 1 ? last_piece_sum(l[t]) : l[t];
+      }
+      float* sp = o.segm_out + sidx * D + ch;
+#pragma unroll
+      for (int u = 0; u < OPL / 4; ++u)
+        reinterpret_cast<float4*>(sp)[u] = float4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    uint32_t w[OPL / 2];
-#pragma unroll
-    for (int e = 0; e < OPL / 2; ++e) w[e] = pack_bf16x2(x[2 * e] * inv, x[2 * e + 1] * inv);
-    u32x4* op = reinterpret_cast<u32x4*>(o.out + (int64_t)qt * o.o_st + (int64_t)head * o.o_sh + ch);
-#pragma unroll
-    for (int u = 0; u < OPL / 8; ++u) op[u] = u32x4{w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]};
-  } else {
-    const int64_t sidx = (int64_t)qt * o.seg_st + (int64_t)head * o.seg_sh + part;
-    if (first) {
-      o.segm_max[sidx] = m;
-      o.segm_sum[sidx] = part == nparts - 1 ? last_piece_sum(l) : l;
-    }
-    float* sp = o.segm_out + sidx * D + ch;
-#pragma unroll
-    for (int u = 0; u < OPL / 4; ++u)
-      reinterpret_cast<float4*>(sp)[u] = float4{x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]};
   }
 }
 
-template <int D, bool PACK>
+template <int D, bool PACK, int NR>
 __global__ __launch_bounds__(WAVE * FP4_WAVES) __attribute__((amdgpu_waves_per_eu(1, 2))) void fp4_attn_kernel(Fp4AttnArgs args) {
   touch_args();
   const AttnArgs& a = args.a;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int rt = a.rt, ksplit = a.ksplit, kspl = div_row_tiles(wave, rt), rtile = wave - kspl * rt;
+  const int rw = a.rt / NR, ksplit = a.ksplit, kspl = wave / rw, rtile = NR * (wave - kspl * rw);
   extern __shared__ __attribute__((aligned(1024))) uint8_t fp4_lds[];
   uint8_t* ring = fp4_lds + wave * FP4_SLOTS * fp4_slot(D);
   int solo = 0;
   walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
-    const int row0 = (rg * rt + rtile) * (PACK ? 8 : 16);
+    const int row0 = (rg * a.rt + rtile) * (PACK ? 8 : 16);
     // (a piece for all key splits, or a short one for one of them: one call, the code is long)
     const bool all = ksplit > 1 && c1 - c0 >= a.coop;
     if (all || solo % ksplit == kspl)
-      attend_fp4<D, PACK>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, all ? kspl : 0, all ? ksplit : 1, rtile, part, nparts, ring, lane);
+      attend_fp4<D, PACK, NR>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, all ? kspl : 0, all ? ksplit : 1, part, nparts, ring, lane);
     if (!all) ++solo;
   });
 }
@@ -950,13 +988,15 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   if (rows > INT32_MAX / 4) return fail("%s: grid too large", nm);
   // the row tile: 8 rows where that holds all of a request's rows; else 16
   const bool pack = rows <= 8;
-  const int rt = (int)std::min<int64_t>(MAX_ROW_TILES, (rows + 15) / 16);
+  // a wavefront takes one row tile or, of more rows than one tile holds, two: it converts a tile's keys once for both
+  const int nr = rows <= 16 ? 1 : 2;
+  const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : MAX_ROW_TILES, rw = rt / nr;
   const Tuning tune = read_tuning();
   const bool cut = num_splits > 1 && segm_rows > 0;
   const int most = cut ? MAX_ROW_TILES : FP4_WAVES;
   const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
                      : !cut || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? most : DEFAULT_KSPLIT;
-  const int ks = std::max(1, std::min(ks_max, most / rt)), waves = rt * ks;
+  const int ks = std::max(1, std::min(ks_max, most / rw)), waves = rw * ks;
   Fp4AttnArgs b;
   b.s = Fp4Scales{const_cast<uint8_t*>(k_scale), const_cast<uint8_t*>(v_scale), s_sb, s_sh};
   b.lse = lse; b.lse_st = lse_st;
@@ -985,8 +1025,9 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
                                        : (int)PLAN_FAST_MAX;
   a.seg_cost = seg_cost_units(tune, 0);
   const size_t lds = (size_t)waves * FP4_SLOTS * fp4_slot((int)head_dim);
-  void (*kern)(Fp4AttnArgs) = head_dim == 128 ? (pack ? fp4_attn_kernel<128, true> : fp4_attn_kernel<128, false>)
-                                              : (pack ? fp4_attn_kernel<64, true> : fp4_attn_kernel<64, false>);
+  void (*kern)(Fp4AttnArgs) =
+      head_dim == 128 ? (pack ? fp4_attn_kernel<128, true, 1> : nr == 1 ? fp4_attn_kernel<128, false, 1> : fp4_attn_kernel<128, false, 2>)
+                      : (pack ? fp4_attn_kernel<64, true, 1> : nr == 1 ? fp4_attn_kernel<64, false, 1> : fp4_attn_kernel<64, false, 2>);
   const int64_t tw = target_waves > 0 ? target_waves
                      : cut            ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
                                       : (int64_t)device_cus() * waves;
