@@ -236,7 +236,10 @@ constexpr int fp4_accs(int d, bool pack) { return pack ? d / 32 : d / 16; }
 constexpr int fp4_merge_fields(int d, bool pack) { return 4 * fp4_accs(d, pack) + 2; }
 // Wavefronts of a workgroup: what its registers and LDS leave room for. Segments that are not cut are shared by all of them.
 constexpr int FP4_WAVES = 8;
-constexpr int FP4_SLOTS = 4;
+// Tiles of a wavefront's ring. Up to 8 query rows a key's products are few and the loads are what it waits for: 4 (ragged decode,
+// 96 requests of up to 32768 keys: 58 us; 2 slots, with twice the workgroups on a unit, 67). More rows: 2, where the products
+// cover the loads and more workgroups fit (24 requests of 4 rows: 23 us; 4 slots 27).
+constexpr int fp4_slots(bool pack) { return pack ? 4 : 2; }
 constexpr int FP4_DMA_AUX = 2;   // streaming: K and V are read once
 
 // 16 query rows as the MFMA's second operand: lane (n, g) holds row n's channels (D / 4) g + 8 s .. + 7 in step s.
@@ -325,7 +328,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   constexpr int RT = PACK ? 8 : 16;        // rows of a tile
   static_assert(!PACK || NR == 1, "at most 8 rows are one tile");
   constexpr int VT = D / 16, NA = fp4_accs(D, PACK), SB = D / FP4_GROUP;
-  constexpr int S = FP4_SLOTS, SLOT = fp4_slot(D), HALF = fp4_half(D), CODES = fp4_codes(D), CH = fp4_chunks(D);
+  constexpr int S = fp4_slots(PACK), SLOT = fp4_slot(D), HALF = fp4_half(D), CODES = fp4_codes(D), CH = fp4_chunks(D);
   constexpr int DMAS = CODES / 1024, OPS = 2 * (DMAS + 1);   // DMAs of a half's codes; vector memory operations of a tile
   static_assert(S * OPS < 64, "vmcnt range");
   const int G = PACK ? a.G >> 1 : a.G;     // (PACK: the plan counts 16 columns a tile, two a row)
@@ -408,13 +411,13 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
     for (int b = 0; b < 2; ++b)
       next[b] = ((const __attribute__((address_space(4))) int*)bt)[__builtin_amdgcn_readfirstlane(half_key(j, b) >> lbs)];
   };
-  auto load = [&](int slot, int j) {   // tile j, whose page ids are here
+  auto load = [&](uint32_t slot, int j) {   // tile j, whose page ids are here; slot: its offset in the ring
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const int id = __builtin_amdgcn_readfirstlane(next[b]), p = (unsigned)id < (unsigned)num_blocks ? id : 0;
       const uint32_t of = half_key(j, b) & (bs - 1);
       const uint64_t co = (uint64_t)(uint32_t)p * c_sb + of * c_sn, so = (uint64_t)(uint32_t)p * s_sb + of * SB;
-      uint8_t* dst = lds + slot * SLOT + b * HALF;
+      uint8_t* dst = lds + slot + b * HALF;
 #pragma unroll
       for (int u = 0; u < DMAS; ++u)
         __builtin_amdgcn_global_load_lds((const void*)(src[u] + co), (__attribute__((address_space(3))) void*)(dst + 1024 * u), 16, 0, FP4_DMA_AUX);
@@ -427,7 +430,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 #pragma unroll
     for (int j = 0; j < S - 1; ++j)
       if (j < nt) {
-        load(j, j);
+        load(j * SLOT, j);
         fetch(j + 1);
       }
 #pragma unroll
@@ -450,18 +453,17 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   }
   const uint32_t pshift = PACK && n >= 8 ? 16 : 0;   // PACK: where the column's weights stand beside zeros
 
-  // tile j in `slot`; vm: this wavefront's vector memory operations behind the tile's own (the reads' statements wait for
-  // themselves: the compiler sees neither the DMAs nor that they are done)
-  auto compute = [&](auto masked_t, auto vm_t, auto slot_t, int j) {
+  // tile j, at `slot` of the ring (the reads' statements wait for themselves: the compiler sees neither the DMAs nor that they
+  // are done)
+  auto compute = [&](auto masked_t, uint32_t slot, int j) {
     constexpr bool MASKED = decltype(masked_t)::value;
-    constexpr int VM = decltype(vm_t)::value, AT = decltype(slot_t)::value * SLOT;
     const int n0 = tile(j) * TILE;
     uint32_t kw[2][D / 32], ksw[2], v[8], vs[2][D / 32];
     if constexpr (D == 128) {
       u32x4 k0, k1;
-      asm volatile("s_waitcnt vmcnt(%c6)\n\tds_read_b128 %0, %4 offset:%c7\n\tds_read_b128 %1, %4 offset:%c8\n\t"
-                   "ds_read_u8 %2, %5 offset:%c7\n\tds_read_u8 %3, %5 offset:%c8\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(k0), "=&v"(k1), "=&v"(ksw[0]), "=&v"(ksw[1]) : "v"(kadr), "v"(ksadr), "n"(VM), "n"(AT), "n"(AT + HALF) : "memory");
+      asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%c6\n\t"
+                   "ds_read_u8 %2, %5\n\tds_read_u8 %3, %5 offset:%c6\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(k0), "=&v"(k1), "=&v"(ksw[0]), "=&v"(ksw[1]) : "v"(kadr + slot), "v"(ksadr + slot), "n"(HALF) : "memory");
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         kw[0][i] = k0[i];
@@ -469,9 +471,9 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       }
     } else {
       u32x2 k0, k1;
-      asm volatile("s_waitcnt vmcnt(%c6)\n\tds_read_b64 %0, %4 offset:%c7\n\tds_read_b64 %1, %4 offset:%c8\n\t"
-                   "ds_read_u8 %2, %5 offset:%c7\n\tds_read_u8 %3, %5 offset:%c8\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(k0), "=&v"(k1), "=&v"(ksw[0]), "=&v"(ksw[1]) : "v"(kadr), "v"(ksadr), "n"(VM), "n"(AT), "n"(AT + HALF) : "memory");
+      asm volatile("ds_read_b64 %0, %4\n\tds_read_b64 %1, %4 offset:%c6\n\t"
+                   "ds_read_u8 %2, %5\n\tds_read_u8 %3, %5 offset:%c6\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(k0), "=&v"(k1), "=&v"(ksw[0]), "=&v"(ksw[1]) : "v"(kadr + slot), "v"(ksadr + slot), "n"(HALF) : "memory");
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         kw[0][i] = k0[i];
@@ -484,13 +486,13 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
     for (int b = 0; b < 2; ++b) fp4_scores<D, NR>(kw[b], ksw[b], q, b, z);
     if constexpr (D == 128) {   // (while the products run)
       u32x4 x0, x1;
-      asm volatile("ds_read_b32 %0, %10 offset:%c15\n\tds_read_b32 %1, %11 offset:%c15\n\tds_read_b32 %2, %12 offset:%c15\n\t"
-                   "ds_read_b32 %3, %13 offset:%c15\n\tds_read_b32 %4, %10 offset:%c16\n\tds_read_b32 %5, %11 offset:%c16\n\t"
-                   "ds_read_b32 %6, %12 offset:%c16\n\tds_read_b32 %7, %13 offset:%c16\n\tds_read_b128 %8, %14 offset:%c15\n\t"
-                   "ds_read_b128 %9, %14 offset:%c16\n\ts_waitcnt lgkmcnt(0)"
+      asm volatile("ds_read_b32 %0, %10\n\tds_read_b32 %1, %11\n\tds_read_b32 %2, %12\n\t"
+                   "ds_read_b32 %3, %13\n\tds_read_b32 %4, %10 offset:%c15\n\tds_read_b32 %5, %11 offset:%c15\n\t"
+                   "ds_read_b32 %6, %12 offset:%c15\n\tds_read_b32 %7, %13 offset:%c15\n\tds_read_b128 %8, %14\n\t"
+                   "ds_read_b128 %9, %14 offset:%c15\n\ts_waitcnt lgkmcnt(0)"
                    : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
                      "=&v"(x0), "=&v"(x1)
-                   : "v"(vadr[0]), "v"(vadr[1]), "v"(vadr[2]), "v"(vadr[3]), "v"(vsadr), "n"(AT), "n"(AT + HALF) : "memory");
+                   : "v"(vadr[0] + slot), "v"(vadr[1] + slot), "v"(vadr[2] + slot), "v"(vadr[3] + slot), "v"(vsadr + slot), "n"(HALF) : "memory");
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         vs[0][i] = x0[i];
@@ -498,13 +500,13 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       }
     } else {
       u32x2 x0, x1;
-      asm volatile("ds_read_u16 %0, %10 offset:%c15\n\tds_read_u16 %1, %11 offset:%c15\n\tds_read_u16 %2, %12 offset:%c15\n\t"
-                   "ds_read_u16 %3, %13 offset:%c15\n\tds_read_u16 %4, %10 offset:%c16\n\tds_read_u16 %5, %11 offset:%c16\n\t"
-                   "ds_read_u16 %6, %12 offset:%c16\n\tds_read_u16 %7, %13 offset:%c16\n\tds_read_b64 %8, %14 offset:%c15\n\t"
-                   "ds_read_b64 %9, %14 offset:%c16\n\ts_waitcnt lgkmcnt(0)"
+      asm volatile("ds_read_u16 %0, %10\n\tds_read_u16 %1, %11\n\tds_read_u16 %2, %12\n\t"
+                   "ds_read_u16 %3, %13\n\tds_read_u16 %4, %10 offset:%c15\n\tds_read_u16 %5, %11 offset:%c15\n\t"
+                   "ds_read_u16 %6, %12 offset:%c15\n\tds_read_u16 %7, %13 offset:%c15\n\tds_read_b64 %8, %14\n\t"
+                   "ds_read_b64 %9, %14 offset:%c15\n\ts_waitcnt lgkmcnt(0)"
                    : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]),
                      "=&v"(x0), "=&v"(x1)
-                   : "v"(vadr[0]), "v"(vadr[1]), "v"(vadr[2]), "v"(vadr[3]), "v"(vsadr), "n"(AT), "n"(AT + HALF) : "memory");
+                   : "v"(vadr[0] + slot), "v"(vadr[1] + slot), "v"(vadr[2] + slot), "v"(vadr[3] + slot), "v"(vsadr + slot), "n"(HALF) : "memory");
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         vs[0][i] = x0[i];
@@ -612,55 +614,39 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
     }
   };
 
-  // S - 1 tiles in flight. The last ones have fewer behind them: they wait for all.
-  if (nt > 0) {
-    const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
-    const int j_full = min(nt - (S - 1), full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0);
-    int j0 = 0;
-    for (; j0 + S <= j_full; j0 += S) {
-      auto step = [&](auto s_t) {
-        constexpr int s = decltype(s_t)::value;
-        load((s + S - 1) % S, j0 + s + S - 1);
-        compute(std::false_type{}, std::integral_constant<int, (S - 1) * OPS>{}, s_t, j0 + s);
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-      if constexpr (S > 2) step(std::integral_constant<int, 2 % S>{});
-      if constexpr (S > 3) step(std::integral_constant<int, 3 % S>{});
+  // S - 1 tiles in flight. One body for whole tiles and one for those at some row's limit, whatever their place in the ring: a
+  // piece is a few tiles, and the first pass through code costs more than the second.
+  const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
+  const int j_full = full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0;
+  uint32_t slot = 0, free = (S - 1) * SLOT;
+#pragma unroll 1
+  for (int j = 0; j < nt; ++j) {
+    if (j + S - 1 < nt) {
+      load(free, j + S - 1);
+      wait_vm<(S - 1) * OPS>();   // this wavefront's operations behind the tile's own
+    } else {
+      wait_vm<0>();
     }
-    for (; j0 < nt; j0 += S) {
-      auto step = [&](auto s_t) {
-        constexpr int s = decltype(s_t)::value;
-        const int j = j0 + s;
-        if (j >= nt) return;
-        if (j + S - 1 < nt) {
-          load((s + S - 1) % S, j + S - 1);
-          compute(std::true_type{}, std::integral_constant<int, (S - 1) * OPS>{}, s_t, j);
-        } else {
-          compute(std::true_type{}, std::integral_constant<int, 0>{}, s_t, j);
-        }
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-      if constexpr (S > 2) step(std::integral_constant<int, 2 % S>{});
-      if constexpr (S > 3) step(std::integral_constant<int, 3 % S>{});
-    }
+    if (j < j_full) compute(std::false_type{}, slot, j);
+    else compute(std::true_type{}, slot, j);
+    free = slot;
+    slot = slot + SLOT == S * SLOT ? 0 : slot + SLOT;
   }
 
-  // ---- the key splits' merge, half of them into the other half at a time ----
+  // ---- the key splits' merge, half of them into the other half at a time, one row tile after the other ----
 #pragma unroll
   for (int t = 0; t < NR; ++t) l[t] = group4_sum(l[t]);
   if (KS > 1) {
     // (each wavefront hands over in its own ring, which is done with)
     constexpr int FIELDS = fp4_merge_fields(D, PACK);
-    static_assert(NR * FIELDS * WAVE * 4 <= S * SLOT, "merge fields in the ring");
+    static_assert(FIELDS * WAVE * 4 <= S * SLOT, "merge fields in the ring");
     auto mem = [&](int k) { return reinterpret_cast<float*>(lds + (k - ks) * (a.rt / NR) * S * SLOT) + lane; };
     for (int half = KS, width = KS; width > 1; width = half) {
       half = (width + 1) / 2;
-      if (active && ks >= half && ks < width) {
-        float* to = mem(ks);
 #pragma unroll
-        for (int t = 0; t < NR; ++t, to += FIELDS * WAVE) {
+      for (int t = 0; t < NR; ++t) {
+        if (active && ks >= half && ks < width) {
+          float* to = mem(ks);
 #pragma unroll
           for (int c = 0; c < NA; ++c)
 #pragma unroll
@@ -668,12 +654,9 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
           to[(4 * NA) * WAVE] = m[t];
           to[(4 * NA + 1) * WAVE] = l[t];
         }
-      }
-      __syncthreads();
-      if (active && ks + half < width) {
-        const float* from = mem(ks + half);
-#pragma unroll
-        for (int t = 0; t < NR; ++t, from += FIELDS * WAVE) {
+        __syncthreads();
+        if (active && ks + half < width) {
+          const float* from = mem(ks + half);
           const float mo = from[(4 * NA) * WAVE], M = __builtin_fmaxf(m[t], mo);
           const float w0 = __builtin_amdgcn_exp2f(m[t] - M), w1 = __builtin_amdgcn_exp2f(mo - M);
           l[t] = __builtin_fmaf(w1, from[(4 * NA + 1) * WAVE], l[t] * w0);
@@ -683,8 +666,8 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
             for (int i = 0; i < 4; ++i) acc[t][c][i] = __builtin_fmaf(w1, from[(4 * c + i) * WAVE], acc[t][c][i] * w0);
           m[t] = M;
         }
+        __syncthreads();
       }
-      __syncthreads();
     }
   }
   if (ks > 0 || !active) return;
@@ -759,7 +742,7 @@ __global__ __launch_bounds__(WAVE * FP4_WAVES) __attribute__((amdgpu_waves_per_e
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int rw = a.rt / NR, ksplit = a.ksplit, kspl = wave / rw, rtile = NR * (wave - kspl * rw);
   extern __shared__ __attribute__((aligned(1024))) uint8_t fp4_lds[];
-  uint8_t* ring = fp4_lds + wave * FP4_SLOTS * fp4_slot(D);
+  uint8_t* ring = fp4_lds + wave * fp4_slots(PACK) * fp4_slot(D);
   int solo = 0;
   walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
     const int row0 = (rg * a.rt + rtile) * (PACK ? 8 : 16);
@@ -988,13 +971,14 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   if (rows > INT32_MAX / 4) return fail("%s: grid too large", nm);
   // the row tile: 8 rows where that holds all of a request's rows; else 16
   const bool pack = rows <= 8;
-  // a wavefront takes one row tile or, of more rows than one tile holds, two: it converts a tile's keys once for both
-  const int nr = rows <= 16 ? 1 : 2;
-  const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : MAX_ROW_TILES, rw = rt / nr;
   const Tuning tune = read_tuning();
   const bool cut = num_splits > 1 && segm_rows > 0;
-  const int most = cut ? MAX_ROW_TILES : FP4_WAVES;
-  const int ks_max = tune.ksplit ? std::max(1, std::min(MAX_ROW_TILES, atoi(tune.ksplit)))
+  // More rows than a tile holds: a wavefront to each tile of rows, or one to two of them, which converts a key once for both but
+  // keeps half as many wavefronts busy. Cut segments are short and take the first (16 requests of 8 rows, 4 heads a KV head:
+  // 24 us against 29; 64 such: 63 against 60), whole ones the second (64 of 4096 keys each: 64 against 77).
+  const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : MAX_ROW_TILES, nr = cut || rt == 1 ? 1 : 2, rw = rt / nr;
+  const int most = cut && rt == 1 ? MAX_ROW_TILES : FP4_WAVES;
+  const int ks_max = tune.ksplit ? std::max(1, std::min(FP4_WAVES, atoi(tune.ksplit)))
                      : !cut || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? most : DEFAULT_KSPLIT;
   const int ks = std::max(1, std::min(ks_max, most / rw)), waves = rw * ks;
   Fp4AttnArgs b;
@@ -1024,7 +1008,7 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
                                        : (int)PLAN_FAST_MAX;
   a.seg_cost = seg_cost_units(tune, 0);
-  const size_t lds = (size_t)waves * FP4_SLOTS * fp4_slot((int)head_dim);
+  const size_t lds = (size_t)waves * fp4_slots(pack) * fp4_slot((int)head_dim);
   void (*kern)(Fp4AttnArgs) =
       head_dim == 128 ? (pack ? fp4_attn_kernel<128, true, 1> : nr == 1 ? fp4_attn_kernel<128, false, 1> : fp4_attn_kernel<128, false, 2>)
                       : (pack ? fp4_attn_kernel<64, true, 1> : nr == 1 ? fp4_attn_kernel<64, false, 1> : fp4_attn_kernel<64, false, 2>);
