@@ -614,23 +614,34 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
     }
   };
 
-  // S - 1 tiles in flight. One body for whole tiles and one for those at some row's limit, whatever their place in the ring: a
-  // piece is a few tiles, and the first pass through code costs more than the second.
+  // S - 1 tiles in flight. One body for whole tiles and one for those at some row's limit or at the end, whatever their place in
+  // the ring: a piece is a few tiles, and the first pass through code costs more than the second (a body to each slot: 1 request
+  // of 4096 keys 13.3 us against 12.7, 64 of 8 rows 64 against 60; 128 of 32768 keys 359 against 361).
   const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
   const int j_full = full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0;
   uint32_t slot = 0, free = (S - 1) * SLOT;
+  auto turn = [&] {
+    free = slot;
+    slot = slot + SLOT == S * SLOT ? 0 : slot + SLOT;
+  };
+  int j = 0;
 #pragma unroll 1
-  for (int j = 0; j < nt; ++j) {
+  for (const int end = min(j_full, nt - (S - 1)); j < end; ++j) {
+    load(free, j + S - 1);
+    wait_vm<(S - 1) * OPS>();   // this wavefront's operations behind the tile's own
+    compute(std::false_type{}, slot, j);
+    turn();
+  }
+#pragma unroll 1
+  for (; j < nt; ++j) {
     if (j + S - 1 < nt) {
       load(free, j + S - 1);
-      wait_vm<(S - 1) * OPS>();   // this wavefront's operations behind the tile's own
+      wait_vm<(S - 1) * OPS>();
     } else {
       wait_vm<0>();
     }
-    if (j < j_full) compute(std::false_type{}, slot, j);
-    else compute(std::true_type{}, slot, j);
-    free = slot;
-    slot = slot + SLOT == S * SLOT ? 0 : slot + SLOT;
+    compute(std::true_type{}, slot, j);
+    turn();
   }
 
   // ---- the key splits' merge, half of them into the other half at a time, one row tile after the other ----
