@@ -240,7 +240,9 @@ constexpr int FP4_WAVES = 8;
 // 96 requests of up to 32768 keys: 58 us; 2 slots, with twice the workgroups on a unit, 67). More rows: 2, where the products
 // cover the loads and more workgroups fit (24 requests of 4 rows: 23 us; 4 slots 27).
 constexpr int fp4_slots(bool pack) { return pack ? 4 : 2; }
-constexpr int FP4_DMA_AUX = 2;   // streaming: K and V are read once
+// The DMAs' cache policy: streaming (2) where K and V are read once; the wavefronts of several row tiles read the same lines
+// (verification, 16 requests of 8 rows: 22.5 us against 24.4; 24 of 4: 23.0 against 25.2; 64 of 4: 37.4 against 35.7).
+constexpr int fp4_dma_aux(bool pack) { return pack ? 2 : 0; }
 
 // 16 query rows as the MFMA's second operand: lane (n, g) holds row n's channels (D / 4) g + 8 s .. + 7 in step s.
 template <int D>
@@ -420,8 +422,8 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       uint8_t* dst = lds + slot + b * HALF;
 #pragma unroll
       for (int u = 0; u < DMAS; ++u)
-        __builtin_amdgcn_global_load_lds((const void*)(src[u] + co), (__attribute__((address_space(3))) void*)(dst + 1024 * u), 16, 0, FP4_DMA_AUX);
-      __builtin_amdgcn_global_load_lds((const void*)(ssrc + so), (__attribute__((address_space(3))) void*)(dst + CODES), 4, 0, FP4_DMA_AUX);
+        __builtin_amdgcn_global_load_lds((const void*)(src[u] + co), (__attribute__((address_space(3))) void*)(dst + 1024 * u), 16, 0, fp4_dma_aux(PACK));
+      __builtin_amdgcn_global_load_lds((const void*)(ssrc + so), (__attribute__((address_space(3))) void*)(dst + CODES), 4, 0, fp4_dma_aux(PACK));
     }
   };
 
@@ -983,14 +985,14 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   // the row tile: 8 rows where that holds all of a request's rows; else 16
   const bool pack = rows <= 8;
   const Tuning tune = read_tuning();
-  const bool cut = num_splits > 1 && segm_rows > 0;
-  // More rows than a tile holds: a wavefront to each tile of rows, or one to two of them, which converts a key once for both but
-  // keeps half as many wavefronts busy. Cut segments are short and take the first (16 requests of 8 rows, 4 heads a KV head:
-  // 24 us against 29; 64 such: 63 against 60), whole ones the second (64 of 4096 keys each: 64 against 77).
-  const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : MAX_ROW_TILES, nr = cut || rt == 1 ? 1 : 2, rw = rt / nr;
+  const bool cut = num_splits > 1 && segm_rows > 0, few = num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS;
+  // More rows than a tile holds: a wavefront to each tile of rows, or one to two of them, which loads and converts a key once for
+  // both but keeps half as many wavefronts busy. Few pairs of a request and a KV head, cut, take the first (16 requests of 8 rows,
+  // 28 heads on 4: 22.5 us against 26), others the second (64 such requests: 54 against 62; 64 of 4096 keys, whole: 59 against 76).
+  const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : MAX_ROW_TILES, nr = rt == 1 || (cut && few) ? 1 : 2, rw = rt / nr;
   const int most = cut && rt == 1 ? MAX_ROW_TILES : FP4_WAVES;
   const int ks_max = tune.ksplit ? std::max(1, std::min(FP4_WAVES, atoi(tune.ksplit)))
-                     : !cut || num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS ? most : DEFAULT_KSPLIT;
+                     : !cut || few ? most : DEFAULT_KSPLIT;
   const int ks = std::max(1, std::min(ks_max, most / rw)), waves = rw * ks;
   Fp4AttnArgs b;
   b.s = Fp4Scales{const_cast<uint8_t*>(k_scale), const_cast<uint8_t*>(v_scale), s_sb, s_sh};
