@@ -354,7 +354,7 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
 
 /* Quantize rows into slots: for t < num_tokens whose slot is in [0, nb * bs), others are skipped. Of a group's 32 values x, with
  * top = max |x| (finite x):  e = floor(log2 top) - 2, one more where top 2^-e > 7, from -100 to 125; byte e + 127; codes the
- * nearest of x 2^-e, ties to the even code, at most 6 (infinities too); a NaN is 0. Bit-reproducible. */
+ * nearest of x 2^-e, ties to the even code, at most 6 (infinities too); a NaN is 0. A slot occurs once. Bit-reproducible. */
 int kvq_quant_fp4_cache(const void* key, int64_t key_st, int64_t key_sh, const void* value, int64_t val_st, int64_t val_sh,
                         uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t kc_sh, uint8_t* v_cache, int64_t vc_sb,
                         int64_t vc_sn, int64_t vc_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads,
@@ -391,8 +391,9 @@ int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const v
 /* Attention over a 4-bit cache for requests with 1 <= q_len <= qmax: o = softmax(q k^T softmax_scale) v, bottom-right causal,
  * bf16 q and out; a row that sees no key is zero, another whose q holds a NaN or an infinity is NaN. Cached values are exact.
  * Rounded: the weights, to bf16 (2^-8 of each). lse (fp32 [T, Hq], row stride lse_st, or NULL): the rows' natural
- * log-sum-exp, -inf where no key is seen. softmax_scale from 1e-16 to 1e16. Rows, skipped requests, split buffers and the other
- * arguments as kvq_block_decode_attention. */
+ * log-sum-exp, -inf where no key is seen. softmax_scale from 1e-16 to 1e16. K's and V's page and slot strides are the same.
+ * max_query_len picks the launch: requests with more tokens, up to qmax, are served too. Rows, skipped requests, split buffers
+ * and the other arguments as kvq_block_decode_attention. */
 int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,
                              int64_t k_sh, const uint8_t* v_cache, int64_t v_sb, int64_t v_sn, int64_t v_sh,
                              int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
@@ -420,7 +421,7 @@ int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t
  * weights[r, h, m .. n - 1] become 0. kept[r, h, i] (int32, strides (kp_sr, kp_sh, 1)): the position that row i held before;
  * new_lens[r] = min(n, m). Where n <= m nothing moves (kept[r, h, i] = i). Entries of kept from new_lens[r] on and cache rows
  * from there on are left as they are. The pages of a call's requests must be theirs alone. Page ids outside [0, nb) read as page
- * 0, and are not written. Bit-reproducible. */
+ * 0, and are not written. A table has at most 2^28 slots (bt_cols * block_size). Bit-reproducible. */
 int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, uint8_t* v_cache, int64_t v_sb, int64_t v_sn,
                   int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, uint8_t* k_scale,
                   uint8_t* v_scale, int64_t s_sb, int64_t s_sh, float* weights, int64_t w_sr, int64_t w_sh, int64_t w_cols,

@@ -54,6 +54,8 @@ __device__ __forceinline__ void eight_of(const void* p, bool bf16, int64_t i, fl
 // (i, i + rd / 2) or, INTER, (2 i, 2 i + 1); fp32 throughout, one rounding to bf16. A lane holds 8 pairs of a row, so a
 // pair never leaves its lane, a row's mean is a sum over D / 16 lanes, and a token's cos and sin, which all of its heads
 // share, are read once by the wavefront that takes them.
+// Bound by memory: 16384 tokens of 32 + 8 heads of 128 (344 MB): 66 us, 5.2 TB/s, what a stream of as many bytes read as
+// written reaches (5.3 .. 5.5). 32 tokens of 28 + 4 heads: 3.5 us, a launch.
 template <int D, bool INTER, bool BF16_TABLE>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeArgs a) {
   constexpr int LPR = D / 16, RPW = WAVE / LPR;   // lanes per row, rows per wavefront

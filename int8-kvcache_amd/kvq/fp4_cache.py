@@ -127,7 +127,7 @@ def fp4_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block
     """Attention over a 4-bit cache for the requests with at most SHORT_Q query tokens (others are skipped), with
     decode_attention's arguments: out rows softmax(q k^T softmax_scale) v, bottom-right causal, of the cached values and the
     bf16 q. Rounded: the weights, to bf16 (2^-8 of each). A row that sees no key is zero, another with a NaN or an infinity
-    in q NaN. segm: split buffers (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces. lse
+    in q NaN. The caches have the same page and slot strides. segm: split buffers (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces. lse
     (float32 [T, q heads]): filled with the rows' natural log-sum-exp, -inf for a row that sees no key."""
     name = "fp4_decode_attention"
     so, sm, ss = segm if segm is not None else (None, None, None)
@@ -253,7 +253,8 @@ def evict_keys(k_cache, v_cache, scales, weights, seq_lens, keep, recent, block_
     request may keep]): filled with the position that each row held; new_lens (int32 [requests]): min(seq_lens, keep), the
     lengths from now on: the next token's slot is the one behind, while its position for the rotation goes on counting. keep
     counts as at most kept.shape[2] and as at least 0. A request within its budget is left as it is. The pages of the
-    requests must be theirs alone. Returns new_lens."""
+    requests must be theirs alone, a prefix that two requests share is not evicted from. A table has at most 2^28 slots.
+    Returns new_lens."""
     name = "evict_keys"
     if ck._served(ck.ext(), name, k_cache, v_cache, scales["k_scale"], scales["v_scale"], weights, seq_lens, keep, recent,
                   block_table, kept, new_lens):

@@ -201,6 +201,18 @@ def test_c_entry_sizes():
     assert _c("fp4_prefill_attention", (21, 64)) == (1, "fp4_prefill_attention: work list tiles must be 128 rows")
 
 
+def test_c_entry_layouts():
+    """The strides that the kernels' 32-bit offsets, or one address for a key's K and V, leave out."""
+    for name, at in (("quant_fp4_cache", 7), ("quant_fp4_cache", 20), ("read_fp4_cache", 5), ("fp4_pages", 1),
+                     ("fp4_decode_attention", 4), ("fp4_key_weights", 4), ("fp4_evict", 14), ("fp4_evict", 5)):
+        for far in (1 << 32, -2048):
+            assert _c(name, (at, far)) == (1, f"{name}: pages 4 GiB apart or more"), (name, at)
+    same = "fp4_decode_attention: K and V caches must have the same page and slot strides"
+    assert _c("fp4_decode_attention", (8, 4096)) == (1, same)
+    assert _c("fp4_decode_attention", (9, 128)) == (1, same)
+    assert _c("fp4_evict", (25, (1 << 23) + 1)) == (1, "fp4_evict: tables of more than 2^28 slots")
+
+
 ROPE = [16, 3584, 128, 16, 512, 128, 16, 3584, 128, 16, 512, 128, 5, 28, 4, 128, 16, 64, 16, 64, 100, 64, 0, 16, 16, 1, 1e-6, 0, None]
 
 

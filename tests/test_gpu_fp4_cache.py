@@ -378,6 +378,121 @@ def test_many_requests_and_bad_pages():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("most", [1, 2, 100])
+@pytest.mark.parametrize("split", [False, True])
+def test_longest_query_is_a_hint(most, split):
+    """max_query_len picks the launch; rows of longer requests are served all the same."""
+    lens, q_lens = [700, 33, 5000, 8], [8, 1, 5, 8]
+    c = filled(4, 128, 16, lens)
+    cu = cumsum(q_lens)
+    q = torch.randn(cu[-1], 28, 128, generator=gen(9)).to(torch.bfloat16).to(DEV)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device=DEV)
+    fc.fp4_decode_attention(q, c.kc, c.vc, out, i32(cu), i32(lens), c.table, 0.09, c.scales,
+                            nan_segm(cu[-1], 28, 16, 128) if split else None, most, lse)
+    want, bound, of, of_bound = R.attention(q, c.kc, c.vc, c.scales, cu, lens, c.table, 0.09)
+    R.check(out, want, bound, most)
+    R.check_lse(lse, of, of_bound, most)
+
+
+@pytest.mark.parametrize("splits", ["1", "3", "5", "8"])
+@pytest.mark.parametrize("hq,h,d", [(28, 4, 128), (14, 2, 64), (32, 1, 128)])
+@pytest.mark.parametrize("qlen", [1, 4, 8])
+def test_other_numbers_of_key_splits(splits, hq, h, d, qlen, monkeypatch):
+    monkeypatch.setenv("KVQ_KSPLIT", splits)
+    lens = [0, 9, 100, 33, 700, 2049]
+    c = filled(h, d, 16, lens)
+    q_lens = [qlen] * len(lens)
+    attend(c, hq, q_lens, lens)
+    attend(c, hq, q_lens, lens, nan_segm(sum(q_lens), hq, 8, d))
+
+
+@pytest.mark.parametrize("hq,h,d", [(28, 4, 128), (14, 2, 64)])
+@pytest.mark.parametrize("qlen", [3, 8])
+def test_many_pairs_of_many_rows(hq, h, d, qlen):
+    """More pairs of a request and a kv head than take a wavefront a row tile, cut and whole; some of fewer tokens."""
+    r = np.random.RandomState(1)
+    lens = [int(x) for x in r.randint(8, 600, 40)]
+    q_lens = [int(x) for x in r.randint(0, qlen + 1, 40)]
+    q_lens[0] = qlen
+    c = filled(h, d, 32, lens)
+    attend(c, hq, q_lens, lens)
+    attend(c, hq, q_lens, lens, nan_segm(sum(q_lens) + 2, hq, 8, d))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("order", ["heads first", "V first", "padded rows", "slots first"])
+def test_other_orders_of_a_cache(d, order):
+    """Caches of other strides through every operator that reads them, against the same calls on the usual layout."""
+    lens, q_lens, h, bs, hq = [300, 20, 0, 1000], [1, 8, 1, 3], 4, 32, 12
+    ref = filled(h, d, bs, lens)
+    nb = ref.kc.shape[0]
+    full = lambda *shape: torch.full(shape, 0xff, dtype=torch.uint8, device=DEV)  # noqa: E731
+    c = Cache(h, d, bs, nb)
+    if order == "heads first":
+        c.kc, c.vc = (full(nb, h, bs, d // 2).transpose(1, 2) for _ in range(2))
+    elif order == "V first":
+        kv = full(nb, bs, h, d)
+        c.kc, c.vc = kv[..., d // 2:], kv[..., :d // 2]
+    elif order == "padded rows":
+        c.kc, c.vc = (full(nb + 1, bs + 3, h + 1, d // 2 + 16)[:nb, :bs, 1:, :d // 2] for _ in range(2))
+    else:
+        c.kc, c.vc = (full(bs, nb, h, d // 2).transpose(0, 1) for _ in range(2))
+    fc.quant_fp4_cache(ref.k.to(DEV), ref.v.to(DEV), c.kc, c.vc, c.scales, slots_of(ref.host, lens, bs).to(DEV))
+    for x, y in zip(c.parts(), ref.parts()):
+        assert torch.equal(x, y)
+    c.host, c.table = ref.host, ref.table
+    segm = [nan_segm(sum(q_lens), hq, 8, d) for _ in range(2)]
+    a, b = attend(c, hq, q_lens, lens, segm[0]), attend(ref, hq, q_lens, lens, segm[1])
+    assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+    attend(c, hq, [1, 20, 1, 40], lens)
+    w = [torch.zeros(len(lens), h, 1000, device=DEV) for _ in range(2)]
+    kept = [torch.zeros(len(lens), h, 64, dtype=torch.int32, device=DEV) for _ in range(2)]
+    for i, (x, of) in enumerate(((c, a), (ref, b))):
+        fc.add_key_weights(of[0], x.kc, x.scales, of[2], w[i], i32(cumsum(q_lens)), i32(lens), x.table, d ** -0.5, 8)
+        fc.evict_keys(x.kc, x.vc, x.scales, w[i], i32(lens), i32([64] * 4), 8, x.table, kept[i], i32([0] * 4))
+    assert torch.equal(w[0], w[1]) and torch.equal(kept[0], kept[1])
+    for x, y in zip(c.parts(), ref.parts()):
+        assert torch.equal(x, y)
+
+
+def test_two_graphs_share_buffers():
+    """Graphs of two batches over one cache, with the same split buffers, replayed in turn with eager work between."""
+    lens = [3000, 17, 0, 900]
+    c = filled(4, 128, 16, lens)
+    segm = nan_segm(32, 28, 16, 128)
+    batches = []
+    for q_lens, short in (([1, 1, 1, 1], lens), ([8, 3, 1, 8], [2000, 10, 0, 901 - 1])):
+        cu = cumsum(q_lens)
+        q = torch.randn(cu[-1], 28, 128, generator=gen(cu[-1])).to(torch.bfloat16).to(DEV)
+        x = dict(q=q, out=torch.zeros_like(q), lse=torch.zeros(q.shape[:2], device=DEV), cu=i32(cu), lens=i32(short),
+                 most=max(q_lens), w=torch.zeros(4, 4, 3000, device=DEV))
+        batches.append(x)
+
+    def run(x):
+        fc.fp4_paged_attention(x["q"], c.kc, c.vc, x["out"], x["cu"], x["lens"], c.table, x["most"], 0.09, c.scales, None, segm,
+                               x["lse"])
+        x["w"].zero_()
+        fc.add_key_weights(x["q"], c.kc, c.scales, x["lse"], x["w"], x["cu"], x["lens"], c.table, 0.09, x["most"])
+
+    want, graphs = [], []
+    for x in batches:
+        run(x)
+        torch.cuda.synchronize()
+        want.append([x[n].clone() for n in ("out", "lse", "w")])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(x)
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 1, 0):
+        for n in ("out", "lse", "w"):
+            batches[i][n].fill_(7.0)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(batches[i][n], y) for n, y in zip(("out", "lse", "w"), want[i])), i
+        run(batches[1 - i])
+        assert all(torch.equal(batches[1 - i][n], y) for n, y in zip(("out", "lse", "w"), want[1 - i])), i
+
+
 # ------------------------------------------------------------------------------------------------ weights
 def weigh(c, hq, q_lens, lens, cols, seed=5, lse=None, most=None, pad=1):
     h, d, bs = c.geom
