@@ -390,7 +390,7 @@ int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const v
 
 /* Attention over a 4-bit cache for requests with 1 <= q_len <= qmax: o = softmax(q k^T softmax_scale) v, bottom-right causal,
  * bf16 q and out; a row that sees no key is zero, another whose q holds a NaN or an infinity is NaN. Cached values are exact.
- * Rounded: the weights, to bf16 (2^-8 of each). lse (fp32 [T, Hq], row stride lse_st, or NULL): the rows' natural
+ * Rounded: the weights, to a sum of two bf16 (2^-14 of each). lse (fp32 [T, Hq], row stride lse_st, or NULL): the rows' natural
  * log-sum-exp, -inf where no key is seen. softmax_scale from 1e-16 to 1e16. K's and V's page and slot strides are the same.
  * max_query_len picks the launch: requests with more tokens, up to qmax, are served too. Rows, skipped requests, split buffers
  * and the other arguments as kvq_block_decode_attention. */

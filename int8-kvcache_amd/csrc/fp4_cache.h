@@ -206,7 +206,9 @@ __global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
 //                      makes two codes and their exponent two bf16 operands, exactly; q as it is
 //   e    = S scale     m: the row's largest e plus BLOCK_REF, raised where it lags by more than 8
 //   P    = 2^(e - m),  l += P
-//   O   += V^T . P     v_mfma_f32_16x16x32_bf16: V's values as bf16 (exact), P rounded to bf16 (2^-8 of each weight)
+//   O   += V^T . P     v_mfma_f32_16x16x32_bf16, twice: V's values as bf16 (exact), P as a sum of two bf16, cut off (2^-14
+//                      of each weight; one bf16 was as far off as the output's own rounding, 2.3e-3 in all in place of 1.7e-3, and
+//                      decode of 128 x 32768 keys 360 us in place of 371, verification of 64 x 8 tokens 51 in place of 56)
 // A conversion leaves two channels of a key side by side; the product sums over what is side by side. Not PACK: v_perm pairs
 // keys of a channel, two for four values. PACK (at most 8 (token, q head) rows per kv head): the rows are the columns 0 .. 7 and
 // again 8 .. 15, and the product runs over (key, channel of the pair): P stands beside zeros, in columns 0 .. 7 for the even
@@ -216,10 +218,10 @@ __global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
 // Weights are kept below 2^-24 (BLOCK_REF), so that a sum over a million keys of V's largest values (6 2^125) stays finite.
 //
 // What bounds it, and the time (4 KV heads of 128, 7 q heads each):
-//   decode, 128 requests of 32768 keys   360 us for 2.29 GB: 6.4 TB/s of the 6.9 that a plain stream reads (whole lines, below)
+//   decode, 128 requests of 32768 keys   371 us for 2.29 GB: 6.2 TB/s of the 6.9 that a plain stream reads (whole lines, below)
 //   decode, 1 request of 4096 keys       9.3 us and 3.8 for the merge: latency of launch, plan, table, first tile and merge
-//   64 requests of 8 rows, 512 .. 8192 keys   45 us and 8 for the merge, for 89 MB: issue of vector instructions. Of a tile and
-//                  16 rows it needs 64 conversions, 32 v_perm and some 80 others; two row tiles a wavefront share the first two
+//   64 requests of 8 rows, 512 .. 8192 keys   48 us and 8 for the merge, for 89 MB: issue of vector instructions. Of a tile and
+//                  16 rows it needs 64 conversions, 32 v_perm and some 100 others; two row tiles a wavefront share the first two
 // 12 or 16 wavefronts to a workgroup, 3 or 4 to a SIMD, change neither of the last two (62 .. 64 us where 8 took 63).
 // ------------------------------------------------------------------------------------------------
 struct Fp4AttnArgs {
@@ -281,6 +283,8 @@ struct Fp4Query {
     odd = group4_sum(odd);
   }
 };
+// what a float's upper half, as bf16, leaves of it (exact)
+__device__ __forceinline__ float behind_bf16(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 // S^T[key][row] of 16 keys and NR row tiles: lane (n, g) holds row n's keys 4 g + i. The keys are converted once.
 template <int D, int NR>
 __device__ __forceinline__ void fp4_scores(const uint32_t (&k)[D / 32], uint32_t byte, const Fp4Query<D> (&q)[NR], int b, f32x4 (&z)[NR][2]) {
@@ -466,7 +470,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 #pragma unroll
     for (int c = 0; c < NA; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const uint32_t pshift = PACK && n >= 8 ? 16 : 0;   // PACK: where the column's weights stand beside zeros
+  const uint32_t pick = n >= 8 ? 0x03020c0cu : 0x0c0c0302u;   // PACK: a weight's upper half to where the column has it, beside 0
 
   // tile j, at `slot` of the ring (the reads' statements wait for themselves: the compiler sees neither the DMAs nor that they
   // are done)
@@ -572,11 +576,14 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       if (MASKED) vsc[e] = n0 + 16 * (e / 4) + 4 * g + e % 4 < L ? vsc[e] : 0.f;
     }
     if constexpr (PACK) {
-      u32x4 pw[2];
+      u32x4 pw[2], pl[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pw[b][i] = pack_bf16x2_rne(p[0][b][i], 0.f) << pshift;
+        for (int i = 0; i < 4; ++i) {
+          pw[b][i] = __builtin_amdgcn_perm(0, __float_as_uint(p[0][b][i]), pick);
+          pl[b][i] = __builtin_amdgcn_perm(0, __float_as_uint(behind_bf16(p[0][b][i])), pick);
+        }
       auto pair = [&](auto byte_t) {   // the channels 2 B and 2 B + 1 of the lane's
         constexpr int B = decltype(byte_t)::value;
 #pragma unroll
@@ -585,8 +592,9 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[4 * b + i], vsc[4 * b + i], B));
-          acc[0][B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&w), *reinterpret_cast<bf16x8*>(&pw[b]),
-                                                              acc[0][B], 0, 0, 0);
+          const bf16x8 x = *reinterpret_cast<bf16x8*>(&w);
+          acc[0][B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, *reinterpret_cast<bf16x8*>(&pw[b]), acc[0][B], 0, 0, 0);
+          acc[0][B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, *reinterpret_cast<bf16x8*>(&pl[b]), acc[0][B], 0, 0, 0);
         }
       };
       pair(std::integral_constant<int, 0>{});
@@ -596,12 +604,18 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
         pair(std::integral_constant<int, 3>{});
       }
     } else {
-      bf16x8 pop[NR];   // the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i
+      bf16x8 pop[NR], plo[NR];   // the MFMA's key 8 g + 4 b + i: key 16 b + 4 g + i
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
-        u32x4 pw = {pack_bf16x2_rne(p[t][0][0], p[t][0][1]), pack_bf16x2_rne(p[t][0][2], p[t][0][3]),
-                    pack_bf16x2_rne(p[t][1][0], p[t][1][1]), pack_bf16x2_rne(p[t][1][2], p[t][1][3])};
+        u32x4 pw, pl;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = p[t][i / 2][2 * (i % 2)], y = p[t][i / 2][2 * (i % 2) + 1];
+          pw[i] = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+          pl[i] = __builtin_amdgcn_perm(__float_as_uint(behind_bf16(y)), __float_as_uint(behind_bf16(x)), 0x07060302u);
+        }
         pop[t] = *reinterpret_cast<bf16x8*>(&pw);
+        plo[t] = *reinterpret_cast<bf16x8*>(&pl);
       }
       auto pair = [&](auto byte_t) {
         constexpr int B = decltype(byte_t)::value;
@@ -618,6 +632,8 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
         for (int t = 0; t < NR; ++t) {
           acc[t][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), pop[t], acc[t][2 * B], 0, 0, 0);
           acc[t][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), pop[t], acc[t][2 * B + 1], 0, 0, 0);
+          acc[t][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&even), plo[t], acc[t][2 * B], 0, 0, 0);
+          acc[t][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&odd), plo[t], acc[t][2 * B + 1], 0, 0, 0);
         }
       };
       pair(std::integral_constant<int, 0>{});

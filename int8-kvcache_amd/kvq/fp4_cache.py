@@ -126,9 +126,10 @@ def fp4_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block
                          max_query_len=1, lse=None):
     """Attention over a 4-bit cache for the requests with at most SHORT_Q query tokens (others are skipped), with
     decode_attention's arguments: out rows softmax(q k^T softmax_scale) v, bottom-right causal, of the cached values and the
-    bf16 q. Rounded: the weights, to bf16 (2^-8 of each). A row that sees no key is zero, another with a NaN or an infinity
-    in q NaN. The caches have the same page and slot strides. segm: split buffers (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces. lse
-    (float32 [T, q heads]): filled with the rows' natural log-sum-exp, -inf for a row that sees no key."""
+    bf16 q. Rounded: the weights, to a sum of two bf16 (2^-14 of each). A row that sees no key is zero, another with a
+    NaN or an infinity in q NaN. The caches have the same page and slot strides. segm: split buffers
+    (cuda_kernels.split_buffers), which allow a (request, kv head) to be cut into pieces. lse (float32 [T, q heads]): filled
+    with the rows' natural log-sum-exp, -inf for a row that sees no key."""
     name = "fp4_decode_attention"
     so, sm, ss = segm if segm is not None else (None, None, None)
     if ck._served(ck.ext(), name, q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, scales["k_scale"],

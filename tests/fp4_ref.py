@@ -103,10 +103,11 @@ def attention(q, kc, vc, scales, cu, lens, table, softmax_scale, short_q=8):
             shape = (b - a, g, d)
             o, mag = (p.view(-1, n) @ v).view(shape), (p.view(-1, n) @ v.abs()).view(shape)
             off = _score_error(x, k, softmax_scale)
-            # a score's error once in the numerator and once in the denominator; the weights to bf16; fp32 sums; a weight is at
+            # a score's error once in the numerator and once in the denominator; the weights to bf16, of short requests to a
+            # sum of two, both cut off (a step, 2^-7, of what is left, itself below 2^-7); fp32 sums; a weight is at
             # least 2^-40 of itself in fp32 (a maximum that lags by 8, and 32 more), so one below 2^(40 - 126) of the row's may
             # be lost, and all of them together
-            err = torch.expm1(2 * off) * mag + U * mag + 1e-5 * mag + n * 2.0 ** -86 * v.abs().max()
+            err = torch.expm1(2 * off) * mag + (U if b - a > short_q else 2.0 ** -14) * mag + 1e-5 * mag + n * 2.0 ** -86 * v.abs().max()
             out[a:b, h * g:(h + 1) * g] = o
             bound[a:b, h * g:(h + 1) * g] = U * (o.abs() + err) + err + 1e-38
             lse[a:b, h * g:(h + 1) * g] = of

@@ -199,7 +199,7 @@ def attend(c, hq, q_lens, lens, segm=None, seed=3, scale=None, pad=2, q=None):
     plan = ck.plan_long(cu, lens, bs)
     got = fc.fp4_paged_attention(q, c.kc, c.vc, out, i32(cu), i32(lens), c.table, max(q_lens), scale, c.scales, plan, segm, lse)
     assert got is out
-    want, bound, of, of_bound = R.attention(q, c.kc, c.vc, c.scales, cu, lens, c.table, scale)
+    want, bound, of, of_bound = R.attention(q, c.kc, c.vc, c.scales, cu, lens, c.table, scale, ck.SHORT_Q)
     assert bool((out[cu[-1]:] == 7.0).all()) and bool((lse[cu[-1]:] == 7.0).all())
     R.check(out[:cu[-1]], want[:cu[-1]], bound[:cu[-1]], (q_lens, lens))
     for r, n in enumerate(q_lens):
