@@ -208,7 +208,7 @@ __global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
 //   P    = 2^(e - m),  l += P
 //   O   += V^T . P     v_mfma_f32_16x16x32_bf16, twice: V's values as bf16 (exact), P as a sum of two bf16, cut off (2^-14
 //                      of each weight; one bf16 was as far off as the output's own rounding, 2.3e-3 in all in place of 1.7e-3, and
-//                      decode of 128 x 32768 keys 360 us in place of 371, verification of 64 x 8 tokens 51 in place of 56)
+//                      decode of 128 x 32768 keys 354 us in place of 364, verification of 64 x 8 tokens 51 in place of 56)
 // A conversion leaves two channels of a key side by side; the product sums over what is side by side. Not PACK: v_perm pairs
 // keys of a channel, two for four values. PACK (at most 8 (token, q head) rows per kv head): the rows are the columns 0 .. 7 and
 // again 8 .. 15, and the product runs over (key, channel of the pair): P stands beside zeros, in columns 0 .. 7 for the even
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
 // Weights are kept below 2^-24 (BLOCK_REF), so that a sum over a million keys of V's largest values (6 2^125) stays finite.
 //
 // What bounds it, and the time (4 KV heads of 128, 7 q heads each):
-//   decode, 128 requests of 32768 keys   371 us for 2.29 GB: 6.2 TB/s of the 6.9 that a plain stream reads (whole lines, below)
+//   decode, 128 requests of 32768 keys   364 us for 2.29 GB: 6.3 TB/s of the 6.9 that a plain stream reads (whole lines, below)
 //   decode, 1 request of 4096 keys       9.3 us and 3.8 for the merge: latency of launch, plan, table, first tile and merge
 //   64 requests of 8 rows, 512 .. 8192 keys   48 us and 8 for the merge, for 89 MB: issue of vector instructions. Of a tile and
 //                  16 rows it needs 64 conversions, 32 v_perm and some 100 others; two row tiles a wavefront share the first two
@@ -251,10 +251,12 @@ constexpr int fp4_accs(int d, bool pack) { return pack ? d / 32 : d / 16; }
 constexpr int fp4_merge_fields(int d, bool pack) { return 4 * fp4_accs(d, pack) + 2; }
 // Wavefronts of a workgroup: what its registers and LDS leave room for. Segments that are not cut are shared by all of them.
 constexpr int FP4_WAVES = 8;
-// Tiles of a wavefront's ring. Up to 8 query rows a key's products are few and the loads are what it waits for: 4 (ragged decode,
-// 96 requests of up to 32768 keys: 58 us; 2 slots, with twice the workgroups on a unit, 67). More rows: 2, where the products
-// cover the loads and more workgroups fit (24 requests of 4 rows: 23 us; 4 slots 27).
-constexpr int fp4_slots(bool pack) { return pack ? 4 : 2; }
+// Tiles of a wavefront's ring. Up to 8 query rows a key's products are few and the loads are what it waits for. In segments that
+// are cut, of few wavefronts: 4 (ragged decode, 96 requests of up to 32768 keys: 58 us; 2 slots, with twice the workgroups on a
+// unit, 67). Whole ones: 2 (128 requests of 32768 keys 364 us, of 4096 74; 4 slots 372 and 77; the units are full either way and
+// ask for less at once; 12 and 16 wavefronts of 2 slots: 370, 366). More rows: 2, where the products cover the loads and more
+// workgroups fit (24 requests of 4 rows: 23 us; 4 slots 27).
+constexpr int fp4_slots(bool pack, bool cut) { return pack && cut ? 4 : 2; }
 // The DMAs' cache policy: streaming (2) where K and V are read once; the wavefronts of several row tiles read the same lines
 // (verification, 16 requests of 8 rows: 22.5 us against 24.4; 24 of 4: 23.0 against 25.2; 64 of 4: 37.4 against 35.7).
 constexpr int fp4_dma_aux(bool pack) { return pack ? 2 : 0; }
@@ -339,7 +341,7 @@ __device__ __forceinline__ int fp4_place(bool apart, int r, int p) {
 }
 
 // One wavefront's share of a piece: NR row tiles from row0 on, key tiles c_begin + ks, c_begin + ks + KS, .. below c_end.
-template <int D, bool PACK, int NR>
+template <int D, bool PACK, int NR, int S>
 __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqlen, int kvh, int row0, int c_begin, int c_end,
                                            int ks, int KS, int part, int nparts, uint8_t* lds, int lane) {
   const Fp4AttnArgs& args = fresh_fp4();
@@ -347,7 +349,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   constexpr int RT = PACK ? 8 : 16;        // rows of a tile
   static_assert(!PACK || NR == 1, "at most 8 rows are one tile");
   constexpr int VT = D / 16, NA = fp4_accs(D, PACK), SB = D / FP4_GROUP;
-  constexpr int S = fp4_slots(PACK), SLOT = fp4_slot(D), HALF = fp4_half(D), CODES = fp4_codes(D), CH = fp4_chunks(D);
+  constexpr int SLOT = fp4_slot(D), HALF = fp4_half(D), CODES = fp4_codes(D), CH = fp4_chunks(D);
   constexpr int DMAS = CODES / 1024, OPS = 2 * (DMAS + 1);   // DMAs of a half's codes; vector memory operations of a tile
   static_assert(S * OPS < 64, "vmcnt range");
   const int G = PACK ? a.G >> 1 : a.G;     // (PACK: the plan counts 16 columns a tile, two a row)
@@ -777,23 +779,29 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   }
 }
 
-template <int D, bool PACK, int NR>
+template <int D, bool PACK, int NR, int S>
 __global__ __launch_bounds__(WAVE * FP4_WAVES) __attribute__((amdgpu_waves_per_eu(1, 2))) void fp4_attn_kernel(Fp4AttnArgs args) {
   touch_args();
   const AttnArgs& a = args.a;
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int rw = a.rt / NR, ksplit = a.ksplit, kspl = wave / rw, rtile = NR * (wave - kspl * rw);
   extern __shared__ __attribute__((aligned(1024))) uint8_t fp4_lds[];
-  uint8_t* ring = fp4_lds + wave * fp4_slots(PACK) * fp4_slot(D);
+  uint8_t* ring = fp4_lds + wave * S * fp4_slot(D);
   int solo = 0;
   walk_pieces(a, lane, [&](int r, const ReqWork& w, int kvh, int rg, int c0, int c1, int part, int nparts) {
     const int row0 = (rg * a.rt + rtile) * (PACK ? 8 : 16);
     // (a piece for all key splits, or a short one for one of them: one call, the code is long)
     const bool all = ksplit > 1 && c1 - c0 >= a.coop;
     if (all || solo % ksplit == kspl)
-      attend_fp4<D, PACK, NR>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, all ? kspl : 0, all ? ksplit : 1, part, nparts, ring, lane);
+      attend_fp4<D, PACK, NR, S>(r, w.tok, w.qlen, w.len, kvh, row0, c0, c1, all ? kspl : 0, all ? ksplit : 1, part, nparts, ring, lane);
     if (!all) ++solo;
   });
+}
+
+template <int D>
+auto fp4_attn_of(bool pack, bool cut, int nr) -> void (*)(Fp4AttnArgs) {
+  if (pack) return cut ? fp4_attn_kernel<D, true, 1, fp4_slots(true, true)> : fp4_attn_kernel<D, true, 1, fp4_slots(true, false)>;
+  return nr == 1 ? fp4_attn_kernel<D, false, 1, fp4_slots(false, true)> : fp4_attn_kernel<D, false, 2, fp4_slots(false, true)>;
 }
 
 // split_reduce_kernel, with the rows' log-sum-exp
@@ -1050,10 +1058,9 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   a.plan_fast_max = tune.plan_fast_max ? (int)std::max(1ll, std::min(PLAN_FAST_MAX, atoll(tune.plan_fast_max)))
                                        : (int)PLAN_FAST_MAX;
   a.seg_cost = seg_cost_units(tune, 0);
-  const size_t lds = (size_t)waves * fp4_slots(pack) * fp4_slot((int)head_dim);
-  void (*kern)(Fp4AttnArgs) =
-      head_dim == 128 ? (pack ? fp4_attn_kernel<128, true, 1> : nr == 1 ? fp4_attn_kernel<128, false, 1> : fp4_attn_kernel<128, false, 2>)
-                      : (pack ? fp4_attn_kernel<64, true, 1> : nr == 1 ? fp4_attn_kernel<64, false, 1> : fp4_attn_kernel<64, false, 2>);
+  const int slots = fp4_slots(pack, cut);
+  const size_t lds = (size_t)waves * slots * fp4_slot((int)head_dim);
+  void (*kern)(Fp4AttnArgs) = head_dim == 128 ? fp4_attn_of<128>(pack, cut, nr) : fp4_attn_of<64>(pack, cut, nr);
   const int64_t tw = target_waves > 0 ? target_waves
                      : cut            ? (int64_t)device_cus() * resident_waves((const void*)kern, WAVE * waves, lds)
                                       : (int64_t)device_cus() * waves;
