@@ -2,6 +2,7 @@
 //
 //   key_weights_kernel   adds what each cached key gets of a step's rows to its running sum
 //   evict_kernel         chooses each request's and kv head's keys and moves them to the front of its pages
+//   evict_lens_kernel    the lengths from then on, where they replace what evict_kernel reads
 #pragma once
 
 namespace {
@@ -147,7 +148,7 @@ struct EvictArgs {
   const int* keep;
   const int* block_table;
   int* kept;
-  int* new_lens;
+  int* new_lens;   // NULL: evict_lens_kernel writes them
   int64_t k_sb, k_sn, k_sh, v_sb, v_sn, v_sh, w_sr, w_sh, bt_stride, kp_sr, kp_sh;
   int heads, num_blocks, lbs, cols, bt_cols, kept_cols, recent;
 };
@@ -165,6 +166,19 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// request r's keys, and how many of them each kv head may hold
+__device__ __forceinline__ int evict_keys_of(const EvictArgs& a, int r) {
+  return min(max(a.seq_lens[r], 0), (int)min((int64_t)a.bt_cols << a.lbs, (int64_t)INT32_MAX));
+}
+__device__ __forceinline__ int evict_most_of(const EvictArgs& a, int r) { return min(max(a.keep[r], 0), a.kept_cols); }
+
+// The lengths in a launch behind evict_kernel's, for a call whose new_lens is its seq_lens or keep: a head's workgroup may start
+// after another of its request has ended, and reads both. (Elsewhere the first head's workgroup writes them: a launch less.)
+__global__ __launch_bounds__(256) void evict_lens_kernel(EvictArgs a, int* new_lens, int num_seqs) {
+  const int r = blockIdx.x * 256 + threadIdx.x;
+  if (r < num_seqs) new_lens[r] = min(evict_keys_of(a, r), evict_most_of(a, r));
+}
+
 template <int D>
 __global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
   constexpr int SB = D / FP4_GROUP, CH = D / 32;   // exponent bytes, 16-byte chunks of a row's codes
@@ -175,11 +189,10 @@ __global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int r = blockIdx.x / a.heads, h = blockIdx.x - r * a.heads;
   const int* bt = a.block_table + (int64_t)r * a.bt_stride;
-  const int n = min(max(a.seq_lens[r], 0), (int)min((int64_t)a.bt_cols << a.lbs, (int64_t)INT32_MAX));
-  const int m = min(max(a.keep[r], 0), a.kept_cols), len = min(n, m);
+  const int n = evict_keys_of(a, r), m = evict_most_of(a, r);
   int* kept = a.kept + (int64_t)r * a.kp_sr + (int64_t)h * a.kp_sh;
   float* w = a.w + (int64_t)r * a.w_sr + (int64_t)h * a.w_sh;
-  if (h == 0 && tid == 0) a.new_lens[r] = len;
+  if (a.new_lens && h == 0 && tid == 0) a.new_lens[r] = min(n, m);
   if (n <= m) {   // all of them stay where they are
     for (int i = tid; i < n; i += EV_THREADS) kept[i] = i;
     return;
@@ -438,9 +451,15 @@ int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, ui
     return fail("%s: null pointer", nm);
   if (bt_cols > (1 << 28) / block_size) return fail("%s: tables of more than 2^28 slots", nm);   // (32-bit byte offsets)
   if (num_seqs > INT32_MAX / num_heads) return fail("%s: too many requests and heads for one call", nm);
+  // (element r of new_lens follows from element r of the others alone)
+  for (const int32_t* in : {seq_lens, keep})
+    if (in != new_lens && (uintptr_t)in < (uintptr_t)(new_lens + num_seqs) && (uintptr_t)new_lens < (uintptr_t)(in + num_seqs))
+      return fail("%s: new_lens may be seq_lens or keep, but not overlap them otherwise", nm);
+  const bool in_place = new_lens == seq_lens || new_lens == keep;
   EvictArgs a;
   a.kc = k_cache; a.vc = v_cache; a.s = Fp4Scales{k_scale, v_scale, s_sb, s_sh}; a.w = weights;
-  a.seq_lens = seq_lens; a.keep = keep; a.block_table = block_table; a.kept = kept; a.new_lens = new_lens;
+  a.seq_lens = seq_lens; a.keep = keep; a.block_table = block_table; a.kept = kept;
+  a.new_lens = in_place ? nullptr : new_lens;
   a.k_sb = k_sb; a.k_sn = k_sn; a.k_sh = k_sh; a.v_sb = v_sb; a.v_sn = v_sn; a.v_sh = v_sh; a.w_sr = w_sr; a.w_sh = w_sh;
   a.bt_stride = bt_stride; a.kp_sr = kp_sr; a.kp_sh = kp_sh;
   a.heads = (int)num_heads; a.num_blocks = (int)num_blocks; a.lbs = log2i(block_size); a.cols = (int)w_cols;
@@ -449,7 +468,10 @@ int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, ui
   const dim3 grid((unsigned)(num_seqs * num_heads));
   if (head_dim == 128) hipLaunchKernelGGL(evict_kernel<128>, grid, dim3(EV_THREADS), 0, st, a);
   else hipLaunchKernelGGL(evict_kernel<64>, grid, dim3(EV_THREADS), 0, st, a);
-  return launched(nm);
+  const int rc = launched(nm);
+  if (rc != KVQ_OK || !in_place) return rc;
+  hipLaunchKernelGGL(evict_lens_kernel, dim3((unsigned)((num_seqs + 255) / 256)), dim3(256), 0, st, a, new_lens, (int)num_seqs);
+  return launched("fp4_evict: lengths");
 }
 
 }  // extern "C"

@@ -252,7 +252,8 @@ def evict_keys(k_cache, v_cache, scales, weights, seq_lens, keep, recent, block_
     (add_key_weights; ties to the lowest position, a NaN counts as the largest); their rows move to the request's first positions
     in their order, their weights with them, and the weights behind become 0. kept (int32 [requests, kv heads, most that a
     request may keep]): filled with the position that each row held; new_lens (int32 [requests]): min(seq_lens, keep), the
-    lengths from now on: the next token's slot is the one behind, while its position for the rotation goes on counting. keep
+    lengths from now on: the next token's slot is the one behind, while its position for the rotation goes on counting. new_lens
+    may be seq_lens (or keep) itself, which is then updated in place, by a launch more; it overlaps them in no other way. keep
     counts as at most kept.shape[2] and as at least 0. A request within its budget is left as it is. The pages of the
     requests must be theirs alone, a prefix that two requests share is not evicted from. A table has at most 2^28 slots.
     Returns new_lens."""

@@ -213,6 +213,15 @@ def test_c_entry_layouts():
     assert _c("fp4_evict", (25, (1 << 23) + 1)) == (1, "fp4_evict: tables of more than 2^28 slots")
 
 
+@pytest.mark.parametrize("seq_lens,keep,new_lens", [(64, 80, 68), (64, 80, 60), (80, 64, 68), (80, 64, 60), (64, 64, 68),
+                                                    (64, 68, 64), (68, 64, 64)])
+def test_new_lengths_that_overlap_others(seq_lens, keep, new_lens):
+    """The workgroups of a request's heads read seq_lens and keep while new_lens is written: two requests' lengths (8 bytes)
+    that are neither one of the others' nor apart from them."""
+    assert _c("fp4_evict", (20, seq_lens), (21, keep), (31, new_lens)) == (
+        1, "fp4_evict: new_lens may be seq_lens or keep, but not overlap them otherwise")
+
+
 ROPE = [16, 3584, 128, 16, 512, 128, 16, 3584, 128, 16, 512, 128, 5, 28, 4, 128, 16, 64, 16, 64, 100, 64, 0, 16, 16, 1, 1e-6, 0, None]
 
 

@@ -642,6 +642,35 @@ def test_evict_bounds_of_its_arguments():
     assert all(torch.equal(a, b) for a, b in zip(before, c.parts())) and int(new) == 20
 
 
+@pytest.mark.parametrize("where", ["seq_lens", "keep", "both", "beside"])
+def test_evict_updates_lengths_in_place(where):
+    """new_lens as seq_lens or keep themselves, or right behind them: every head's choice, rows and sums as with lengths of
+    their own. More workgroups (60 requests of 16 heads) than run at once, so that some start after others have ended."""
+    h, d, bs = 16, 64, 16
+    lens = [200 + 3 * r if r % 5 else 40 for r in range(60)]
+    keep = lens if where == "both" else [64 + r for r in range(60)]
+    a, b = (filled(h, d, bs, lens) for _ in range(2))
+    w = [torch.rand(60, h, 400, generator=gen(5)).to(DEV) for _ in range(2)]
+    kept = [torch.full((60, h, 100), -7, dtype=torch.int32, device=DEV) for _ in range(2)]
+    own = i32([-7] * 60)
+    fc.evict_keys(a.kc, a.vc, a.scales, w[0], i32(lens), i32(keep), 16, a.table, kept[0], own)
+    both = i32(lens + [-7] * 60)
+    at, budget = both[:60], i32(keep)
+    if where == "both":
+        budget = at
+    new = {"seq_lens": at, "keep": budget, "both": at, "beside": both[60:]}[where]
+    for _ in range(2):   # (again: nothing is left to do, the lengths stay)
+        got = fc.evict_keys(b.kc, b.vc, b.scales, w[1], at, budget, 16, b.table, kept[1], new)
+        assert got is new and torch.equal(new, own)
+        if where != "seq_lens":
+            break
+    assert new.cpu().tolist() == [min(n, k, 100) for n, k in zip(lens, keep)]
+    assert torch.equal(*w)
+    assert all(torch.equal(x, y) for x, y in zip(a.parts(), b.parts()))
+    if where != "seq_lens":
+        assert torch.equal(*kept)
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("hq,h,d,bs", [(28, 4, 128, 16), (14, 2, 64, 64)])
 def test_generation_captured_and_replayed(hq, h, d, bs):
