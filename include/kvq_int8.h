@@ -349,8 +349,9 @@ int kvq_block_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const
  * A cached value is an e2m1 code (0, 1/2, 1, 3/2, 2, 3, 4, 6 or their negatives) times 2^(byte - 127), one exponent byte for
  * each 32 channels of a row (page, slot, head), K's and V's apart. Caches are bytes [nb, bs, H, D / 2], strides (sb, sn, sh, 1)
  * in bytes, multiples of 16, pages below 4 GiB apart, channel 2 c in the low half of byte c; exponent bytes k_scale / v_scale
- * [nb, H, bs, D / 32], strides (s_sb, s_sh, D / 32, 1), 16-byte aligned as well. Tables and lengths as above; head_dim 64 or 128. An exponent byte
- * that the write does not make (above 252: 255 would be no number) may give any value for its own row, and counts nowhere else. */
+ * [nb, H, bs, D / 32], strides (s_sb, s_sh, D / 32, 1), 16-byte aligned as well. Tables and lengths as above; head_dim 64 or
+ * 128. An exponent byte that the write does not make (above 252: 255 would be no number) may give any value for its own row and for
+ * the query rows that see it, and counts nowhere else. */
 
 /* Quantize rows into slots: for t < num_tokens whose slot is in [0, nb * bs), others are skipped. Of a group's 32 values x, with
  * top = max |x| (finite x):  e = floor(log2 top) - 2, one more where top 2^-e > 7, from -100 to 125; byte e + 127; codes the

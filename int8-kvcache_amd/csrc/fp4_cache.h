@@ -574,8 +574,11 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
       // the lane's byte as an exponent: the conversion reads no other bits of its scale (D = 64: two keys' bytes to a word)
       const uint32_t w = D == 128 ? vs[e / 4][e % 4] : vs[e / 4][e % 4 / 2];
       vsc[e] = __uint_as_float(__builtin_amdgcn_alignbit(w, w, D == 128 || e % 2 == 0 ? vrot : vrot + 16));
-      // whatever lies behind the last key is finite: it meets weights of 0
-      if (MASKED) vsc[e] = n0 + 16 * (e / 4) + 4 * g + e % 4 < L ? vsc[e] : 0.f;
+      // what lies behind the last key, and keys whose byte no write makes, are finite: they meet weights of 0 (in the tiles that
+      // every row sees whole no weight is masked, and such a byte is its key's alone)
+      if (MASKED)
+        vsc[e] = n0 + 16 * (e / 4) + 4 * g + e % 4 < L
+                     ? __uint_as_float(min(__float_as_uint(vsc[e]) & 0x7f800000u, (uint32_t)FP4_MAX_E << 23)) : 0.f;
     }
     if constexpr (PACK) {
       u32x4 pw[2], pl[2];

@@ -348,6 +348,32 @@ def test_rows_that_are_no_number_stay_their_own(q_lens, split):
         R.check_lse(lse, of, of_bound)
 
 
+@pytest.mark.parametrize("byte", [253, 254, 255])
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("hq,h,d,q_lens", [(28, 4, 128, [8, 2, 5, 3]), (4, 4, 128, [8, 2, 5, 3]), (14, 2, 64, [4, 2, 3, 2]),
+                                           (16, 16, 64, [7, 2, 8, 3]), (28, 4, 128, [20, 40, 9, 300])])
+def test_exponent_bytes_that_no_write_makes(hq, h, d, q_lens, split, byte):
+    """A byte above 252 at a request's last key, K's and V's: query rows that do not see that key, all but the request's last,
+    are what they are over the clean cache."""
+    lens = [3000, 33, 400, 301]
+    c = filled(h, d, 16, lens)
+    cu = cumsum(q_lens)
+    q = torch.randn(cu[-1], hq, d, generator=gen(2)).to(torch.bfloat16).to(DEV)
+    want, bound, of, of_bound = R.attention(q, c.kc, c.vc, c.scales, cu, lens, c.table, d ** -0.5)
+    for r, n in enumerate(lens):
+        for s in c.scales.values():
+            s[int(c.host[r, (n - 1) // 16]), :, (n - 1) % 16] = byte
+    segm = nan_segm(cu[-1], hq, 16, d) if split else None
+    out, lse = torch.full_like(q, 7.0), torch.zeros(cu[-1], hq, device=DEV)
+    fc.fp4_paged_attention(q, c.kc, c.vc, out, i32(cu), i32(lens), c.table, max(q_lens), d ** -0.5, c.scales,
+                           ck.plan_long(cu, lens, 16), segm, lse)
+    seen = torch.ones(cu[-1], dtype=torch.bool)
+    seen[torch.tensor(cu[1:]) - 1] = False
+    R.check(out[seen], want[seen], bound[seen], q_lens)
+    if max(q_lens) <= ck.SHORT_Q:
+        R.check_lse(lse[seen], of[seen], of_bound[seen])
+
+
 @pytest.mark.parametrize("short_q", [1, 1_000_000])
 def test_other_short_query_limits(short_q, monkeypatch):
     """KVQ_SHORT_Q's other uses: verification rows through the long path, whole prompts through the short one."""
