@@ -379,8 +379,8 @@ int kvq_fp4_pages(const uint8_t* k_cache, int64_t kc_sb, int64_t kc_sn, int64_t 
                   const int32_t* src_j, int64_t num_pages, void* stream);
 
 /* The attention below for the rows of a work list, as kvq_paged_prefill_attention_ex takes it (tile_piece NULL: every entry
- * reads all of its rows' keys), over pages that kvq_fp4_pages left (pages_table [num_seqs, ..], row stride pt_stride). q is
- * taken as it is, the weights are rounded to bf16. */
+ * reads all of its rows' keys), over pages that kvq_fp4_pages left (pages_table [num_seqs, ..], row stride pt_stride), with the
+ * same q and weights. */
 int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k_pages, const void* v_pages,
                               const float* page_scales, int64_t num_pages, int64_t block_size, int64_t num_kv_heads,
                               int64_t head_dim, void* out, int64_t o_st, int64_t o_sh, const int32_t* cu_seqlens_q,

@@ -5,7 +5,8 @@
 //
 //   quant_fp4_kernel   quantize a step's new K/V rows into their slots
 //   read_fp4_kernel    ranges of the requests' keys back to bf16 rows
-//   fp4_pages_kernel   pages back to a contiguous bf16 cache, for the prefill
+//   fp4_pages_kernel   pages back to a contiguous bf16 cache
+//   fp4_prefill_kernel attention of long queries over that
 //   fp4_attn_kernel    attention of short queries
 #pragma once
 
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(256) void read_fp4_kernel(ReadFp4Args a) {
 // block_table[src_req[p], src_j[p]]. A lane converts 8 channels of one (slot, head), K or V by blockIdx.z; lanes in the order
 // of the output. The prefill over it is the block-scaled cache's, whose weights leave room for large values: every scale 1.
 // A chunk's queries are many per key, so that its keys are converted once, and not by each tile of queries. 3,533 keys of 8 heads
-// (18 MB): 6.2 us, 3 TB/s, of the 37 us that the prefill over them takes.
+// (18 MB): 6.2 us, 3 TB/s.
 // ------------------------------------------------------------------------------------------------
 struct Fp4PagesArgs {
   const uint8_t* kc;
@@ -198,6 +199,15 @@ __global__ __launch_bounds__(256) void fp4_pages_kernel(Fp4PagesArgs a) {
     const uint32_t w = *reinterpret_cast<const uint32_t*>(cache + t * sn + h * sh + 4 * c);
     out[i] = fp4_to_bf16(w, fp4_finite(scale[h * a.s.sh + t * (D / FP4_GROUP) + c / 4]));
   }
+}
+
+// The bf16 prefill over those pages. Its weights are a sum of two bf16, as the short queries' below, so that a row's accuracy does
+// not depend on how many tokens its request has: 1.6e-3 against 64 bits, the output's own rounding, where one bf16 had 2.1e-3.
+// The second product over V costs what it adds to the matrix cores' work, half as much again: 2 x 8,192 tokens of 32 / 8 heads x
+// 128 1,260 us with the copy in place of 910, 700 tokens and 333 behind 2,167 keys 53.6 in place of 47.7.
+template <int D, bool SPLIT>
+__global__ __launch_bounds__(256, D == 64 ? 4 : 3) void fp4_prefill_kernel(PrefillArgs a) {
+  prefill_body<D, PR_SRC_BF16_FP4, SPLIT>(a);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -981,8 +991,8 @@ int kvq_fp4_prefill_attention(const void* q, int64_t q_st, int64_t q_sh, const v
   const dim3 grid((unsigned)num_tiles, (unsigned)num_kv_heads);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   void (*kern)(PrefillArgs) = head_dim == 128
-      ? (tile_piece ? block_codes_prefill_kernel<128, true> : block_codes_prefill_kernel<128, false>)
-      : (tile_piece ? block_codes_prefill_kernel<64, true> : block_codes_prefill_kernel<64, false>);
+      ? (tile_piece ? fp4_prefill_kernel<128, true> : fp4_prefill_kernel<128, false>)
+      : (tile_piece ? fp4_prefill_kernel<64, true> : fp4_prefill_kernel<64, false>);
   hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
   const int rc = launched(nm);
   if (rc != KVQ_OK || !tile_piece || num_merge == 0) return rc;

@@ -2189,12 +2189,13 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rne(float a, float b) {
 // (prefill_i8_kernel below), converted tile by tile either as dequant_pages converts them (bf16 of
 // code x scale) or as exact bf16 codes with the scales folded into q (K) and the output (V).
 // PR_SRC_BF16_BLOCK: a bf16 temporary cache of a block-scaled cache's codes, each 16-key half tile's K scale a factor of
-// its scores and its V scale's log2 an addend of P's exponent (block_cache.h).
-constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2, PR_SRC_BF16_BLOCK = 3;
+// its scores and its V scale's log2 an addend of P's exponent (block_cache.h). PR_SRC_BF16_FP4: the same over a 4-bit cache's
+// values, every scale 1, with P as a sum of two bf16 (fp4_cache.h).
+constexpr int PR_SRC_BF16 = 0, PR_SRC_I8 = 1, PR_SRC_I8_FOLD = 2, PR_SRC_BF16_BLOCK = 3, PR_SRC_BF16_FP4 = 4;
 
 template <int D, int SRC, bool SPLIT>
 __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
-  constexpr bool BLK = SRC == PR_SRC_BF16_BLOCK;
+  constexpr bool TWO = SRC == PR_SRC_BF16_FP4, BLK = SRC == PR_SRC_BF16_BLOCK || TWO;
   constexpr bool I8 = SRC != PR_SRC_BF16 && !BLK;
   constexpr bool FOLD = SRC == PR_SRC_I8_FOLD;
   constexpr int DS = D / 32;                // 32-channel chunks of the QK contraction
@@ -2685,17 +2686,21 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   auto softmax_pv = [&](auto st_t) {
     const uint32_t so = stage_vofs(st_t);
     const int SOI = stage_iofs(st_t);
-    bf16x8 pop[RB];
+    bf16x8 pop[RB], plo[TWO ? RB : 1];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       float p[2][4], psum = 0.f;
-      if constexpr (BLK) {   // (the denominators below, on the matrix cores)
+      if constexpr (BLK) {   // (the denominators below, on the matrix cores; TWO: here, there the tile loop would spill)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const float f = ent[b][0] * a.sm_log2, e0 = ent[b][1] - m[rb];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], f, e0));
+          for (int i = 0; i < 4; ++i) {
+            p[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rb][b][i], f, e0));
+            if constexpr (TWO) psum += p[b][i];
+          }
         }
+        if constexpr (TWO) l[rb] += psum;
       } else {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -2712,6 +2717,13 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       pw.z = pack_bf16x2_rne(p[1][0], p[1][1]);
       pw.w = pack_bf16x2_rne(p[1][2], p[1][3]);
       pop[rb] = *reinterpret_cast<bf16x8*>(&pw);
+      if constexpr (TWO) {   // what the rounding left (exact in fp32), to a bf16 as well: 2^-18 of a weight is lost
+        u32x4 lw;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          lw[j] = pack_bf16x2_rne(p[j / 2][2 * (j % 2)] - bf16_lo(pw[j]), p[j / 2][2 * (j % 2) + 1] - bf16_hi(pw[j]));
+        plo[rb] = *reinterpret_cast<bf16x8*>(&lw);
+      }
     }
     // V^T operands (lane (n, g): V[4g + k][16 tt + n] and V[16 + 4g + k][16 tt + n], k = 0..3). The
     // transposing reads are issued from inline assembly, 4 channel tiles per statement, each statement
@@ -2747,11 +2759,15 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
           acc[rb][t0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rb], acc[rb][t0 + u], 0, 0, 0);
+        if constexpr (TWO)
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb)
+            acc[rb][t0 + u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, plo[rb], acc[rb][t0 + u], 0, 0, 0);
       }
     }
     // BLK: the sums of the rounded P by half, each over its V scale: row b of the first operand picks the keys of half b, so
     // they stand in the lanes of group 0
-    if constexpr (BLK) {
+    if constexpr (BLK && !TWO) {
       u32x4 pw = {n == 0 ? 0x3f803f80u : 0u, 0u, n == 1 ? 0x3f803f80u : 0u, 0u};
       pw.y = pw.x;
       pw.w = pw.z;

@@ -167,8 +167,8 @@ def fp4_decode_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block
 
 def fp4_long_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, plan, softmax_scale, scales):
     """Attention over a 4-bit cache for the plan's long requests (cuda_kernels.plan_long; the others' rows are left as they
-    were): fp4_decode_attention's formula, over a temporary bf16 copy of their pages (exact, 4 bytes per key, channel and kv
-    head); q as it is, the weights rounded to bf16. Inside a graph capture the plan's lists must be on the GPU already
+    were): fp4_decode_attention's formula and roundings, over a temporary bf16 copy of their pages (exact, 4 bytes per key,
+    channel and kv head). Inside a graph capture the plan's lists must be on the GPU already
     (plan.gpu, plan.work: an earlier call with the plan made them)."""
     name, e = "fp4_long_attention", ck.ext()
     bs, h, d = *k_cache.shape[1:3], 2 * k_cache.shape[3]

@@ -245,6 +245,17 @@ def test_long_queries(hq, h, d, bs):
     attend(c, hq, [9, 20, 333, 130], lens)
 
 
+@pytest.mark.parametrize("hq,h,d", HEADS)
+def test_long_queries_hold_their_weights_as_short_ones(hq, h, d):
+    """A row's weights are a sum of two bf16 (2^-14 of each and less) whatever its request's number of tokens."""
+    lens, q_lens = [9, 40, 333, 700, 5000], [9, 20, 333, 130, 10]
+    c = filled(h, d, 32, lens)
+    q, out, _ = attend(c, hq, q_lens, lens, pad=0)
+    cu = cumsum(q_lens)
+    want, bound, _, _ = R.attention(q, c.kc, c.vc, c.scales, cu, lens, c.table, d ** -0.5, short_q=max(q_lens))
+    R.check(out, want, bound)
+
+
 def test_mixed_batch_and_few_rows_over_many_keys():
     lens = [500, 20, 64, 2000, 9000]
     c = filled(4, 128, 32, lens)
