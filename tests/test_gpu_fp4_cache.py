@@ -781,6 +781,97 @@ def test_generation_captured_and_replayed(hq, h, d, bs):
     attend(b.c, hq, [1] * n, lens)
 
 
+@pytest.mark.parametrize("hq,h,d,bs", [(28, 4, 128, 16), (14, 2, 64, 64)])
+def test_steps_of_a_generation_against_plain_forms(hq, h, d, bs):
+    """Norm and rotation, write, attention, key weights and eviction (lengths in place) in one captured graph: what each replay
+    leaves against the plain forms of what it found."""
+    prompts, budget, recent, cols = [37, 5, 128, 300], 64, 8, 320
+    n = len(prompts)
+    table, nb = page_table([max(p, budget) + 2 for p in prompts], bs, 3)
+    dtab, cu = table.to(DEV), i32(range(n + 1))
+    angle = torch.arange(400)[:, None] * 1000.0 ** (-torch.arange(0, d, 2) / d)
+    cos_sin = torch.cat([angle.cos(), angle.sin()], -1).to(DEV)
+    weight = [(1 + 0.1 * torch.randn(d, generator=gen(s))).to(DEV) for s in (1, 2)]
+    c = Cache(h, d, bs, nb)
+    k, v = rows(sum(prompts), h, d, 4)
+    fc.quant_fp4_cache(k.to(DEV), v.to(DEV), c.kc, c.vc, c.scales, slots_of(table, prompts, bs).to(DEV))
+    lens, pos = i32(prompts), torch.tensor(prompts, device=DEV)
+    qkv = torch.zeros(n, (hq + 2 * h) * d, dtype=torch.bfloat16, device=DEV)
+    q = qkv[:, :hq * d].view(n, hq, d)
+    k, v = (x.view(n, h, d) for x in qkv[:, hq * d:].chunk(2, -1))
+    w, lse, out = torch.zeros(n, h, cols, device=DEV), torch.zeros(n, hq, device=DEV), torch.zeros_like(q)
+    segm = ck.split_buffers(n, hq, d, 16, DEV)
+    keep, kept = i32([budget] * n), torch.zeros(n, h, budget, dtype=torch.int32, device=DEV)
+
+    def step():
+        rope.norm_rope(q, k, pos, cos_sin, *weight)
+        slots = (dtab.gather(1, (lens // bs).long()[:, None])[:, 0] * bs + lens % bs).long()
+        lens.add_(1)
+        fc.quant_fp4_cache(k, v, c.kc, c.vc, c.scales, slots)
+        fc.fp4_paged_attention(q, c.kc, c.vc, out, cu, lens, dtab, 1, d ** -0.5, c.scales, None, segm, lse)
+        fc.add_key_weights(q, c.kc, c.scales, lse, w, cu, lens, dtab, d ** -0.5)
+        fc.evict_keys(c.kc, c.vc, c.scales, w, lens, keep, recent, dtab, kept, lens)
+        pos.add_(1)
+
+    state = (*c.parts(), lens, pos, w)
+    start = [t.clone() for t in state]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for t, x in zip(state, start):
+        t.copy_(x)
+    for i in range(6):
+        qkv.copy_(torch.randn(qkv.shape, generator=gen(100 + i)))
+        q0, k0 = q.clone(), k.clone()
+        kc, vc, ks, vs, lens0, pos0, w0 = [t.clone() for t in state]
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, got, g in ((q0, q, weight[0]), (k0, k, weight[1])):
+            R.check(got, *R.norm_rope(x, pos0, cos_sin, g, 1e-6, False), i)
+        assert torch.equal(pos, pos0 + 1)
+        slots = torch.tensor([int(table[r, m // bs]) * bs + m % bs for r, m in enumerate(lens0.tolist())])
+        scales = {"k_scale": ks, "v_scale": vs}
+        for x, cache, scale in ((k, kc, ks), (v, vc, vs)):
+            R.write(x.cpu(), cache, scale, slots)
+        now = [m + 1 for m in lens0.tolist()]
+        want, bound, of, of_bound = R.attention(q, kc, vc, scales, cu.tolist(), now, dtab, d ** -0.5)
+        R.check(out, want, bound, i)
+        R.check_lse(lse, of, of_bound, i)
+        add, off = R.key_weights(q, kc, scales, lse, w.shape, cu.tolist(), now, dtab, d ** -0.5)
+        sums = (w0.double() + add).cpu()
+        off = (off + sums.to(DEV) * 2.0 ** -23).cpu()
+        old, new = [t.cpu() for t in (kc, vc, ks, vs)], [t.cpu() for t in c.parts()]
+        at, got = kept.cpu().long(), w.cpu().double()
+        assert lens.tolist() == [min(m, budget) for m in now]
+        for r, m in enumerate(now):
+            left = min(m, budget)
+            for g in range(h):
+                mine = at[r, g, :left]
+                if m <= budget:
+                    assert mine.tolist() == list(range(m))
+                else:
+                    # in order, the latest, and none of the rest that is surely below one that was left
+                    assert bool((mine[1:] > mine[:-1]).all()) and mine[-recent:].tolist() == list(range(m - recent, m))
+                    gone = torch.ones(m, dtype=torch.bool)
+                    gone[mine] = False
+                    least = (sums[r, g, mine] + off[r, g, mine])[:left - recent].min()
+                    assert bool(((sums[r, g, :m] - off[r, g, :m])[gone] <= least).all()), (i, r, g)
+                    assert bool((got[r, g, left:] == 0).all())
+                assert bool(((got[r, g, :left] - sums[r, g, mine]).abs() <= off[r, g, mine]).all()), (i, r, g)
+                dst, src = torch.arange(left), mine
+                ids = table[r].long()
+                for side_old, side_new in zip(old[:2], new[:2]):
+                    assert torch.equal(side_new[ids[dst // bs], dst % bs, g], side_old[ids[src // bs], src % bs, g])
+                for side_old, side_new in zip(old[2:], new[2:]):
+                    assert torch.equal(side_new[ids[dst // bs], g, dst % bs], side_old[ids[src // bs], g, src % bs])
+
+
 def test_caches_past_two_and_four_gib():
     """A cache of more than 4 GiB a side: the pages used lie at its ends and around 2 and 4 GiB."""
     h, d, bs = 8, 128, 64
