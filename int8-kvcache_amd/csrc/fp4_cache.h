@@ -477,7 +477,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
   for (int t = 0; t < NR; ++t) {
     rs[t] = a.sm_log2 + q[t].odd;
     lim[t] = rtok[t] < qlen ? L - qlen + 1 + rtok[t] : L;
-    m[t] = -1e30f;
+    m[t] = FP4_NO_SCORE;
     l[t] = 0.f;
 #pragma unroll
     for (int c = 0; c < NA; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};

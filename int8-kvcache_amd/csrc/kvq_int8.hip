@@ -60,6 +60,9 @@ constexpr float MIN_V_SCALE = 0x1p-70f;     // and a V scale as this (8.5e-22; t
 // (V scales of 2^121); P stays a normal number down to weights of 2^-67 of the largest at the write's smallest V scale, of
 // 2^-24 at MIN_V_SCALE.
 constexpr float BLOCK_REF = 32.f;
+// What a row's maximum starts from in the 4-bit cache's attention: below any score, and its difference from any of them is still
+// no NaN. (The other kernels start from -1e30, as the reference does, and take scores below it for none.)
+constexpr float FP4_NO_SCORE = -3e38f;
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
@@ -2198,6 +2201,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   constexpr bool TWO = SRC == PR_SRC_BF16_FP4, BLK = SRC == PR_SRC_BF16_BLOCK || TWO;
   constexpr bool I8 = SRC != PR_SRC_BF16 && !BLK;
   constexpr bool FOLD = SRC == PR_SRC_I8_FOLD;
+  constexpr float NO_SCORE = TWO ? FP4_NO_SCORE : -1e30f;
   constexpr int DS = D / 32;                // 32-channel chunks of the QK contraction
   constexpr int VT = D / 16;                // PV channel tiles
   constexpr int RB = PR_RB;
@@ -2558,7 +2562,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   f32x4 acc[RB][VT];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
-    m[rb] = -1e30f;
+    m[rb] = NO_SCORE;
     l[rb] = 0.f;
 #pragma unroll
     for (int tt = 0; tt < VT; ++tt) acc[rb][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -2872,7 +2876,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       next_tile(c_lo, lin_t, std::true_type{});
       row_top();
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) m[rb] = __builtin_fmaxf(top[rb], -1e30f);
+      for (int rb = 0; rb < RB; ++rb) m[rb] = __builtin_fmaxf(top[rb], NO_SCORE);
       softmax_pv(scur);
       advance();
       int c = c_lo + 1;
@@ -2926,7 +2930,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     if (__syncthreads_or(jump)) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        m[rb] = -1e30f;
+        m[rb] = NO_SCORE;
         l[rb] = 0.f;
 #pragma unroll
         for (int tt = 0; tt < VT; ++tt) acc[rb][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -3034,7 +3038,7 @@ __global__ __launch_bounds__(WAVE * PR_MERGE_WAVES) void prefill_merge_kernel(Pr
   if (lane < P) ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (row0 + lane * step));
   const float* po = a.part_out + row0 * D + CPL * lane;
   const bool seen = !(ml.y == 0.f);
-  const float M = wave_max(seen ? ml.x : -1e30f);
+  const float M = wave_max(seen ? ml.x : -INFINITY);
   const float wt = seen ? __builtin_amdgcn_exp2f(ml.x - M) : 0.f;
   const float den = wave_sum(wt * ml.y);
   const float inv = den > 0.f ? 1.f / den : 0.f;

@@ -329,6 +329,43 @@ def test_largest_values_stay_finite():
 
 
 @pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("hq,h,d,q_lens", [(28, 4, 128, [1, 1, 1]), (28, 4, 128, [8, 2, 3]), (14, 2, 64, [4, 1, 8]), (28, 4, 128, [30, 9, 200]),
+                                           (16, 16, 64, [9, 40, 300])])
+def test_scores_of_any_size(hq, h, d, q_lens, sign, split):
+    """Scores of some +-1e36: a row is the mean of V over the keys of the larger score, of which every row sees some, its
+    log-sum-exp that score and the logarithm of their number."""
+    lens = [3000, 40, 700]
+    table, nb = page_table(lens, 16, 1)
+    c = Cache(h, d, 16, nb)
+    n, cu = sum(lens), cumsum(q_lens)
+    far = torch.cat([torch.arange(m) % 3 != 2 for m in lens])       # position 2, 5, .. have the larger score
+    k = sign * 2.0 ** 57 * torch.where(far, 2.0 if sign < 0 else 1.0, 1.0 if sign < 0 else 2.0)[:, None, None].expand(n, h, d)
+    v = rows(n, h, d, 3)[1]
+    fc.quant_fp4_cache(k.to(torch.bfloat16).contiguous().to(DEV), v.to(DEV), c.kc, c.vc, c.scales, slots_of(table, lens, 16).to(DEV))
+    c.table = table.to(DEV)
+    q = torch.full((cu[-1], hq, d), 2.0 ** 57, dtype=torch.bfloat16, device=DEV)
+    out, lse = torch.full_like(q, 7.0), torch.zeros(cu[-1], hq, device=DEV)
+    segm = nan_segm(cu[-1], hq, 16, d) if split else None
+    fc.fp4_paged_attention(q, c.kc, c.vc, out, i32(cu), i32(lens), c.table, max(q_lens), d ** -0.5, c.scales,
+                           ck.plan_long(cu, lens, 16), segm, lse)
+    top = sign * d ** 0.5 * 2.0 ** 114 * (1 if sign < 0 else 2)
+    for r, m in enumerate(lens):
+        vs = R.values(c.vc, c.scales["v_scale"], c.table[r], m)
+        for t in range(cu[r], cu[r + 1]):
+            at = vs[:, 2:m - cu[r + 1] + t + 1:3]
+            if at.shape[1] == 0:
+                continue
+            want = at.mean(1).repeat_interleave(hq // h, 0)
+            mag = at.abs().mean(1).repeat_interleave(hq // h, 0)
+            # equal weights: their rounding (2^-14), fp32 sums, the output's half step
+            err = (2.0 ** -14 + 1e-5) * mag
+            R.check(out[t], want, R.U * (want.abs() + err) + err, (r, t))
+            if q_lens[r] <= ck.SHORT_Q:
+                assert bool(((lse[t].double() - top).abs() <= abs(top) * d * 2.0 ** -22).all()), (r, t)
+
+
+@pytest.mark.parametrize("split", [False, True])
 @pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [8, 8, 3, 8], [40, 9, 300, 12]])
 def test_rows_that_are_no_number_stay_their_own(q_lens, split):
     """A NaN or an infinity in one q row makes that row and its log-sum-exp NaN and no other's; rows of zeros average."""
