@@ -421,8 +421,8 @@ int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t
  * position, a NaN the largest; 0 from w_cols on). Their rows move to positions 0 .. m - 1 in order, their weights with them;
  * weights[r, h, m .. n - 1] become 0. kept[r, h, i] (int32, strides (kp_sr, kp_sh, 1)): the position that row i held before;
  * new_lens[r] = min(n, m); new_lens may be seq_lens or keep itself (one launch more), and overlaps them in no other way. Where
- * n <= m nothing moves (kept[r, h, i] = i). Entries of kept from new_lens[r] on and cache rows from there on are left as they are. The pages of a call's requests must be theirs alone. Page ids outside [0, nb) read as page
- * 0, and are not written. A table has at most 2^28 slots (bt_cols * block_size). Bit-reproducible. */
+ * n <= m nothing moves (kept[r, h, i] = i). Entries of kept from new_lens[r] on and cache rows from there on are left as they are.
+ * The pages of a call's requests must be theirs alone. Page ids outside [0, nb) read as page 0, and are not written. A table has at most 2^28 slots (bt_cols * block_size). Bit-reproducible. */
 int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, uint8_t* v_cache, int64_t v_sb, int64_t v_sn,
                   int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, uint8_t* k_scale,
                   uint8_t* v_scale, int64_t s_sb, int64_t s_sh, float* weights, int64_t w_sr, int64_t w_sh, int64_t w_cols,

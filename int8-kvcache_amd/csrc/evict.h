@@ -13,8 +13,8 @@ namespace {
 // tiles, so a key's sum has one owner in a call: nothing is atomic, the result does not depend on the order of workgroups);
 // a piece's tiles go round the workgroup's wavefronts. A wavefront holds RT row tiles' planes; more rows take another round
 // over the piece's tiles, whose keys' sums the same lanes then add to again.
-// Bound by memory: 16 requests of 16384 keys, 8 KV heads of 128, 8 tokens of 4 q heads: 57 us for 160 MB, of K's codes and the
-// sums. Where K's and V's codes of a key share a line, the half that is V's comes along: 290 MB, 5.1 TB/s. A ragged batch of 24
+// Bound by memory: 16 requests of 16384 keys, 8 KV heads of 128, 8 tokens of 4 q heads: 58 us for 160 MB, of K's codes and the
+// sums. Where K's and V's codes of a key share a line, the half that is V's comes along: 290 MB, 5.0 TB/s. A ragged batch of 24
 // decoding requests: 6.7 us. Rings of 3 and 4 tiles, 8 wavefronts and loads without the streaming hint were all slower.
 // ------------------------------------------------------------------------------------------------
 struct KeyWeightArgs {
@@ -134,10 +134,12 @@ __global__ __launch_bounds__(WAVE * KW_WAVES) void key_weights_kernel(KeyWeightA
 //            64 answers of the u-th; so counts, ties and places are a scan over lanes and one over wavefronts
 //   move     row i takes the row of the i-th kept position, which is i or later: rows are read into registers, in order, a
 //            batch at a time, and written after a barrier, so that nothing is overwritten that is still to be read
-// One workgroup, because a choice needs all of a head's sums and the moves its order: nothing leaves the workgroup, and two
-// launches less. 64 requests of 1024 .. 32768 keys, 8 heads, to 2048 each: 90 us, of which 46 are the moves (285 MB read and
-// written: 6.2 TB/s) and 44 the choice, from 35 MB of sums that it reads two or three times (select, list). 1 request of 4096
-// keys to 1024, 4 heads: 16 us, 9 of them the choice: latency of its passes and barriers.
+// One workgroup: a choice needs all of a head's sums, its counts and places stay within the workgroup, and there is one launch.
+// (Rows whose source lies at or behind m meet no destination and could be moved by any number of workgroups, in a launch more.)
+// 64 requests of 1024 .. 32768 keys, 8 heads, to 2048 each (51 of them have more): 88 .. 103 us from box to box. In a pass that
+// finds the rows moved already it takes 42: the choice, from 19 MB of sums that it reads two or three times (select, list) by one
+// workgroup for the longest head. The rest are the moves, 225 MB read and written, some 4 TB/s, and the clearing of 16 MB of sums.
+// 1 request of 4096 keys to 1024, 4 heads: 16 us, 9 of them the choice: latency of its passes and barriers.
 // ------------------------------------------------------------------------------------------------
 struct EvictArgs {
   uint8_t* kc;

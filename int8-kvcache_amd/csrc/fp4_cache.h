@@ -229,10 +229,11 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 3) void fp4_prefill_kernel(Prefi
 //
 // What bounds it, and the time (4 KV heads of 128, 7 q heads each):
 //   decode, 128 requests of 32768 keys   364 us for 2.29 GB: 6.3 TB/s of the 6.9 that a plain stream reads (whole lines, below)
-//   decode, 1 request of 4096 keys       9.3 us and 3.8 for the merge: latency of launch, plan, table, first tile and merge
-//   64 requests of 8 rows, 512 .. 8192 keys   48 us and 8 for the merge, for 89 MB: issue of vector instructions. Of a tile and
+//   decode, 1 request of 4096 keys       9.3 us and 3.9 for the merge: latency of launch, plan, table, first tile and merge
+//   64 requests of 8 tokens, 512 .. 8192 keys 49 us and 8 for the merge, for 89 MB: issue of vector instructions. Of a tile and
 //                  16 rows it needs 64 conversions, 32 v_perm and some 100 others; two row tiles a wavefront share the first two
-// 12 or 16 wavefronts to a workgroup, 3 or 4 to a SIMD, change neither of the last two (62 .. 64 us where 8 took 63).
+// 12 or 16 wavefronts to a workgroup, 3 or 4 to a SIMD, change neither of the last two (the third, when a weight was one bf16 and
+// each row tile had a wavefront: 62 .. 64 us where 8 took 63).
 // ------------------------------------------------------------------------------------------------
 struct Fp4AttnArgs {
   AttnArgs a;   // (first: fresh_args)
@@ -262,13 +263,14 @@ constexpr int fp4_merge_fields(int d, bool pack) { return 4 * fp4_accs(d, pack) 
 // Wavefronts of a workgroup: what its registers and LDS leave room for. Segments that are not cut are shared by all of them.
 constexpr int FP4_WAVES = 8;
 // Tiles of a wavefront's ring. Up to 8 query rows a key's products are few and the loads are what it waits for. In segments that
-// are cut, of few wavefronts: 4 (ragged decode, 96 requests of up to 32768 keys: 58 us; 2 slots, with twice the workgroups on a
-// unit, 67). Whole ones: 2 (128 requests of 32768 keys 364 us, of 4096 74; 4 slots 372 and 77; the units are full either way and
+// are cut, of few wavefronts: 4 (ragged decode, 96 requests of up to 32768 keys: 66 us; 2 slots, with twice the workgroups on a
+// unit, 71). Whole ones: 2 (128 requests of 32768 keys 367 us, of 4096 74; 4 slots 374 and 76; the units are full either way and
 // ask for less at once; 12 and 16 wavefronts of 2 slots: 370, 366). More rows: 2, where the products cover the loads and more
-// workgroups fit (24 requests of 4 rows: 23 us; 4 slots 27).
+// workgroups fit (24 requests of 4 tokens: 24.3 us; 4 slots 26.5).
 constexpr int fp4_slots(bool pack, bool cut) { return pack && cut ? 4 : 2; }
 // The DMAs' cache policy: streaming (2) where K and V are read once; the wavefronts of several row tiles read the same lines
-// (verification, 16 requests of 8 rows: 22.5 us against 24.4; 24 of 4: 23.0 against 25.2; 64 of 4: 37.4 against 35.7).
+// (verification, 16 requests of 8 tokens: 23.6 us against 25.4; 24 of 4: 24.3 against 25.9; 64 of 8: 54.7 against 56.9; 64 of 4
+// over 4096 keys each: 42.0 against 40.9).
 constexpr int fp4_dma_aux(bool pack) { return pack ? 2 : 0; }
 
 // 16 query rows as the MFMA's second operand: lane (n, g) holds row n's channels (D / 4) g + 8 s .. + 7 in step s.
@@ -310,16 +312,14 @@ __device__ __forceinline__ void fp4_scores(const uint32_t (&k)[D / 32], uint32_t
       z[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(&w), q[t].op[s], z[t][b], 0, 0, 0);
   }
 }
-// A streaming load of each lane's own `off` from a base that the wavefront shares, through a buffer descriptor: the base and
-// `uni` stay in scalar registers, a lane's part is 32 bits (as 64-bit addresses they took two vector registers and an addition
-// a load: 14 of a tile's 160 vector instructions).
+// key_weights_kernel's loads: a streaming load of each lane's own `off` from a base that the wavefront shares, through a buffer
+// descriptor. The base and `uni` stay in scalar registers, a lane's part is 32 bits (64-bit addresses take two vector registers
+// and an addition a load).
 template <typename T>
 __device__ __forceinline__ T load_at(const uint8_t* base, uint32_t off, uint32_t uni) {
   const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, INT32_MAX, QC_RSRC_WORD3);
   if constexpr (sizeof(T) == 16) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b128(r, off, uni, QC_LOAD_AUX));
   else if constexpr (sizeof(T) == 8) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b64(r, off, uni, QC_LOAD_AUX));
-  else if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, uni, QC_LOAD_AUX));
-  else if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, uni, QC_LOAD_AUX));
   else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b8(r, off, uni, QC_LOAD_AUX));
 }
 // page p of `base`: strides are below 4 GiB (check_fp4)
@@ -662,7 +662,7 @@ __device__ __forceinline__ void attend_fp4(int seq, int tok, int qlen, int seqle
 
   // S - 1 tiles in flight. One body for whole tiles and one for those at some row's limit or at the end, whatever their place in
   // the ring: a piece is a few tiles, and the first pass through code costs more than the second (a body to each slot: 1 request
-  // of 4096 keys 13.3 us against 12.7, 64 of 8 rows 64 against 60; 128 of 32768 keys 359 against 361).
+  // of 4096 keys 13.3 us against 12.7, 64 of 8 tokens 64 against 60, 128 of 32768 keys 359 against 361, when weights were one bf16).
   const int full_end = lim_lo > 0 ? lim_lo / TILE : 0;
   const int j_full = full_end > c_begin + ks ? (full_end - c_begin - ks + KS - 1) / KS : 0;
   uint32_t slot = 0, free = (S - 1) * SLOT;
@@ -1037,8 +1037,9 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
   const Tuning tune = read_tuning();
   const bool cut = num_splits > 1 && segm_rows > 0, few = num_seqs * num_kv_heads <= WIDE_SPLIT_PAIRS;
   // More rows than a tile holds: a wavefront to each tile of rows, or one to two of them, which loads and converts a key once for
-  // both but keeps half as many wavefronts busy. Few pairs of a request and a KV head, cut, take the first (16 requests of 8 rows,
-  // 28 heads on 4: 22.5 us against 26), others the second (64 such requests: 54 against 62; 64 of 4096 keys, whole: 59 against 76).
+  // both but keeps half as many wavefronts busy. Few pairs of a request and a KV head, cut, take the first (16 requests of 8 tokens,
+  // 28 heads on 4: 23.6 us against 27.0), others the second (64 such requests: 54.7 against 62.4; 64 of 4096 keys, whole: 69
+  // against 81).
   const int rt = rows <= 16 ? 1 : rows <= 32 ? 2 : MAX_ROW_TILES, nr = rt == 1 || (cut && few) ? 1 : 2, rw = rt / nr;
   const int most = cut && rt == 1 ? MAX_ROW_TILES : FP4_WAVES;
   const int ks_max = tune.ksplit ? std::max(1, std::min(FP4_WAVES, atoi(tune.ksplit)))
