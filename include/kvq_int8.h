@@ -408,7 +408,7 @@ int kvq_fp4_decode_attention(const void* q, int64_t q_st, int64_t q_sh, const ui
 /* Add the attention weights of a step's rows to running sums: for requests with 1 <= q_len <= qmax and j < w_cols,
  *   weights[r, h, j] += sum over r's tokens and h's q heads that see key j of exp(q . k_j softmax_scale - lse)
  * weights fp32 [B, Hkv, w_cols], strides (w_sr, w_sh, 1); lse as kvq_fp4_decode_attention leaves it, rows whose lse is not
- * finite add nothing. Row r of weights belongs to request r alone. Bit-reproducible. */
+ * finite add nothing. Row r of weights belongs to request r alone, and no two rows overlap. Bit-reproducible. */
 int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* k_cache, int64_t k_sb, int64_t k_sn,
                         int64_t k_sh, int64_t num_blocks, int64_t block_size, int64_t num_kv_heads, int64_t head_dim,
                         const uint8_t* k_scale, int64_t s_sb, int64_t s_sh, const float* lse, int64_t lse_st, float* weights,
@@ -422,7 +422,8 @@ int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t
  * weights[r, h, m .. n - 1] become 0. kept[r, h, i] (int32, strides (kp_sr, kp_sh, 1)): the position that row i held before;
  * new_lens[r] = min(n, m); new_lens may be seq_lens or keep itself (one launch more), and overlaps them in no other way. Where
  * n <= m nothing moves (kept[r, h, i] = i). Entries of kept from new_lens[r] on and cache rows from there on are left as they are.
- * The pages of a call's requests must be theirs alone. Page ids outside [0, nb) read as page 0, and are not written. A table has at most 2^28 slots (bt_cols * block_size). Bit-reproducible. */
+ * Rows (r, h) of weights do not overlap, nor do kept's. The pages of a call's requests must be theirs alone. Page ids outside
+ * [0, nb) read as page 0, and are not written. A table has at most 2^28 slots (bt_cols * block_size). Bit-reproducible. */
 int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, uint8_t* v_cache, int64_t v_sb, int64_t v_sn,
                   int64_t v_sh, int64_t num_blocks, int64_t block_size, int64_t num_heads, int64_t head_dim, uint8_t* k_scale,
                   uint8_t* v_scale, int64_t s_sb, int64_t s_sh, float* weights, int64_t w_sr, int64_t w_sh, int64_t w_cols,

@@ -380,6 +380,15 @@ __global__ __launch_bounds__(EV_THREADS) void evict_kernel(EvictArgs a) {
   for (int i = m + tid; i < min(n, a.cols); i += EV_THREADS) w[i] = 0.f;
 }
 
+// rows of `cols` elements, n0 x n1 of them at multiples of s0 and s1, of which no two share an element (any order of the two; a
+// workgroup updates each in place)
+bool rows_apart(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t cols) {
+  if (cols == 0) return true;
+  if (n0 <= 1) return n1 <= 1 || s1 >= cols;
+  if (n1 <= 1) return s0 >= cols;
+  return s0 >= s1 ? s1 >= cols && s0 - cols >= (n1 - 1) * s1 : s0 >= cols && s1 - cols >= (n0 - 1) * s0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -401,6 +410,7 @@ int kvq_fp4_key_weights(const void* q, int64_t q_st, int64_t q_sh, const uint8_t
     return fail("%s: bad head counts Hq=%lld Hkv=%lld", nm, (long long)num_q_heads, (long long)num_kv_heads);
   if (!q || !lse || !weights || !cu_seqlens_q || !seq_lens || !block_table) return fail("%s: null pointer", nm);
   if (!aligned16(q) || (q_st | q_sh) % 8) return fail("%s: rows must be 16-byte aligned (base pointers and strides)", nm);
+  if (!rows_apart(num_seqs, w_sr, num_kv_heads, w_sh, w_cols)) return fail("%s: rows of weights overlap", nm);
   const int G = (int)(num_q_heads / num_kv_heads);
   const int64_t most = std::min<int64_t>(qmax, INT32_MAX / 4);
   if (G * most > INT32_MAX / 4) return fail("%s: too many rows for one kv head", nm);
@@ -453,6 +463,8 @@ int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, ui
     return fail("%s: null pointer", nm);
   if (bt_cols > (1 << 28) / block_size) return fail("%s: tables of more than 2^28 slots", nm);   // (32-bit byte offsets)
   if (num_seqs > INT32_MAX / num_heads) return fail("%s: too many requests and heads for one call", nm);
+  if (!rows_apart(num_seqs, w_sr, num_heads, w_sh, w_cols)) return fail("%s: rows of weights overlap", nm);
+  if (!rows_apart(num_seqs, kp_sr, num_heads, kp_sh, kept_cols)) return fail("%s: rows of kept overlap", nm);
   // (element r of new_lens follows from element r of the others alone)
   for (const int32_t* in : {seq_lens, keep})
     if (in != new_lens && (uintptr_t)in < (uintptr_t)(new_lens + num_seqs) && (uintptr_t)new_lens < (uintptr_t)(in + num_seqs))

@@ -216,7 +216,7 @@ def fp4_paged_attention(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_
 
 def add_key_weights(q, k_cache, scales, lse, weights, cu_seqlens_q, seq_lens, block_table, softmax_scale, max_query_len=1):
     """Add the attention that each cached key gets of a step's rows to its running sum, weights (float32 [requests, kv heads,
-    keys], the last dim contiguous; row r is request r's alone): the softmax's weights, summed over the request's query tokens
+    keys], the last dim contiguous, no rows in common; row r is request r's alone): the softmax's weights, summed over the request's query tokens
     and the kv head's q heads. For the requests with at most SHORT_Q query tokens; keys behind weights' last column are not
     counted. q, lse: fp4_decode_attention's of the same rows (rows whose lse is not finite add nothing). A prompt's keys are
     judged by its last tokens: attend with those rows of q as a short request over all of its keys, then call this with them.
@@ -256,7 +256,8 @@ def evict_keys(k_cache, v_cache, scales, weights, seq_lens, keep, recent, block_
     may be seq_lens (or keep) itself, which is then updated in place, by a launch more; it overlaps them in no other way. keep
     counts as at most kept.shape[2] and as at least 0. A request within its budget is left as it is. The pages of the
     requests must be theirs alone, a prefix that two requests share is not evicted from. A table has at most 2^28 slots.
-    Returns new_lens."""
+    Rows of weights, or of kept, have nothing in common (sums that a request's heads share are copied for each head). Returns
+    new_lens."""
     name = "evict_keys"
     if ck._served(ck.ext(), name, k_cache, v_cache, scales["k_scale"], scales["v_scale"], weights, seq_lens, keep, recent,
                   block_table, kept, new_lens):

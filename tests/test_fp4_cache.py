@@ -222,6 +222,20 @@ def test_new_lengths_that_overlap_others(seq_lens, keep, new_lens):
         1, "fp4_evict: new_lens may be seq_lens or keep, but not overlap them otherwise")
 
 
+def test_rows_that_overlap():
+    """Sums that requests or heads share (an expanded tensor's strides of 0) would be updated by several workgroups; rows apart in
+    any order are taken (and these calls refused for what is looked at next)."""
+    for sr, sh in ((384, 96), (96, 192), (1000, 97), (97, 1000)):
+        assert _c("fp4_key_weights", (17, sr), (18, sh), (25, 65528), (28, 1 << 30))[1] == "fp4_key_weights: too many rows for one kv head"
+        assert "new_lens may be" in _c("fp4_evict", (17, sr), (18, sh), (20, 64), (31, 68))[1]
+    assert "new_lens may be" in _c("fp4_evict", (28, 4), (29, 8), (20, 64), (31, 68))[1]
+    for name in ("fp4_key_weights", "fp4_evict"):
+        for sr, sh in ((0, 96), (384, 0), (0, 0), (384, 95), (383, 96), (95, 190), (96, 191)):
+            assert _c(name, (17, sr), (18, sh)) == (1, f"{name}: rows of weights overlap"), (name, sr, sh)
+    for sr, sh in ((0, 4), (16, 0), (16, 3), (15, 4)):
+        assert _c("fp4_evict", (28, sr), (29, sh)) == (1, "fp4_evict: rows of kept overlap"), (sr, sh)
+
+
 ROPE = [16, 3584, 128, 16, 512, 128, 16, 3584, 128, 16, 512, 128, 5, 28, 4, 128, 16, 64, 16, 64, 100, 64, 0, 16, 16, 1, 1e-6, 0, None]
 
 

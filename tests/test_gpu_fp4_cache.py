@@ -745,6 +745,31 @@ def test_evict_updates_lengths_in_place(where):
         assert torch.equal(*kept)
 
 
+def test_sums_in_other_orders():
+    """weights and kept as views of heads-first buffers, requests side by side; expanded over heads they are refused."""
+    lens, h = [300, 40, 700], 4
+    a, b = (filled(h, 128, 16, lens) for _ in range(2))
+    w = torch.rand(3, h, 704, generator=gen(1)).to(DEV)
+    v = w.transpose(0, 1).contiguous().transpose(0, 1)
+    q = torch.randn(3, 28, 128, generator=gen(2)).to(torch.bfloat16).to(DEV)
+    lse = torch.full((3, 28), 5.0, device=DEV)
+    kept = torch.full((3, h, 100), -7, dtype=torch.int32, device=DEV)
+    kept2 = torch.full((h, 3, 100), -7, dtype=torch.int32, device=DEV).transpose(0, 1)
+    new = [i32([0] * 3) for _ in range(2)]
+    for c, x, k, n in ((a, w, kept, new[0]), (b, v, kept2, new[1])):
+        fc.add_key_weights(q, c.kc, c.scales, lse, x, i32([0, 1, 2, 3]), i32(lens), c.table, 0.1)
+        fc.evict_keys(c.kc, c.vc, c.scales, x, i32(lens), i32([100] * 3), 10, c.table, k, n)
+    assert torch.equal(w, v) and torch.equal(kept, kept2) and torch.equal(*new)
+    assert all(torch.equal(x, y) for x, y in zip(a.parts(), b.parts()))
+    shared = torch.rand(3, 1, 704, device=DEV).expand(3, h, 704)
+    with pytest.raises(RuntimeError, match="rows of weights overlap"):
+        fc.evict_keys(a.kc, a.vc, a.scales, shared, i32(lens), i32([50] * 3), 10, a.table, kept, new[0])
+    with pytest.raises(RuntimeError, match="rows of weights overlap"):
+        fc.add_key_weights(q, a.kc, a.scales, lse, shared, i32([0, 1, 2, 3]), i32(lens), a.table, 0.1)
+    with pytest.raises(RuntimeError, match="rows of kept overlap"):
+        fc.evict_keys(a.kc, a.vc, a.scales, w, i32(lens), i32([50] * 3), 10, a.table, kept[:, :1].expand(3, h, 100), new[0])
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("hq,h,d,bs", [(28, 4, 128, 16), (14, 2, 64, 64)])
 def test_generation_captured_and_replayed(hq, h, d, bs):
