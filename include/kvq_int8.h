@@ -437,7 +437,8 @@ int kvq_fp4_evict(uint8_t* k_cache, int64_t k_sb, int64_t k_sn, int64_t k_sh, ui
  * for the pairs of the first rotary_dim channels: (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where interleaved. q / k and their
  * outputs bf16 [T, H, D], strides (st, sh, 1), an output may be its input; positions int32 or int64 (position_bits); table
  * [num_positions, rotary_dim] (row stride t_st) fp32 or bf16: rotary_dim / 2 cosines, then as many sines; weights [D] fp32 or
- * bf16, both NULL: no norm. fp32 throughout, one rounding. rotary_dim a multiple of 16. No counterpart in the reference. */
+ * bf16, both NULL: no norm. fp32 throughout, the sum of a row's squares too (values within 2^-60 .. 2^60, smaller ones where eps
+ * is not 0), one rounding. rotary_dim a multiple of 16. No counterpart in the reference. */
 int kvq_norm_rope(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, void* q_out,
                   int64_t qo_st, int64_t qo_sh, void* k_out, int64_t ko_st, int64_t ko_sh, int64_t num_tokens,
                   int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, const void* positions, int64_t position_bits,

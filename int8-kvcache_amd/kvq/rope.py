@@ -19,8 +19,9 @@ def norm_rope(q, k, positions, cos_sin, q_weight=None, k_weight=None, eps=1e-6, 
 
     cos_sin (float32 or bf16 [positions, R], R a multiple of 16 up to D): row p holds position p's R / 2 cosines, then its sines.
     A pair is (i, i + R / 2), or (2 i, 2 i + 1) where interleaved. positions: int32 or int64 [T]; the rows of a token whose
-    position the table does not have are left as they are. float32 throughout, one rounding. q_out, k_out: where the results
-    go, q and k themselves by default (no other overlap). Returns (q_out, k_out)."""
+    position the table does not have are left as they are. float32 throughout, the sum of a row's squares too (so for values
+    within 2^-60 .. 2^60, smaller ones where eps is not 0), one rounding. q_out, k_out: where the results go,
+    q and k themselves by default (no other overlap). Returns (q_out, k_out)."""
     name = "norm_rope"
     q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
     if ck._served(ck.ext(), name, q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out):
